@@ -85,14 +85,12 @@ def draw(rng):
     dtype = rng.choice(list(TYPES))
     if op == "norm":
         dim = _spread(rng, 16, 8192)
-        if rng.random() < 0.6:
-            dim = _even(dim)
+        dim = _even(dim) if rng.random() < 0.6 else dim | 1
         return _norm(rng.choice(["forward", "gradient"]), _spread(rng, 1, min(65536, 64_000_000 // dim)), dim, dtype,
                      rng.choice([1, 1, 1, 4]))
     if op == "adapt":
         d_in, d_out = _spread(rng, 32, 4096), _spread(rng, 32, 4096)
-        if rng.random() < 0.7:
-            d_in, d_out = _even(d_in), _even(d_out)
+        d_in, d_out = (_even(d_in), _even(d_out)) if rng.random() < 0.7 else (d_in | 1, d_out | 1)
         single = rng.random() < 0.25
         # (what a row costs in single precision is more than in 16 bits)
         most = int((60e9 if dtype == "float32" else 240e9) / (2 * d_in * d_out))
