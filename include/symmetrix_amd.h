@@ -288,6 +288,84 @@ int smx_nlist_arrays(smx_nlist* nl, const int** num_neigh, const int** first_nei
 int smx_nlist_copy_to_host(smx_nlist* nl, int* num_neigh, int* neigh_indices, int* neigh_types, int* neigh_shift,
                            double* xyz, double* r);
 
+/* ---- Operators for heads that are fine-tuned on the engine's descriptors (H1, M1, H2) and served beside it.  They have
+ * no counterpart in the reference.  Every array is in device memory, work is enqueued on `stream` (a hipStream_t, or
+ * NULL) without synchronising, nothing is allocated (a workspace, where one is needed, is the caller's, its size asked
+ * for beforehand, and free again when the call's work on the stream is done), and calls can be captured into a graph.
+ * Arrays need the alignment of their element type only; strides are in elements, from row to row.  Results do not
+ * depend on the order in which thread blocks run. */
+enum {
+    SMX_TYPE_F32 = 0,
+    SMX_TYPE_BF16 = 1,
+    SMX_TYPE_F16 = 2
+};
+
+/* Layer norm over rows of dim numbers: y = (x - mean) rstd weight + bias, rstd = 1 / sqrt(var + eps).  weight[dim] and
+ * bias[dim] (either may be NULL) are of weight_type: the features' type or SMX_TYPE_F32.  mean[rows] and rstd[rows] may
+ * be NULL.  Sums are in single precision. */
+int smx_layer_norm_forward(int type, int weight_type, long rows, long dim, const void* d_x, long x_stride,
+                           const void* d_weight, const void* d_bias, double eps, void* d_y, long y_stride,
+                           float* d_mean, float* d_rstd, void* stream);
+/* Its gradient.  dx[rows][dim], dweight[dim] and dbias[dim] (of weight_type) may be NULL; the sums over rows behind the
+ * latter need the workspace. */
+int smx_layer_norm_backward_workspace(long rows, long dim, long* bytes);
+int smx_layer_norm_backward(int type, int weight_type, long rows, long dim, const void* d_dy, long dy_stride,
+                            const void* d_x, long x_stride, const float* d_mean, const float* d_rstd,
+                            const void* d_weight, void* d_dx, long dx_stride, void* d_dweight, void* d_dbias,
+                            void* d_workspace, long workspace_bytes, void* stream);
+
+/* A projection shared by all rows, and a low-rank adapter per row beside it:
+ *   y_i = weight x_i + scale_a B_a (A_a x_i),  a = index_i
+ * weight[d_out][d_in] (rows weight_stride apart), A[num_adapters][rank][d_in], B[num_adapters][d_out][rank] and x are of
+ * one type; scale[num_adapters] may be NULL (ones).  index[rows] names a row's adapter, in any order; -1: none.  A row
+ * whose index is neither has NaN for results and no part in the gradients.  What one adapter holds, infinities and NaN
+ * too, has no effect on other adapters' rows. */
+typedef struct {
+    int type;
+    int d_in, d_out, rank, num_adapters;
+    long rows;
+    const void* x;
+    long x_stride;
+    const void* weight;
+    long weight_stride;
+    const void *A, *B;
+    const float* scale;
+    const int* index;
+} smx_adapted_linear;
+#define SMX_ADAPTER_MAX_RANK 128
+#define SMX_ADAPTER_MAX_COUNT 4096
+int smx_adapted_linear_workspace(const smx_adapted_linear* p, int backward, long* bytes);
+int smx_adapted_linear_forward(const smx_adapted_linear* p, void* d_y, long y_stride, void* d_workspace,
+                               long workspace_bytes, void* stream);
+/* Gradients of x, A and B with weight and scale fixed: dx[rows][d_in], dA[num_adapters][rank][d_in],
+ * dB[num_adapters][d_out][rank], all of p->type; each may be NULL.  Adapters without a row get zeros. */
+int smx_adapted_linear_backward(const smx_adapted_linear* p, const void* d_dy, long dy_stride, void* d_dx,
+                                long dx_stride, void* d_dA, void* d_dB, void* d_workspace, long workspace_bytes,
+                                void* stream);
+
+/* One AdamW step over `count` tensors (a host array of descriptions, read before the call returns):
+ *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,
+ *   p = (1 - lr weight_decay) p - lr / (1 - beta1^step) m / (sqrt(v / (1 - beta2^step)) + eps)
+ * param is of param_type, grad of grad_type (the same, or SMX_TYPE_F32).  master: parameters in single precision that
+ * the step goes by, of which param gets a rounded copy (parameters in 16 bits; for all tensors of a call or none).
+ * state_bits 32: exp_avg and exp_avg_sq are float[numel].  state_bits 8: they are codes, signed and unsigned chars
+ * [numel], and scale_avg, scale_avg_sq hold a float for every SMX_MOMENT_BLOCK of them:
+ *   m = scale c |c| / 127^2,  v = scale (c / 255)^4.  Zeros are a valid start. */
+typedef struct {
+    void* param;
+    const void* grad;
+    float* master;
+    void *exp_avg, *exp_avg_sq;
+    float *scale_avg, *scale_avg_sq;
+    long numel;
+} smx_adamw_tensor;
+#define SMX_MOMENT_BLOCK 256
+int smx_adamw_step(int param_type, int grad_type, int state_bits, const smx_adamw_tensor* tensors, int count, double lr,
+                   double beta1, double beta2, double eps, double weight_decay, long step, void* stream);
+/* What moments in 8 bits stand for, as floats; either output may be NULL. */
+int smx_moment_values(long numel, const void* d_code_avg, const float* d_scale_avg, const void* d_code_avg_sq,
+                      const float* d_scale_avg_sq, float* d_exp_avg, float* d_exp_avg_sq, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,384 @@
+"""Operators for heads that are fine-tuned on the engine's descriptors and served beside it: layer norm, a shared projection
+with a low-rank adapter per row (systems, datasets or users, each with its own), and AdamW over many tensors.
+
+Tensors are torch's, on the GPU, in float32, bfloat16 or float16; work goes to torch's current stream of their device.  The
+forward and backward calls are plain functions; layer_norm and adapted_linear are the same for torch's automatic
+differentiation.  Wrong arguments raise ValueError (TypeError for element types) before anything is launched."""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import _lib
+
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+MOMENT_BLOCK = 256          # moments in 8 bits: numbers to a scale
+MAX_RANK = 128
+MAX_ADAPTERS = 4096
+
+
+class _Adapted(C.Structure):
+    _fields_ = [("type", C.c_int), ("d_in", C.c_int), ("d_out", C.c_int), ("rank", C.c_int), ("num_adapters", C.c_int), ("rows", C.c_long),
+                ("x", C.c_void_p), ("x_stride", C.c_long), ("weight", C.c_void_p), ("weight_stride", C.c_long), ("A", C.c_void_p),
+                ("B", C.c_void_p), ("scale", C.c_void_p), ("index", C.c_void_p)]
+
+
+class _AdamwTensor(C.Structure):
+    _fields_ = [("param", C.c_void_p), ("grad", C.c_void_p), ("master", C.c_void_p), ("exp_avg", C.c_void_p), ("exp_avg_sq", C.c_void_p),
+                ("scale_avg", C.c_void_p), ("scale_avg_sq", C.c_void_p), ("numel", C.c_long)]
+
+
+_functions = None
+
+
+def _lib_functions():
+    global _functions
+    if _functions is None:
+        L = _lib.lib()
+        p, i, n, d = C.c_void_p, C.c_int, C.c_long, C.c_double
+        for name, args in (
+                ("smx_layer_norm_forward", [i, i, n, n, p, n, p, p, d, p, n, p, p, p]),
+                ("smx_layer_norm_backward_workspace", [n, n, p]),
+                ("smx_layer_norm_backward", [i, i, n, n, p, n, p, n, p, p, p, p, n, p, p, p, n, p]),
+                ("smx_adapted_linear_workspace", [p, i, p]),
+                ("smx_adapted_linear_forward", [p, p, n, p, n, p]),
+                ("smx_adapted_linear_backward", [p, p, n, p, n, p, p, p, n, p]),
+                ("smx_adamw_step", [i, i, i, p, i, d, d, d, d, d, n, p]),
+                ("smx_moment_values", [n, p, p, p, p, p, p, p])):
+            getattr(L, name).argtypes = args
+        _functions = L
+    return _functions
+
+
+def _type(t, what):
+    try:
+        return _TYPES[t.dtype]
+    except KeyError:
+        raise TypeError(f"{what}: float32, bfloat16 or float16, not {t.dtype}") from None
+
+
+def _need(holds, what):
+    if not holds:
+        raise ValueError(what)
+
+
+def _rows(t, dim, what):
+    """t[..., dim] as rows, and the stride from one to the next (a copy where the rows have none)."""
+    if t.shape[-1] != dim:
+        raise ValueError(f"{what}: rows of {dim} numbers expected, not {t.shape[-1]}")
+    if t.dim() != 2:
+        t = t.reshape(-1, dim)
+    rows = t.shape[0]
+    if rows > 1:
+        stride = t.stride(0)
+        if stride < dim or (dim > 1 and t.stride(1) != 1):
+            t, stride = t.contiguous(), dim
+    else:
+        stride = dim
+        if dim > 1 and t.stride(1) != 1:
+            t = t.contiguous()
+    return t, rows, stride
+
+
+class _On:
+    """The device of a call's tensors, made the current one where it is not, and the stream to use."""
+    __slots__ = ("device", "before")
+
+    def __init__(self, t, *others):
+        if not t.is_cuda:
+            raise ValueError("tensors on the GPU expected: there is no CPU path")
+        self.device = t.device
+        for o in others:
+            if o is not None and o.device != t.device:
+                raise ValueError(f"tensors on one device expected: {t.device} and {o.device}")
+
+    def __enter__(self):
+        self.before = torch.cuda.current_device()
+        if self.before != self.device.index:
+            torch.cuda.set_device(self.device)
+        return torch.cuda.current_stream(self.device).cuda_stream
+
+    def __exit__(self, *exc):
+        if self.before != self.device.index:
+            torch.cuda.set_device(self.before)
+
+
+# ---- layer norm
+
+def _affine(x, weight, bias):
+    dim, kind = x.shape[-1], None
+    for t, what in ((weight, "weight"), (bias, "bias")):
+        if t is None:
+            continue
+        _need(t.dim() == 1 and t.shape[0] == dim and (dim == 1 or t.stride(0) == 1), f"{what}: {dim} contiguous numbers expected")
+        if t.dtype != x.dtype and t.dtype != torch.float32:
+            raise TypeError(f"{what}: {x.dtype} or float32, not {t.dtype}")
+        _need(kind in (None, t.dtype), "weight and bias: one type expected")
+        kind = t.dtype
+    return x.dtype if kind is None else kind
+
+
+def layer_norm_forward(x, weight=None, bias=None, eps=1e-5):
+    """y = (x - mean) rstd weight + bias over the last dimension of x; returns y, mean and rstd (float32, a number a row)."""
+    kind = _type(x, "x")
+    _need(x.dim() >= 1 and x.shape[-1] >= 1, "x: rows of at least one number expected")
+    dim = x.shape[-1]
+    weights = _TYPES[_affine(x, weight, bias)]
+    rows_of, rows, stride = _rows(x, dim, "x")
+    with _On(x, weight, bias) as stream:
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        stats = torch.empty((2,) + x.shape[:-1], dtype=torch.float32, device=x.device)
+        mean, rstd = stats[0], stats[1]
+        _lib.check(_lib_functions().smx_layer_norm_forward(
+            kind, weights, rows, dim, rows_of.data_ptr(), stride, 0 if weight is None else weight.data_ptr(), 0 if bias is None else bias.data_ptr(),
+            eps, y.data_ptr(), dim, mean.data_ptr(), rstd.data_ptr(), stream))
+    return y, mean, rstd
+
+
+def layer_norm_backward(dy, x, mean, rstd, weight=None, need=(True, True, True)):
+    """Gradients of x, weight and bias (None where `need` says so); the latter two in weight's type."""
+    kind = _type(x, "x")
+    dim = x.shape[-1]
+    _need(dy.shape == x.shape and dy.dtype == x.dtype, "dy: shape and type of x expected")
+    _need(mean.dtype == rstd.dtype == torch.float32 and mean.shape == rstd.shape == x.shape[:-1] and mean.is_contiguous() and rstd.is_contiguous(),
+          "mean and rstd: float32, a number a row expected")
+    weights = _affine(x, weight, None)
+    x_rows, rows, x_stride = _rows(x, dim, "x")
+    dy_rows, _, dy_stride = _rows(dy, dim, "dy")
+    with _On(x, dy, mean, rstd, weight) as stream:
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need[0] else None
+        sums = torch.empty((2, dim), dtype=weights, device=x.device) if need[1] or need[2] else None
+        dw, db = (sums[0] if need[1] else None, sums[1] if need[2] else None) if sums is not None else (None, None)
+        work = None
+        if sums is not None:
+            size = C.c_long()
+            _lib.check(_lib_functions().smx_layer_norm_backward_workspace(rows, dim, C.byref(size)))
+            work = torch.empty(size.value, dtype=torch.uint8, device=x.device)
+        _lib.check(_lib_functions().smx_layer_norm_backward(
+            kind, _TYPES[weights], rows, dim, dy_rows.data_ptr(), dy_stride, x_rows.data_ptr(), x_stride, mean.data_ptr(), rstd.data_ptr(),
+            0 if weight is None else weight.data_ptr(), 0 if dx is None else dx.data_ptr(), dim, 0 if dw is None else dw.data_ptr(),
+            0 if db is None else db.data_ptr(), 0 if work is None else work.data_ptr(), 0 if work is None else work.numel(), stream))
+    return dx, dw, db
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        y, mean, rstd = layer_norm_forward(x, weight, bias, eps)
+        ctx.save_for_backward(x, weight, mean, rstd)
+        ctx.bias_type = None if bias is None else bias.dtype
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, mean, rstd = ctx.saved_tensors
+        dx, dw, db = layer_norm_backward(dy, x, mean, rstd, weight, ctx.needs_input_grad[:3])
+        return dx, dw, db if db is None else db.to(ctx.bias_type), None
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5):
+    """Layer norm over the last dimension, differentiable once."""
+    return _LayerNorm.apply(x, weight, bias, eps)
+
+
+# ---- a shared projection with a low-rank adapter per row
+
+def _describe(x, weight, A, B, scale, index):
+    kind = _type(x, "x")
+    _need(weight.dim() == 2, "weight: [d_out, d_in] expected")
+    d_out, d_in = weight.shape
+    _need(d_in >= 1 and d_out >= 1, "weight: at least one row and column expected")
+    _need(A.dim() == 3 and B.dim() == 3, "A: [adapters, rank, d_in] and B: [adapters, d_out, rank] expected")
+    n, rank = A.shape[0], A.shape[1]
+    _need(A.shape[2] == d_in and B.shape == (n, d_out, rank), "A: [adapters, rank, d_in] and B: [adapters, d_out, rank] expected")
+    if not (weight.dtype == A.dtype == B.dtype == x.dtype):
+        raise TypeError("x, weight, A and B: one type expected")
+    _need(1 <= rank <= MAX_RANK and n <= MAX_ADAPTERS, f"rank: 1 to {MAX_RANK}, adapters: up to {MAX_ADAPTERS}")
+    rows_of, rows, stride = _rows(x, d_in, "x")
+    weight, _, weight_stride = _rows(weight, d_in, "weight")
+    A, B = A.contiguous(), B.contiguous()
+    if index.dtype != torch.int32:
+        raise TypeError(f"index: int32 expected, not {index.dtype}")
+    _need(index.shape == x.shape[:-1] and index.is_contiguous(), "index: a contiguous number a row expected")
+    if scale is not None:
+        if scale.dtype != torch.float32:
+            raise TypeError(f"scale: float32 expected, not {scale.dtype}")
+        _need(scale.shape == (n,) and scale.is_contiguous(), "scale: a contiguous number an adapter expected")
+    keep = (rows_of, weight, A, B)          # (copies live until the call is made)
+    p = _Adapted(kind, d_in, d_out, rank, n, rows, rows_of.data_ptr(), stride, weight.data_ptr(), weight_stride, A.data_ptr(), B.data_ptr(),
+                 0 if scale is None else scale.data_ptr(), index.data_ptr())
+    return p, keep
+
+
+def _workspace(p, backward, device):
+    size = C.c_long()
+    _lib.check(_lib_functions().smx_adapted_linear_workspace(C.byref(p), backward, C.byref(size)))
+    return torch.empty(size.value, dtype=torch.uint8, device=device)
+
+
+def adapted_linear_forward(x, weight, A, B, scale, index):
+    """y = weight x + scale[a] B[a] (A[a] x) for every row of x, a = index of the row (int32; -1: no adapter).
+
+    x[..., d_in], weight[d_out, d_in], A[adapters, rank, d_in] and B[adapters, d_out, rank] are of one type, scale[adapters] is
+    float32 (None: ones).  Rows may come in any order.  A row whose index is out of range is NaN."""
+    with _On(x, weight, A, B, scale, index) as stream:
+        p, keep = _describe(x, weight, A, B, scale, index)
+        y = torch.empty(x.shape[:-1] + (p.d_out,), dtype=x.dtype, device=x.device)
+        work = _workspace(p, 0, x.device)
+        _lib.check(_lib_functions().smx_adapted_linear_forward(C.byref(p), y.data_ptr(), p.d_out, work.data_ptr(), work.numel(), stream))
+    return y
+
+
+def adapted_linear_backward(dy, x, weight, A, B, scale, index, need=(True, True, True)):
+    """Gradients of x, A and B (None where `need` says so); weight and scale are fixed."""
+    with _On(x, dy, weight, A, B, scale, index) as stream:
+        p, keep = _describe(x, weight, A, B, scale, index)
+        _need(dy.shape == x.shape[:-1] + (p.d_out,), "dy: a row of d_out numbers for every row of x expected")
+        if dy.dtype != x.dtype:
+            raise TypeError("dy: the type of x expected")
+        dy_rows, _, dy_stride = _rows(dy, p.d_out, "dy")
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need[0] else None
+        dA = torch.empty(A.shape, dtype=A.dtype, device=x.device) if need[1] else None
+        dB = torch.empty(B.shape, dtype=B.dtype, device=x.device) if need[2] else None
+        work = _workspace(p, 1, x.device)
+        _lib.check(_lib_functions().smx_adapted_linear_backward(
+            C.byref(p), dy_rows.data_ptr(), dy_stride, 0 if dx is None else dx.data_ptr(), p.d_in, 0 if dA is None else dA.data_ptr(),
+            0 if dB is None else dB.data_ptr(), work.data_ptr(), work.numel(), stream))
+    return dx, dA, dB
+
+
+class _AdaptedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, A, B, scale, index):
+        ctx.save_for_backward(x, weight, A, B, scale, index)
+        return adapted_linear_forward(x, weight, A, B, scale, index)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, A, B, scale, index = ctx.saved_tensors
+        wanted = ctx.needs_input_grad
+        dx, dA, dB = adapted_linear_backward(dy, x, weight, A, B, scale, index, (wanted[0], wanted[2], wanted[3]))
+        return dx, None, dA, dB, None, None
+
+
+def adapted_linear(x, weight, A, B, scale, index):
+    """adapted_linear_forward, differentiable once with respect to x, A and B; weight and scale have to be fixed."""
+    _need(not weight.requires_grad and not (scale is not None and scale.requires_grad), "weight and scale are fixed: they cannot require gradients")
+    return _AdaptedLinear.apply(x, weight, A, B, scale, index)
+
+
+# ---- AdamW
+
+def moment_values(code_avg, scale_avg, code_avg_sq, scale_avg_sq):
+    """The numbers that moments in 8 bits stand for: codes (int8, uint8) of one tensor and a float32 scale for every 256 of them."""
+    n = code_avg.numel()
+    if code_avg.dtype != torch.int8 or code_avg_sq.dtype != torch.uint8 or not scale_avg.dtype == scale_avg_sq.dtype == torch.float32:
+        raise TypeError("codes in int8 and uint8, scales in float32 expected")
+    blocks = -(-n // MOMENT_BLOCK)
+    _need(code_avg_sq.numel() == n and scale_avg.numel() == scale_avg_sq.numel() == blocks, f"{n} codes and {blocks} scales expected")
+    _need(all(t.is_contiguous() for t in (code_avg, scale_avg, code_avg_sq, scale_avg_sq)), "contiguous tensors expected")
+    with _On(code_avg, scale_avg, code_avg_sq, scale_avg_sq) as stream:
+        m = torch.empty(code_avg.shape, dtype=torch.float32, device=code_avg.device)
+        v = torch.empty_like(m)
+        _lib.check(_lib_functions().smx_moment_values(n, code_avg.data_ptr(), scale_avg.data_ptr(), code_avg_sq.data_ptr(), scale_avg_sq.data_ptr(),
+                                                      m.data_ptr(), v.data_ptr(), stream))
+    return m, v
+
+
+class AdamW:
+    """AdamW over many tensors at once, a launch for up to 56 of them.
+
+    state_bits 32: moments in single precision; 8: in codes of 8 bits, 256 to a scale.  masters: parameters in single
+    precision for params in 16 bits, a list like params; True makes them from params.  states: moments to go on with, a tuple a
+    tensor, (exp_avg, exp_avg_sq) or (code_avg, scale_avg, code_avg_sq, scale_avg_sq); they are used in place, as params and
+    masters are, and so is what self.states holds otherwise (zeros at first).  step: steps taken before."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, masters=None, states=None, step=0):
+        self.params = list(params)
+        _need(state_bits in (32, 8), "state_bits: 32 or 8")
+        _need(0 <= betas[0] < 1 and 0 <= betas[1] < 1, "betas: 0 up to, not including, 1")
+        _need(lr >= 0 and eps >= 0 and weight_decay >= 0, "lr, eps and weight_decay: numbers from 0 on")
+        _need(step >= 0, "step: steps taken before, none or more")
+        self.lr, self.betas, self.eps, self.weight_decay, self.state_bits, self.step_count = lr, tuple(betas), eps, weight_decay, state_bits, step
+        for p in self.params:
+            _type(p, "parameters")
+            _need(p.is_contiguous(), "parameters: contiguous tensors expected")
+            _need(p.is_cuda and p.device == self.params[0].device, "parameters on one GPU expected: there is no CPU path")
+            if p.dtype != self.params[0].dtype:
+                raise TypeError("parameters of one type expected: an optimizer for each")
+        if masters is True:
+            masters = [p.detach().float() for p in self.params]
+        if masters is not None:
+            masters = list(masters)
+            _need(len(masters) == len(self.params), "masters: one for every parameter expected")
+            for m, p in zip(masters, self.params):
+                _need(p.dtype != torch.float32, "masters are for parameters in 16 bits")
+                _need(m.dtype == torch.float32 and m.shape == p.shape and m.is_contiguous() and m.device == p.device,
+                      "masters: contiguous, float32, of the parameters' shapes and on their device expected")
+        self.masters = masters
+        if states is None:
+            states = [self._zeros(p) for p in self.params]
+        self.states = [tuple(s) for s in states]
+        _need(len(self.states) == len(self.params), "states: a tuple for every parameter expected")
+        kinds = (torch.float32, torch.float32) if state_bits == 32 else (torch.int8, torch.float32, torch.uint8, torch.float32)
+        for s, p in zip(self.states, self.params):
+            n = p.numel()
+            counts = (n, n) if state_bits == 32 else (n, -(-n // MOMENT_BLOCK)) * 2
+            _need(len(s) == len(kinds) and all(t.dtype == k and t.numel() == c and t.is_contiguous() and t.device == p.device
+                                               for t, k, c in zip(s, kinds, counts)),
+                  "states: (exp_avg, exp_avg_sq) in float32, or (code_avg int8, scale_avg float32, code_avg_sq uint8, scale_avg_sq float32), "
+                  "contiguous and on the parameters' device, expected")
+
+    def _zeros(self, p):
+        n, blocks = p.numel(), -(-p.numel() // MOMENT_BLOCK)
+        make = lambda k, dtype: torch.zeros(k, dtype=dtype, device=p.device)          # noqa: E731
+        if self.state_bits == 32:
+            return make(n, torch.float32), make(n, torch.float32)
+        return make(n, torch.int8), make(blocks, torch.float32), make(n, torch.uint8), make(blocks, torch.float32)
+
+    def step(self, grads=None):
+        """One step with the given gradients, one for every parameter (None: the parameters' own).  A parameter without a gradient
+        (None) is left as it is.  Gradients are of the parameters' type or all in float32."""
+        if grads is None:
+            grads = [p.grad for p in self.params]
+        _need(len(grads) == len(self.params), "a gradient (or None) for every parameter expected")
+        if not self.params:
+            self.step_count += 1
+            return
+        eight, first = self.state_bits == 8, self.params[0]
+        table = (_AdamwTensor * len(grads))()
+        kind, count, keep = None, 0, []
+        for i, (p, g) in enumerate(zip(self.params, grads)):
+            if g is None:
+                continue
+            if kind is None:
+                kind = g.dtype
+                if kind != first.dtype and kind != torch.float32:
+                    raise TypeError(f"gradients: {first.dtype} or float32, not {kind}")
+            if g.dtype != kind:
+                raise TypeError("gradients of one type expected")
+            if g.shape != p.shape or g.device != p.device:
+                raise ValueError("gradients of the parameters' shapes and on their device expected")
+            if not g.is_contiguous():
+                g = g.contiguous()
+                keep.append(g)
+            s, t = self.states[i], table[count]
+            t.param, t.grad, t.numel = p.data_ptr(), g.data_ptr(), p.numel()
+            t.exp_avg = s[0].data_ptr()
+            if eight:
+                t.scale_avg, t.exp_avg_sq, t.scale_avg_sq = s[1].data_ptr(), s[2].data_ptr(), s[3].data_ptr()
+            else:
+                t.exp_avg_sq = s[1].data_ptr()
+            if self.masters is not None:
+                t.master = self.masters[i].data_ptr()
+            count += 1
+        with _On(first) as stream:
+            _lib.check(_lib_functions().smx_adamw_step(
+                _TYPES[first.dtype], _TYPES[kind or first.dtype], self.state_bits, C.addressof(table), count, self.lr, self.betas[0], self.betas[1],
+                self.eps, self.weight_decay, self.step_count + 1, stream))
+        # (as torch's own operations in place do: a backward pass that saved the old values says so)
+        torch.autograd.graph.increment_version([p for p, g in zip(self.params, grads) if g is not None])
+        self.step_count += 1
