@@ -54,6 +54,30 @@ __device__ __forceinline__ void store_run(T* p, long left, const float (&v)[V])
     }
 }
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// 1 KB of a wavefront from global memory (16 bytes per lane, from an address that is a multiple of 16) into LDS at `to` + 16 lane.
+// In assembly: next to the compiler's own form of this load it lets every read of the LDS wait for all loads in flight; here
+// wait_loads waits by count.  The LDS address goes through m0, which the load may read one wait state after the write (s_nop) and has
+// read when it is issued; m0 belongs to the compiler and is given back as it was.
+__device__ __forceinline__ void load_into_lds(const void* from, unsigned to)
+{
+    unsigned m0;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
+                 : "=&s"(m0) : "v"(from), "s"(to) : "memory");
+}
+// all but the N youngest loads have arrived, and every read and write of the LDS is done
+template <int N>
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"(N) : "memory"); }
+// a barrier that waits for nothing but the wavefronts (__syncthreads would wait for loads in flight too)
+__device__ __forceinline__ void barrier_only()
+{
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+__device__ __forceinline__ unsigned lds_address(const void* p) { return (unsigned)(unsigned long)(__attribute__((address_space(3))) const void*)p; }
+
 // sum over groups of G neighbouring lanes, the same in all of them
 template <int G>
 __device__ __forceinline__ float group_sum(float x)
