@@ -56,15 +56,15 @@ __device__ __forceinline__ void store_run(T* p, long left, const float (&v)[V])
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-// 1 KB of a wavefront from global memory (16 bytes per lane, from an address that is a multiple of 16) into LDS at `to` + 16 lane.
+// 1 KB of a wavefront from global memory (16 bytes per lane, at base + offset, a multiple of 16) into LDS at `to` + 16 lane.
 // In assembly: next to the compiler's own form of this load it lets every read of the LDS wait for all loads in flight; here
 // wait_loads waits by count.  The LDS address goes through m0, which the load may read one wait state after the write (s_nop) and has
 // read when it is issued; m0 belongs to the compiler and is given back as it was.
-__device__ __forceinline__ void load_into_lds(const void* from, unsigned to)
+__device__ __forceinline__ void load_into_lds(const void* base, unsigned offset, unsigned to)
 {
     unsigned m0;
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
-                 : "=&s"(m0) : "v"(from), "s"(to) : "memory");
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
+                 : "=&s"(m0) : "v"(offset), "s"(base), "s"(to) : "memory");
 }
 // all but the N youngest loads have arrived, and every read and write of the LDS is done
 template <int N>

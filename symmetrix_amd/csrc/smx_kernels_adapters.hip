@@ -77,45 +77,163 @@ struct Layout {
     const void* src;
     long src_each, src_row, src_k;      // strides of a matrix, a row and a number
     void* dst;
-    long dst_each, part;                // strides of a matrix and a part
-    int rows, k, k_padded;
+    long dst_each, part;                // strides of a matrix and a part; part 0: one part, as it is
+    int rows, k, k_padded, matrices;
 };
+inline __host__ __device__ long layout_blocks(const Layout& p) { return (long)((p.k_padded + 63) / 64) * ((p.rows + 63) / 64) * p.matrices; }
 // a block takes 64 rows and 64 numbers of them
-template <typename T, bool SPLIT>
-__global__ __launch_bounds__(256) void k_lay_out(const Layout p)
+template <typename T>
+__device__ __forceinline__ void lay_out(const Layout& p, long block, T (*tile)[65])
 {
-    __shared__ T tile[64][65];
-    const int row0 = blockIdx.y * 64, k0 = blockIdx.x * 64;
-    const T* src = static_cast<const T*>(p.src) + blockIdx.z * p.src_each;
-    const bool along = p.src_k == 1;
-    for (int i = threadIdx.x; i < 64 * 64; i += 256) {
-        const int r = along ? i / 64 : i % 64, k = along ? i % 64 : i / 64;
-        tile[r][k] = row0 + r < p.rows && k0 + k < p.k ? src[(row0 + r) * p.src_row + (k0 + k) * p.src_k] : (T)0.0f;
+    const int across = (p.k_padded + 63) / 64, down = (p.rows + 63) / 64;
+    const int k0 = (int)(block % across) * 64, row0 = (int)(block / across % down) * 64, matrix = (int)(block / across / down);
+    const T* src = static_cast<const T*>(p.src) + matrix * p.src_each;
+    T x[16];
+    // (neighbouring threads where neighbouring numbers are)
+    if (p.src_k == 1) {
+        const int k = threadIdx.x & 63;
+#pragma unroll
+        for (int u = 0; u < 16; ++u) {
+            const int r = (threadIdx.x >> 6) + 4 * u;
+            x[u] = row0 + r < p.rows && k0 + k < p.k ? src[(row0 + r) * p.src_row + k0 + k] : (T)0.0f;
+        }
+#pragma unroll
+        for (int u = 0; u < 16; ++u) tile[(threadIdx.x >> 6) + 4 * u][k] = x[u];
+    } else {
+        const int r = threadIdx.x & 63;
+#pragma unroll
+        for (int u = 0; u < 16; ++u) {
+            const int k = (threadIdx.x >> 6) + 4 * u;
+            x[u] = row0 + r < p.rows && k0 + k < p.k ? src[(row0 + r) * p.src_row + (k0 + k) * p.src_k] : (T)0.0f;
+        }
+#pragma unroll
+        for (int u = 0; u < 16; ++u) tile[r][(threadIdx.x >> 6) + 4 * u] = x[u];
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < 64 * 32; i += 256) {
-        const int r = i / 32, k = i % 32 * 2;
-        if (row0 + r >= p.rows || k0 + k >= p.k_padded) continue;
-        const long at = blockIdx.z * p.dst_each + (long)(row0 + r) * p.k_padded + k0 + k;
-        if constexpr (SPLIT) {
-            const float x[2] = {(float)tile[r][k] * kSplitScale, (float)tile[r][k + 1] * kSplitScale};
-            bf16 part[3][2];
-            split(x, part);
 #pragma unroll
-            for (int s = 0; s < 3; ++s) {
-                const bf16x2 v = {part[s][0], part[s][1]};
-                *reinterpret_cast<bf16x2*>(static_cast<bf16*>(p.dst) + s * p.part + at) = v;
-            }
+    for (int u = 0; u < 8; ++u) {
+        const int r = (threadIdx.x >> 5) + 8 * u, k = (threadIdx.x & 31) * 2;
+        if (row0 + r >= p.rows || k0 + k >= p.k_padded) continue;
+        const long at = matrix * p.dst_each + (long)(row0 + r) * p.k_padded + k0 + k;
+        if (std::is_same_v<T, float> && p.part) {
+            const float v[2] = {(float)tile[r][k] * kSplitScale, (float)tile[r][k + 1] * kSplitScale};
+            bf16 part[3][2];
+            split(v, part);
+#pragma unroll
+            for (int q = 0; q < 3; ++q) *reinterpret_cast<bf16x2*>(static_cast<bf16*>(p.dst) + q * p.part + at) = bf16x2{part[q][0], part[q][1]};
         } else {
-            T* dst = static_cast<T*>(p.dst) + at;
-            dst[0] = tile[r][k]; dst[1] = tile[r][k + 1];
+            typedef T pair __attribute__((ext_vector_type(2)));
+            *reinterpret_cast<pair*>(static_cast<T*>(p.dst) + at) = pair{tile[r][k], tile[r][k + 1]};
         }
     }
 }
-template <typename T, bool SPLIT>
-void lay_out(const Layout& p, int matrices, hipStream_t s)
+
+// ---- rows sorted by adapter, in their order: places [start[a], start[a + 1]) of perm hold adapter a's; rows with no adapter, and with an
+// index out of range, come last.  Pieces of at most `piece` rows of one adapter: [first[a], first[a + 1]).
+
+struct Groups {
+    const int* index;
+    int adapters, blocks, rows_per_block, piece;
+    long rows;
+    int* count;              // [block][key]: rows of a block
+    int *start, *first;      // [adapters + 1]
+    int* perm;
+};
+__device__ __forceinline__ int key_of(int a, int n) { return has_adapter(a, n) ? a : (a == -1 ? n : n + 1); }
+constexpr int kMostKeys = SMX_ADAPTER_MAX_COUNT + 2;
+
+__device__ __forceinline__ void count_rows(const Groups& p, int block, int* hist)
 {
-    hipLaunchKernelGGL((k_lay_out<T, SPLIT>), dim3((p.k_padded + 63) / 64, (p.rows + 63) / 64, matrices), dim3(256), 0, s, p);
+    const int keys = p.adapters + 2;
+    for (int k = threadIdx.x; k < keys; k += 256) hist[k] = 0;
+    __syncthreads();
+    const long begin = (long)block * p.rows_per_block, end = min(begin + p.rows_per_block, p.rows);
+    for (long i = begin + threadIdx.x; i < end; i += 256) atomicAdd(&hist[key_of(p.index[i], p.adapters)], 1);
+    __syncthreads();
+    for (int k = threadIdx.x; k < keys; k += 256) p.count[(long)block * keys + k] = hist[k];
+}
+__device__ __forceinline__ int wave_exclusive(int x, int lane, int& total)
+{
+    int sum = x;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const int y = __shfl_up(sum, d, 64);
+        if (lane >= d) sum += y;
+    }
+    total = __shfl(sum, 63, 64);
+    return sum - x;
+}
+// One wavefront places the rows of a block.
+__device__ __forceinline__ void place_rows(const Groups& p, int block, int lane, int* base)
+{
+    const int keys = p.adapters + 2;
+    int rows = 0, pieces = 0;
+    for (int k0 = 0; k0 < keys; k0 += 64) {
+        const int k = min(k0 + lane, keys - 1);
+        int all = 0, before = 0;
+#pragma unroll 8
+        for (int b = 0; b < p.blocks; ++b) {
+            const int x = p.count[(long)b * keys + k];
+            all += x;
+            before += b < block ? x : 0;
+        }
+        if (k0 + lane >= keys) all = 0;
+        int row_total, piece_total;
+        const int row_before = rows + wave_exclusive(all, lane, row_total);
+        const int piece_before = pieces + wave_exclusive(k0 + lane < p.adapters ? (all + p.piece - 1) / p.piece : 0, lane, piece_total);
+        if (k0 + lane < keys) base[k0 + lane] = row_before + before;
+        if (block == 0 && k0 + lane <= p.adapters) {
+            p.start[k0 + lane] = row_before;
+            p.first[k0 + lane] = piece_before;
+        }
+        rows += row_total;
+        pieces += piece_total;
+    }
+    const long begin = (long)block * p.rows_per_block, end = min(begin + p.rows_per_block, p.rows);
+    for (long i = begin; i < end; i += 64) {
+        const bool live = i + lane < end;
+        const int key = live ? key_of(p.index[i + lane], p.adapters) : keys;
+        unsigned long same = __ballot(live);
+        for (int bit = 0; (1 << bit) <= keys; ++bit) {
+            const unsigned long set = __ballot(key >> bit & 1);
+            same &= key >> bit & 1 ? set : ~set;
+        }
+        const int before = __popcll(same & ((1ul << lane) - 1));
+        // (the wavefront's own LDS operations, which are done in order; the fences keep the compiler to it)
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        const int at = live ? base[key] + before : 0;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (live) {
+            p.perm[at] = (int)(i + lane);
+            if (before == 0) base[key] = at + __popcll(same);
+        }
+    }
+}
+
+// What the other kernels need beforehand: two layouts, and the rows of every adapter counted.
+struct Prepare {
+    Layout layout[2];
+    long blocks[2];
+    Groups groups;
+};
+template <typename T>
+__global__ __launch_bounds__(256) void k_prepare(const Prepare p)
+{
+    __shared__ union {
+        T tile[64][65];
+        int hist[kMostKeys];
+    } lds;
+    long block = blockIdx.x;
+    if (block < p.blocks[0]) {
+        lay_out<T>(p.layout[0], block, lds.tile);
+        return;
+    }
+    block -= p.blocks[0];
+    if (block < p.blocks[1]) {
+        lay_out<T>(p.layout[1], block, lds.tile);
+        return;
+    }
+    count_rows(p.groups, (int)(block - p.blocks[1]), lds.hist);
 }
 
 // ---- h[row][r] = c_a sum over k of in[row][k] F_a(r, k); zero for r from the rank on and for rows without an adapter
@@ -131,53 +249,121 @@ struct Down {
     long rows;
     float* h;
 };
+// one or two of them, and beside them the rows placed by adapter
+struct Downs {
+    Down down[2];
+    int blocks[2];
+    Groups groups;
+};
 
-// A block takes 16 rows; its wavefronts have 128 bytes of a row by turns, and their sums are added in order.
-template <typename T, int RT>
-__global__ __launch_bounds__(256) void k_down(const Down p)
+// A block takes 16 MT rows; its wavefronts have 128 bytes of a row by turns, and their sums are added in order.
+template <typename T, int RT, int MT>
+__global__ __launch_bounds__(256) void k_down(const Downs both)
 {
     constexpr int V = kRun<T>, UNIT = 8 * V;
-    __shared__ f32x4 part[4][RT][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
-    const long row = min((long)blockIdx.x * 16 + n, p.rows - 1);
-    const bool live = (long)blockIdx.x * 16 + n < p.rows;
-    const int a = p.index[row];
-    const bool good = live && has_adapter(a, p.adapters);
-    const T* in = static_cast<const T*>(p.in) + row * p.in_stride;
-    if (live && !good && wave == 0)
+    typedef typename Operand<T>::type frag;
+    __shared__ union {
+        f32x4 part[4][MT * RT][64];
+        int base[kMostKeys];
+    } lds;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
+    int block = blockIdx.x;
+    if (block >= both.blocks[0] + both.blocks[1]) {
+        if (wave == 0) place_rows(both.groups, block - both.blocks[0] - both.blocks[1], lane, lds.base);
+        return;
+    }
+    const bool second = block >= both.blocks[0];
+    if (second) block -= both.blocks[0];
+    const Down& p = both.down[second];
+    long row[MT];
+    int a[MT];
+    bool good[MT];
+    unsigned left[MT];
+    const T* in[MT];
 #pragma unroll
-        for (int q = 0; q < RT; ++q)
-            if (16 * q < p.padded) *reinterpret_cast<f32x4*>(p.h + row * p.padded + 16 * q + 4 * g) = f32x4{0, 0, 0, 0};
-    unsigned left = (unsigned)__ballot(good) & 0xffffu;
-    while (left) {
-        const int cur = __builtin_amdgcn_readlane(a, __builtin_ctz(left));
-        const bool mine = good && a == cur;
-        left &= ~(unsigned)__ballot(mine);
-        f32x4 acc[RT];
+    for (int i = 0; i < MT; ++i) {
+        const long at = ((long)block * MT + i) * 16 + n;
+        row[i] = min(at, p.rows - 1);
+        a[i] = p.index[row[i]];
+        good[i] = at < p.rows && has_adapter(a[i], p.adapters);
+        left[i] = (unsigned)__ballot(good[i]) & 0xffffu;
+        in[i] = static_cast<const T*>(p.in) + row[i] * p.in_stride + g * V;
+        if (at < p.rows && !good[i] && wave == 0)
 #pragma unroll
-        for (int q = 0; q < RT; ++q) acc[q] = f32x4{0, 0, 0, 0};
-        const T* F = static_cast<const T*>(p.F) + cur * p.f_each;
-        for (int k0 = wave * UNIT; k0 < p.k; k0 += 4 * UNIT)
+            for (int q = 0; q < RT; ++q)
+                if (16 * q < p.padded) *reinterpret_cast<f32x4*>(p.h + row[i] * p.padded + 16 * q + 4 * g) = f32x4{0, 0, 0, 0};
+    }
+    for (;;) {
+        int cur = -1;
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int k = k0 + u * (UNIT / 2) + g * V;
-                const auto x = load_operand(in + k, p.k - k);
+        for (int i = 0; i < MT; ++i)
+            if (cur < 0 && left[i]) cur = __builtin_amdgcn_readlane(a[i], __builtin_ctz(left[i]));
+        if (cur < 0) break;
+        bool mine[MT];
 #pragma unroll
-                for (int q = 0; q < RT; ++q) {
-                    const int r = 16 * q + n;
-                    const auto f = load_operand(F + (long)min(r, p.rank - 1) * p.f_row + k, r < p.rank ? p.k - k : 0);
-                    acc[q] = mma(f, x, acc[q]);
-                }
+        for (int i = 0; i < MT; ++i) {
+            mine[i] = good[i] && a[i] == cur;
+            left[i] &= ~(unsigned)__ballot(mine[i]);
+        }
+        f32x4 acc[MT][RT];
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int q = 0; q < RT; ++q) acc[i][q] = f32x4{0, 0, 0, 0};
+        const T* F[RT];
+#pragma unroll
+        for (int q = 0; q < RT; ++q) F[q] = static_cast<const T*>(p.F) + cur * p.f_each + (long)min(16 * q + n, p.rank - 1) * p.f_row + g * V;
+        const int full = p.k / UNIT;
+        int u = wave;
+#pragma unroll 2
+        for (; u < full; u += 4) {
+            const long k = (long)u * UNIT;
+            frag x[MT][2], f[RT][2];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+#pragma unroll
+                for (int i = 0; i < MT; ++i) x[i][half] = *reinterpret_cast<const typename Run<T, V>::loose*>(in[i] + k + half * (UNIT / 2));
+#pragma unroll
+                for (int q = 0; q < RT; ++q) f[q][half] = *reinterpret_cast<const typename Run<T, V>::loose*>(F[q] + k + half * (UNIT / 2));
             }
 #pragma unroll
-        for (int q = 0; q < RT; ++q) part[wave][q][lane] = acc[q];
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int q = 0; q < RT; ++q) acc[i][q] = mma(f[q][half], x[i][half], acc[i][q]);
+        }
+        if (u == full && p.k % UNIT) {      // (the end of the rows, for one wavefront)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int k = full * UNIT + half * (UNIT / 2), rest = p.k - k - g * V;
+                frag x[MT];
+#pragma unroll
+                for (int i = 0; i < MT; ++i) x[i] = load_operand(in[i] + k, rest);
+#pragma unroll
+                for (int q = 0; q < RT; ++q) {
+                    const frag f = load_operand(F[q] + k, rest);
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) acc[i][q] = mma(f, x[i], acc[i][q]);
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int q = 0; q < RT; ++q) lds.part[wave][i * RT + q][lane] = acc[i][q];
         __syncthreads();
         const float c = p.scale ? p.scale[cur] : 1.0f;
-        for (int q = wave; q < RT; q += 4) {
-            f32x4 sum = part[0][q][lane];
 #pragma unroll
-            for (int w = 1; w < 4; ++w) sum += part[w][q][lane];
-            if (mine && 16 * q < p.padded) *reinterpret_cast<f32x4*>(p.h + row * p.padded + 16 * q + 4 * g) = sum * c;
+        for (int at = 0; at < MT * RT; ++at) {
+            if (at % 4 != wave) continue;
+            const int i = at / RT, q = at % RT;
+            f32x4 sum = lds.part[0][at][lane];
+#pragma unroll
+            for (int w = 1; w < 4; ++w) sum += lds.part[w][at][lane];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sum[j] = 16 * q + 4 * g + j < p.rank ? sum[j] * c : 0.0f;
+            if (mine[i] && 16 * q < p.padded) *reinterpret_cast<f32x4*>(p.h + row[i] * p.padded + 16 * q + 4 * g) = sum;
         }
         __syncthreads();
     }
@@ -192,13 +378,19 @@ __global__ __launch_bounds__(256) void k_down_few(const Down p)
     const int lane = threadIdx.x & 63, r = blockIdx.y * 4 + (threadIdx.x >> 6), a = p.index[row];
     float sum = 0.0f;
     if (has_adapter(a, p.adapters) && r < p.rank) {
-        const T* in = static_cast<const T*>(p.in) + row * p.in_stride;
-        const T* F = static_cast<const T*>(p.F) + a * p.f_each + (long)r * p.f_row;
+        const T* in = static_cast<const T*>(p.in) + row * p.in_stride + lane * V;
+        const T* F = static_cast<const T*>(p.F) + a * p.f_each + (long)r * p.f_row + lane * V;
+        const int full = p.k / (64 * V) * (64 * V);
 #pragma unroll 4
-        for (int k = lane * V; k < p.k; k += 64 * V) {
+        for (int k = 0; k < full; k += 64 * V) {
+            const typename Operand<T>::type x = *reinterpret_cast<const typename Run<T, V>::loose*>(in + k), f = *reinterpret_cast<const typename Run<T, V>::loose*>(F + k);
+#pragma unroll
+            for (int j = 0; j < V; ++j) sum = fmaf((float)x[j], (float)f[j], sum);
+        }
+        if (full < p.k) {
             float x[V], f[V];
-            load_run<V>(in + k, p.k - k, x);
-            load_run<V>(F + k, p.k - k, f);
+            load_run<V>(in + full, p.k - full - lane * V, x);
+            load_run<V>(F + full, p.k - full - lane * V, f);
 #pragma unroll
             for (int j = 0; j < V; ++j) sum = fmaf(x[j], f[j], sum);
         }
@@ -218,6 +410,7 @@ struct Product {
     long w0_col, w0_k;
     const void* F;
     long f_each, f_col, f_r;
+    bool f_runs;
     const float* h;
     const int* index;
     int adapters, rank, padded, k, k_padded, cols;
@@ -238,19 +431,129 @@ __device__ __forceinline__ bool tile_of(const Product& p, int& rt, int& ct)
     return true;
 }
 
+// The product of a factor's columns and rows of h, 32 r at a time (single precision: 16).  Sixteen bits: on the bf16 instructions, h in two
+// bf16 parts (what is left out is below 2^-16 of a product; the result is rounded to 2^-9 or 2^-11), and numbers of float16 in two, which
+// hold them exactly.
+template <typename T>
+struct AdapterProduct {
+    static constexpr int CHUNK = 32, F_PARTS = std::is_same_v<T, f16> ? 2 : 1;
+    struct Factor {
+        bf16x8 part[F_PARTS];
+    };
+    __device__ static __forceinline__ void parts_of(const float (&x)[8], bf16x8 (&part)[2])
+    {
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+            const f32x2 v = {x[j], x[j + 1]};
+            const bf16x2 h = __builtin_convertvector(v, bf16x2);
+            f32x2 rest = v - __builtin_convertvector(h, f32x2);
+            if (rest[0] != rest[0]) rest[0] = 0.0f;      // (infinities are their first part)
+            if (rest[1] != rest[1]) rest[1] = 0.0f;
+            const bf16x2 l = __builtin_convertvector(rest, bf16x2);
+            part[0][j] = h[0]; part[0][j + 1] = h[1];
+            part[1][j] = l[0]; part[1][j + 1] = l[1];
+        }
+    }
+    // F(r) at from + r * stride, r = r0 + 8 g + 0..7; runs: eight numbers of a rank that is a multiple of eight, side by side.  (No branch
+    // depends on the lane, here and below: what is behind the rank is read from its end and put to zero.)
+    __device__ static __forceinline__ Factor factor(const T* from, long stride, bool runs, int r0, int g, int rank)
+    {
+        const int r = r0 + 8 * g;
+        typename Operand<T>::type v;
+        if (runs) {
+            v = *reinterpret_cast<const typename Run<T, 8>::loose*>(from + min(r, rank - 8));
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = r < rank ? v[j] : (T)0.0f;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const T x = from[min(r + j, rank - 1) * stride];
+                v[j] = r + j < rank ? x : (T)0.0f;
+            }
+        }
+        Factor f;
+        if constexpr (F_PARTS == 1) f.part[0] = v;
+        else {
+            float x[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = (float)v[j];
+            parts_of(x, f.part);
+        }
+        return f;
+    }
+    struct Row {
+        bf16x8 part[2];
+    };
+    __device__ static __forceinline__ Row row(const float* h, int r0, int g, int padded, int)
+    {
+        const int r = r0 + 8 * g;
+        const f32x4* from = reinterpret_cast<const f32x4*>(h + min(r, padded - 8));
+        const f32x4 u = from[0], v = from[1];
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = r < padded ? (j < 4 ? u[j % 4] : v[j % 4]) : 0.0f;
+        Row both;
+        parts_of(x, both.part);
+        return both;
+    }
+    __device__ static __forceinline__ f32x4 run(const Factor& f, const Row& h, f32x4 c, int, int)
+    {
+        c = mma(f.part[0], h.part[1], c);
+        if constexpr (F_PARTS == 2) c = mma(f.part[1], h.part[0], c);
+        return mma(f.part[0], h.part[0], c);
+    }
+};
+template <>
+struct AdapterProduct<float> {
+    static constexpr int CHUNK = 16;
+    // lane g has r0 + 4 j + g: instructions of r beyond the rank are left out
+    struct Factor {
+        float x[4];
+    };
+    typedef Factor Row;
+    __device__ static __forceinline__ Factor factor(const float* from, long stride, bool, int r0, int g, int rank)
+    {
+        Factor f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (r0 + 4 * j >= rank) break;
+            const float x = from[min(r0 + 4 * j + g, rank - 1) * stride];
+            f.x[j] = r0 + 4 * j + g < rank ? x : 0.0f;
+        }
+        return f;
+    }
+    __device__ static __forceinline__ Row row(const float* h, int r0, int g, int, int rank)
+    {
+        Row v;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v.x[j] = h[r0 + 4 * j + g];
+        return v;
+    }
+    __device__ static __forceinline__ f32x4 run(const Factor& f, const Row& h, f32x4 c, int r0, int rank)
+    {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (r0 + 4 * j < rank) c = __builtin_amdgcn_mfma_f32_16x16x4f32(f.x[j], h.x[j], c, 0, 0, 0);
+        return c;
+    }
+};
+
 // Adds the adapters' part to sums of NM tiles of 16 rows and NT of 16 columns.  Lane (n, g) holds of tile (i, t) row i * 16 + n and
-// columns 4 NT g + 4 t + 0..3.
+// columns 4 NT g + 4 t + 0..3.  For every tile of rows one adapter after the other of those that occur in it; the first r of a factor,
+// which mostly are all of them, stay for the next tile of rows.
 template <typename T, int NM, int NT>
 __device__ __forceinline__ void add_adapters(const Product& p, int lane, long row0, int col0, f32x4 (&acc)[NM][NT])
 {
+    typedef AdapterProduct<T> Op;
     const int n = lane & 15, g = lane >> 4;
-    const T* F[NT];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) F[t] = static_cast<const T*>(p.F) + min(col0 + 4 * NT * (n >> 2) + 4 * t + (n & 3), p.cols - 1) * p.f_col;
+    __builtin_amdgcn_sched_barrier(0);
+    const float* h = p.h + min(row0 + n, p.rows - 1) * p.padded;
+    int a = p.index[min(row0 + n, p.rows - 1)];
+    typename Op::Row first = Op::row(h, 0, g, p.padded, p.rank);
+    int held = -1;
+    typename Op::Factor f[NT];
 #pragma unroll
     for (int i = 0; i < NM; ++i) {
-        const long row = min(row0 + 16 * i + n, p.rows - 1);
-        const int a = p.index[row];
         const bool good = row0 + 16 * i + n < p.rows && has_adapter(a, p.adapters);
         unsigned left = (unsigned)__ballot(good) & 0xffffu;
         while (left) {
@@ -260,25 +563,28 @@ __device__ __forceinline__ void add_adapters(const Product& p, int lane, long ro
             f32x4 sum[NT];
 #pragma unroll
             for (int t = 0; t < NT; ++t) sum[t] = f32x4{0, 0, 0, 0};
-            for (int r = 4 * g; r < p.padded; r += 16) {
-                const f32x4 h = *reinterpret_cast<const f32x4*>(p.h + row * p.padded + r);
+            for (int r0 = 0; r0 < p.rank; r0 += Op::CHUNK) {
+                const typename Op::Row hr = r0 == 0 ? first : Op::row(h, r0, g, p.padded, p.rank);
+                if (cur != held || r0 > 0) {
 #pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    const T* from = F[t] + cur * p.f_each + r * p.f_r;
-                    float f[4];
-                    if (p.f_r == 1) load_run<4>(from, p.rank - r, f);
-                    else {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) f[j] = r + j < p.rank ? (float)from[j * p.f_r] : 0.0f;
-                    }
-                    sum[t] = mma(f32x4{f[0], f[1], f[2], f[3]}, h, sum[t]);
+                    for (int t = 0; t < NT; ++t)
+                        f[t] = Op::factor(static_cast<const T*>(p.F) + cur * p.f_each + min(col0 + 4 * NT * (n >> 2) + 4 * t + (n & 3), p.cols - 1) * p.f_col, p.f_r, p.f_runs, r0, g, p.rank);
+                    held = r0 == 0 ? cur : -1;
                 }
+#pragma unroll
+                for (int t = 0; t < NT; ++t) sum[t] = Op::run(f[t], hr, sum[t], r0, p.rank);
             }
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) acc[i][t][j] += mine ? sum[t][j] : 0.0f;
         }
+        if (i + 1 < NM) {
+            h = p.h + min(row0 + 16 * (i + 1) + n, p.rows - 1) * p.padded;
+            a = p.index[min(row0 + 16 * (i + 1) + n, p.rows - 1)];
+            first = Op::row(h, 0, g, p.padded, p.rank);
+        }
+        __builtin_amdgcn_sched_barrier(0);
     }
 }
 template <typename T, int NM, int NT>
@@ -302,13 +608,14 @@ __device__ __forceinline__ void store_tiles(const Product& p, int lane, long row
     }
 }
 
-// 16-bit types.  Tiles of 32 terms come straight from memory into LDS, three steps ahead, four places; WM x WN wavefronts share the
-// tile.  16 bytes of a row lie at a place that depends on the row, so that lanes that read together meet different banks.
-template <typename T, int BM, int BN, int WM, int WN>
+// 16-bit types.  Tiles of 64 terms come straight from memory into LDS, STAGES of them under way; WM x WN wavefronts share the tile.
+// A load brings eight rows of 128 bytes; the 16-byte pieces of a row lie in an order that depends on the row, so that lanes that read
+// together meet different banks.  A step of 32 terms has its operands fetched during the step before.
+template <typename T, int BM, int BN, int WM, int WN, int STAGES>
 __global__ __launch_bounds__(64 * WM * WN, 2) void k_product16(const Product p)
 {
-    constexpr int WAVES = WM * WN, NM = BM / WM / 16, NT = BN / WN / 16, PER = (BM + BN) / 16 / WAVES, STAGES = 4, AHEAD = 3, STAGE = (BM + BN) * 64;
-    static_assert((BM + BN) / 16 % WAVES == 0, "loads of a wavefront");
+    constexpr int WAVES = WM * WN, NM = BM / WM / 16, NT = BN / WN / 16, PER = (BM + BN) / 8 / WAVES, STAGE = (BM + BN) * 128;
+    static_assert((BM + BN) / 8 % WAVES == 0, "loads of a wavefront");
     typedef typename Operand<T>::type frag;
     extern __shared__ __align__(16) unsigned char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
@@ -316,23 +623,42 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_product16(const Product p)
     if (!tile_of(p, rt, ct)) return;
     const long row0 = (long)rt * BM;
     const int col0 = ct * BN;
-    const char* from[PER];
+    const char* x_base = static_cast<const char*>(p.in) + 2 * row0 * p.in_stride;
+    const char* w_base = static_cast<const char*>(p.W) + 2 * (long)col0 * p.w_stride;
+    unsigned from[PER];
+    unsigned second = 0;      // loads whose piece is in the second half of its row's 128 bytes
 #pragma unroll
     for (int u = 0; u < PER; ++u) {
         const int chunk = wave + u * WAVES;
-        if (chunk < BM / 16) {
-            const int r = chunk * 16 + lane / 4;
-            from[u] = static_cast<const char*>(p.in) + 2 * min(row0 + r, p.rows - 1) * p.in_stride + 16 * ((lane & 3) ^ (r >> 1 & 3));
+        int piece;
+        if (chunk < BM / 8) {
+            const int r = chunk * 8 + lane / 8;
+            piece = (lane & 7) ^ (r & 7);
+            from[u] = (unsigned)(2 * min((long)r, p.rows - 1 - row0) * p.in_stride) + 16 * piece;
         } else {
-            const int r = (chunk - BM / 16) * 16 + lane / 4;
-            from[u] = static_cast<const char*>(p.W) + 2 * (long)min(col0 + r, p.cols - 1) * p.w_stride + 16 * ((lane & 3) ^ ((r >> 1 & 1) | (r / (4 * NT) & 1) << 1));
+            const int r = (chunk - BM / 8) * 8 + lane / 8;
+            piece = (lane & 7) ^ ((r & 3) | (r / (4 * NT) & 1) << 2);
+            from[u] = (unsigned)(2 * min(r, p.cols - 1 - col0) * p.w_stride) + 16 * piece;
         }
+        second |= (unsigned)(piece >> 2) << u;
     }
     const unsigned lds0 = lds_address(lds);
-    const int steps = p.k_padded / kPiece;
+    const int steps = p.k_padded / kPiece, stages = (steps + 1) / 2;
     auto request = [&](int s) {
+        const unsigned to = lds0 + s % STAGES * STAGE + wave * 1024;
 #pragma unroll
-        for (int u = 0; u < PER; ++u) load_into_lds(from[u] + (long)s * 64, lds0 + s % STAGES * STAGE + (wave + u * WAVES) * 1024);
+        for (int u = 0; u < PER; ++u)
+            load_into_lds((wave + u * WAVES < BM / 8 ? x_base : w_base) + (long)s * 128, from[u], to + u * WAVES * 1024);
+    };
+    auto request_half = [&](int s) {      // of rows that end in the middle: the first half twice
+        const unsigned to = lds0 + s % STAGES * STAGE + wave * 1024;
+#pragma unroll
+        for (int u = 0; u < PER; ++u)
+            load_into_lds((wave + u * WAVES < BM / 8 ? x_base : w_base) + (long)s * 128, from[u] - (second >> u & 1) * 64, to + u * WAVES * 1024);
+    };
+    auto request_last = [&](int s) {
+        if (2 * s + 1 == steps) request_half(s);
+        else request(s);
     };
     f32x4 acc[NM][NT];
 #pragma unroll
@@ -340,26 +666,70 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_product16(const Product p)
 #pragma unroll
         for (int t = 0; t < NT; ++t) acc[i][t] = f32x4{0, 0, 0, 0};
     const int wm = wave / WN, wn = wave % WN;
-    const unsigned char* xs = lds + (wm * NM * 16 + n) * 64 + 16 * (g ^ (n >> 1 & 3));
-    const unsigned char* ws = lds + (BM + wn * NT * 16 + 4 * NT * (n >> 2) + (n & 3)) * 64 + 16 * (g ^ ((n >> 1 & 1) | (n >> 2 & 1) << 1));
+    const unsigned char* xs[2];
+    const unsigned char* ws[2];
 #pragma unroll
-    for (int s = 0; s < AHEAD; ++s)
-        if (s < steps) request(s);
-    for (int s = 0; s < steps; ++s) {
-        if (s + AHEAD <= steps) wait_loads<(AHEAD - 1) * PER>();
-        else wait_loads<0>();
-        barrier_only();      // this step's tiles are there, and everybody has read those of the step before
-        if (s + AHEAD < steps) request(s + AHEAD);
-        const int at = s % STAGES * STAGE;
+    for (int h = 0; h < 2; ++h) {
+        xs[h] = lds + (wm * NM * 16 + n) * 128 + 16 * ((4 * h + g) ^ (n & 7));
+        ws[h] = lds + (BM + wn * NT * 16 + 4 * NT * (n >> 2) + (n & 3)) * 128 + 16 * ((4 * h + g) ^ ((n & 3) | (n >> 2 & 1) << 2));
+    }
+    struct Frags {
         frag x[NM], w[NT];
+    };
+    auto fetch = [&](int s, int h, Frags& f) {
+        const int at = s % STAGES * STAGE;
 #pragma unroll
-        for (int t = 0; t < NT; ++t) w[t] = *reinterpret_cast<const frag*>(ws + at + t * 256);
+        for (int t = 0; t < NT; ++t) f.w[t] = *reinterpret_cast<const frag*>(ws[h] + at + t * 512);
 #pragma unroll
-        for (int i = 0; i < NM; ++i) x[i] = *reinterpret_cast<const frag*>(xs + at + i * 1024);
+        for (int i = 0; i < NM; ++i) f.x[i] = *reinterpret_cast<const frag*>(xs[h] + at + i * 2048);
+    };
+    auto sums = [&](const Frags& now) {
 #pragma unroll
         for (int i = 0; i < NM; ++i)
 #pragma unroll
-            for (int t = 0; t < NT; ++t) acc[i][t] = mma(w[t], x[i], acc[i][t]);
+            for (int t = 0; t < NT; ++t) acc[i][t] = mma(now.w[t], now.x[i], acc[i][t]);
+    };
+    auto woven = [&] {      // sums and the fetches beside them, by turns
+#pragma unroll
+        for (int i = 0; i < NM + NT; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, NM * NT / (NM + NT), 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, NM * NT - NM * NT / (NM + NT) * (NM + NT), 0);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+#pragma unroll
+    for (int s = 0; s < STAGES; ++s)
+        if (s < stages) request_last(s);
+    if (STAGES <= stages) wait_loads<(STAGES - 1) * PER>();
+    else wait_loads<0>();
+    barrier_only();
+    Frags f[2];
+    fetch(0, 0, f[0]);
+    int s = 0;
+#pragma unroll 1
+    for (; s + STAGES + 1 < stages; ++s) {
+        fetch(s, 1, f[1]);
+        sums(f[0]);
+        woven();
+        wait_loads<(STAGES - 2) * PER>();
+        barrier_only();      // the next tiles are there, and everybody has read these
+        request(s + STAGES);
+        fetch(s + 1, 0, f[0]);
+        sums(f[1]);
+        woven();
+    }
+#pragma unroll 1
+    for (; s < stages; ++s) {      // the last request, and none
+        if (2 * s + 1 < steps) fetch(s, 1, f[1]);
+        sums(f[0]);
+        if (s + 1 < stages) {
+            wait_loads<0>();
+            barrier_only();
+            if (s + STAGES < stages) request_last(s + STAGES);
+            fetch(s + 1, 0, f[0]);
+        }
+        if (2 * s + 1 < steps) sums(f[1]);
     }
     const long row_w = row0 + wm * NM * 16;
     const int col_w = col0 + wn * NT * 16;
@@ -531,95 +901,6 @@ __global__ __launch_bounds__(512) void k_product_few(const Product p)
     }
 }
 
-// ---- rows sorted by adapter, in their order: places [start[a], start[a + 1]) of perm hold adapter a's; rows with no adapter, and with an
-// index out of range, come last.  Pieces of kPieceRows rows of one adapter: [first[a], first[a + 1]).
-
-__device__ __forceinline__ int key_of(int a, int n) { return has_adapter(a, n) ? a : (a == -1 ? n : n + 1); }
-
-struct Groups {
-    const int* index;
-    int adapters, blocks, rows_per_block, piece;
-    long rows;
-    int *count;      // [key][block], later its exclusive sums over blocks
-    int *total;      // [key]
-    int *start, *first;      // [adapters + 1]
-    int *perm;
-};
-__global__ __launch_bounds__(64) void k_group_count(const Groups p)
-{
-    extern __shared__ int hist[];
-    for (int k = threadIdx.x; k < p.adapters + 2; k += 64) hist[k] = 0;
-    __syncthreads();
-    const long begin = (long)blockIdx.x * p.rows_per_block, end = min(begin + p.rows_per_block, p.rows);
-    for (long i = begin + threadIdx.x; i < end; i += 64) atomicAdd(&hist[key_of(p.index[i], p.adapters)], 1);
-    __syncthreads();
-    for (int k = threadIdx.x; k < p.adapters + 2; k += 64) p.count[(long)k * p.blocks + blockIdx.x] = hist[k];
-}
-__device__ __forceinline__ int wave_exclusive(int x, int lane, int& total)
-{
-    int sum = x;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const int y = __shfl_up(sum, d, 64);
-        if (lane >= d) sum += y;
-    }
-    total = __shfl(sum, 63, 64);
-    return sum - x;
-}
-__global__ __launch_bounds__(256) void k_group_scan(const Groups p)
-{
-    const int key = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (key >= p.adapters + 2) return;
-    int run = 0;
-    int* count = p.count + (long)key * p.blocks;
-    for (int b = 0; b < p.blocks; b += 64) {
-        int total;
-        const int x = b + lane < p.blocks ? count[b + lane] : 0, before = wave_exclusive(x, lane, total);
-        if (b + lane < p.blocks) count[b + lane] = run + before;
-        run += total;
-    }
-    if (lane == 0) p.total[key] = run;
-}
-__global__ __launch_bounds__(64) void k_group_place(const Groups p)
-{
-    extern __shared__ int base[];
-    const int lane = threadIdx.x, keys = p.adapters + 2;
-    int rows = 0, pieces = 0;
-    for (int k = 0; k < keys; k += 64) {
-        int row_total, piece_total;
-        const int x = k + lane < keys ? p.total[k + lane] : 0;
-        const int row_before = rows + wave_exclusive(x, lane, row_total);
-        const int piece_before = pieces + wave_exclusive(k + lane < p.adapters ? (x + p.piece - 1) / p.piece : 0, lane, piece_total);
-        if (k + lane < keys) base[k + lane] = row_before + p.count[(long)(k + lane) * p.blocks + blockIdx.x];
-        if (blockIdx.x == 0 && k + lane <= p.adapters) {
-            p.start[k + lane] = row_before;
-            p.first[k + lane] = piece_before;
-        }
-        rows += row_total;
-        pieces += piece_total;
-    }
-    __syncthreads();
-    const long begin = (long)blockIdx.x * p.rows_per_block, end = min(begin + p.rows_per_block, p.rows);
-    for (long i = begin; i < end; i += 64) {
-        const bool live = i + lane < end;
-        const int key = live ? key_of(p.index[i + lane], p.adapters) : keys;
-        unsigned long same = __ballot(live);
-        for (int bit = 0; (1 << bit) <= keys; ++bit) {
-            const unsigned long set = __ballot(key >> bit & 1);
-            same &= key >> bit & 1 ? set : ~set;
-        }
-        const int before = __popcll(same & ((1ul << lane) - 1));
-        int at = 0;
-        if (live) at = base[key] + before;
-        __syncthreads();
-        if (live) {
-            p.perm[at] = (int)(i + lane);
-            if (before == 0) base[key] = at + __popcll(same);
-        }
-        __syncthreads();
-    }
-}
-
 // ---- sums over rows of h[row][r] in[row][col], by pieces of an adapter's rows
 
 struct Outer {
@@ -632,12 +913,19 @@ struct Outer {
     void* out;
     long out_each, out_r, out_col;
 };
+struct Outers {
+    Outer outer[2];
+    int blocks[2];      // of columns
+};
 // A block takes a piece, 64 r at most, and 64 V columns; a wavefront 16 V of them, four rows at a time.
 template <typename T, int RT>
-__global__ __launch_bounds__(256) void k_outer(const Outer p)
+__global__ __launch_bounds__(256) void k_outer(const Outers both)
 {
     constexpr int V = kRun<T>, U = 4;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4, item = blockIdx.x;
+    const bool second = (int)blockIdx.y >= both.blocks[0];
+    const Outer& p = both.outer[second];
+    const int slab = second ? blockIdx.y - both.blocks[0] : blockIdx.y;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4, item = blockIdx.x;
     if (item >= p.first[p.adapters]) return;
     int low = 0, high = p.adapters;
     while (high - low > 1) {
@@ -646,32 +934,42 @@ __global__ __launch_bounds__(256) void k_outer(const Outer p)
         else high = mid;
     }
     const int begin = p.start[low] + (item - p.first[low]) * p.piece, end = min(begin + p.piece, p.start[low + 1]);
-    const int col = (blockIdx.y * 4 + wave) * 16 * V + V * n, r0 = blockIdx.z * 64;
-    if ((blockIdx.y * 4 + wave) * 16 * V >= p.cols) return;
+    const int col = (slab * 4 + wave) * 16 * V + V * n, r0 = blockIdx.z * 64;
+    if ((slab * 4 + wave) * 16 * V >= p.cols) return;
     const T* in = static_cast<const T*>(p.in) + col;
     const float* h = p.h + r0 + n;
+    const bool whole = (slab * 4 + wave + 1) * 16 * V <= p.cols;
     f32x4 acc[RT][V];
 #pragma unroll
     for (int q = 0; q < RT; ++q)
 #pragma unroll
         for (int t = 0; t < V; ++t) acc[q][t] = f32x4{0, 0, 0, 0};
-    for (int at = begin; at < end; at += 4 * U) {
-        float x[U][V], hv[U][RT];
+    for (int at = begin; at < end; at += 64) {
+        const int mine = p.perm[min(at + lane, end - 1)];      // the rows of the next 64
+#pragma unroll 1
+        for (int i0 = 0; i0 < min(64, end - at); i0 += 4 * U) {
+            typename Operand<T>::type x[U];
+            float hv[U][RT];
+            bool live[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int i = at + 4 * u + g;
-            const bool live = i < end;
-            const long row = p.perm[min(i, end - 1)];
-            load_run<V>(in + row * p.in_stride, live ? p.cols - col : 0, x[u]);
+            for (int u = 0; u < U; ++u) {
+                const int i = i0 + 4 * u + g;
+                live[u] = at + i < end;
+                const long row = __shfl(mine, i, 64);
+                if (whole) x[u] = *reinterpret_cast<const typename Run<T, V>::loose*>(in + row * p.in_stride);
+                else x[u] = load_operand(in + row * p.in_stride, p.cols - col);
 #pragma unroll
-            for (int q = 0; q < RT; ++q) hv[u][q] = live && r0 + 16 * q + n < p.rank ? h[row * p.padded + 16 * q] : 0.0f;
+                for (int q = 0; q < RT; ++q) hv[u][q] = r0 + 16 * q + n < p.rank ? h[row * p.padded + 16 * q] : 0.0f;
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int t = 0; t < V; ++t) {
+                    const float v = live[u] ? (float)x[u][t] : 0.0f;
+#pragma unroll
+                    for (int q = 0; q < RT; ++q) acc[q][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(live[u] ? hv[u][q] : 0.0f, v, acc[q][t], 0, 0, 0);
+                }
         }
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int q = 0; q < RT; ++q)
-#pragma unroll
-                for (int t = 0; t < V; ++t) acc[q][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(hv[u][q], x[u][t], acc[q][t], 0, 0, 0);
     }
     float* out = p.partial + (long)item * p.rank * p.cols + col;
 #pragma unroll
@@ -685,15 +983,28 @@ __global__ __launch_bounds__(256) void k_outer(const Outer p)
             if (r < p.rank) store_run<V>(out + (long)r * p.cols, p.cols - col, v);
         }
 }
+// The pieces of an adapter, in order: a block takes 64 numbers, four threads each.
 template <typename T>
-__global__ __launch_bounds__(256) void k_join(const Outer p)
+__global__ __launch_bounds__(256) void k_join(const Outers both)
 {
-    const int a = blockIdx.y, each = p.rank * p.cols, e = blockIdx.x * 256 + threadIdx.x;
-    if (e >= each) return;
+    __shared__ float part[4][64];
+    const Outer& p = both.outer[blockIdx.z];
+    const int a = blockIdx.y, each = p.rank * p.cols, lane = threadIdx.x & 63, q = threadIdx.x >> 6, e = blockIdx.x * 64 + lane;
+    if ((int)blockIdx.x * 64 >= each) return;
     float sum = 0.0f;
-    for (int i = p.first[a]; i < p.first[a + 1]; ++i) sum += p.partial[(long)i * each + e];
-    const int r = e / p.cols, col = e % p.cols;
-    static_cast<T*>(p.out)[a * p.out_each + r * p.out_r + col * p.out_col] = (T)sum;
+    if (e < each) {
+        const float* from = p.partial + e;
+        const int last = p.first[a + 1];
+#pragma unroll 4
+        for (int i = p.first[a] + q; i < last; i += 4) sum += from[(long)i * each];
+    }
+    part[q][lane] = sum;
+    __syncthreads();
+    if (q == 0 && e < each) {
+        sum = (part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]);
+        const int r = e / p.cols, col = e % p.cols;
+        static_cast<T*>(p.out)[a * p.out_each + r * p.out_r + col * p.out_col] = (T)sum;
+    }
 }
 
 // ---- host side
@@ -727,7 +1038,11 @@ struct Arena {
 };
 
 // rows that direct loads into LDS can take as they are
-bool as_it_is(const void* p, long stride, long k) { return (reinterpret_cast<size_t>(p) & 15) == 0 && stride % 8 == 0 && k % kPiece == 0; }
+// (the offsets inside a tile have 32 bits)
+bool as_it_is(const void* p, long stride, long k) { return (reinterpret_cast<size_t>(p) & 15) == 0 && stride % 8 == 0 && stride <= 1 << 22 && k % kPiece == 0; }
+
+template <int N>
+using Int = std::integral_constant<int, N>;
 
 struct Call {
     const smx_adapted_linear& p;
@@ -735,46 +1050,103 @@ struct Call {
     Arena arena;
     const bool dry;      // nothing is launched, the workspace is counted
     const int padded;
+    Prepare prepare{};
+    Downs downs{};
+    int num_layouts = 0, num_downs = 0;
     Call(const smx_adapted_linear& p_, void* base, hipStream_t s_, bool dry_)
         : p(p_), s(s_), arena{static_cast<char*>(base)}, dry(dry_), padded((int)up(p_.rank, 16)) {}
 
     template <typename T>
-    void down(const T* in, long in_stride, const T* F, long f_each, long f_row, int k, float* h, bool few)
+    void lay_out(const void* src, long src_each, long src_row, long src_k, void* dst, long part, long rows, int k, int matrices)
     {
-        if (dry) return;
-        const Down d{in, in_stride, F, f_each, f_row, p.scale, p.index, p.num_adapters, p.rank, padded, k, p.rows, h};
-        if (few) {
-            hipLaunchKernelGGL((k_down_few<T>), dim3((unsigned)p.rows, padded / 4), dim3(256), 0, s, d);
-            return;
+        const int k_padded = (int)up(k, kPiece);
+        // (rows in 32 bits)
+        for (long r = 0; r < rows; r += 1 << 30) {
+            if (num_layouts == 2) flush_layouts<T>();
+            const Layout l{static_cast<const T*>(src) + r * src_row, src_each, src_row, src_k, static_cast<T*>(dst) + r * k_padded, rows * k_padded, part,
+                           (int)std::min(1L << 30, rows - r), k, k_padded, matrices};
+            prepare.blocks[num_layouts] = layout_blocks(l);
+            prepare.layout[num_layouts++] = l;
         }
-        const dim3 grid((unsigned)((p.rows + 15) / 16));
-        auto go = [&](auto rt) { hipLaunchKernelGGL((k_down<T, decltype(rt)::value>), grid, dim3(256), 0, s, d); };
-        if (padded == 16) go(std::integral_constant<int, 1>{});
-        else if (padded == 32) go(std::integral_constant<int, 2>{});
-        else if (padded <= 64) go(std::integral_constant<int, 4>{});
-        else go(std::integral_constant<int, 8>{});
+    }
+    // launches what is laid out, and the count of rows if it is due
+    template <typename T>
+    void flush_layouts(bool count = false)
+    {
+        const long blocks = prepare.blocks[0] + prepare.blocks[1] + (count ? prepare.groups.blocks : 0);
+        refuse_unless(blocks <= 0x7fffffffL, "more blocks than a launch takes");
+        if (!dry && blocks) hipLaunchKernelGGL((k_prepare<T>), dim3((unsigned)blocks), dim3(256), 0, s, prepare);
+        prepare.blocks[0] = prepare.blocks[1] = 0;
+        num_layouts = 0;
     }
 
-    // out[rows][cols] = in W^T + adapters' part; W(col, k) = W[col * w_col + k * w_k], F(col, r) = F[a][col * f_col + r * f_r]
     template <typename T>
-    void product(const T* in, long in_stride, const T* W, long w_col, long w_k, const T* F, long f_each, long f_col, long f_r, const float* h, int k, int cols,
-                 T* out, long out_stride, bool few)
+    void down(const T* in, long in_stride, const T* F, long f_each, long f_row, int k, float* h)
+    {
+        downs.down[num_downs++] = Down{in, in_stride, F, f_each, f_row, p.scale, p.index, p.num_adapters, p.rank, padded, k, p.rows, h};
+    }
+    template <typename T>
+    void flush_downs(bool place)
+    {
+        if (dry) return;
+        auto go = [&](auto rt, auto mt) {
+            constexpr int RT = decltype(rt)::value, MT = decltype(mt)::value;
+            for (int i = 0; i < num_downs; ++i) downs.blocks[i] = (int)((p.rows + 16 * MT - 1) / (16 * MT));
+            const long blocks = (long)downs.blocks[0] + downs.blocks[1] + (place ? downs.groups.blocks : 0);
+            refuse_unless(blocks <= 0x7fffffffL, "more blocks than a launch takes");
+            if (blocks) hipLaunchKernelGGL((k_down<T, RT, MT>), dim3((unsigned)blocks), dim3(256), 0, s, downs);
+        };
+        if (padded == 16) go(Int<1>{}, Int<2>{});
+        else if (padded == 32) go(Int<2>{}, Int<2>{});
+        else if (padded <= 64) go(Int<4>{}, Int<2>{});
+        else go(Int<8>{}, Int<1>{});
+    }
+
+    // out[rows][cols] = in W^T + adapters' part; W(col, k) = W[col * w_col + k * w_k], F(col, r) = F[a][col * f_col + r * f_r].
+    // First what has to be laid out for it, then the product itself.
+    template <typename T>
+    Product product(const T* in, long in_stride, const T* W, long w_col, long w_k, const T* F, long f_each, long f_col, long f_r, const float* h, int k, int cols, T* out,
+                    long out_stride, bool few)
     {
         Product q{};
-        q.in = in; q.in_stride = in_stride; q.W0 = W; q.w0_col = w_col; q.w0_k = w_k; q.F = F; q.f_each = f_each; q.f_col = f_col; q.f_r = f_r; q.h = h;
+        q.in = in; q.in_stride = in_stride; q.W0 = W; q.w0_col = w_col; q.w0_k = w_k; q.F = F; q.f_each = f_each; q.f_col = f_col; q.f_r = f_r; q.f_runs = f_r == 1 && p.rank % 8 == 0; q.h = h;
         q.index = p.index; q.adapters = p.num_adapters; q.rank = p.rank; q.padded = padded; q.k = k; q.k_padded = (int)up(k, kPiece); q.cols = cols;
         q.rows = p.rows; q.out = out; q.out_stride = out_stride;
+        if (few) return q;
+        if constexpr (std::is_same_v<T, float>) {
+            q.w_part = (long)cols * q.k_padded;
+            bf16* parts = arena.take<bf16>(3 * q.w_part);
+            lay_out<float>(W, 0, w_col, w_k, parts, q.w_part, cols, k, 1);
+            q.W = parts; q.w_stride = q.k_padded;
+        } else {
+            q.W = W; q.w_stride = w_col;
+            if (!(w_k == 1 && as_it_is(W, w_col, k))) {
+                T* laid = arena.take<T>((long)cols * q.k_padded);
+                lay_out<T>(W, 0, w_col, w_k, laid, 0, cols, k, 1);
+                q.W = laid; q.w_stride = q.k_padded;
+            }
+            if (!as_it_is(in, in_stride, k)) {
+                T* laid = arena.take<T>(p.rows * q.k_padded);
+                lay_out<T>(in, 0, in_stride, 1, laid, 0, p.rows, k, 1);
+                q.in = laid; q.in_stride = q.k_padded;
+            }
+        }
+        return q;
+    }
+    template <typename T>
+    void launch(Product q, bool few)
+    {
+        if (dry) return;
         if (few) {
-            if (dry) return;
-            auto go = [&](auto mt) { hipLaunchKernelGGL((k_product_few<T, decltype(mt)::value>), dim3((cols + 15) / 16), dim3(512), 0, s, q); };
-            if (p.rows <= 16) go(std::integral_constant<int, 1>{});
-            else if (p.rows <= 32) go(std::integral_constant<int, 2>{});
-            else go(std::integral_constant<int, 4>{});
+            auto go = [&](auto mt) { hipLaunchKernelGGL((k_product_few<T, decltype(mt)::value>), dim3((q.cols + 15) / 16), dim3(512), 0, s, q); };
+            if (p.rows <= 16) go(Int<1>{});
+            else if (p.rows <= 32) go(Int<2>{});
+            else go(Int<4>{});
             return;
         }
         auto tiles = [&](int bm, int bn) {
             q.row_tiles = (int)((p.rows + bm - 1) / bm);
-            q.col_tiles = (cols + bn - 1) / bn;
+            q.col_tiles = (q.cols + bn - 1) / bn;
             return (long)q.row_tiles * q.col_tiles;
         };
         auto blocks = [&] {
@@ -783,42 +1155,24 @@ struct Call {
             return dim3((unsigned)((t + 7) / 8 * 8));
         };
         if constexpr (std::is_same_v<T, float>) {
-            bf16* parts = arena.take<bf16>(3L * cols * q.k_padded);
-            if (dry) return;
-            lay_out<float, true>(Layout{W, 0, w_col, w_k, parts, 0, (long)cols * q.k_padded, cols, k, q.k_padded}, 1, s);
-            q.W = parts; q.w_stride = q.k_padded; q.w_part = (long)cols * q.k_padded;
             if (tiles(128, 128) >= 256) hipLaunchKernelGGL((k_product32<4, 4>), blocks(), dim3(256), 0, s, q);
             else {
                 tiles(64, 64);
                 hipLaunchKernelGGL((k_product32<2, 2>), blocks(), dim3(256), 0, s, q);
             }
         } else {
-            if (!(w_k == 1 && as_it_is(W, w_col, k))) {
-                T* laid = arena.take<T>((long)cols * q.k_padded);
-                if (!dry) lay_out<T, false>(Layout{W, 0, w_col, w_k, laid, 0, 0, cols, k, q.k_padded}, 1, s);
-                q.W = laid; q.w_stride = q.k_padded;
-            } else {
-                q.W = W; q.w_stride = w_col;
-            }
-            if (!as_it_is(in, in_stride, k)) {
-                T* laid = arena.take<T>(p.rows * q.k_padded);
-                for (long r = 0; !dry && r < p.rows; r += 4000000)      // (the rows of a grid)
-                    lay_out<T, false>(Layout{in + r * in_stride, 0, in_stride, 1, laid + r * q.k_padded, 0, 0, (int)std::min(4000000L, p.rows - r), k, q.k_padded}, 1, s);
-                q.in = laid; q.in_stride = q.k_padded;
-            }
-            if (dry) return;
-            auto go = [&](auto bm, auto bn, auto wm, auto wn) {
-                constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value, WM = decltype(wm)::value, WN = decltype(wn)::value;
-                constexpr int bytes = 4 * (BM + BN) * 64;
+            auto go = [&](auto bm, auto bn, auto wm, auto wn, auto stages) {
+                constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value, WM = decltype(wm)::value, WN = decltype(wn)::value, S = decltype(stages)::value;
+                constexpr int bytes = S * (BM + BN) * 128;
                 if constexpr (bytes > 64 * 1024)
-                    hip_ok(hipFuncSetAttribute(reinterpret_cast<const void*>(&k_product16<T, BM, BN, WM, WN>), hipFuncAttributeMaxDynamicSharedMemorySize, bytes), "LDS");
-                hipLaunchKernelGGL((k_product16<T, BM, BN, WM, WN>), blocks(), dim3(64 * WM * WN), bytes, s, q);
+                    hip_ok(hipFuncSetAttribute(reinterpret_cast<const void*>(&k_product16<T, BM, BN, WM, WN, S>), hipFuncAttributeMaxDynamicSharedMemorySize, bytes), "LDS");
+                hipLaunchKernelGGL((k_product16<T, BM, BN, WM, WN, S>), blocks(), dim3(64 * WM * WN), bytes, s, q);
             };
-            if (tiles(256, 256) >= 192) go(std::integral_constant<int, 256>{}, std::integral_constant<int, 256>{}, std::integral_constant<int, 2>{}, std::integral_constant<int, 4>{});
-            else if (tiles(128, 128) >= 192) go(std::integral_constant<int, 128>{}, std::integral_constant<int, 128>{}, std::integral_constant<int, 2>{}, std::integral_constant<int, 2>{});
+            if (tiles(256, 256) >= 192) go(Int<256>{}, Int<256>{}, Int<2>{}, Int<4>{}, Int<2>{});
+            else if (tiles(128, 128) >= 192) go(Int<128>{}, Int<128>{}, Int<2>{}, Int<2>{}, Int<2>{});
             else {
                 tiles(64, 64);
-                go(std::integral_constant<int, 64>{}, std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{}, std::integral_constant<int, 2>{});
+                go(Int<64>{}, Int<64>{}, Int<2>{}, Int<2>{}, Int<3>{});
             }
         }
     }
@@ -829,22 +1183,12 @@ struct Call {
         const bool few = p.rows <= kMostFew;
         const T *x = static_cast<const T*>(p.x), *W = static_cast<const T*>(p.weight), *A = static_cast<const T*>(p.A), *B = static_cast<const T*>(p.B);
         float* h = arena.take<float>(p.rows * padded);
-        down(x, p.x_stride, A, (long)p.rank * p.d_in, p.d_in, p.d_in, h, few);
-        product(x, p.x_stride, W, p.weight_stride, 1, B, (long)p.rank * p.d_out, p.rank, 1, h, p.d_in, p.d_out, y, y_stride, few);
-    }
-
-    template <typename T>
-    void outer(Outer q, long most, const T* in, long in_stride, const float* h, int cols, void* out, long out_each, long out_r, long out_col)
-    {
-        q.in = in; q.in_stride = in_stride; q.h = h; q.cols = cols; q.out = out; q.out_each = out_each; q.out_r = out_r; q.out_col = out_col;
-        const int slab = 64 * kRun<T>;
-        if (p.rows > 0) {
-            const dim3 grid((unsigned)most, (cols + slab - 1) / slab, (p.rank + 63) / 64);
-            if (padded == 16) hipLaunchKernelGGL((k_outer<T, 1>), grid, dim3(256), 0, s, q);
-            else if (padded == 32) hipLaunchKernelGGL((k_outer<T, 2>), grid, dim3(256), 0, s, q);
-            else hipLaunchKernelGGL((k_outer<T, 4>), grid, dim3(256), 0, s, q);
-        }
-        hipLaunchKernelGGL((k_join<T>), dim3((p.rank * cols + 255) / 256, p.num_adapters), dim3(256), 0, s, q);
+        const Product q = product(x, p.x_stride, W, p.weight_stride, 1, B, (long)p.rank * p.d_out, p.rank, 1, h, p.d_in, p.d_out, y, y_stride, few);
+        flush_layouts<T>();
+        down(x, p.x_stride, A, (long)p.rank * p.d_in, p.d_in, p.d_in, h);
+        if (!few) flush_downs<T>(false);
+        else if (!dry) hipLaunchKernelGGL((k_down_few<T>), dim3((unsigned)p.rows, padded / 4), dim3(256), 0, s, downs.down[0]);
+        launch<T>(q, few);
     }
 
     template <typename T>
@@ -853,41 +1197,62 @@ struct Call {
         const T *x = static_cast<const T*>(p.x), *W = static_cast<const T*>(p.weight), *A = static_cast<const T*>(p.A), *B = static_cast<const T*>(p.B);
         const long each_a = (long)p.rank * p.d_in, each_b = (long)p.rank * p.d_out;
         const int n = p.num_adapters;
-        const bool sums = (dA || dB || dry) && n > 0;
-        float *h = arena.take<float>(p.rows * padded), *g = arena.take<float>(p.rows * padded);
-        if (p.rows > 0) {
-            // B_a^T, so that sums over d_out run along rows
-            const int k_padded = (int)up(p.d_out, kPiece);
-            T* Bt = arena.take<T>((long)n * p.rank * k_padded);
-            if (!dry && (dx || dA)) {
-                if (n) lay_out<T, false>(Layout{B, each_b, 1, p.rank, Bt, (long)p.rank * k_padded, 0, p.rank, p.d_out, k_padded}, n, s);
-                down(dy, dy_stride, Bt, (long)p.rank * k_padded, k_padded, p.d_out, g, false);
-            }
-            if (!dry && dB) down(x, p.x_stride, A, each_a, p.d_in, p.d_in, h, false);
-            if (dx || dry) product(dy, dy_stride, W, 1, p.weight_stride, A, each_a, 1, p.d_in, g, p.d_out, p.d_in, dx, dx_stride, false);
+        const bool rows = p.rows > 0, want_x = rows && (dx || dry), want_a = n > 0 && (dA || dry), want_b = n > 0 && (dB || dry), sums = want_a || want_b;
+        float *h = arena.take<float>(want_b ? p.rows * padded : 0), *g = arena.take<float>(want_x || want_a ? p.rows * padded : 0);
+        Groups& groups = prepare.groups;
+        long most = 0;
+        float *partial_a = nullptr, *partial_b = nullptr;
+        if (sums) {
+            groups.index = p.index; groups.adapters = n; groups.rows = p.rows;
+            // (a block that places rows reads the counts of all blocks)
+            const long most_blocks = std::max(1, std::min(256, 16384 / (n + 2)));
+            groups.rows_per_block = (int)std::max(256L, up((p.rows + most_blocks - 1) / most_blocks, 64));
+            groups.blocks = (int)std::max(1L, (p.rows + groups.rows_per_block - 1) / groups.rows_per_block);
+            groups.piece = (int)std::max(64L, up((p.rows + 511) / 512, 64));
+            groups.count = arena.take<int>((long)(n + 2) * groups.blocks);
+            groups.start = arena.take<int>(n + 1);
+            groups.first = arena.take<int>(n + 1);
+            groups.perm = arena.take<int>(p.rows);
+            most = std::min<long>(p.rows, p.rows / groups.piece + n);      // pieces: of an adapter's rows, one that is not full
+            if (want_a) partial_a = arena.take<float>(most * each_a);
+            if (want_b) partial_b = arena.take<float>(most * each_b);
+            downs.groups = groups;
         }
-        if (!sums) return;
-        Groups q{};
-        q.index = p.index; q.adapters = n; q.rows = p.rows;
-        q.rows_per_block = (int)std::max(256L, up((p.rows + 1023) / 1024, 64));
-        q.blocks = (int)std::max(1L, (p.rows + q.rows_per_block - 1) / q.rows_per_block);
-        q.piece = (int)std::max(64L, up((p.rows + 511) / 512, 16));
-        q.count = arena.take<int>((long)(n + 2) * q.blocks);
-        q.total = arena.take<int>(n + 2);
-        q.start = arena.take<int>(n + 1);
-        q.first = arena.take<int>(n + 1);
-        q.perm = arena.take<int>(p.rows);
-        const long most = std::min<long>(p.rows, p.rows / q.piece + n);      // pieces: of an adapter's rows, one that is not full
-        float* partial = arena.take<float>(most * p.rank * std::max(p.d_in, p.d_out));
-        if (dry) return;
-        const unsigned lds = (n + 2) * sizeof(int);
-        hipLaunchKernelGGL(k_group_count, dim3(q.blocks), dim3(64), lds, s, q);
-        hipLaunchKernelGGL(k_group_scan, dim3((n + 2 + 3) / 4), dim3(256), 0, s, q);
-        hipLaunchKernelGGL(k_group_place, dim3(q.blocks), dim3(64), lds, s, q);
+        Product q{};
+        // B_a^T, so that sums over d_out run along rows
+        const int k_padded = (int)up(p.d_out, kPiece);
+        T* Bt = nullptr;
+        if (want_x || (want_a && rows)) {
+            Bt = arena.take<T>((long)n * p.rank * k_padded);
+            if (n) lay_out<T>(B, each_b, 1, p.rank, Bt, 0, p.rank, p.d_out, n);
+            down(dy, dy_stride, Bt, (long)p.rank * k_padded, k_padded, p.d_out, g);
+        }
+        if (want_b && rows) down(x, p.x_stride, A, each_a, p.d_in, p.d_in, h);
+        if (want_x) q = product(dy, dy_stride, W, 1, p.weight_stride, A, each_a, 1, p.d_in, g, p.d_out, p.d_in, dx, dx_stride, false);
+        flush_layouts<T>(sums);
+        flush_downs<T>(sums);
+        if (want_x) launch<T>(q, false);
+        if (!sums || dry) return;
+        Outers both{};
         Outer o{};
-        o.start = q.start; o.first = q.first; o.perm = q.perm; o.adapters = n; o.rank = p.rank; o.padded = padded; o.piece = q.piece; o.partial = partial;
-        if (dA) outer(o, most, x, p.x_stride, g, p.d_in, dA, each_a, p.d_in, 1);
-        if (dB) outer(o, most, dy, dy_stride, h, p.d_out, dB, each_b, 1, p.rank);
+        o.start = groups.start; o.first = groups.first; o.perm = groups.perm; o.adapters = n; o.rank = p.rank; o.padded = padded; o.piece = groups.piece;
+        int num = 0, across = 0, widest = 0;
+        auto add = [&](const T* in, long in_stride, const float* factor, int cols, float* partial, T* out, long each, long out_r, long out_col) {
+            o.in = in; o.in_stride = in_stride; o.h = factor; o.cols = cols; o.partial = partial; o.out = out; o.out_each = each; o.out_r = out_r; o.out_col = out_col;
+            both.blocks[num] = (cols + 64 * kRun<T> - 1) / (64 * kRun<T>);
+            across += both.blocks[num];
+            widest = std::max(widest, cols);
+            both.outer[num++] = o;
+        };
+        if (want_a) add(x, p.x_stride, g, p.d_in, partial_a, dA, each_a, p.d_in, 1);
+        if (want_b) add(dy, dy_stride, h, p.d_out, partial_b, dB, each_b, 1, p.rank);
+        if (rows) {
+            const dim3 grid((unsigned)most, across, (p.rank + 63) / 64);
+            if (padded == 16) hipLaunchKernelGGL((k_outer<T, 1>), grid, dim3(256), 0, s, both);
+            else if (padded == 32) hipLaunchKernelGGL((k_outer<T, 2>), grid, dim3(256), 0, s, both);
+            else hipLaunchKernelGGL((k_outer<T, 4>), grid, dim3(256), 0, s, both);
+        }
+        hipLaunchKernelGGL((k_join<T>), dim3((unsigned)(((long)p.rank * widest + 63) / 64), n, num), dim3(256), 0, s, both);
     }
 };
 
