@@ -77,9 +77,19 @@ struct Layout {
     const void* src;
     long src_each, src_row, src_k;      // strides of a matrix, a row and a number
     void* dst;
-    long dst_each, part;                // strides of a matrix and a part; part 0: one part, as it is
+    long dst_each;                      // stride of a matrix
     int rows, k, k_padded, matrices;
+    bool parts;    // single precision in three bf16 parts, in the order of k_product32
+    int live;      // rows that there are; zeros behind them
 };
+// First part of number k of a row, in [128 rows][32 numbers][part][row][32]: what a block takes at a step lies as it goes into LDS, the
+// four pieces of a row in an order that depends on the row, for the banks.
+constexpr int kPartRows = 128;
+__device__ __forceinline__ long split_place(int row, int k, int k_padded)
+{
+    const int r = row % kPartRows, piece = (k % kPiece / 8) ^ (r >> 1 & 3);
+    return ((long)(row / kPartRows) * (k_padded / kPiece) + k / kPiece) * 3 * kPartRows * kPiece + r * kPiece + piece * 8 + k % 8;
+}
 inline __host__ __device__ long layout_blocks(const Layout& p) { return (long)((p.k_padded + 63) / 64) * ((p.rows + 63) / 64) * p.matrices; }
 // a block takes 64 rows and 64 numbers of them
 template <typename T>
@@ -95,7 +105,7 @@ __device__ __forceinline__ void lay_out(const Layout& p, long block, T (*tile)[6
 #pragma unroll
         for (int u = 0; u < 16; ++u) {
             const int r = (threadIdx.x >> 6) + 4 * u;
-            x[u] = row0 + r < p.rows && k0 + k < p.k ? src[(row0 + r) * p.src_row + k0 + k] : (T)0.0f;
+            x[u] = row0 + r < p.live && k0 + k < p.k ? src[(row0 + r) * p.src_row + k0 + k] : (T)0.0f;
         }
 #pragma unroll
         for (int u = 0; u < 16; ++u) tile[(threadIdx.x >> 6) + 4 * u][k] = x[u];
@@ -104,7 +114,7 @@ __device__ __forceinline__ void lay_out(const Layout& p, long block, T (*tile)[6
 #pragma unroll
         for (int u = 0; u < 16; ++u) {
             const int k = (threadIdx.x >> 6) + 4 * u;
-            x[u] = row0 + r < p.rows && k0 + k < p.k ? src[(row0 + r) * p.src_row + (k0 + k) * p.src_k] : (T)0.0f;
+            x[u] = row0 + r < p.live && k0 + k < p.k ? src[(row0 + r) * p.src_row + (k0 + k) * p.src_k] : (T)0.0f;
         }
 #pragma unroll
         for (int u = 0; u < 16; ++u) tile[r][(threadIdx.x >> 6) + 4 * u] = x[u];
@@ -114,16 +124,16 @@ __device__ __forceinline__ void lay_out(const Layout& p, long block, T (*tile)[6
     for (int u = 0; u < 8; ++u) {
         const int r = (threadIdx.x >> 5) + 8 * u, k = (threadIdx.x & 31) * 2;
         if (row0 + r >= p.rows || k0 + k >= p.k_padded) continue;
-        const long at = matrix * p.dst_each + (long)(row0 + r) * p.k_padded + k0 + k;
-        if (std::is_same_v<T, float> && p.part) {
+        if (std::is_same_v<T, float> && p.parts) {
             const float v[2] = {(float)tile[r][k] * kSplitScale, (float)tile[r][k + 1] * kSplitScale};
             bf16 part[3][2];
             split(v, part);
+            bf16* to = static_cast<bf16*>(p.dst) + split_place(row0 + r, k0 + k, p.k_padded);
 #pragma unroll
-            for (int q = 0; q < 3; ++q) *reinterpret_cast<bf16x2*>(static_cast<bf16*>(p.dst) + q * p.part + at) = bf16x2{part[q][0], part[q][1]};
+            for (int q = 0; q < 3; ++q) *reinterpret_cast<bf16x2*>(to + q * kPartRows * kPiece) = bf16x2{part[q][0], part[q][1]};
         } else {
             typedef T pair __attribute__((ext_vector_type(2)));
-            *reinterpret_cast<pair*>(static_cast<T*>(p.dst) + at) = pair{tile[r][k], tile[r][k + 1]};
+            *reinterpret_cast<pair*>(static_cast<T*>(p.dst) + matrix * p.dst_each + (long)(row0 + r) * p.k_padded + k0 + k) = pair{tile[r][k], tile[r][k + 1]};
         }
     }
 }
@@ -404,8 +414,8 @@ __global__ __launch_bounds__(256) void k_down_few(const Down p)
 struct Product {
     const void* in;
     long in_stride;
-    const void* W;               // laid out: rows (columns of the result) w_stride apart, of a multiple of 32 numbers
-    long w_stride, w_part;
+    const void* W;               // laid out: rows (columns of the result) w_stride apart, of a multiple of 32 numbers; or three bf16 parts
+    long w_stride;
     const void* W0;              // as the caller has it
     long w0_col, w0_k;
     const void* F;
@@ -506,52 +516,75 @@ struct AdapterProduct {
 template <>
 struct AdapterProduct<float> {
     static constexpr int CHUNK = 16;
-    // lane g has r0 + 4 j + g: instructions of r beyond the rank are left out
+    // Of the r of a chunk lane g has EACH neighbours (1, 2 or 4, for as many instructions): r0 + EACH g + 0..EACH-1, one load where they are
+    // all there.
+    __device__ static __forceinline__ int each(int r0, int rank) { return rank - r0 <= 4 ? 1 : (rank - r0 <= 8 ? 2 : 4); }
     struct Factor {
-        float x[4];
+        f32x4 x;
     };
     typedef Factor Row;
     __device__ static __forceinline__ Factor factor(const float* from, long stride, bool, int r0, int g, int rank)
     {
+        const int e = each(r0, rank), r = r0 + e * g;
         Factor f;
+        if (stride == 1 && rank - r0 >= 16) f.x = *reinterpret_cast<const Run<float, 4>::loose*>(from + r);
+        else if (stride == 1 && rank - r0 == 8) {
+            const Run<float, 2>::type v = *reinterpret_cast<const Run<float, 2>::loose*>(from + r);
+            f.x = f32x4{v[0], v[1], 0.0f, 0.0f};
+        } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (r0 + 4 * j >= rank) break;
-            const float x = from[min(r0 + 4 * j + g, rank - 1) * stride];
-            f.x[j] = r0 + 4 * j + g < rank ? x : 0.0f;
+            for (int j = 0; j < 4; ++j) {
+                f.x[j] = 0.0f;
+                if (j >= e) continue;
+                const float x = from[min(r + j, rank - 1) * stride];
+                f.x[j] = r + j < rank ? x : 0.0f;
+            }
         }
         return f;
     }
     __device__ static __forceinline__ Row row(const float* h, int r0, int g, int, int rank)
     {
+        const int e = each(r0, rank);
         Row v;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v.x[j] = h[r0 + 4 * j + g];
+        if (e == 4) v.x = *reinterpret_cast<const f32x4*>(h + r0 + 4 * g);
+        else if (e == 2) {
+            const Run<float, 2>::type u = *reinterpret_cast<const Run<float, 2>::type*>(h + r0 + 2 * g);
+            v.x = f32x4{u[0], u[1], 0.0f, 0.0f};
+        } else v.x = f32x4{h[r0 + g], 0.0f, 0.0f, 0.0f};
         return v;
     }
     __device__ static __forceinline__ f32x4 run(const Factor& f, const Row& h, f32x4 c, int r0, int rank)
     {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (r0 + 4 * j < rank) c = __builtin_amdgcn_mfma_f32_16x16x4f32(f.x[j], h.x[j], c, 0, 0, 0);
+        const int e = each(r0, rank);
+        c = __builtin_amdgcn_mfma_f32_16x16x4f32(f.x[0], h.x[0], c, 0, 0, 0);
+        if (e >= 2) c = __builtin_amdgcn_mfma_f32_16x16x4f32(f.x[1], h.x[1], c, 0, 0, 0);
+        if (e == 4) {
+            c = __builtin_amdgcn_mfma_f32_16x16x4f32(f.x[2], h.x[2], c, 0, 0, 0);
+            c = __builtin_amdgcn_mfma_f32_16x16x4f32(f.x[3], h.x[3], c, 0, 0, 0);
+        }
         return c;
     }
 };
 
-// Adds the adapters' part to sums of NM tiles of 16 rows and NT of 16 columns.  Lane (n, g) holds of tile (i, t) row i * 16 + n and
-// columns 4 NT g + 4 t + 0..3.  For every tile of rows one adapter after the other of those that occur in it; the first r of a factor,
-// which mostly are all of them, stay for the next tile of rows.
+// Lane (n, g) holds of tile (i, t) row i * 16 + n and four columns.  In 16 bits these are 4 NT g + 4 t + 0..3, so that a lane has 4 NT
+// neighbours to store; in single precision 16 t + 4 g + 0..3.
+template <typename T, int NT>
+__device__ __forceinline__ int column_of(int t, int m) { return std::is_same_v<T, float> ? 16 * t + m : 4 * NT * (m >> 2) + 4 * t + (m & 3); }
+
+// Adds the adapters' part to sums of NM tiles of 16 rows and NT of 16 columns.  For every tile of rows one adapter after the other of
+// those that occur in it, four tiles of columns at a time; a factor that is held as a whole stays for the next tile of rows.
 template <typename T, int NM, int NT>
 __device__ __forceinline__ void add_adapters(const Product& p, int lane, long row0, int col0, f32x4 (&acc)[NM][NT])
 {
     typedef AdapterProduct<T> Op;
+    constexpr int GT = NT < 4 ? NT : 4;
     const int n = lane & 15, g = lane >> 4;
     __builtin_amdgcn_sched_barrier(0);
     const float* h = p.h + min(row0 + n, p.rows - 1) * p.padded;
     int a = p.index[min(row0 + n, p.rows - 1)];
     typename Op::Row first = Op::row(h, 0, g, p.padded, p.rank);
     int held = -1;
-    typename Op::Factor f[NT];
+    typename Op::Factor f[GT];
 #pragma unroll
     for (int i = 0; i < NM; ++i) {
         const bool good = row0 + 16 * i + n < p.rows && has_adapter(a, p.adapters);
@@ -559,25 +592,28 @@ __device__ __forceinline__ void add_adapters(const Product& p, int lane, long ro
         while (left) {
             const int cur = __builtin_amdgcn_readlane(a, __builtin_ctz(left));
             const bool mine = good && a == cur;
-            left &= ~(unsigned)__ballot(mine);
-            f32x4 sum[NT];
-#pragma unroll
-            for (int t = 0; t < NT; ++t) sum[t] = f32x4{0, 0, 0, 0};
+            const unsigned whose = (unsigned)__ballot(mine) & 0xffffu;
+            left &= ~whose;
             for (int r0 = 0; r0 < p.rank; r0 += Op::CHUNK) {
                 const typename Op::Row hr = r0 == 0 ? first : Op::row(h, r0, g, p.padded, p.rank);
-                if (cur != held || r0 > 0) {
 #pragma unroll
-                    for (int t = 0; t < NT; ++t)
-                        f[t] = Op::factor(static_cast<const T*>(p.F) + cur * p.f_each + min(col0 + 4 * NT * (n >> 2) + 4 * t + (n & 3), p.cols - 1) * p.f_col, p.f_r, p.f_runs, r0, g, p.rank);
-                    held = r0 == 0 ? cur : -1;
+                for (int t0 = 0; t0 < NT; t0 += GT) {
+                    if (NT > GT || cur != held || r0 > 0) {
+#pragma unroll
+                        for (int t = 0; t < GT; ++t)
+                            f[t] = Op::factor(static_cast<const T*>(p.F) + cur * p.f_each + min(col0 + column_of<T, NT>(t0 + t, n), p.cols - 1) * p.f_col, p.f_r, p.f_runs, r0,
+                                              g, p.rank);
+                        held = p.rank <= Op::CHUNK ? cur : -1;
+                    }
+#pragma unroll
+                    for (int t = 0; t < GT; ++t) {
+                        const f32x4 sum = Op::run(f[t], hr, f32x4{0, 0, 0, 0}, r0, p.rank);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) acc[i][t0 + t][j] += mine ? sum[j] : 0.0f;
+                    }
+                    if (NT > GT) __builtin_amdgcn_sched_barrier(0);
                 }
-#pragma unroll
-                for (int t = 0; t < NT; ++t) sum[t] = Op::run(f[t], hr, sum[t], r0, p.rank);
             }
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][t][j] += mine ? sum[t][j] : 0.0f;
         }
         if (i + 1 < NM) {
             h = p.h + min(row0 + 16 * (i + 1) + n, p.rows - 1) * p.padded;
@@ -590,20 +626,29 @@ __device__ __forceinline__ void add_adapters(const Product& p, int lane, long ro
 template <typename T, int NM, int NT>
 __device__ __forceinline__ void store_tiles(const Product& p, int lane, long row0, int col0, const f32x4 (&acc)[NM][NT])
 {
-    constexpr int V = kRun<T>, N = 4 * NT < V ? 4 * NT : V;
-    const int n = lane & 15, g = lane >> 4, col = col0 + 4 * NT * g;
+    constexpr int N = std::is_same_v<T, float> || NT == 1 ? 4 : 8;
+    const int n = lane & 15, g = lane >> 4;
 #pragma unroll
     for (int i = 0; i < NM; ++i) {
         const long row = row0 + 16 * i + n;
         if (row >= p.rows) continue;
-        const bool bad = is_bad(p.index[row], p.adapters);
-        T* out = static_cast<T*>(p.out) + row * p.out_stride + col;
+        T* out = static_cast<T*>(p.out) + row * p.out_stride;
 #pragma unroll
-        for (int u = 0; u < 4 * NT; u += N) {
+        for (int t = 0; t < NT; t += N / 4) {
+            const int col = col0 + column_of<T, NT>(t, 4 * g);
             float v[N];
 #pragma unroll
-            for (int j = 0; j < N; ++j) v[j] = bad ? std::numeric_limits<float>::quiet_NaN() : acc[i][(u + j) / 4][(u + j) % 4];
-            store_run<N>(out + u, p.cols - col - u, v);
+            for (int j = 0; j < N; ++j) v[j] = acc[i][t + j / 4][j % 4];
+            store_run<N>(out + col, p.cols - col, v);
+        }
+        if (__builtin_expect(is_bad(p.index[row], p.adapters), 0)) {
+            const float none[4] = {std::numeric_limits<float>::quiet_NaN(), std::numeric_limits<float>::quiet_NaN(), std::numeric_limits<float>::quiet_NaN(),
+                                   std::numeric_limits<float>::quiet_NaN()};
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const int col = col0 + column_of<T, NT>(t, 4 * g);
+                store_run<4>(out + col, p.cols - col, none);
+            }
         }
     }
 }
@@ -738,119 +783,128 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_product16(const Product p)
 }
 
 // Single precision on the bf16 matrix instructions: both operands in three parts, exactly, of whose products the six largest are formed
-// (what is left out is below 1.002 2^-24 of a product), small ones first.  The rows' numbers are split here, W's beforehand.  Numbers are
-// brought up by 2^24 first, so that the parts of small ones are normal numbers; sums that are not finite for it, or are not at all, are
-// formed again in single precision.
+// (what is left out is below 1.002 2^-24 of a product), small ones first.  Numbers are brought up by 2^24 first, so that the parts of
+// small ones are normal numbers; sums that are not finite for it, or are not at all, are formed again in single precision.
+// A wavefront has 16 NM rows of its own, which it reads and splits in registers, a step of 32 terms ahead; W's parts, split beforehand, lie
+// in memory as they go into LDS, where the four wavefronts share them.
 template <int NM, int NT>
-__global__ __launch_bounds__(256, 2) void k_product32(const Product p)
+__global__ __launch_bounds__(256, NM == 1 ? 4 : 3) void k_product32(const Product p)
 {
-    constexpr int BM = 32 * NM, BN = 32 * NT, XR = BM * 4 / 256, WR = 3 * BN * 4 / 256;
-    __shared__ __align__(16) unsigned char lds[3 * (BM + BN) * 64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
+    constexpr int BM = 64 * NM, BN = 16 * NT, STAGE = 3 * BN * 64, PER = STAGE / 4096;
+    __shared__ __align__(16) unsigned char lds[2 * STAGE];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
     int rt, ct;
     if (!tile_of(p, rt, ct)) return;
-    const long row0 = (long)rt * BM;
-    const int col0 = ct * BN;
-    const float* from[XR];
-    const bf16* wfrom[WR];
-    int to[XR], wto[WR];
+    const long row0 = (long)rt * BM + wave * 16 * NM;
+    const int col0 = ct * BN, steps = p.k_padded / kPiece;
+    const float* from[NM];
 #pragma unroll
-    for (int u = 0; u < XR; ++u) {
-        const int i = threadIdx.x + 256 * u, r = i / 4;
-        from[u] = static_cast<const float*>(p.in) + min(row0 + r, p.rows - 1) * p.in_stride + 8 * (i & 3);
-        to[u] = r * 64 + 16 * ((i & 3) ^ (r >> 1 & 3));
-    }
-#pragma unroll
-    for (int u = 0; u < WR; ++u) {
-        const int i = threadIdx.x + 256 * u, part = i / (BN * 4), r = i / 4 % BN;
-        wfrom[u] = static_cast<const bf16*>(p.W) + part * p.w_part + (long)min(col0 + r, p.cols - 1) * p.w_stride + 8 * (i & 3);
-        wto[u] = 3 * BM * 64 + part * BN * 64 + r * 64 + 16 * ((i & 3) ^ ((r >> 1 & 1) | (r / (4 * NT) & 1) << 1));
-    }
-    float x[XR][8];
-    bf16x8 w[WR];
+    for (int i = 0; i < NM; ++i) from[i] = static_cast<const float*>(p.in) + min(row0 + 16 * i + n, p.rows - 1) * p.in_stride;
+    const char* w_base = static_cast<const char*>(p.W) + (long)(col0 / kPartRows) * steps * (3 * kPartRows * 64) + col0 % kPartRows * 64;
+    const unsigned lds0 = lds_address(lds) + wave * PER * 1024;
+    f32x4 raw[NM][2];
     auto request = [&](int s) {
-        const int k = s * kPiece;
 #pragma unroll
-        for (int u = 0; u < XR; ++u) load_run<8>(from[u] + k, p.k - k - 8 * (int)(threadIdx.x & 3), x[u]);
+        for (int u = 0; u < PER; ++u) {
+            const int chunk = wave * PER + u, part = chunk / NT;
+            load_into_lds(w_base + (long)s * (3 * kPartRows * 64) + part * kPartRows * 64 + chunk % NT * 1024, lane * 16, lds0 + s % 2 * STAGE + u * 1024);
+        }
+        const int k = s * kPiece + 8 * g;
+        if ((s + 1) * kPiece <= p.k) {
 #pragma unroll
-        for (int u = 0; u < WR; ++u) w[u] = *reinterpret_cast<const bf16x8*>(wfrom[u] + k);
+            for (int i = 0; i < NM; ++i)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) raw[i][h] = *reinterpret_cast<const Run<float, 4>::loose*>(from[i] + k + 4 * h);
+        } else {
+#pragma unroll
+            for (int i = 0; i < NM; ++i)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float x = from[i][min(k + j, p.k - 1)];
+                    raw[i][j / 4][j % 4] = k + j < p.k ? x : 0.0f;
+                }
+        }
+        asm volatile("" ::: "memory");      // (asked for here, not where they are used)
     };
     f32x4 acc[NM][NT];
 #pragma unroll
     for (int i = 0; i < NM; ++i)
 #pragma unroll
         for (int t = 0; t < NT; ++t) acc[i][t] = f32x4{0, 0, 0, 0};
-    const int wm = wave >> 1, wn = wave & 1;
-    const unsigned char* xs = lds + (wm * NM * 16 + n) * 64 + 16 * (g ^ (n >> 1 & 3));
-    const unsigned char* ws = lds + 3 * BM * 64 + (wn * NT * 16 + 4 * NT * (n >> 2) + (n & 3)) * 64 + 16 * (g ^ ((n >> 1 & 1) | (n >> 2 & 1) << 1));
-    const int steps = p.k_padded / kPiece;
+    const unsigned char* ws = lds + n * 64 + 16 * (g ^ (n >> 1 & 3));
     request(0);
+#pragma unroll 1
     for (int s = 0; s < steps; ++s) {
-        __syncthreads();      // everybody has read the step before
-#pragma unroll
-        for (int u = 0; u < XR; ++u) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[u][j] *= kSplitScale;
-            bf16 part[3][8];
-            split(x[u], part);
-#pragma unroll
-            for (int q = 0; q < 3; ++q) {
-                bf16x8 v;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = part[q][j];
-                *reinterpret_cast<bf16x8*>(lds + q * BM * 64 + to[u]) = v;
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < WR; ++u) *reinterpret_cast<bf16x8*>(lds + wto[u]) = w[u];
-        __syncthreads();
-        if (s + 1 < steps) request(s + 1);
-        bf16x8 wf[NT][3];
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int q = 0; q < 3; ++q) wf[t][q] = *reinterpret_cast<const bf16x8*>(ws + q * BN * 64 + t * 256);
+        bf16x8 x[NM][3];
 #pragma unroll
         for (int i = 0; i < NM; ++i) {
-            bf16x8 xf[3];
+            float v[8];
 #pragma unroll
-            for (int q = 0; q < 3; ++q) xf[q] = *reinterpret_cast<const bf16x8*>(xs + q * BM * 64 + i * 1024);
+            for (int j = 0; j < 8; ++j) v[j] = raw[i][j / 4][j % 4] * kSplitScale;
+            bf16 part[3][8];
+            split(v, part);
+#pragma unroll
+            for (int q = 0; q < 3; ++q)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[i][q][j] = part[q][j];
+        }
+        wait_loads<0>();
+        barrier_only();      // this step's parts are there, and everybody has read those of the step before
+        if (s + 1 < steps) request(s + 1);
+        const unsigned char* at = ws + s % 2 * STAGE;
+        // two tiles of columns at a time, the operands of the next two under way
+        bf16x8 w[2][2][3];
+        auto fetch = [&](int t) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int q = 0; q < 3; ++q) w[t / 2 % 2][c][q] = *reinterpret_cast<const bf16x8*>(at + q * BN * 64 + (t + c) * 1024);
+        };
+        fetch(0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
+#pragma unroll
+        for (int t = 0; t < NT; t += 2) {
+            if (t + 2 < NT) fetch(t + 2);
             constexpr int ix[6] = {2, 0, 1, 1, 0, 0}, iw[6] = {0, 2, 1, 0, 1, 0};
 #pragma unroll
             for (int o = 0; o < 6; ++o)
 #pragma unroll
-                for (int t = 0; t < NT; ++t) acc[i][t] = mma(wf[t][iw[o]], xf[ix[o]], acc[i][t]);
+                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                    for (int i = 0; i < NM; ++i) acc[i][t + c] = mma(w[t / 2 % 2][c][iw[o]], x[i][ix[o]], acc[i][t + c]);
+            if (t + 2 < NT) __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, 12 * NM, 0);
         }
     }
     constexpr float kBack = 1.0f / (kSplitScale * kSplitScale);
-    const long row_w = row0 + wm * NM * 16;
-    const int col_w = col0 + wn * NT * 16;
 #pragma unroll
     for (int i = 0; i < NM; ++i) {
-        bool fine = true;
+        float none[4] = {0.0f, 0.0f, 0.0f, 0.0f};      // NaN if a sum is not finite
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
+                none[j] = fmaf(acc[i][t][j], 0.0f, none[j]);
                 acc[i][t][j] *= kBack;
-                fine = fine && fabsf(acc[i][t][j]) <= std::numeric_limits<float>::max();
             }
-        if (__builtin_expect(!fine, 0)) {
-            const float* row = static_cast<const float*>(p.in) + min(row_w + 16 * i + n, p.rows - 1) * p.in_stride;
+        const float any = (none[0] + none[1]) + (none[2] + none[3]);
+        if (__builtin_expect(__any(any != any), 0)) {
+            const float* row = static_cast<const float*>(p.in) + min(row0 + 16 * i + n, p.rows - 1) * p.in_stride;
 #pragma unroll
             for (int t = 0; t < NT; ++t)
+#pragma unroll 1
+                for (int j = 0; j < 4; ++j) {
+                    const float* wc = static_cast<const float*>(p.W0) + min(col0 + 16 * t + 4 * g + j, p.cols - 1) * p.w0_col;
+                    float sum = 0.0f;
+                    for (int k = 0; k < p.k; ++k) sum = fmaf(row[k], wc[k * p.w0_k], sum);
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (!(fabsf(acc[i][t][j]) <= std::numeric_limits<float>::max())) {
-                        const float* wc = static_cast<const float*>(p.W0) + min(col_w + 4 * NT * g + 4 * t + j, p.cols - 1) * p.w0_col;
-                        float sum = 0.0f;
-                        for (int k = 0; k < p.k; ++k) sum = fmaf(row[k], wc[k * p.w0_k], sum);
-                        acc[i][t][j] = sum;
-                    }
+                    for (int c = 0; c < 4; ++c)
+                        if (c == j && !(fabsf(acc[i][t][c]) <= std::numeric_limits<float>::max())) acc[i][t][c] = sum;
+                }
         }
     }
-    add_adapters<float, NM, NT>(p, lane, row_w, col_w, acc);
-    store_tiles<float, NM, NT>(p, lane, row_w, col_w, acc);
+    add_adapters<float, NM, NT>(p, lane, row0, col0, acc);
+    store_tiles<float, NM, NT>(p, lane, row0, col0, acc);
 }
 
 // Few rows: a block takes 16 columns and all rows; eight wavefronts have 128 bytes of W's rows by turns.
@@ -1057,17 +1111,14 @@ struct Call {
         : p(p_), s(s_), arena{static_cast<char*>(base)}, dry(dry_), padded((int)up(p_.rank, 16)) {}
 
     template <typename T>
-    void lay_out(const void* src, long src_each, long src_row, long src_k, void* dst, long part, long rows, int k, int matrices)
+    void lay_out(const void* src, long src_each, long src_row, long src_k, void* dst, bool parts, long rows, int k, int matrices)
     {
         const int k_padded = (int)up(k, kPiece);
-        // (rows in 32 bits)
-        for (long r = 0; r < rows; r += 1 << 30) {
-            if (num_layouts == 2) flush_layouts<T>();
-            const Layout l{static_cast<const T*>(src) + r * src_row, src_each, src_row, src_k, static_cast<T*>(dst) + r * k_padded, rows * k_padded, part,
-                           (int)std::min(1L << 30, rows - r), k, k_padded, matrices};
-            prepare.blocks[num_layouts] = layout_blocks(l);
-            prepare.layout[num_layouts++] = l;
-        }
+        if (num_layouts == 2) flush_layouts<T>();
+        const long padded_rows = parts ? up(rows, kPartRows) : rows;
+        const Layout l{src, src_each, src_row, src_k, dst, padded_rows * k_padded, (int)padded_rows, k, k_padded, matrices, parts, (int)rows};
+        prepare.blocks[num_layouts] = layout_blocks(l);
+        prepare.layout[num_layouts++] = l;
     }
     // launches what is laid out, and the count of rows if it is due
     template <typename T>
@@ -1114,20 +1165,19 @@ struct Call {
         q.rows = p.rows; q.out = out; q.out_stride = out_stride;
         if (few) return q;
         if constexpr (std::is_same_v<T, float>) {
-            q.w_part = (long)cols * q.k_padded;
-            bf16* parts = arena.take<bf16>(3 * q.w_part);
-            lay_out<float>(W, 0, w_col, w_k, parts, q.w_part, cols, k, 1);
-            q.W = parts; q.w_stride = q.k_padded;
+            bf16* parts = arena.take<bf16>(3 * up(cols, kPartRows) * q.k_padded);
+            lay_out<float>(W, 0, w_col, w_k, parts, true, cols, k, 1);
+            q.W = parts;
         } else {
             q.W = W; q.w_stride = w_col;
             if (!(w_k == 1 && as_it_is(W, w_col, k))) {
                 T* laid = arena.take<T>((long)cols * q.k_padded);
-                lay_out<T>(W, 0, w_col, w_k, laid, 0, cols, k, 1);
+                lay_out<T>(W, 0, w_col, w_k, laid, false, cols, k, 1);
                 q.W = laid; q.w_stride = q.k_padded;
             }
             if (!as_it_is(in, in_stride, k)) {
                 T* laid = arena.take<T>(p.rows * q.k_padded);
-                lay_out<T>(in, 0, in_stride, 1, laid, 0, p.rows, k, 1);
+                lay_out<T>(in, 0, in_stride, 1, laid, false, p.rows, k, 1);
                 q.in = laid; q.in_stride = q.k_padded;
             }
         }
@@ -1144,9 +1194,9 @@ struct Call {
             else go(Int<4>{});
             return;
         }
-        auto tiles = [&](int bm, int bn) {
-            q.row_tiles = (int)((p.rows + bm - 1) / bm);
-            q.col_tiles = (q.cols + bn - 1) / bn;
+        auto tiles = [&](int tile_rows, int tile_cols) {
+            q.row_tiles = (int)((q.rows + tile_rows - 1) / tile_rows);
+            q.col_tiles = (q.cols + tile_cols - 1) / tile_cols;
             return (long)q.row_tiles * q.col_tiles;
         };
         auto blocks = [&] {
@@ -1154,11 +1204,28 @@ struct Call {
             refuse_unless(t < 0x7ffffff0L / 8, "more tiles than a launch takes");
             return dim3((unsigned)((t + 7) / 8 * 8));
         };
+        // Tiles that run at once are done at about the same time: where those of the last such round are few, their rows get a launch of
+        // smaller tiles.  (What is left for it is in q then, and whether there is anything.)
+        auto rounds = [&](int tile_rows, int tile_cols, long at_once, auto&& go) {
+            const long all = tiles(tile_rows, tile_cols), over = all % at_once;
+            const long main_rows = all > at_once && over > 0 && over <= at_once / 2 ? (all - over) / q.col_tiles * tile_rows : q.rows;
+            const Product whole = q;
+            q.rows = main_rows;
+            tiles(tile_rows, tile_cols);
+            go();
+            q = whole;
+            q.rows -= main_rows;
+            q.in = static_cast<const T*>(q.in) + main_rows * q.in_stride;
+            q.out = static_cast<T*>(q.out) + main_rows * q.out_stride;
+            q.h += main_rows * q.padded;
+            q.index += main_rows;
+            return q.rows > 0;
+        };
         if constexpr (std::is_same_v<T, float>) {
-            if (tiles(128, 128) >= 256) hipLaunchKernelGGL((k_product32<4, 4>), blocks(), dim3(256), 0, s, q);
+            if (tiles(128, 128) >= 256) hipLaunchKernelGGL((k_product32<2, 8>), blocks(), dim3(256), 0, s, q);
             else {
                 tiles(64, 64);
-                hipLaunchKernelGGL((k_product32<2, 2>), blocks(), dim3(256), 0, s, q);
+                hipLaunchKernelGGL((k_product32<1, 4>), blocks(), dim3(256), 0, s, q);
             }
         } else {
             auto go = [&](auto bm, auto bn, auto wm, auto wn, auto stages) {
@@ -1168,12 +1235,10 @@ struct Call {
                     hip_ok(hipFuncSetAttribute(reinterpret_cast<const void*>(&k_product16<T, BM, BN, WM, WN, S>), hipFuncAttributeMaxDynamicSharedMemorySize, bytes), "LDS");
                 hipLaunchKernelGGL((k_product16<T, BM, BN, WM, WN, S>), blocks(), dim3(64 * WM * WN), bytes, s, q);
             };
-            if (tiles(256, 256) >= 192) go(Int<256>{}, Int<256>{}, Int<2>{}, Int<4>{}, Int<2>{});
-            else if (tiles(128, 128) >= 192) go(Int<128>{}, Int<128>{}, Int<2>{}, Int<2>{}, Int<2>{});
-            else {
-                tiles(64, 64);
-                go(Int<64>{}, Int<64>{}, Int<2>{}, Int<2>{}, Int<3>{});
-            }
+            if (tiles(256, 256) >= 192 && !rounds(256, 256, 256, [&] { go(Int<256>{}, Int<256>{}, Int<2>{}, Int<4>{}, Int<2>{}); })) return;
+            if (tiles(128, 128) >= 192 && !rounds(128, 128, 512, [&] { go(Int<128>{}, Int<128>{}, Int<2>{}, Int<2>{}, Int<2>{}); })) return;
+            tiles(64, 64);
+            go(Int<64>{}, Int<64>{}, Int<2>{}, Int<2>{}, Int<3>{});
         }
     }
 
@@ -1224,7 +1289,7 @@ struct Call {
         T* Bt = nullptr;
         if (want_x || (want_a && rows)) {
             Bt = arena.take<T>((long)n * p.rank * k_padded);
-            if (n) lay_out<T>(B, each_b, 1, p.rank, Bt, 0, p.rank, p.d_out, n);
+            if (n) lay_out<T>(B, each_b, 1, p.rank, Bt, false, p.rank, p.d_out, n);
             down(dy, dy_stride, Bt, (long)p.rank * k_padded, k_padded, p.d_out, g);
         }
         if (want_b && rows) down(x, p.x_stride, A, each_a, p.d_in, p.d_in, h);
