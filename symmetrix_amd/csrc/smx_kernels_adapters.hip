@@ -49,6 +49,21 @@ __device__ __forceinline__ typename Operand<T>::type load_operand(const T* p, lo
     return x;
 }
 
+// 16 rows of 64 bytes, 16 bytes a lane: from lane 4 n + g, where neighbouring lanes have asked for neighbouring bytes of row n, to lane
+// 16 g + n, which has them in an operand.  (Asked for in the order of an operand, with every lane in another row than its neighbours, a
+// load takes about 100 cycles instead of 16, caches or not.)
+template <typename V>
+__device__ __forceinline__ V to_operand(const V& x, int lane)
+{
+    typedef int i32x4 __attribute__((ext_vector_type(4)));
+    const int from = (4 * (lane & 15) + (lane >> 4)) * 4;
+    const i32x4 u = __builtin_bit_cast(i32x4, x);
+    i32x4 v;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = __builtin_amdgcn_ds_bpermute(from, u[j]);
+    return __builtin_bit_cast(V, v);
+}
+
 __device__ __forceinline__ bool has_adapter(int a, int n) { return a >= 0 && a < n; }
 __device__ __forceinline__ bool is_bad(int a, int n) { return a < -1 || a >= n; }
 
@@ -267,13 +282,13 @@ struct Downs {
 };
 
 // A block takes 16 MT rows; its wavefronts have 128 bytes of a row by turns, and their sums are added in order.
-template <typename T, int RT, int MT>
-__global__ __launch_bounds__(256) void k_down(const Downs both)
+template <typename T, int RT, int MT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void k_down(const Downs both)
 {
     constexpr int V = kRun<T>, UNIT = 8 * V;
     typedef typename Operand<T>::type frag;
     __shared__ union {
-        f32x4 part[4][MT * RT][64];
+        f32x4 part[WAVES][MT * RT][64];
         int base[kMostKeys];
     } lds;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
@@ -285,6 +300,9 @@ __global__ __launch_bounds__(256) void k_down(const Downs both)
     const bool second = block >= both.blocks[0];
     if (second) block -= both.blocks[0];
     const Down& p = both.down[second];
+    // the blocks of a die (every eighth) take neighbouring rows, whose factors its L2 holds: rows of one adapter mostly are neighbours
+    block = block % 8 * (both.blocks[second] / 8) + block / 8;
+    if ((long)block * 16 * MT >= p.rows) return;
     long row[MT];
     int a[MT];
     bool good[MT];
@@ -297,85 +315,126 @@ __global__ __launch_bounds__(256) void k_down(const Downs both)
         a[i] = p.index[row[i]];
         good[i] = at < p.rows && has_adapter(a[i], p.adapters);
         left[i] = (unsigned)__ballot(good[i]) & 0xffffu;
-        in[i] = static_cast<const T*>(p.in) + row[i] * p.in_stride + g * V;
+        in[i] = static_cast<const T*>(p.in) + min(((long)block * MT + i) * 16 + lane / 4, p.rows - 1) * p.in_stride + (lane & 3) * V;
         if (at < p.rows && !good[i] && wave == 0)
 #pragma unroll
             for (int q = 0; q < RT; ++q)
                 if (16 * q < p.padded) *reinterpret_cast<f32x4*>(p.h + row[i] * p.padded + 16 * q + 4 * g) = f32x4{0, 0, 0, 0};
     }
-    for (;;) {
-        int cur = -1;
+    // the sums of rows with up to ADAPTERS adapters in one sweep over their numbers
+    auto sweep = [&](auto adapters, const int (&cur)[2]) {
+        constexpr int ADAPTERS = decltype(adapters)::value;
+        f32x4 acc[ADAPTERS][MT][RT];
+        const T* F[ADAPTERS][RT];
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
-            if (cur < 0 && left[i]) cur = __builtin_amdgcn_readlane(a[i], __builtin_ctz(left[i]));
-        if (cur < 0) break;
-        bool mine[MT];
+        for (int c = 0; c < ADAPTERS; ++c) {
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            mine[i] = good[i] && a[i] == cur;
-            left[i] &= ~(unsigned)__ballot(mine[i]);
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int q = 0; q < RT; ++q) acc[c][i][q] = f32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int q = 0; q < RT; ++q) F[c][q] = static_cast<const T*>(p.F) + cur[c] * p.f_each + (long)min(16 * q + lane / 4, p.rank - 1) * p.f_row + (lane & 3) * V;
         }
-        f32x4 acc[MT][RT];
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int q = 0; q < RT; ++q) acc[i][q] = f32x4{0, 0, 0, 0};
-        const T* F[RT];
-#pragma unroll
-        for (int q = 0; q < RT; ++q) F[q] = static_cast<const T*>(p.F) + cur * p.f_each + (long)min(16 * q + n, p.rank - 1) * p.f_row + g * V;
         const int full = p.k / UNIT;
-        int u = wave;
-#pragma unroll 2
-        for (; u < full; u += 4) {
-            const long k = (long)u * UNIT;
-            frag x[MT][2], f[RT][2];
+        struct Unit {
+            frag x[MT][2], f[ADAPTERS][RT][2];
+        };
+        auto fetch = [&](int u, Unit& v) {
+            const long k = (long)min(u, full - 1) * UNIT;
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
 #pragma unroll
-                for (int i = 0; i < MT; ++i) x[i][half] = *reinterpret_cast<const typename Run<T, V>::loose*>(in[i] + k + half * (UNIT / 2));
+                for (int i = 0; i < MT; ++i) v.x[i][half] = *reinterpret_cast<const typename Run<T, V>::loose*>(in[i] + k + half * (UNIT / 2));
 #pragma unroll
-                for (int q = 0; q < RT; ++q) f[q][half] = *reinterpret_cast<const typename Run<T, V>::loose*>(F[q] + k + half * (UNIT / 2));
+                for (int c = 0; c < ADAPTERS; ++c)
+#pragma unroll
+                    for (int q = 0; q < RT; ++q) v.f[c][q][half] = *reinterpret_cast<const typename Run<T, V>::loose*>(F[c][q] + k + half * (UNIT / 2));
             }
+            asm volatile("" ::: "memory");      // (asked for here, not where they are used)
+        };
+        auto sums = [&](const Unit& v) {
 #pragma unroll
-            for (int half = 0; half < 2; ++half)
+            for (int half = 0; half < 2; ++half) {
+                frag x[MT];
 #pragma unroll
-                for (int i = 0; i < MT; ++i)
+                for (int i = 0; i < MT; ++i) x[i] = to_operand(v.x[i][half], lane);
 #pragma unroll
-                    for (int q = 0; q < RT; ++q) acc[i][q] = mma(f[q][half], x[i][half], acc[i][q]);
+                for (int c = 0; c < ADAPTERS; ++c)
+#pragma unroll
+                    for (int q = 0; q < RT; ++q) {
+                        const frag f = to_operand(v.f[c][q][half], lane);
+#pragma unroll
+                        for (int i = 0; i < MT; ++i) acc[c][i][q] = mma(f, x[i], acc[c][i][q]);
+                    }
+            }
+        };
+        int u = wave;
+        if (u < full) {
+            Unit even, odd;
+            fetch(u, even);
+#pragma unroll 1
+            for (;;) {
+                fetch(u + WAVES, odd);
+                sums(even);
+                if ((u += WAVES) >= full) break;
+                fetch(u + WAVES, even);
+                sums(odd);
+                if ((u += WAVES) >= full) break;
+            }
         }
         if (u == full && p.k % UNIT) {      // (the end of the rows, for one wavefront)
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                const int k = full * UNIT + half * (UNIT / 2), rest = p.k - k - g * V;
+                const int k = full * UNIT + half * (UNIT / 2), rest = p.k - k - (lane & 3) * V;
                 frag x[MT];
 #pragma unroll
-                for (int i = 0; i < MT; ++i) x[i] = load_operand(in[i] + k, rest);
+                for (int i = 0; i < MT; ++i) x[i] = to_operand(load_operand(in[i] + k, rest), lane);
 #pragma unroll
-                for (int q = 0; q < RT; ++q) {
-                    const frag f = load_operand(F[q] + k, rest);
+                for (int c = 0; c < ADAPTERS; ++c)
 #pragma unroll
-                    for (int i = 0; i < MT; ++i) acc[i][q] = mma(f, x[i], acc[i][q]);
-                }
+                    for (int q = 0; q < RT; ++q) {
+                        const frag f = to_operand(load_operand(F[c][q] + k, rest), lane);
+#pragma unroll
+                        for (int i = 0; i < MT; ++i) acc[c][i][q] = mma(f, x[i], acc[c][i][q]);
+                    }
             }
         }
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
+        for (int c = 0; c < ADAPTERS; ++c) {
 #pragma unroll
-            for (int q = 0; q < RT; ++q) lds.part[wave][i * RT + q][lane] = acc[i][q];
-        __syncthreads();
-        const float c = p.scale ? p.scale[cur] : 1.0f;
+            for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int at = 0; at < MT * RT; ++at) {
-            if (at % 4 != wave) continue;
-            const int i = at / RT, q = at % RT;
-            f32x4 sum = lds.part[0][at][lane];
+                for (int q = 0; q < RT; ++q) lds.part[wave][i * RT + q][lane] = acc[c][i][q];
+            __syncthreads();
+            const float scale = p.scale ? p.scale[cur[c]] : 1.0f;
 #pragma unroll
-            for (int w = 1; w < 4; ++w) sum += lds.part[w][at][lane];
+            for (int at = 0; at < MT * RT; ++at) {
+                if (at % WAVES != wave) continue;
+                const int i = at / RT, q = at % RT;
+                f32x4 sum = lds.part[0][at][lane];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) sum[j] = 16 * q + 4 * g + j < p.rank ? sum[j] * c : 0.0f;
-            if (mine[i] && 16 * q < p.padded) *reinterpret_cast<f32x4*>(p.h + row[i] * p.padded + 16 * q + 4 * g) = sum;
+                for (int w = 1; w < WAVES; ++w) sum += lds.part[w][at][lane];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) sum[j] = 16 * q + 4 * g + j < p.rank ? sum[j] * scale : 0.0f;
+                if (good[i] && a[i] == cur[c] && 16 * q < p.padded) *reinterpret_cast<f32x4*>(p.h + row[i] * p.padded + 16 * q + 4 * g) = sum;
+            }
+            __syncthreads();
         }
-        __syncthreads();
+    };
+    auto next = [&] {
+        int cur = -1;
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+            if (cur < 0 && left[i]) cur = __builtin_amdgcn_readlane(a[i], __builtin_ctz(left[i]));
+#pragma unroll
+        for (int i = 0; i < MT; ++i) left[i] &= ~(unsigned)__ballot(good[i] && a[i] == cur);
+        return cur;
+    };
+    // (two at a time: the blocks in which one adapter's rows end and another's begin would be the last ones otherwise)
+    for (int cur[2] = {next(), 0}; cur[0] >= 0; cur[0] = next()) {
+        cur[1] = next();
+        if (cur[1] >= 0) sweep(std::integral_constant<int, 2>{}, cur);
+        else sweep(std::integral_constant<int, 1>{}, cur);
     }
 }
 
@@ -1140,17 +1199,18 @@ struct Call {
     void flush_downs(bool place)
     {
         if (dry) return;
-        auto go = [&](auto rt, auto mt) {
-            constexpr int RT = decltype(rt)::value, MT = decltype(mt)::value;
-            for (int i = 0; i < num_downs; ++i) downs.blocks[i] = (int)((p.rows + 16 * MT - 1) / (16 * MT));
+        auto go = [&](auto rt, auto mt, auto waves) {
+            constexpr int RT = decltype(rt)::value, MT = decltype(mt)::value, WAVES = decltype(waves)::value;
+            for (int i = 0; i < num_downs; ++i) downs.blocks[i] = (int)up((p.rows + 16 * MT - 1) / (16 * MT), 8);
             const long blocks = (long)downs.blocks[0] + downs.blocks[1] + (place ? downs.groups.blocks : 0);
             refuse_unless(blocks <= 0x7fffffffL, "more blocks than a launch takes");
-            if (blocks) hipLaunchKernelGGL((k_down<T, RT, MT>), dim3((unsigned)blocks), dim3(256), 0, s, downs);
+            if (blocks) hipLaunchKernelGGL((k_down<T, RT, MT, WAVES>), dim3((unsigned)blocks), dim3(64 * WAVES), 0, s, downs);
         };
-        if (padded == 16) go(Int<1>{}, Int<2>{});
-        else if (padded == 32) go(Int<2>{}, Int<2>{});
-        else if (padded <= 64) go(Int<4>{}, Int<2>{});
-        else go(Int<8>{}, Int<1>{});
+        const bool few_blocks = p.rows / 16 * num_downs < 4096 && downs.down[0].k >= 1024;
+        if (padded == 16) few_blocks ? go(Int<1>{}, Int<2>{}, Int<8>{}) : go(Int<1>{}, Int<2>{}, Int<4>{});
+        else if (padded == 32) few_blocks ? go(Int<2>{}, Int<2>{}, Int<8>{}) : go(Int<2>{}, Int<2>{}, Int<4>{});
+        else if (padded <= 64) few_blocks ? go(Int<4>{}, Int<1>{}, Int<8>{}) : go(Int<4>{}, Int<2>{}, Int<4>{});
+        else go(Int<8>{}, Int<1>{}, Int<4>{});
     }
 
     // out[rows][cols] = in W^T + adapters' part; W(col, k) = W[col * w_col + k * w_k], F(col, r) = F[a][col * f_col + r * f_r].
