@@ -64,6 +64,19 @@ __device__ __forceinline__ V to_operand(const V& x, int lane)
     return __builtin_bit_cast(V, v);
 }
 
+// and back: what lane 16 g + n has of row n goes to lane 4 n + g
+template <typename V>
+__device__ __forceinline__ V from_operand(const V& x, int lane)
+{
+    typedef int i32x4 __attribute__((ext_vector_type(4)));
+    const int from = (16 * (lane & 3) + (lane >> 2)) * 4;
+    const i32x4 u = __builtin_bit_cast(i32x4, x);
+    i32x4 v;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = __builtin_amdgcn_ds_bpermute(from, u[j]);
+    return __builtin_bit_cast(V, v);
+}
+
 __device__ __forceinline__ bool has_adapter(int a, int n) { return a >= 0 && a < n; }
 __device__ __forceinline__ bool is_bad(int a, int n) { return a < -1 || a >= n; }
 
@@ -500,6 +513,11 @@ __device__ __forceinline__ bool tile_of(const Product& p, int& rt, int& ct)
     return true;
 }
 
+// Lane (n, g) holds of tile (i, t) row i * 16 + n and four columns: in single precision 16 t + 4 g + 0..3; in 16 bits 8 g + 4 (t % 2) + 0..3 of
+// the 32 columns of two tiles, so that a lane has eight neighbours of them to store.
+template <typename T>
+__device__ __forceinline__ int column_of(int t, int m) { return std::is_same_v<T, float> ? 16 * t + m : 32 * (t >> 1) + 8 * (m >> 2) + 4 * (t & 1) + (m & 3); }
+
 // The product of a factor's columns and rows of h, 32 r at a time (single precision: 16).  Sixteen bits: on the bf16 instructions, h in two
 // bf16 parts (what is left out is below 2^-16 of a product; the result is rounded to 2^-9 or 2^-11), and numbers of float16 in two, which
 // hold them exactly.
@@ -523,21 +541,25 @@ struct AdapterProduct {
             part[1][j] = l[0]; part[1][j + 1] = l[1];
         }
     }
-    // F(r) at from + r * stride, r = r0 + 8 g + 0..7; runs: eight numbers of a rank that is a multiple of eight, side by side.  (No branch
-    // depends on the lane, here and below: what is behind the rank is read from its end and put to zero.)
-    __device__ static __forceinline__ Factor factor(const T* from, long stride, bool runs, int r0, int g, int rank)
+    // F(col, r) = base[col * f_col + r * f_r] for the columns of a tile, r = r0 + 8 g + 0..7; eight numbers at a time where they are side by side
+    // and the rank is a multiple of eight.  (No branch depends on the lane, here and below: what is behind the rank is read from its end and
+    // put to zero.)
+    __device__ static __forceinline__ Factor factor(const Product& p, const T* base, int col0, int t, int r0, int lane)
     {
-        const int r = r0 + 8 * g;
         typename Operand<T>::type v;
-        if (runs) {
-            v = *reinterpret_cast<const typename Run<T, 8>::loose*>(from + min(r, rank - 8));
+        if (p.f_runs) {
+            const int r = r0 + 8 * (lane & 3);
+            v = *reinterpret_cast<const typename Run<T, 8>::loose*>(base + min(col0 + column_of<T>(t, lane >> 2), p.cols - 1) * p.f_col + min(r, p.rank - 8));
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = r < rank ? v[j] : (T)0.0f;
+            for (int j = 0; j < 8; ++j) v[j] = r < p.rank ? v[j] : (T)0.0f;
+            v = to_operand(v, lane);
         } else {
+            const int r = r0 + 8 * (lane >> 4);
+            const T* from = base + min(col0 + column_of<T>(t, lane & 15), p.cols - 1) * p.f_col;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const T x = from[min(r + j, rank - 1) * stride];
-                v[j] = r + j < rank ? x : (T)0.0f;
+                const T x = from[min(r + j, p.rank - 1) * p.f_r];
+                v[j] = r + j < p.rank ? x : (T)0.0f;
             }
         }
         Factor f;
@@ -553,82 +575,97 @@ struct AdapterProduct {
     struct Row {
         bf16x8 part[2];
     };
-    __device__ static __forceinline__ Row row(const float* h, int r0, int g, int padded, int)
+    // h of the rows of a tile
+    __device__ static __forceinline__ Row row(const Product& p, long row0, int r0, int lane)
     {
-        const int r = r0 + 8 * g;
-        const f32x4* from = reinterpret_cast<const f32x4*>(h + min(r, padded - 8));
-        const f32x4 u = from[0], v = from[1];
-        float x[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = r < padded ? (j < 4 ? u[j % 4] : v[j % 4]) : 0.0f;
+        const int r = r0 + 8 * (lane & 3);
+        const f32x4* from = reinterpret_cast<const f32x4*>(p.h + min(row0 + lane / 4, p.rows - 1) * p.padded + min(r, p.padded - 8));
+        f32x4 u = from[0], v = from[1];
+        if (r >= p.padded) u = v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        u = to_operand(u, lane);
+        v = to_operand(v, lane);
+        const float x[8] = {u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]};
         Row both;
         parts_of(x, both.part);
         return both;
     }
-    __device__ static __forceinline__ f32x4 run(const Factor& f, const Row& h, f32x4 c, int, int)
+    __device__ static __forceinline__ f32x4 run(const Factor& f, const Row& h, f32x4 c)
     {
         c = mma(f.part[0], h.part[1], c);
         if constexpr (F_PARTS == 2) c = mma(f.part[1], h.part[0], c);
         return mma(f.part[0], h.part[0], c);
     }
 };
-template <>
-struct AdapterProduct<float> {
-    static constexpr int CHUNK = 16;
-    // Of the r of a chunk lane g has EACH neighbours (1, 2 or 4, for as many instructions): r0 + EACH g + 0..EACH-1, one load where they are
-    // all there.
-    __device__ static __forceinline__ int each(int r0, int rank) { return rank - r0 <= 4 ? 1 : (rank - r0 <= 8 ? 2 : 4); }
-    struct Factor {
-        f32x4 x;
-    };
-    typedef Factor Row;
-    __device__ static __forceinline__ Factor factor(const float* from, long stride, bool, int r0, int g, int rank)
-    {
-        const int e = each(r0, rank), r = r0 + e * g;
-        Factor f;
-        if (stride == 1 && rank - r0 >= 16) f.x = *reinterpret_cast<const Run<float, 4>::loose*>(from + r);
-        else if (stride == 1 && rank - r0 == 8) {
-            const Run<float, 2>::type v = *reinterpret_cast<const Run<float, 2>::loose*>(from + r);
-            f.x = f32x4{v[0], v[1], 0.0f, 0.0f};
-        } else {
+// In single precision for NM tiles of rows that all belong to adapter a, sixteen r at a time: lane g has four of them, or where the rest of the
+// rank is 8 or 4, so that half or three quarters would be zeros, two or one, for as many instructions.
+__device__ __forceinline__ f32x4 deal(f32x4 x, int e, int lane)
+{
+    if (e == 4) return to_operand(x, lane);
+    const int n = lane & 15, g = lane >> 4, from = (4 * n + (e == 2 ? g >> 1 : 0)) * 4;
+    f32x4 y;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                f.x[j] = 0.0f;
-                if (j >= e) continue;
-                const float x = from[min(r + j, rank - 1) * stride];
-                f.x[j] = r + j < rank ? x : 0.0f;
+    for (int j = 0; j < 4; ++j) y[j] = __int_as_float(__builtin_amdgcn_ds_bpermute(from, __float_as_int(x[j])));
+    if (e == 2) return g & 1 ? f32x4{y[2], y[3], 0.0f, 0.0f} : f32x4{y[0], y[1], 0.0f, 0.0f};
+    return f32x4{g & 2 ? (g & 1 ? y[3] : y[2]) : (g & 1 ? y[1] : y[0]), 0.0f, 0.0f, 0.0f};
+}
+template <int NM, int NT>
+__device__ __forceinline__ void add_adapter(const Product& p, int lane, long row0, int col0, int a, f32x4 (&acc)[NM][NT])
+{
+    const int n = lane & 15, g = lane >> 4;
+    const float* F = static_cast<const float*>(p.F) + a * p.f_each;
+    const bool runs = p.f_r == 1 && p.rank % 4 == 0;
+#pragma unroll 1
+    for (int r0 = 0; r0 < p.rank; r0 += 16) {
+        const int e = p.rank - r0 == 4 ? 1 : (p.rank - r0 == 8 ? 2 : 4), r = r0 + 4 * (lane & 3);
+        f32x4 h[NM], f[NT];
+#pragma unroll
+        for (int i = 0; i < NM; ++i) h[i] = *reinterpret_cast<const f32x4*>(p.h + min(row0 + 16 * i + lane / 4, p.rows - 1) * p.padded + r);
+        if (runs) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+                f[t] = *reinterpret_cast<const Run<float, 4>::loose*>(F + min(col0 + 16 * t + lane / 4, p.cols - 1) * p.f_col + min(r, p.rank - 4));
+        } else {      // (the instructions' own order)
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) f[t][j] = F[min(col0 + 16 * t + n, p.cols - 1) * p.f_col + min(r0 + e * g + j, p.rank - 1) * p.f_r];
+        }
+#pragma unroll
+        for (int i = 0; i < NM; ++i) h[i] = deal(h[i], e, lane);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            if (runs) {
+                if (r >= p.rank) f[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                f[t] = deal(f[t], e, lane);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) f[t][j] = r0 + e * g + j < p.rank ? f[t][j] : 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < NM; ++i) {
+                acc[i][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(f[t][0], h[i][0], acc[i][t], 0, 0, 0);
+                if (e >= 2) acc[i][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(f[t][1], h[i][1], acc[i][t], 0, 0, 0);
+                if (e == 4) {
+                    acc[i][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(f[t][2], h[i][2], acc[i][t], 0, 0, 0);
+                    acc[i][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(f[t][3], h[i][3], acc[i][t], 0, 0, 0);
+                }
             }
         }
-        return f;
     }
-    __device__ static __forceinline__ Row row(const float* h, int r0, int g, int, int rank)
-    {
-        const int e = each(r0, rank);
-        Row v;
-        if (e == 4) v.x = *reinterpret_cast<const f32x4*>(h + r0 + 4 * g);
-        else if (e == 2) {
-            const Run<float, 2>::type u = *reinterpret_cast<const Run<float, 2>::type*>(h + r0 + 2 * g);
-            v.x = f32x4{u[0], u[1], 0.0f, 0.0f};
-        } else v.x = f32x4{h[r0 + g], 0.0f, 0.0f, 0.0f};
-        return v;
-    }
-    __device__ static __forceinline__ f32x4 run(const Factor& f, const Row& h, f32x4 c, int r0, int rank)
-    {
-        const int e = each(r0, rank);
-        c = __builtin_amdgcn_mfma_f32_16x16x4f32(f.x[0], h.x[0], c, 0, 0, 0);
-        if (e >= 2) c = __builtin_amdgcn_mfma_f32_16x16x4f32(f.x[1], h.x[1], c, 0, 0, 0);
-        if (e == 4) {
-            c = __builtin_amdgcn_mfma_f32_16x16x4f32(f.x[2], h.x[2], c, 0, 0, 0);
-            c = __builtin_amdgcn_mfma_f32_16x16x4f32(f.x[3], h.x[3], c, 0, 0, 0);
-        }
-        return c;
-    }
-};
-
-// Lane (n, g) holds of tile (i, t) row i * 16 + n and four columns.  In 16 bits these are 4 NT g + 4 t + 0..3, so that a lane has 4 NT
-// neighbours to store; in single precision 16 t + 4 g + 0..3.
-template <typename T, int NT>
-__device__ __forceinline__ int column_of(int t, int m) { return std::is_same_v<T, float> ? 16 * t + m : 4 * NT * (m >> 2) + 4 * t + (m & 3); }
+}
+// The adapter of all rows of NM tiles (-1: all have none; -2: they differ).  A row behind the last one has the last one's.
+template <int NM>
+__device__ __forceinline__ int one_adapter(const Product& p, int lane, long row0)
+{
+    int a[NM];
+#pragma unroll
+    for (int i = 0; i < NM; ++i) a[i] = p.index[min(row0 + 16 * i + (lane & 15), p.rows - 1)];
+    const int first = __builtin_amdgcn_readfirstlane(a[0]);
+    bool same = true;
+#pragma unroll
+    for (int i = 0; i < NM; ++i) same = same && a[i] == first;
+    return __all(same) ? (has_adapter(first, p.adapters) ? first : -1) : -2;
+}
 
 // Adds the adapters' part to sums of NM tiles of 16 rows and NT of 16 columns.  For every tile of rows one adapter after the other of
 // those that occur in it, four tiles of columns at a time; a factor that is held as a whole stays for the next tile of rows.
@@ -637,11 +674,10 @@ __device__ __forceinline__ void add_adapters(const Product& p, int lane, long ro
 {
     typedef AdapterProduct<T> Op;
     constexpr int GT = NT < 4 ? NT : 4;
-    const int n = lane & 15, g = lane >> 4;
+    const int n = lane & 15;
     __builtin_amdgcn_sched_barrier(0);
-    const float* h = p.h + min(row0 + n, p.rows - 1) * p.padded;
     int a = p.index[min(row0 + n, p.rows - 1)];
-    typename Op::Row first = Op::row(h, 0, g, p.padded, p.rank);
+    typename Op::Row first = Op::row(p, row0, 0, lane);
     int held = -1;
     typename Op::Factor f[GT];
 #pragma unroll
@@ -654,19 +690,18 @@ __device__ __forceinline__ void add_adapters(const Product& p, int lane, long ro
             const unsigned whose = (unsigned)__ballot(mine) & 0xffffu;
             left &= ~whose;
             for (int r0 = 0; r0 < p.rank; r0 += Op::CHUNK) {
-                const typename Op::Row hr = r0 == 0 ? first : Op::row(h, r0, g, p.padded, p.rank);
+                const typename Op::Row hr = r0 == 0 ? first : Op::row(p, row0 + 16 * i, r0, lane);
 #pragma unroll
                 for (int t0 = 0; t0 < NT; t0 += GT) {
                     if (NT > GT || cur != held || r0 > 0) {
 #pragma unroll
                         for (int t = 0; t < GT; ++t)
-                            f[t] = Op::factor(static_cast<const T*>(p.F) + cur * p.f_each + min(col0 + column_of<T, NT>(t0 + t, n), p.cols - 1) * p.f_col, p.f_r, p.f_runs, r0,
-                                              g, p.rank);
+                            f[t] = Op::factor(p, static_cast<const T*>(p.F) + cur * p.f_each, col0, t0 + t, r0, lane);
                         held = p.rank <= Op::CHUNK ? cur : -1;
                     }
 #pragma unroll
                     for (int t = 0; t < GT; ++t) {
-                        const f32x4 sum = Op::run(f[t], hr, f32x4{0, 0, 0, 0}, r0, p.rank);
+                        const f32x4 sum = Op::run(f[t], hr, f32x4{0, 0, 0, 0});
 #pragma unroll
                         for (int j = 0; j < 4; ++j) acc[i][t0 + t][j] += mine ? sum[j] : 0.0f;
                     }
@@ -675,9 +710,8 @@ __device__ __forceinline__ void add_adapters(const Product& p, int lane, long ro
             }
         }
         if (i + 1 < NM) {
-            h = p.h + min(row0 + 16 * (i + 1) + n, p.rows - 1) * p.padded;
             a = p.index[min(row0 + 16 * (i + 1) + n, p.rows - 1)];
-            first = Op::row(h, 0, g, p.padded, p.rank);
+            first = Op::row(p, row0 + 16 * (i + 1), 0, lane);
         }
         __builtin_amdgcn_sched_barrier(0);
     }
@@ -685,30 +719,30 @@ __device__ __forceinline__ void add_adapters(const Product& p, int lane, long ro
 template <typename T, int NM, int NT>
 __device__ __forceinline__ void store_tiles(const Product& p, int lane, long row0, int col0, const f32x4 (&acc)[NM][NT])
 {
-    constexpr int N = std::is_same_v<T, float> || NT == 1 ? 4 : 8;
-    const int n = lane & 15, g = lane >> 4;
+    // (64 bytes of a row by four neighbouring lanes)
+    constexpr int STEP = std::is_same_v<T, float> ? 1 : 2, N = 4 * STEP;
 #pragma unroll
     for (int i = 0; i < NM; ++i) {
-        const long row = row0 + 16 * i + n;
-        if (row >= p.rows) continue;
+        const long row = row0 + 16 * i + lane / 4;
+        const bool live = row < p.rows;
         T* out = static_cast<T*>(p.out) + row * p.out_stride;
 #pragma unroll
-        for (int t = 0; t < NT; t += N / 4) {
-            const int col = col0 + column_of<T, NT>(t, 4 * g);
-            float v[N];
+        for (int t = 0; t < NT; t += STEP) {
+            typename Run<T, N>::type v;
 #pragma unroll
-            for (int j = 0; j < N; ++j) v[j] = acc[i][t + j / 4][j % 4];
-            store_run<N>(out + col, p.cols - col, v);
-        }
-        if (__builtin_expect(is_bad(p.index[row], p.adapters), 0)) {
-            const float none[4] = {std::numeric_limits<float>::quiet_NaN(), std::numeric_limits<float>::quiet_NaN(), std::numeric_limits<float>::quiet_NaN(),
-                                   std::numeric_limits<float>::quiet_NaN()};
+            for (int j = 0; j < N; ++j) v[j] = (T)acc[i][t + j / 4][j % 4];
+            v = from_operand(v, lane);
+            const int col = col0 + 16 * t + N * (lane & 3);
+            if (!live) continue;
+            if (p.cols - col >= N) *reinterpret_cast<typename Run<T, N>::loose*>(out + col) = v;
+            else {
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                const int col = col0 + column_of<T, NT>(t, 4 * g);
-                store_run<4>(out + col, p.cols - col, none);
+                for (int j = 0; j < N; ++j)
+                    if (col + j < p.cols) out[col + j] = v[j];
             }
         }
+        if (__builtin_expect(live && is_bad(p.index[row], p.adapters), 0))
+            for (int c = col0 + (lane & 3); c < min(col0 + 16 * NT, p.cols); c += 4) out[c] = (T)std::numeric_limits<float>::quiet_NaN();
     }
 }
 
@@ -741,7 +775,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_product16(const Product p)
             from[u] = (unsigned)(2 * min((long)r, p.rows - 1 - row0) * p.in_stride) + 16 * piece;
         } else {
             const int r = (chunk - BM / 8) * 8 + lane / 8;
-            piece = (lane & 7) ^ ((r & 3) | (r / (4 * NT) & 1) << 2);
+            piece = (lane & 7) ^ ((r & 3) | (r >> 3 & 1) << 2);
             from[u] = (unsigned)(2 * min(r, p.cols - 1 - col0) * p.w_stride) + 16 * piece;
         }
         second |= (unsigned)(piece >> 2) << u;
@@ -775,7 +809,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_product16(const Product p)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         xs[h] = lds + (wm * NM * 16 + n) * 128 + 16 * ((4 * h + g) ^ (n & 7));
-        ws[h] = lds + (BM + wn * NT * 16 + 4 * NT * (n >> 2) + (n & 3)) * 128 + 16 * ((4 * h + g) ^ ((n & 3) | (n >> 2 & 1) << 2));
+        ws[h] = lds + (BM + wn * NT * 16 + column_of<T>(0, n)) * 128 + 16 * ((4 * h + g) ^ ((n & 3) | (n >> 2 & 1) << 2));
     }
     struct Frags {
         frag x[NM], w[NT];
@@ -783,7 +817,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_product16(const Product p)
     auto fetch = [&](int s, int h, Frags& f) {
         const int at = s % STAGES * STAGE;
 #pragma unroll
-        for (int t = 0; t < NT; ++t) f.w[t] = *reinterpret_cast<const frag*>(ws[h] + at + t * 512);
+        for (int t = 0; t < NT; ++t) f.w[t] = *reinterpret_cast<const frag*>(ws[h] + at + column_of<T>(t, 0) * 128);
 #pragma unroll
         for (int i = 0; i < NM; ++i) f.x[i] = *reinterpret_cast<const frag*>(xs[h] + at + i * 2048);
     };
@@ -962,8 +996,60 @@ __global__ __launch_bounds__(256, NM == 1 ? 4 : 3) void k_product32(const Produc
                 }
         }
     }
-    add_adapters<float, NM, NT>(p, lane, row0, col0, acc);
+    const int one = one_adapter<NM>(p, lane, row0);
+    if (one >= 0) add_adapter<NM, NT>(p, lane, row0, col0, one, acc);
     store_tiles<float, NM, NT>(p, lane, row0, col0, acc);
+}
+
+// Where the rows of a wavefront of k_product32 have different adapters, their part is added here, to the stored sums: a block takes
+// eight of the `group` rows of one, a lane a column.  (A launch of its own: the registers for it would cost k_product32 a
+// block on every CU, and the few tiles that are mixed where requests are runs of rows would be its last ones: 95 us against 80 and 8,
+// 50 000 rows of 256 numbers, 512 columns, 12 adapters of rank 8.)
+__global__ __launch_bounds__(256) void k_add_mixed(const Product p, int group)
+{
+    const int lane = threadIdx.x & 63;
+    const long row0 = (long)blockIdx.x * group;
+    const int mine = p.index[min(row0 + lane % group, p.rows - 1)];
+    if (__all(mine == __builtin_amdgcn_readfirstlane(mine))) return;
+    const int col = blockIdx.y * 256 + threadIdx.x;
+    if (col >= p.cols) return;
+    const bool runs = p.f_r == 1 && p.rank % 4 == 0;
+    float* out = static_cast<float*>(p.out) + col;
+    const float* F0 = static_cast<const float*>(p.F) + col * p.f_col;
+    {
+        const int i0 = 8 * blockIdx.z;
+        float y[8], sum[8];
+        const float* F[8];
+        const float* h[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const long row = min(row0 + i0 + u, p.rows - 1);
+            const int a = __builtin_amdgcn_readlane(mine, i0 + u);
+            F[u] = F0 + (has_adapter(a, p.adapters) ? a : 0) * p.f_each;
+            h[u] = p.h + row * p.padded;
+            y[u] = out[row * p.out_stride];
+            sum[u] = 0.0f;
+        }
+#pragma unroll 1
+        for (int r = 0; r < p.rank; r += 4) {
+            f32x4 f[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                if (runs) f[u] = *reinterpret_cast<const Run<float, 4>::loose*>(F[u] + r);
+                else {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) f[u][q] = F[u][min(r + q, p.rank - 1) * p.f_r];
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) sum[u] = r + q < p.rank ? fmaf(h[u][r + q], f[u][q], sum[u]) : sum[u];
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            if (row0 + i0 + u < p.rows && has_adapter(__builtin_amdgcn_readlane(mine, i0 + u), p.adapters)) out[(row0 + i0 + u) * p.out_stride] = y[u] + sum[u];
+    }
 }
 
 // Few rows: a block takes 16 columns and all rows; eight wavefronts have 128 bytes of W's rows by turns.
@@ -1282,11 +1368,15 @@ struct Call {
             return q.rows > 0;
         };
         if constexpr (std::is_same_v<T, float>) {
-            if (tiles(128, 128) >= 256) hipLaunchKernelGGL((k_product32<2, 8>), blocks(), dim3(256), 0, s, q);
+            const bool wide = tiles(128, 128) >= 256;
+            if (wide) hipLaunchKernelGGL((k_product32<2, 8>), blocks(), dim3(256), 0, s, q);
             else {
                 tiles(64, 64);
                 hipLaunchKernelGGL((k_product32<1, 4>), blocks(), dim3(256), 0, s, q);
             }
+            const int group = wide ? 32 : 16;
+            if (p.num_adapters)
+                hipLaunchKernelGGL(k_add_mixed, dim3((unsigned)((q.rows + group - 1) / group), (q.cols + 255) / 256, group / 8), dim3(256), 0, s, q, group);
         } else {
             auto go = [&](auto bm, auto bn, auto wm, auto wn, auto stages) {
                 constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value, WM = decltype(wm)::value, WN = decltype(wn)::value, S = decltype(stages)::value;
