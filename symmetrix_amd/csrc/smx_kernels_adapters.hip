@@ -1057,23 +1057,65 @@ template <typename T, int MT>
 __global__ __launch_bounds__(512) void k_product_few(const Product p)
 {
     constexpr int V = kRun<T>, UNIT = 8 * V;
+    typedef typename Operand<T>::type frag;
     __shared__ f32x4 part[8][MT][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4, col0 = blockIdx.x * 16;
-    const T* W = static_cast<const T*>(p.W0) + (long)min(col0 + n, p.cols - 1) * p.w0_col;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col0 = blockIdx.x * 16, mine = (lane & 3) * V;
+    const T* W = static_cast<const T*>(p.W0) + (long)min(col0 + lane / 4, p.cols - 1) * p.w0_col + mine;
     const T* in[MT];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) in[i] = static_cast<const T*>(p.in) + min(16L * i + n, p.rows - 1) * p.in_stride;
+    for (int i = 0; i < MT; ++i) in[i] = static_cast<const T*>(p.in) + min(16L * i + lane / 4, p.rows - 1) * p.in_stride + mine;
     f32x4 acc[MT];
 #pragma unroll
     for (int i = 0; i < MT; ++i) acc[i] = f32x4{0, 0, 0, 0};
-    for (int k0 = wave * UNIT; k0 < p.k; k0 += 8 * UNIT)
+    struct Unit {
+        frag w[2], x[MT][2];
+    };
+    const int full = p.k / UNIT;
+    auto fetch = [&](int u, Unit& v) {
+        const long k = (long)min(u, full - 1) * UNIT;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int k = k0 + u * (UNIT / 2) + g * V;
-            const auto w = load_operand(W + k, p.k - k);
+        for (int half = 0; half < 2; ++half) {
+            v.w[half] = *reinterpret_cast<const typename Run<T, V>::loose*>(W + k + half * (UNIT / 2));
 #pragma unroll
-            for (int i = 0; i < MT; ++i) acc[i] = mma(w, load_operand(in[i] + k, p.k - k), acc[i]);
+            for (int i = 0; i < MT; ++i) v.x[i][half] = *reinterpret_cast<const typename Run<T, V>::loose*>(in[i] + k + half * (UNIT / 2));
         }
+        asm volatile("" ::: "memory");      // (asked for here, not where they are used)
+    };
+    auto sums = [&](const Unit& v) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const frag w = to_operand(v.w[half], lane);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) acc[i] = mma(w, to_operand(v.x[i][half], lane), acc[i]);
+        }
+    };
+    int u = wave;
+    if (u < full) {
+        Unit unit[4];
+#pragma unroll
+        for (int q = 0; q < 3; ++q) fetch(u + 8 * q, unit[q]);
+#pragma unroll 1
+        for (;;) {
+            bool done = false;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                if (done) continue;
+                fetch(u + 24, unit[(q + 3) % 4]);
+                sums(unit[q]);
+                done = (u += 8) >= full;
+            }
+            if (done) break;
+        }
+    }
+    if (wave == full % 8 && p.k % UNIT) {      // (the end of the rows)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int k = full * UNIT + half * (UNIT / 2);
+            const frag w = to_operand(load_operand(W + k, p.k - k - mine), lane);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) acc[i] = mma(w, to_operand(load_operand(in[i] + k, p.k - k - mine), lane), acc[i]);
+        }
+    }
 #pragma unroll
     for (int i = 0; i < MT; ++i) part[wave][i][lane] = acc[i];
     __syncthreads();
