@@ -7,6 +7,8 @@ differentiation.  Wrong arguments raise ValueError (TypeError for element types)
 from __future__ import annotations
 
 import ctypes as C
+import functools
+import struct
 
 import torch
 
@@ -19,14 +21,22 @@ MAX_ADAPTERS = 4096
 
 
 class _Adapted(C.Structure):
+    """smx_adapted_linear"""
     _fields_ = [("type", C.c_int), ("d_in", C.c_int), ("d_out", C.c_int), ("rank", C.c_int), ("num_adapters", C.c_int), ("rows", C.c_long),
                 ("x", C.c_void_p), ("x_stride", C.c_long), ("weight", C.c_void_p), ("weight_stride", C.c_long), ("A", C.c_void_p),
                 ("B", C.c_void_p), ("scale", C.c_void_p), ("index", C.c_void_p)]
 
 
 class _AdamwTensor(C.Structure):
+    """smx_adamw_tensor"""
     _fields_ = [("param", C.c_void_p), ("grad", C.c_void_p), ("master", C.c_void_p), ("exp_avg", C.c_void_p), ("exp_avg_sq", C.c_void_p),
                 ("scale_avg", C.c_void_p), ("scale_avg_sq", C.c_void_p), ("numel", C.c_long)]
+
+
+# the same as packed bytes, which are made in a fraction of the time
+_ADAPTED = struct.Struct("@5iqPqPqPPPP")
+_ADAMW_TENSOR = struct.Struct("@7Pq")
+assert _ADAPTED.size == C.sizeof(_Adapted) and _ADAMW_TENSOR.size == C.sizeof(_AdamwTensor)
 
 
 _functions = None
@@ -81,42 +91,39 @@ def _rows(t, dim, what):
     return t, rows, stride
 
 
-class _On:
-    """The device of a call's tensors, made the current one where it is not, and the stream to use."""
-    __slots__ = ("device", "before")
+def _on(t, *others):
+    """The ordinal of the tensors' device, which has to be one GPU."""
+    device = t.get_device()
+    if device < 0:
+        raise ValueError("tensors on the GPU expected: there is no CPU path")
+    for o in others:
+        if o is not None and o.get_device() != device:
+            raise ValueError(f"tensors on one device expected: {t.device} and {o.device}")
+    return device
 
-    def __init__(self, t, *others):
-        if not t.is_cuda:
-            raise ValueError("tensors on the GPU expected: there is no CPU path")
-        self.device = t.device
-        for o in others:
-            if o is not None and o.device != t.device:
-                raise ValueError(f"tensors on one device expected: {t.device} and {o.device}")
 
-    def __enter__(self):
-        self.before = torch.cuda.current_device()
-        if self.before != self.device.index:
-            torch.cuda.set_device(self.device)
-        return torch.cuda.current_stream(self.device).cuda_stream
-
-    def __exit__(self, *exc):
-        if self.before != self.device.index:
-            torch.cuda.set_device(self.before)
+def _call(device, entry, *args):
+    """Calls an entry point with the device's current stream as its last argument, and the device as the current one."""
+    if torch.cuda.current_device() == device:
+        code = entry(*args, torch._C._cuda_getCurrentRawStream(device))
+    else:
+        with torch.cuda.device(device):
+            code = entry(*args, torch._C._cuda_getCurrentRawStream(device))
+    if code:
+        _lib.check(code)
 
 
 # ---- layer norm
 
-def _affine(x, weight, bias):
-    dim, kind = x.shape[-1], None
-    for t, what in ((weight, "weight"), (bias, "bias")):
-        if t is None:
-            continue
-        _need(t.dim() == 1 and t.shape[0] == dim and (dim == 1 or t.stride(0) == 1), f"{what}: {dim} contiguous numbers expected")
-        if t.dtype != x.dtype and t.dtype != torch.float32:
-            raise TypeError(f"{what}: {x.dtype} or float32, not {t.dtype}")
-        _need(kind in (None, t.dtype), "weight and bias: one type expected")
-        kind = t.dtype
-    return x.dtype if kind is None else kind
+def _affine(x, dim, weight, bias):
+    kind = x.dtype if weight is None and bias is None else (bias if weight is None else weight).dtype
+    if kind != x.dtype and kind != torch.float32:
+        raise TypeError(f"weight and bias: {x.dtype} or float32, not {kind}")
+    for t in (weight, bias):
+        if t is not None:
+            _need(t.shape == (dim,) and t.is_contiguous(), f"weight and bias: {dim} contiguous numbers expected")
+            _need(t.dtype == kind, "weight and bias: one type expected")
+    return kind
 
 
 def layer_norm_forward(x, weight=None, bias=None, eps=1e-5):
@@ -124,16 +131,21 @@ def layer_norm_forward(x, weight=None, bias=None, eps=1e-5):
     kind = _type(x, "x")
     _need(x.dim() >= 1 and x.shape[-1] >= 1, "x: rows of at least one number expected")
     dim = x.shape[-1]
-    weights = _TYPES[_affine(x, weight, bias)]
+    weights = _affine(x, dim, weight, bias)
+    device = _on(x, weight, bias)
     rows_of, rows, stride = _rows(x, dim, "x")
-    with _On(x, weight, bias) as stream:
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        stats = torch.empty((2,) + x.shape[:-1], dtype=torch.float32, device=x.device)
-        mean, rstd = stats[0], stats[1]
-        _lib.check(_lib_functions().smx_layer_norm_forward(
-            kind, weights, rows, dim, rows_of.data_ptr(), stride, 0 if weight is None else weight.data_ptr(), 0 if bias is None else bias.data_ptr(),
-            eps, y.data_ptr(), dim, mean.data_ptr(), rstd.data_ptr(), stream))
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    mean, rstd = x.new_empty((2,) + x.shape[:-1], dtype=torch.float32).unbind(0)
+    _call(device, _lib_functions().smx_layer_norm_forward, kind, _TYPES[weights], rows, dim, rows_of.data_ptr(), stride,
+          0 if weight is None else weight.data_ptr(), 0 if bias is None else bias.data_ptr(), eps, y.data_ptr(), dim, mean.data_ptr(), rstd.data_ptr())
     return y, mean, rstd
+
+
+@functools.lru_cache(maxsize=1024)
+def _norm_workspace(rows, dim):
+    size = C.c_long()
+    _lib.check(_lib_functions().smx_layer_norm_backward_workspace(rows, dim, C.byref(size)))
+    return size.value
 
 
 def layer_norm_backward(dy, x, mean, rstd, weight=None, need=(True, True, True)):
@@ -143,22 +155,19 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, need=(True, True, True))
     _need(dy.shape == x.shape and dy.dtype == x.dtype, "dy: shape and type of x expected")
     _need(mean.dtype == rstd.dtype == torch.float32 and mean.shape == rstd.shape == x.shape[:-1] and mean.is_contiguous() and rstd.is_contiguous(),
           "mean and rstd: float32, a number a row expected")
-    weights = _affine(x, weight, None)
+    weights = _affine(x, dim, weight, None)
+    device = _on(x, dy, mean, rstd, weight)
     x_rows, rows, x_stride = _rows(x, dim, "x")
     dy_rows, _, dy_stride = _rows(dy, dim, "dy")
-    with _On(x, dy, mean, rstd, weight) as stream:
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need[0] else None
-        sums = torch.empty((2, dim), dtype=weights, device=x.device) if need[1] or need[2] else None
-        dw, db = (sums[0] if need[1] else None, sums[1] if need[2] else None) if sums is not None else (None, None)
-        work = None
-        if sums is not None:
-            size = C.c_long()
-            _lib.check(_lib_functions().smx_layer_norm_backward_workspace(rows, dim, C.byref(size)))
-            work = torch.empty(size.value, dtype=torch.uint8, device=x.device)
-        _lib.check(_lib_functions().smx_layer_norm_backward(
-            kind, _TYPES[weights], rows, dim, dy_rows.data_ptr(), dy_stride, x_rows.data_ptr(), x_stride, mean.data_ptr(), rstd.data_ptr(),
-            0 if weight is None else weight.data_ptr(), 0 if dx is None else dx.data_ptr(), dim, 0 if dw is None else dw.data_ptr(),
-            0 if db is None else db.data_ptr(), 0 if work is None else work.data_ptr(), 0 if work is None else work.numel(), stream))
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format) if need[0] else None
+    dw = db = work = None
+    if need[1] or need[2]:
+        dw, db = x.new_empty((2, dim), dtype=weights).unbind(0)
+        dw, db = dw if need[1] else None, db if need[2] else None
+        work = x.new_empty((_norm_workspace(rows, dim),), dtype=torch.uint8)
+    _call(device, _lib_functions().smx_layer_norm_backward, kind, _TYPES[weights], rows, dim, dy_rows.data_ptr(), dy_stride, x_rows.data_ptr(), x_stride,
+          mean.data_ptr(), rstd.data_ptr(), 0 if weight is None else weight.data_ptr(), 0 if dx is None else dx.data_ptr(), dim,
+          0 if dw is None else dw.data_ptr(), 0 if db is None else db.data_ptr(), 0 if work is None else work.data_ptr(), 0 if work is None else work.numel())
     return dx, dw, db
 
 
@@ -206,16 +215,20 @@ def _describe(x, weight, A, B, scale, index):
         if scale.dtype != torch.float32:
             raise TypeError(f"scale: float32 expected, not {scale.dtype}")
         _need(scale.shape == (n,) and scale.is_contiguous(), "scale: a contiguous number an adapter expected")
-    keep = (rows_of, weight, A, B)          # (copies live until the call is made)
-    p = _Adapted(kind, d_in, d_out, rank, n, rows, rows_of.data_ptr(), stride, weight.data_ptr(), weight_stride, A.data_ptr(), B.data_ptr(),
-                 0 if scale is None else scale.data_ptr(), index.data_ptr())
-    return p, keep
+    p = _ADAPTED.pack(kind, d_in, d_out, rank, n, rows, rows_of.data_ptr(), stride, weight.data_ptr(), weight_stride, A.data_ptr(), B.data_ptr(),
+                      0 if scale is None else scale.data_ptr(), index.data_ptr())
+    # (the copies live until the call is made)
+    return p, (kind, d_in, d_out, rank, n, rows, stride, weight_stride), (rows_of, weight, A, B)
 
 
-def _workspace(p, backward, device):
-    size = C.c_long()
-    _lib.check(_lib_functions().smx_adapted_linear_workspace(C.byref(p), backward, C.byref(size)))
-    return torch.empty(size.value, dtype=torch.uint8, device=device)
+@functools.lru_cache(maxsize=1024)
+def _adapted_workspace(sizes, backward):
+    """Bytes of a call's workspace, which depends on sizes alone."""
+    kind, d_in, d_out, rank, n, rows, stride, weight_stride = sizes
+    size, some = C.c_long(), 256
+    _lib.check(_lib_functions().smx_adapted_linear_workspace(
+        _ADAPTED.pack(kind, d_in, d_out, rank, n, rows, some, stride, some, weight_stride, some, some, 0, some), backward, C.byref(size)))
+    return size.value
 
 
 def adapted_linear_forward(x, weight, A, B, scale, index):
@@ -223,29 +236,29 @@ def adapted_linear_forward(x, weight, A, B, scale, index):
 
     x[..., d_in], weight[d_out, d_in], A[adapters, rank, d_in] and B[adapters, d_out, rank] are of one type, scale[adapters] is
     float32 (None: ones).  Rows may come in any order.  A row whose index is out of range is NaN."""
-    with _On(x, weight, A, B, scale, index) as stream:
-        p, keep = _describe(x, weight, A, B, scale, index)
-        y = torch.empty(x.shape[:-1] + (p.d_out,), dtype=x.dtype, device=x.device)
-        work = _workspace(p, 0, x.device)
-        _lib.check(_lib_functions().smx_adapted_linear_forward(C.byref(p), y.data_ptr(), p.d_out, work.data_ptr(), work.numel(), stream))
+    device = _on(x, weight, A, B, scale, index)
+    p, sizes, keep = _describe(x, weight, A, B, scale, index)
+    y = x.new_empty(x.shape[:-1] + (sizes[2],))
+    work = x.new_empty((_adapted_workspace(sizes, 0),), dtype=torch.uint8)
+    _call(device, _lib_functions().smx_adapted_linear_forward, p, y.data_ptr(), sizes[2], work.data_ptr(), work.numel())
     return y
 
 
 def adapted_linear_backward(dy, x, weight, A, B, scale, index, need=(True, True, True)):
     """Gradients of x, A and B (None where `need` says so); weight and scale are fixed."""
-    with _On(x, dy, weight, A, B, scale, index) as stream:
-        p, keep = _describe(x, weight, A, B, scale, index)
-        _need(dy.shape == x.shape[:-1] + (p.d_out,), "dy: a row of d_out numbers for every row of x expected")
-        if dy.dtype != x.dtype:
-            raise TypeError("dy: the type of x expected")
-        dy_rows, _, dy_stride = _rows(dy, p.d_out, "dy")
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need[0] else None
-        dA = torch.empty(A.shape, dtype=A.dtype, device=x.device) if need[1] else None
-        dB = torch.empty(B.shape, dtype=B.dtype, device=x.device) if need[2] else None
-        work = _workspace(p, 1, x.device)
-        _lib.check(_lib_functions().smx_adapted_linear_backward(
-            C.byref(p), dy_rows.data_ptr(), dy_stride, 0 if dx is None else dx.data_ptr(), p.d_in, 0 if dA is None else dA.data_ptr(),
-            0 if dB is None else dB.data_ptr(), work.data_ptr(), work.numel(), stream))
+    device = _on(x, dy, weight, A, B, scale, index)
+    p, sizes, keep = _describe(x, weight, A, B, scale, index)
+    d_in, d_out = sizes[1:3]
+    _need(dy.shape == x.shape[:-1] + (d_out,), "dy: a row of d_out numbers for every row of x expected")
+    if dy.dtype != x.dtype:
+        raise TypeError("dy: the type of x expected")
+    dy_rows, _, dy_stride = _rows(dy, d_out, "dy")
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format) if need[0] else None
+    dA = torch.empty_like(A, memory_format=torch.contiguous_format) if need[1] else None
+    dB = torch.empty_like(B, memory_format=torch.contiguous_format) if need[2] else None
+    work = x.new_empty((_adapted_workspace(sizes, 1),), dtype=torch.uint8)
+    _call(device, _lib_functions().smx_adapted_linear_backward, p, dy_rows.data_ptr(), dy_stride, 0 if dx is None else dx.data_ptr(), d_in,
+          0 if dA is None else dA.data_ptr(), 0 if dB is None else dB.data_ptr(), work.data_ptr(), work.numel())
     return dx, dA, dB
 
 
@@ -280,11 +293,11 @@ def moment_values(code_avg, scale_avg, code_avg_sq, scale_avg_sq):
     blocks = -(-n // MOMENT_BLOCK)
     _need(code_avg_sq.numel() == n and scale_avg.numel() == scale_avg_sq.numel() == blocks, f"{n} codes and {blocks} scales expected")
     _need(all(t.is_contiguous() for t in (code_avg, scale_avg, code_avg_sq, scale_avg_sq)), "contiguous tensors expected")
-    with _On(code_avg, scale_avg, code_avg_sq, scale_avg_sq) as stream:
-        m = torch.empty(code_avg.shape, dtype=torch.float32, device=code_avg.device)
-        v = torch.empty_like(m)
-        _lib.check(_lib_functions().smx_moment_values(n, code_avg.data_ptr(), scale_avg.data_ptr(), code_avg_sq.data_ptr(), scale_avg_sq.data_ptr(),
-                                                      m.data_ptr(), v.data_ptr(), stream))
+    device = _on(code_avg, scale_avg, code_avg_sq, scale_avg_sq)
+    m = torch.empty_like(code_avg, dtype=torch.float32)
+    v = torch.empty_like(m)
+    _call(device, _lib_functions().smx_moment_values, n, code_avg.data_ptr(), scale_avg.data_ptr(), code_avg_sq.data_ptr(), scale_avg_sq.data_ptr(),
+          m.data_ptr(), v.data_ptr())
     return m, v
 
 
@@ -331,6 +344,9 @@ class AdamW:
                                                for t, k, c in zip(s, kinds, counts)),
                   "states: (exp_avg, exp_avg_sq) in float32, or (code_avg int8, scale_avg float32, code_avg_sq uint8, scale_avg_sq float32), "
                   "contiguous and on the parameters' device, expected")
+        at = (0, 1) if state_bits == 32 else (0, 2, 1, 3)          # of a state: moments, then their scales
+        self._fixed = [(0 if masters is None else self.masters[i].data_ptr(), *(s[k].data_ptr() for k in at), *((0, 0) if state_bits == 32 else ()), p.numel())
+                       for i, (s, p) in enumerate(zip(self.states, self.params))]
 
     def _zeros(self, p):
         n, blocks = p.numel(), -(-p.numel() // MOMENT_BLOCK)
@@ -345,40 +361,26 @@ class AdamW:
         if grads is None:
             grads = [p.grad for p in self.params]
         _need(len(grads) == len(self.params), "a gradient (or None) for every parameter expected")
-        if not self.params:
-            self.step_count += 1
-            return
-        eight, first = self.state_bits == 8, self.params[0]
-        table = (_AdamwTensor * len(grads))()
-        kind, count, keep = None, 0, []
-        for i, (p, g) in enumerate(zip(self.params, grads)):
-            if g is None:
-                continue
-            if kind is None:
-                kind = g.dtype
-                if kind != first.dtype and kind != torch.float32:
-                    raise TypeError(f"gradients: {first.dtype} or float32, not {kind}")
-            if g.dtype != kind:
-                raise TypeError("gradients of one type expected")
-            if g.shape != p.shape or g.device != p.device:
-                raise ValueError("gradients of the parameters' shapes and on their device expected")
-            if not g.is_contiguous():
-                g = g.contiguous()
-                keep.append(g)
-            s, t = self.states[i], table[count]
-            t.param, t.grad, t.numel = p.data_ptr(), g.data_ptr(), p.numel()
-            t.exp_avg = s[0].data_ptr()
-            if eight:
-                t.scale_avg, t.exp_avg_sq, t.scale_avg_sq = s[1].data_ptr(), s[2].data_ptr(), s[3].data_ptr()
-            else:
-                t.exp_avg_sq = s[1].data_ptr()
-            if self.masters is not None:
-                t.master = self.masters[i].data_ptr()
-            count += 1
-        with _On(first) as stream:
-            _lib.check(_lib_functions().smx_adamw_step(
-                _TYPES[first.dtype], _TYPES[kind or first.dtype], self.state_bits, C.addressof(table), count, self.lr, self.betas[0], self.betas[1],
-                self.eps, self.weight_decay, self.step_count + 1, stream))
-        # (as torch's own operations in place do: a backward pass that saved the old values says so)
-        torch.autograd.graph.increment_version([p for p, g in zip(self.params, grads) if g is not None])
+        taken = [i for i, g in enumerate(grads) if g is not None]
+        if taken:
+            params, device = self.params, self.params[0].get_device()
+            kind, own = grads[taken[0]].dtype, self.params[0].dtype
+            if kind != own and kind != torch.float32:
+                raise TypeError(f"gradients: {own} or float32, not {kind}")
+            table, keep = bytearray(len(taken) * _ADAMW_TENSOR.size), []
+            for at, i in enumerate(taken):
+                p, g = params[i], grads[i]
+                if g.dtype != kind:
+                    raise TypeError("gradients of one type expected")
+                if g.shape != p.shape or g.get_device() != device:
+                    raise ValueError("gradients of the parameters' shapes and on their device expected")
+                if not g.is_contiguous():
+                    g = g.contiguous()
+                    keep.append(g)
+                master, m, v, scale_m, scale_v, n = self._fixed[i]
+                _ADAMW_TENSOR.pack_into(table, at * _ADAMW_TENSOR.size, p.data_ptr(), g.data_ptr(), master, m, v, scale_m, scale_v, n)
+            _call(device, _lib_functions().smx_adamw_step, _TYPES[own], _TYPES[kind], self.state_bits, bytes(table), len(taken), self.lr, self.betas[0],
+                  self.betas[1], self.eps, self.weight_decay, self.step_count + 1)
+            # (as torch's own operations in place do: a backward pass that saved the old values says so)
+            torch.autograd.graph.increment_version(params if len(taken) == len(params) else [params[i] for i in taken])
         self.step_count += 1
