@@ -500,6 +500,8 @@ struct Product {
     void* out;
     long out_stride;
     int row_tiles, col_tiles;
+    int splits, split_steps;      // of the sum over k: parts, and steps of each; from two parts on sums go to partial[split][row][col]
+    float* partial;
 };
 
 // Block -> tile: the blocks of a die (every eighth) take neighbouring tiles, four row tiles high, so that they share rows in its L2.
@@ -746,6 +748,24 @@ __device__ __forceinline__ void store_tiles(const Product& p, int lane, long row
     }
 }
 
+// the sums of a part of k
+template <typename T, int NM, int NT>
+__device__ __forceinline__ void store_partial(const Product& p, int lane, long row0, int col0, const f32x4 (&acc)[NM][NT])
+{
+#pragma unroll
+    for (int i = 0; i < NM; ++i) {
+        const long row = row0 + 16 * i + (lane & 15);
+        if (row >= p.rows) continue;
+        float* out = p.partial + ((long)blockIdx.y * p.rows + row) * p.cols;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const int col = col0 + column_of<T>(t, 4 * (lane >> 4));
+            const float v[4] = {acc[i][t][0], acc[i][t][1], acc[i][t][2], acc[i][t][3]};
+            store_run<4>(out + col, p.cols - col, v);
+        }
+    }
+}
+
 // 16-bit types.  Tiles of 64 terms come straight from memory into LDS, STAGES of them under way; WM x WN wavefronts share the tile.
 // A load brings eight rows of 128 bytes; the 16-byte pieces of a row lie in an order that depends on the row, so that lanes that read
 // together meet different banks.  A step of 32 terms has its operands fetched during the step before.
@@ -761,8 +781,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_product16(const Product p)
     if (!tile_of(p, rt, ct)) return;
     const long row0 = (long)rt * BM;
     const int col0 = ct * BN;
-    const char* x_base = static_cast<const char*>(p.in) + 2 * row0 * p.in_stride;
-    const char* w_base = static_cast<const char*>(p.W) + 2 * (long)col0 * p.w_stride;
+    constexpr bool SPLIT = BM == 64;      // (parts of long sums: of the small tiles alone)
+    const int first = SPLIT ? blockIdx.y * p.split_steps : 0;      // (a multiple of two steps)
+    const char* x_base = static_cast<const char*>(p.in) + 2 * (row0 * p.in_stride + first * kPiece);
+    const char* w_base = static_cast<const char*>(p.W) + 2 * ((long)col0 * p.w_stride + first * kPiece);
     unsigned from[PER];
     unsigned second = 0;      // loads whose piece is in the second half of its row's 128 bytes
 #pragma unroll
@@ -781,7 +803,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_product16(const Product p)
         second |= (unsigned)(piece >> 2) << u;
     }
     const unsigned lds0 = lds_address(lds);
-    const int steps = p.k_padded / kPiece, stages = (steps + 1) / 2;
+    const int all = p.k_padded / kPiece, steps = SPLIT ? min(all - first, p.split_steps) : all, stages = (steps + 1) / 2;
     auto request = [&](int s) {
         const unsigned to = lds0 + s % STAGES * STAGE + wave * 1024;
 #pragma unroll
@@ -871,6 +893,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_product16(const Product p)
     }
     const long row_w = row0 + wm * NM * 16;
     const int col_w = col0 + wn * NT * 16;
+    if constexpr (SPLIT)
+        if (p.splits > 1) {
+            store_partial<T, NM, NT>(p, lane, row_w, col_w, acc);
+            return;
+        }
     add_adapters<T, NM, NT>(p, lane, row_w, col_w, acc);
     store_tiles<T, NM, NT>(p, lane, row_w, col_w, acc);
 }
@@ -884,16 +911,18 @@ template <int NM, int NT>
 __global__ __launch_bounds__(256, NM == 1 ? 4 : 3) void k_product32(const Product p)
 {
     constexpr int BM = 64 * NM, BN = 16 * NT, STAGE = 3 * BN * 64, PER = STAGE / 4096;
+    constexpr bool SPLIT = NM == 1;      // (parts of long sums: of the small tiles alone)
     __shared__ __align__(16) unsigned char lds[2 * STAGE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
     int rt, ct;
     if (!tile_of(p, rt, ct)) return;
     const long row0 = (long)rt * BM + wave * 16 * NM;
-    const int col0 = ct * BN, steps = p.k_padded / kPiece;
+    const int col0 = ct * BN, all = p.k_padded / kPiece, first = SPLIT ? blockIdx.y * p.split_steps : 0, steps = SPLIT ? min(all - first, p.split_steps) : all;
+    const int begin = first * kPiece, rest = p.k - begin;      // numbers of a row from this part on
     const float* from[NM];
 #pragma unroll
-    for (int i = 0; i < NM; ++i) from[i] = static_cast<const float*>(p.in) + min(row0 + 16 * i + n, p.rows - 1) * p.in_stride;
-    const char* w_base = static_cast<const char*>(p.W) + (long)(col0 / kPartRows) * steps * (3 * kPartRows * 64) + col0 % kPartRows * 64;
+    for (int i = 0; i < NM; ++i) from[i] = static_cast<const float*>(p.in) + min(row0 + 16 * i + n, p.rows - 1) * p.in_stride + begin;
+    const char* w_base = static_cast<const char*>(p.W) + ((long)(col0 / kPartRows) * all + first) * (3 * kPartRows * 64) + col0 % kPartRows * 64;
     const unsigned lds0 = lds_address(lds) + wave * PER * 1024;
     f32x4 raw[NM][2];
     auto request = [&](int s) {
@@ -903,7 +932,7 @@ __global__ __launch_bounds__(256, NM == 1 ? 4 : 3) void k_product32(const Produc
             load_into_lds(w_base + (long)s * (3 * kPartRows * 64) + part * kPartRows * 64 + chunk % NT * 1024, lane * 16, lds0 + s % 2 * STAGE + u * 1024);
         }
         const int k = s * kPiece + 8 * g;
-        if ((s + 1) * kPiece <= p.k) {
+        if ((s + 1) * kPiece <= rest) {
 #pragma unroll
             for (int i = 0; i < NM; ++i)
 #pragma unroll
@@ -913,8 +942,8 @@ __global__ __launch_bounds__(256, NM == 1 ? 4 : 3) void k_product32(const Produc
             for (int i = 0; i < NM; ++i)
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    const float x = from[i][min(k + j, p.k - 1)];
-                    raw[i][j / 4][j % 4] = k + j < p.k ? x : 0.0f;
+                    const float x = from[i][min(k + j, rest - 1)];
+                    raw[i][j / 4][j % 4] = k + j < rest ? x : 0.0f;
                 }
         }
         asm volatile("" ::: "memory");      // (asked for here, not where they are used)
@@ -989,13 +1018,18 @@ __global__ __launch_bounds__(256, NM == 1 ? 4 : 3) void k_product32(const Produc
                 for (int j = 0; j < 4; ++j) {
                     const float* wc = static_cast<const float*>(p.W0) + min(col0 + 16 * t + 4 * g + j, p.cols - 1) * p.w0_col;
                     float sum = 0.0f;
-                    for (int k = 0; k < p.k; ++k) sum = fmaf(row[k], wc[k * p.w0_k], sum);
+                    for (int k = begin; k < min(p.k, begin + steps * kPiece); ++k) sum = fmaf(row[k], wc[k * p.w0_k], sum);
 #pragma unroll
                     for (int c = 0; c < 4; ++c)
                         if (c == j && !(fabsf(acc[i][t][c]) <= std::numeric_limits<float>::max())) acc[i][t][c] = sum;
                 }
         }
     }
+    if constexpr (SPLIT)
+        if (p.splits > 1) {
+            store_partial<float, NM, NT>(p, lane, row0, col0, acc);
+            return;
+        }
     const int one = one_adapter<NM>(p, lane, row0);
     if (one >= 0) add_adapter<NM, NT>(p, lane, row0, col0, one, acc);
     store_tiles<float, NM, NT>(p, lane, row0, col0, acc);
@@ -1050,6 +1084,36 @@ __global__ __launch_bounds__(256) void k_add_mixed(const Product p, int group)
         for (int u = 0; u < 8; ++u)
             if (row0 + i0 + u < p.rows && has_adapter(__builtin_amdgcn_readlane(mine, i0 + u), p.adapters)) out[(row0 + i0 + u) * p.out_stride] = y[u] + sum[u];
     }
+}
+
+// The parts of a product split along k, in order, with the adapters' part: a thread has a column of a row.
+template <typename T>
+__global__ __launch_bounds__(256) void k_join_splits(const Product p)
+{
+    const long row = blockIdx.x;
+    const int col = blockIdx.y * 256 + threadIdx.x, a = p.index[row];
+    if (col >= p.cols) return;
+    float sum = 0.0f;
+#pragma unroll 4
+    for (int s = 0; s < p.splits; ++s) sum += p.partial[((long)s * p.rows + row) * p.cols + col];
+    if (has_adapter(a, p.adapters)) {
+        const T* F = static_cast<const T*>(p.F) + a * p.f_each + col * p.f_col;
+        const float* h = p.h + row * p.padded;
+        float part = 0.0f;
+        if (p.f_runs) {
+            for (int r = 0; r < p.rank; r += 8) {
+                float f[8];
+                load_run<8>(F + r, 8, f);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) part = fmaf(h[r + j], f[j], part);
+            }
+        } else {
+#pragma unroll 8
+            for (int r = 0; r < p.rank; ++r) part = fmaf(h[r], (float)F[r * p.f_r], part);
+        }
+        sum += part;
+    }
+    static_cast<T*>(p.out)[row * p.out_stride + col] = is_bad(a, p.adapters) ? (T)std::numeric_limits<float>::quiet_NaN() : (T)sum;
 }
 
 // Few rows: a block takes 16 columns and all rows; eight wavefronts have 128 bytes of W's rows by turns.
@@ -1351,7 +1415,17 @@ struct Call {
         q.in = in; q.in_stride = in_stride; q.W0 = W; q.w0_col = w_col; q.w0_k = w_k; q.F = F; q.f_each = f_each; q.f_col = f_col; q.f_r = f_r; q.f_runs = f_r == 1 && p.rank % 8 == 0; q.h = h;
         q.index = p.index; q.adapters = p.num_adapters; q.rank = p.rank; q.padded = padded; q.k = k; q.k_padded = (int)up(k, kPiece); q.cols = cols;
         q.rows = p.rows; q.out = out; q.out_stride = out_stride;
+        q.splits = 1;
+        q.split_steps = q.k_padded / kPiece + 1;
         if (few) return q;
+        // Few tiles and long sums: the sums in parts of at least eight steps, until there are two blocks for every CU.
+        const long few_tiles = (p.rows + 63) / 64 * ((cols + 63) / 64);
+        const int steps = q.k_padded / kPiece;
+        if (few_tiles <= 192 && steps >= 16) {
+            q.split_steps = (int)std::max(8L, up((steps * few_tiles + 511) / 512, 2));
+            q.splits = (steps + q.split_steps - 1) / q.split_steps;
+            if (q.splits > 1) q.partial = arena.take<float>(q.splits * p.rows * cols);
+        }
         if constexpr (std::is_same_v<T, float>) {
             bf16* parts = arena.take<bf16>(3 * up(cols, kPartRows) * q.k_padded);
             lay_out<float>(W, 0, w_col, w_k, parts, true, cols, k, 1);
@@ -1409,7 +1483,14 @@ struct Call {
             q.index += main_rows;
             return q.rows > 0;
         };
+        auto join = [&] { hipLaunchKernelGGL((k_join_splits<T>), dim3((unsigned)q.rows, (q.cols + 255) / 256), dim3(256), 0, s, q); };
         if constexpr (std::is_same_v<T, float>) {
+            if (q.splits > 1) {
+                tiles(64, 64);
+                hipLaunchKernelGGL((k_product32<1, 4>), dim3(blocks().x, q.splits), dim3(256), 0, s, q);
+                join();
+                return;
+            }
             const bool wide = tiles(128, 128) >= 256;
             if (wide) hipLaunchKernelGGL((k_product32<2, 8>), blocks(), dim3(256), 0, s, q);
             else {
@@ -1425,8 +1506,14 @@ struct Call {
                 constexpr int bytes = S * (BM + BN) * 128;
                 if constexpr (bytes > 64 * 1024)
                     hip_ok(hipFuncSetAttribute(reinterpret_cast<const void*>(&k_product16<T, BM, BN, WM, WN, S>), hipFuncAttributeMaxDynamicSharedMemorySize, bytes), "LDS");
-                hipLaunchKernelGGL((k_product16<T, BM, BN, WM, WN, S>), blocks(), dim3(64 * WM * WN), bytes, s, q);
+                hipLaunchKernelGGL((k_product16<T, BM, BN, WM, WN, S>), dim3(blocks().x, q.splits), dim3(64 * WM * WN), bytes, s, q);
             };
+            if (q.splits > 1) {
+                tiles(64, 64);
+                go(Int<64>{}, Int<64>{}, Int<2>{}, Int<2>{}, Int<3>{});
+                join();
+                return;
+            }
             if (tiles(256, 256) >= 192 && !rounds(256, 256, 256, [&] { go(Int<256>{}, Int<256>{}, Int<2>{}, Int<4>{}, Int<2>{}); })) return;
             if (tiles(128, 128) >= 192 && !rounds(128, 128, 512, [&] { go(Int<128>{}, Int<128>{}, Int<2>{}, Int<2>{}, Int<2>{}); })) return;
             tiles(64, 64);
