@@ -1398,10 +1398,13 @@ struct Call {
             refuse_unless(blocks <= 0x7fffffffL, "more blocks than a launch takes");
             if (blocks) hipLaunchKernelGGL((k_down<T, RT, MT, WAVES>), dim3((unsigned)blocks), dim3(64 * WAVES), 0, s, downs);
         };
-        const bool few_blocks = p.rows / 16 * num_downs < 4096 && downs.down[0].k >= 1024;
-        if (padded == 16) few_blocks ? go(Int<1>{}, Int<2>{}, Int<8>{}) : go(Int<1>{}, Int<2>{}, Int<4>{});
-        else if (padded == 32) few_blocks ? go(Int<2>{}, Int<2>{}, Int<8>{}) : go(Int<2>{}, Int<2>{}, Int<4>{});
-        else if (padded <= 64) few_blocks ? go(Int<4>{}, Int<1>{}, Int<8>{}) : go(Int<4>{}, Int<2>{}, Int<4>{});
+        // Wavefronts of a block share its sums.  Few blocks leave most of the chip without work, so they get more wavefronts: 8 where the
+        // sums are long (4 091 rows of 2 048 and 2 048 in f16: 12.1 us with 8 of 32 rows, 13.6 with 16 of 16 rows), and below 4 096 rows in
+        // all 16 of 16 rows each (1 840 rows of 2 207 in single precision: 21 us, and 48 with 4; 300 of 4 096 in bfloat16: 15 and 23).
+        const bool long_rows = downs.down[0].k >= 1024, few_blocks = p.rows / 16 * num_downs < 4096, very_few = p.rows / 32 * num_downs < 128 && downs.down[0].k >= 256;
+        if (padded == 16) very_few ? go(Int<1>{}, Int<1>{}, Int<16>{}) : few_blocks && long_rows ? go(Int<1>{}, Int<2>{}, Int<8>{}) : go(Int<1>{}, Int<2>{}, Int<4>{});
+        else if (padded == 32) very_few ? go(Int<2>{}, Int<1>{}, Int<16>{}) : few_blocks && long_rows ? go(Int<2>{}, Int<2>{}, Int<8>{}) : go(Int<2>{}, Int<2>{}, Int<4>{});
+        else if (padded <= 64) few_blocks && long_rows ? go(Int<4>{}, Int<1>{}, Int<8>{}) : go(Int<4>{}, Int<2>{}, Int<4>{});
         else go(Int<8>{}, Int<1>{}, Int<4>{});
     }
 
