@@ -292,8 +292,9 @@ int smx_nlist_copy_to_host(smx_nlist* nl, int* num_neigh, int* neigh_indices, in
  * no counterpart in the reference.  Every array is in device memory, work is enqueued on `stream` (a hipStream_t, or
  * NULL) without synchronising, nothing is allocated (a workspace, where one is needed, is the caller's, its size asked
  * for beforehand, and free again when the call's work on the stream is done), and calls can be captured into a graph.
- * Arrays need the alignment of their element type only; strides are in elements, from row to row.  Results do not
- * depend on the order in which thread blocks run. */
+ * Arrays need the alignment of their element type only, the adapters' workspace that of 256 bytes; strides are in
+ * elements, from row to row.  Results do not depend on the order in which thread blocks run.  Arguments are checked
+ * before anything is enqueued: non-zero is returned for what is refused, with the reason in smx_last_error(). */
 enum {
     SMX_TYPE_F32 = 0,
     SMX_TYPE_BF16 = 1,
@@ -302,7 +303,7 @@ enum {
 
 /* Layer norm over rows of dim numbers: y = (x - mean) rstd weight + bias, rstd = 1 / sqrt(var + eps).  weight[dim] and
  * bias[dim] (either may be NULL) are of weight_type: the features' type or SMX_TYPE_F32.  mean[rows] and rstd[rows] may
- * be NULL.  Sums are in single precision. */
+ * be NULL.  Sums are in single precision.  rows: up to 2^31 - 1, dim: up to 2^24. */
 int smx_layer_norm_forward(int type, int weight_type, long rows, long dim, const void* d_x, long x_stride,
                            const void* d_weight, const void* d_bias, double eps, void* d_y, long y_stride,
                            float* d_mean, float* d_rstd, void* stream);
@@ -319,7 +320,7 @@ int smx_layer_norm_backward(int type, int weight_type, long rows, long dim, cons
  * weight[d_out][d_in] (rows weight_stride apart), A[num_adapters][rank][d_in], B[num_adapters][d_out][rank] and x are of
  * one type; scale[num_adapters] may be NULL (ones).  index[rows] names a row's adapter, in any order; -1: none.  A row
  * whose index is neither has NaN for results and no part in the gradients.  What one adapter holds, infinities and NaN
- * too, has no effect on other adapters' rows. */
+ * too, has no effect on other adapters' rows.  rows: up to 2^28, d_in and d_out: up to 2^20. */
 typedef struct {
     int type;
     int d_in, d_out, rank, num_adapters;
@@ -350,7 +351,7 @@ int smx_adapted_linear_backward(const smx_adapted_linear* p, const void* d_dy, l
  * the step goes by, of which param gets a rounded copy (parameters in 16 bits; for all tensors of a call or none).
  * state_bits 32: exp_avg and exp_avg_sq are float[numel].  state_bits 8: they are codes, signed and unsigned chars
  * [numel], and scale_avg, scale_avg_sq hold a float for every SMX_MOMENT_BLOCK of them:
- *   m = scale c |c| / 127^2,  v = scale (c / 255)^4.  Zeros are a valid start. */
+ *   m = scale c |c| / 127^2,  v = scale (c / 255)^4.  Zeros are a valid start.  numel: less than 2^36. */
 typedef struct {
     void* param;
     const void* grad;

@@ -12,6 +12,9 @@
 //
 // Every operation is rounded once, in the order written (no fused multiply-adds, IEEE division and root), so that the codes are those
 // of the same formulas elsewhere.
+//
+// What bounds it is memory: 807 us for 150 million parameters in bfloat16 with masters and moments in 32 bits (28 bytes each, 5.2 TB/s).
+// Moments in 8 bits are 2 + 1/32 bytes to read and as many to write; there the divisions and roots that make codes count as much as the bytes.
 #include "smx_finetune.hpp"
 
 #include <algorithm>
@@ -220,7 +223,7 @@ extern "C" int smx_adamw_step(int param_type, int grad_type, int state_bits, con
         bool masters = false, first = true;
         for (int i = 0; i < count; ++i) {
             const smx_adamw_tensor& t = tensors[i];
-            refuse_unless(t.numel >= 0 && t.numel < (1L << 40), "numel: 0 to 2^40");
+            refuse_unless(t.numel >= 0 && t.numel < (1L << 36), "numel: 0 less than 2^36");
             if (t.numel == 0) continue;
             refuse_unless(t.param && t.grad && t.exp_avg && t.exp_avg_sq, "parameters, gradients and moments must not be null");
             refuse_unless(state_bits == 32 || (t.scale_avg && t.scale_avg_sq), "moments in 8 bits need their scales");
@@ -263,7 +266,7 @@ extern "C" int smx_adamw_step(int param_type, int grad_type, int state_bits, con
             hip_ok(hipGetLastError(), "launch");
             a.count = 0;
         };
-        constexpr long kMostChunks = 0x3fffffff;
+        constexpr long kMostChunks = 1L << 23;      // (a launch takes fewer than 2^32 threads, a tensor at most 2^24 chunks)
         for (int i = 0; i < count; ++i) {
             if (tensors[i].numel == 0) continue;
             const long chunks = (tensors[i].numel + kChunk - 1) / kChunk;
@@ -280,13 +283,18 @@ extern "C" int smx_moment_values(long numel, const void* d_code_avg, const float
                                  float* d_exp_avg, float* d_exp_avg_sq, void* stream)
 {
     return finetune_entry("smx_moment_values", [&] {
-        refuse_unless(numel >= 0 && numel < (1L << 40), "numel: 0 to 2^40");
+        refuse_unless(numel >= 0 && numel < (1L << 36), "numel: 0 less than 2^36");
         if (numel == 0 || (!d_exp_avg && !d_exp_avg_sq)) return;
         refuse_unless((!d_exp_avg || (d_code_avg && d_scale_avg)) && (!d_exp_avg_sq || (d_code_avg_sq && d_scale_avg_sq)), "codes and scales must not be null");
         require_gfx950();
-        hipLaunchKernelGGL(k_moment_values, dim3((unsigned)((numel + 1023) / 1024)), dim3(256), 0, static_cast<hipStream_t>(stream), numel,
-                           static_cast<const int8_t*>(d_code_avg), d_scale_avg, static_cast<const uint8_t*>(d_code_avg_sq), d_scale_avg_sq, d_exp_avg,
-                           d_exp_avg_sq);
+        constexpr long kSlab = 1L << 30;      // (a launch takes fewer than 2^32 threads; whole blocks of a scale)
+        for (long at = 0; at < numel; at += kSlab) {
+            const long n = std::min(numel - at, kSlab);
+            hipLaunchKernelGGL(k_moment_values, dim3((unsigned)((n + 1023) / 1024)), dim3(256), 0, static_cast<hipStream_t>(stream), n,
+                               d_exp_avg ? static_cast<const int8_t*>(d_code_avg) + at : nullptr, d_exp_avg ? d_scale_avg + at / kBlock : nullptr,
+                               d_exp_avg_sq ? static_cast<const uint8_t*>(d_code_avg_sq) + at : nullptr, d_exp_avg_sq ? d_scale_avg_sq + at / kBlock : nullptr,
+                               d_exp_avg ? d_exp_avg + at : nullptr, d_exp_avg_sq ? d_exp_avg_sq + at : nullptr);
+        }
         hip_ok(hipGetLastError(), "launch");
     });
 }

@@ -4,8 +4,13 @@
 //   g = c_a B_a^T dy:   dx = W^T dy + A_a^T g,   dA_a = sum over the adapter's rows of g x^T,   dB_a = sum of dy h^T
 //
 // Forward: h of all rows (k_down), then one product that adds the adapters' part to its sums before they are rounded and stored
-// (k_product16, k_product32; few rows: k_down_few, k_product_few).  Gradient: h and g, the product with W^T, and for dA and dB the rows
-// sorted by adapter (k_group_*), sums over pieces of an adapter's rows (k_outer), and the sums of those (k_join).
+// (k_product16, k_product32 with k_add_mixed; long sums of few tiles in parts, k_join_splits; few rows: k_down_few, k_product_few).
+// Gradient: h and g, the product with W^T, and for dA and dB the rows sorted by adapter (counted in k_prepare, placed beside k_down), sums
+// over pieces of an adapter's rows (k_outer), and the sums of those (k_join).  k_prepare also lays out the operands that the products
+// cannot take as they are: W^T, rows that are not aligned, single precision in its parts.
+//
+// What bounds it: 16-bit products of many rows the matrix instructions (8 179 rows, 4 096 x 4 096 in bfloat16: 250 us a call, 1.10
+// PFLOP/s, of which k_down 27), few rows the bytes of W (16 rows of the same: 8.4 us for the product's 34 MB, 4.0 TB/s), single precision the six bf16 products a product is made of (50 000 rows, 256 -> 512: 111 us, 119 TFLOP/s).
 //
 // Rows are taken as they come in the first two: sixteen of them share a matrix instruction, and every adapter that occurs among them is
 // gone through, its result kept by its own rows alone (a choice, not a product with zero: infinities and NaN of an adapter stay with
@@ -81,7 +86,8 @@ __device__ __forceinline__ bool has_adapter(int a, int n) { return a >= 0 && a <
 __device__ __forceinline__ bool is_bad(int a, int n) { return a < -1 || a >= n; }
 
 constexpr int kPiece = 32;           // terms of a sum that a step of a product takes
-constexpr int kMostFew = 64;         // rows of the kernels for few rows
+// Rows of the kernels for few rows (64 rows, 4 096 x 4 096 in bfloat16: 20 us, and 38 with the others).
+constexpr int kMostFew = 64;
 
 // ---- operands laid out anew: rows of a multiple of 32 numbers, zeros behind the last; single precision for products in three bf16 parts
 
@@ -294,7 +300,9 @@ struct Downs {
     Groups groups;
 };
 
-// A block takes 16 MT rows; its wavefronts have 128 bytes of a row by turns, and their sums are added in order.
+// A block takes 16 MT rows; its wavefronts have 128 bytes of a row by turns, and their sums are added in order.  The next 128 bytes are under
+// way during the sums of these.  Bound by the latency of loads, with few wavefronts on a CU: 67 MB of rows in 27 us (8 179 rows of 4 096
+// numbers in bfloat16, 24 adapters of rank 32), 51 MB in 13 (50 000 rows of 256 in single precision, 4.0 TB/s).
 template <typename T, int RT, int MT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void k_down(const Downs both)
 {
@@ -451,7 +459,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_down(const Downs both)
     }
 }
 
-// Few rows: a wavefront per number of h.
+// Few rows: a wavefront per number of h.  (16 rows of 4 096 numbers: 3.6 us, a chain of a load, a sum and a store.)
 template <typename T>
 __global__ __launch_bounds__(256) void k_down_few(const Down p)
 {
@@ -520,7 +528,7 @@ __device__ __forceinline__ bool tile_of(const Product& p, int& rt, int& ct)
 template <typename T>
 __device__ __forceinline__ int column_of(int t, int m) { return std::is_same_v<T, float> ? 16 * t + m : 32 * (t >> 1) + 8 * (m >> 2) + 4 * (t & 1) + (m & 3); }
 
-// The product of a factor's columns and rows of h, 32 r at a time (single precision: 16).  Sixteen bits: on the bf16 instructions, h in two
+// The product of a factor's columns and rows of h, 32 r at a time, for 16-bit types: on the bf16 instructions, h in two
 // bf16 parts (what is left out is below 2^-16 of a product; the result is rounded to 2^-9 or 2^-11), and numbers of float16 in two, which
 // hold them exactly.
 template <typename T>
@@ -670,18 +678,17 @@ __device__ __forceinline__ int one_adapter(const Product& p, int lane, long row0
 }
 
 // Adds the adapters' part to sums of NM tiles of 16 rows and NT of 16 columns.  For every tile of rows one adapter after the other of
-// those that occur in it, four tiles of columns at a time; a factor that is held as a whole stays for the next tile of rows.
+// those that occur in it; a factor that is held as a whole stays for the next tile of rows.
 template <typename T, int NM, int NT>
 __device__ __forceinline__ void add_adapters(const Product& p, int lane, long row0, int col0, f32x4 (&acc)[NM][NT])
 {
     typedef AdapterProduct<T> Op;
-    constexpr int GT = NT < 4 ? NT : 4;
     const int n = lane & 15;
     __builtin_amdgcn_sched_barrier(0);
     int a = p.index[min(row0 + n, p.rows - 1)];
     typename Op::Row first = Op::row(p, row0, 0, lane);
     int held = -1;
-    typename Op::Factor f[GT];
+    typename Op::Factor f[NT];
 #pragma unroll
     for (int i = 0; i < NM; ++i) {
         const bool good = row0 + 16 * i + n < p.rows && has_adapter(a, p.adapters);
@@ -693,21 +700,17 @@ __device__ __forceinline__ void add_adapters(const Product& p, int lane, long ro
             left &= ~whose;
             for (int r0 = 0; r0 < p.rank; r0 += Op::CHUNK) {
                 const typename Op::Row hr = r0 == 0 ? first : Op::row(p, row0 + 16 * i, r0, lane);
+                if (cur != held || r0 > 0) {
 #pragma unroll
-                for (int t0 = 0; t0 < NT; t0 += GT) {
-                    if (NT > GT || cur != held || r0 > 0) {
+                    for (int t = 0; t < NT; ++t)
+                        f[t] = Op::factor(p, static_cast<const T*>(p.F) + cur * p.f_each, col0, t, r0, lane);
+                    held = p.rank <= Op::CHUNK ? cur : -1;
+                }
 #pragma unroll
-                        for (int t = 0; t < GT; ++t)
-                            f[t] = Op::factor(p, static_cast<const T*>(p.F) + cur * p.f_each, col0, t0 + t, r0, lane);
-                        held = p.rank <= Op::CHUNK ? cur : -1;
-                    }
+                for (int t = 0; t < NT; ++t) {
+                    const f32x4 sum = Op::run(f[t], hr, f32x4{0, 0, 0, 0});
 #pragma unroll
-                    for (int t = 0; t < GT; ++t) {
-                        const f32x4 sum = Op::run(f[t], hr, f32x4{0, 0, 0, 0});
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) acc[i][t0 + t][j] += mine ? sum[j] : 0.0f;
-                    }
-                    if (NT > GT) __builtin_amdgcn_sched_barrier(0);
+                    for (int j = 0; j < 4; ++j) acc[i][t][j] += mine ? sum[j] : 0.0f;
                 }
             }
         }
@@ -769,6 +772,9 @@ __device__ __forceinline__ void store_partial(const Product& p, int lane, long r
 // 16-bit types.  Tiles of 64 terms come straight from memory into LDS, STAGES of them under way; WM x WN wavefronts share the tile.
 // A load brings eight rows of 128 bytes; the 16-byte pieces of a row lie in an order that depends on the row, so that lanes that read
 // together meet different banks.  A step of 32 terms has its operands fetched during the step before.
+// Bound by the matrix instructions: 8 179 rows, 4 096 x 4 096 in bfloat16, rank 32: 240 to 265 us with the adapters' part, 1.03 to 1.14 PFLOP/s;
+// 4 091 rows, 2 048 x 2 048 in float16: 46 us, 0.75.  Tiles of 256 x 256 need half the bytes of 128 x 128 ones for a product but leave CUs without
+// work where there are few: the first 268 us, and 316 in tiles of 128 x 128; the second (128 of the large tiles) 63, and 46.
 template <typename T, int BM, int BN, int WM, int WN, int STAGES>
 __global__ __launch_bounds__(64 * WM * WN, 2) void k_product16(const Product p)
 {
@@ -907,6 +913,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_product16(const Product p)
 // small ones are normal numbers; sums that are not finite for it, or are not at all, are formed again in single precision.
 // A wavefront has 16 NM rows of its own, which it reads and splits in registers, a step of 32 terms ahead; W's parts, split beforehand, lie
 // in memory as they go into LDS, where the four wavefronts share them.
+// Six bf16 products a product: 50 000 rows, 256 -> 512 in 80 us, 164 TFLOP/s of single precision, 0.98 PFLOP/s of the instructions; the splits
+// beside them and the short sums (eight steps, then 128 x 128 numbers to store) keep it from more.  The 154 TFLOP/s that a large product on the
+// single-precision instructions reaches would be 85 us.
 template <int NM, int NT>
 __global__ __launch_bounds__(256, NM == 1 ? 4 : 3) void k_product32(const Product p)
 {
@@ -1116,7 +1125,8 @@ __global__ __launch_bounds__(256) void k_join_splits(const Product p)
     static_cast<T*>(p.out)[row * p.out_stride + col] = is_bad(a, p.adapters) ? (T)std::numeric_limits<float>::quiet_NaN() : (T)sum;
 }
 
-// Few rows: a block takes 16 columns and all rows; eight wavefronts have 128 bytes of W's rows by turns.
+// Few rows: a block takes 16 columns and all rows; eight wavefronts have 128 bytes of W's rows by turns, four units of them under way.
+// Bound by W's bytes: 16 rows, 4 096 x 4 096 in bfloat16: 8.4 us, 4.0 TB/s.
 template <typename T, int MT>
 __global__ __launch_bounds__(512) void k_product_few(const Product p)
 {
@@ -1222,7 +1232,9 @@ struct Outers {
     Outer outer[2];
     int blocks[2];      // of columns
 };
-// A block takes a piece, 64 r at most, and 64 V columns; a wavefront 16 V of them, four rows at a time.
+// A block takes a piece, 64 r at most, and 64 V columns; a wavefront 16 V of them, four rows at a time, in single precision whatever the
+// type.  Rows are read once for each 64 r; with the rows' indirection, bound by the latency of loads: 18 us for 4 091 rows of 2 048 and
+// 2 048 numbers in float16, 14 for 20 011 of 256 and 512 in single precision (61 MB, 4.3 TB/s).
 template <typename T, int RT>
 __global__ __launch_bounds__(256) void k_outer(const Outers both)
 {
@@ -1318,7 +1330,7 @@ void check(const smx_adapted_linear* p)
 {
     refuse_unless(p, "the description must not be null");
     (void)type_bytes(p->type);
-    refuse_unless(p->rows >= 0 && p->rows <= 0x7fffffffL - 4096, "rows: 0 to 2^31 - 4097");
+    refuse_unless(p->rows >= 0 && p->rows <= 1L << 28, "rows: 0 to 2^28");
     refuse_unless(p->d_in >= 1 && p->d_out >= 1 && p->d_in <= (1 << 20) && p->d_out <= (1 << 20), "d_in and d_out: 1 to 2^20");
     refuse_unless(p->rank >= 1 && p->rank <= SMX_ADAPTER_MAX_RANK, "rank: 1 to 128");
     refuse_unless(p->num_adapters >= 0 && p->num_adapters <= SMX_ADAPTER_MAX_COUNT, "num_adapters: 0 to 4096");
@@ -1376,7 +1388,7 @@ struct Call {
     void flush_layouts(bool count = false)
     {
         const long blocks = prepare.blocks[0] + prepare.blocks[1] + (count ? prepare.groups.blocks : 0);
-        refuse_unless(blocks <= 0x7fffffffL, "more blocks than a launch takes");
+        refuse_unless(blocks < 1L << 24, "more blocks than a launch takes");      // (of 256 threads, of which there are fewer than 2^32)
         if (!dry && blocks) hipLaunchKernelGGL((k_prepare<T>), dim3((unsigned)blocks), dim3(256), 0, s, prepare);
         prepare.blocks[0] = prepare.blocks[1] = 0;
         num_layouts = 0;
@@ -1390,13 +1402,12 @@ struct Call {
     template <typename T>
     void flush_downs(bool place)
     {
-        if (dry) return;
         auto go = [&](auto rt, auto mt, auto waves) {
             constexpr int RT = decltype(rt)::value, MT = decltype(mt)::value, WAVES = decltype(waves)::value;
             for (int i = 0; i < num_downs; ++i) downs.blocks[i] = (int)up((p.rows + 16 * MT - 1) / (16 * MT), 8);
             const long blocks = (long)downs.blocks[0] + downs.blocks[1] + (place ? downs.groups.blocks : 0);
-            refuse_unless(blocks <= 0x7fffffffL, "more blocks than a launch takes");
-            if (blocks) hipLaunchKernelGGL((k_down<T, RT, MT, WAVES>), dim3((unsigned)blocks), dim3(64 * WAVES), 0, s, downs);
+            refuse_unless(blocks * 64 * WAVES < 1L << 32, "more blocks than a launch takes");
+            if (!dry && blocks) hipLaunchKernelGGL((k_down<T, RT, MT, WAVES>), dim3((unsigned)blocks), dim3(64 * WAVES), 0, s, downs);
         };
         // Wavefronts of a block share its sums.  Few blocks leave most of the chip without work, so they get more wavefronts: 8 where the
         // sums are long (4 091 rows of 2 048 and 2 048 in f16: 12.1 us with 8 of 32 rows, 13.6 with 16 of 16 rows), and below 4 096 rows in
@@ -1421,10 +1432,11 @@ struct Call {
         q.splits = 1;
         q.split_steps = q.k_padded / kPiece + 1;
         if (few) return q;
-        // Few tiles and long sums: the sums in parts of at least eight steps, until there are two blocks for every CU.
+        // Few tiles and long sums: the sums in parts of at least eight steps, until there are two blocks for every CU.  (40 tiles of 128 steps in
+        // bfloat16: 12 us with the joining, 23 without parts; 176 tiles of 64 steps: 18 and 15.)
         const long few_tiles = (p.rows + 63) / 64 * ((cols + 63) / 64);
         const int steps = q.k_padded / kPiece;
-        if (few_tiles <= 192 && steps >= 16) {
+        if (few_tiles <= 128 && steps >= 16) {
             q.split_steps = (int)std::max(8L, up((steps * few_tiles + 511) / 512, 2));
             q.splits = (steps + q.split_steps - 1) / q.split_steps;
             if (q.splits > 1) q.partial = arena.take<float>(q.splits * p.rows * cols);
@@ -1466,11 +1478,12 @@ struct Call {
         };
         auto blocks = [&] {
             const long t = (long)q.row_tiles * q.col_tiles;
-            refuse_unless(t < 0x7ffffff0L / 8, "more tiles than a launch takes");
+            refuse_unless(t < 1L << 22, "more tiles than a launch takes");
             return dim3((unsigned)((t + 7) / 8 * 8));
         };
         // Tiles that run at once are done at about the same time: where those of the last such round are few, their rows get a launch of
-        // smaller tiles.  (What is left for it is in q then, and whether there is anything.)
+        // smaller tiles: 8 500 rows, 4 096 x 4 096 in bfloat16, 544 tiles of 256 x 256: 256 + 32 us, and 326 in one launch.  (What is left for it
+        // is in q then; the answer is whether there is anything.)
         auto rounds = [&](int tile_rows, int tile_cols, long at_once, auto&& go) {
             const long all = tiles(tile_rows, tile_cols), over = all % at_once;
             const long main_rows = all > at_once && over > 0 && over <= at_once / 2 ? (all - over) / q.col_tiles * tile_rows : q.rows;
@@ -1494,6 +1507,7 @@ struct Call {
                 join();
                 return;
             }
+            // (large tiles from one for every CU on: 4 090 rows, 1 024 x 1 024: 56 us, and 60 in small ones; 1 500 rows: 50, and 29)
             const bool wide = tiles(128, 128) >= 256;
             if (wide) hipLaunchKernelGGL((k_product32<2, 8>), blocks(), dim3(256), 0, s, q);
             else {
@@ -1517,6 +1531,8 @@ struct Call {
                 join();
                 return;
             }
+            // Tiles as large as keep three quarters of the CUs busy (figures at k_product16; 512 tiles of 128 x 128: 46 us, and 67 in tiles of
+            // 64 x 64; 96 of them: 23, and 14).
             if (tiles(256, 256) >= 192 && !rounds(256, 256, 256, [&] { go(Int<256>{}, Int<256>{}, Int<2>{}, Int<4>{}, Int<2>{}); })) return;
             if (tiles(128, 128) >= 192 && !rounds(128, 128, 512, [&] { go(Int<128>{}, Int<128>{}, Int<2>{}, Int<2>{}, Int<2>{}); })) return;
             tiles(64, 64);

@@ -5,6 +5,9 @@
 //
 // A row lies in the registers of a group of lanes, or of a block, between its sums and its output, so that memory is read once;
 // the variance is summed from centered values.  All sums are in single precision.
+//
+// What bounds it is memory: forward 55 us for 16 381 rows of 4 096 numbers in bfloat16 (268 MB, 4.9 TB/s), gradient 49 us a call for
+// 50 000 rows of 256 in single precision (154 MB, 3.1 TB/s with the joining of the parts); a few rows cost a launch, 10 us a call.
 #include "smx_finetune.hpp"
 
 #include <algorithm>
@@ -305,6 +308,7 @@ __global__ __launch_bounds__(256) void k_norm_join(const float* partial, int par
 
 constexpr long kMostDim = 1L << 24;      // of a row
 constexpr long kMostRows = 0x7fffffffL;
+constexpr long kMostBlocks = 1L << 22;      // of a launch, which takes fewer than 2^32 threads
 
 constexpr long kMostHeld = 256 * 32;       // numbers of a row that a block holds in registers
 
@@ -317,7 +321,8 @@ long parts_of(long rows, long dim)
     return std::min<long>((rows + per - 1) / per, 1024);
 }
 
-// fn(V, NV, G, WAVES) as integral constants: how a row of dim numbers is shared
+// fn(V, NV, G, WAVES) as integral constants: how a row of dim numbers is shared.  The fewest lanes that hold it with 16 bytes each, then more
+// bytes a lane and last four wavefronts: sums inside a wavefront need no barrier, and no lane is without work while others have two runs.
 template <typename T, typename Fn>
 void shared_rows(int dim, Fn&& fn)
 {
@@ -362,19 +367,29 @@ extern "C" int smx_layer_norm_forward(int type, int weight_type, long rows, long
         refuse_unless(d_x && d_y, "x and y must not be null");
         require_gfx950();
         const hipStream_t s = static_cast<hipStream_t>(stream);
-        const NormForward p{rows, x_stride, y_stride, (int)dim, (float)eps, d_x, d_weight, d_bias, d_y, d_mean, d_rstd};
+        NormForward p{rows, x_stride, y_stride, (int)dim, (float)eps, d_x, d_weight, d_bias, d_y, d_mean, d_rstd};
         with_type(type, [&](auto t) {
             using T = decltype(t);
+            // fn(blocks) for as many rows at a time as kMostBlocks blocks take, of `per` rows each
+            auto in_slabs = [&](long per, auto&& fn) {
+                for (long left = rows; left > 0; left -= p.rows) {
+                    p.rows = std::min(left, per * kMostBlocks);
+                    fn(dim3((unsigned)((p.rows + per - 1) / per)));
+                    p.x = static_cast<const T*>(p.x) + p.rows * x_stride;
+                    p.y = static_cast<T*>(p.y) + p.rows * y_stride;
+                    if (p.mean) p.mean += p.rows;
+                    if (p.rstd) p.rstd += p.rows;
+                }
+            };
             auto go = [&](auto tw) {
                 using TW = decltype(tw);
                 if (dim > kMostHeld) {
-                    hipLaunchKernelGGL((k_norm_fwd_long<T, TW>), dim3((unsigned)rows), dim3(256), 0, s, p);
+                    in_slabs(1, [&](dim3 blocks) { hipLaunchKernelGGL((k_norm_fwd_long<T, TW>), blocks, dim3(256), 0, s, p); });
                     return;
                 }
                 shared_rows<T>((int)dim, [&](auto v, auto nv, auto g, auto waves) {
-                    constexpr int PER = decltype(waves)::value > 1 ? 1 : 256 / decltype(g)::value;
-                    hipLaunchKernelGGL((k_norm_fwd<T, TW, decltype(v)::value, decltype(nv)::value, decltype(g)::value, decltype(waves)::value>),
-                                       dim3((unsigned)((rows + PER - 1) / PER)), dim3(256), 0, s, p);
+                    constexpr int V = decltype(v)::value, NV = decltype(nv)::value, G = decltype(g)::value, WAVES = decltype(waves)::value;
+                    in_slabs(WAVES > 1 ? 1 : 256 / G, [&](dim3 blocks) { hipLaunchKernelGGL((k_norm_fwd<T, TW, V, NV, G, WAVES>), blocks, dim3(256), 0, s, p); });
                 });
             };
             if (weight_type == type) go(T{});
@@ -415,6 +430,7 @@ extern "C" int smx_layer_norm_backward(int type, int weight_type, long rows, lon
             auto go = [&](auto tw) {
                 using TW = decltype(tw);
                 if (rows > 0 && dim > kMostHeld) {
+                    refuse_unless(rows < 1L << 24, "more rows than a launch takes");      // (of more than 8 192 numbers)
                     if (d_dx) hipLaunchKernelGGL((k_norm_bwd_long<T, TW>), dim3((unsigned)rows), dim3(256), 0, s, p);
                     if (sums) hipLaunchKernelGGL((k_norm_bwd_columns<T>), dim3((unsigned)((dim + 255) / 256), (unsigned)parts), dim3(256), 0, s, p);
                 } else if (rows > 0) {

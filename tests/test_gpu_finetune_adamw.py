@@ -290,3 +290,16 @@ def test_c_entry_refuses_without_touching_a_device():
     one[0].numel = 0
     assert call() == 0
     assert L.smx_moment_values(-1, 0, 0, 0, 0, 0, 0, 0) == -1 and L.smx_moment_values(0, 0, 0, 0, 0, 0, 0, 0) == 0
+
+
+@pytest.mark.gpu
+def test_values_of_more_codes_than_a_launch_takes():
+    from symmetrix_amd import finetune
+    n = (1 << 30) + 600
+    cm, cv = torch.zeros(n, dtype=torch.int8, device="cuda"), torch.zeros(n, dtype=torch.uint8, device="cuda")
+    cm[-600:] = torch.randint(-127, 128, (600,), device="cuda").to(torch.int8)
+    cv[-600:] = torch.randint(0, 256, (600,), device="cuda").to(torch.uint8)
+    sm, sv = torch.rand((n + 255) // 256, device="cuda") + 0.5, torch.rand((n + 255) // 256, device="cuda") + 0.5
+    m, v = finetune.moment_values(cm, sm, cv, sv)
+    m0, v0 = finetune.moment_values(cm[-600:].clone(), sm[-3:].clone(), cv[-600:].clone(), sv[-3:].clone())
+    assert torch.equal(m[-600:], m0) and torch.equal(v[-600:], v0)

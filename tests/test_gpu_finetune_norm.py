@@ -293,3 +293,18 @@ def test_c_entry_refuses_without_touching_a_device():
     assert b"workspace" in L.smx_last_error()
     with pytest.raises(ValueError):
         _lib.check(-1)
+
+
+@pytest.mark.gpu
+def test_more_rows_than_a_launch_takes():
+    """Short rows share a block by 32: 2^22 blocks take 2^27 of them, the rest is another launch."""
+    from symmetrix_amd import finetune
+    rows, dim = (1 << 27) + 77, 2
+    x = torch.zeros(rows, dim, device="cuda")
+    some = torch.randn(200, dim, device="cuda")
+    x[-200:] = some
+    w, b = torch.randn(dim, device="cuda"), torch.randn(dim, device="cuda")
+    y, mean, rstd = finetune.layer_norm_forward(x, w, b)
+    y0, mean0, rstd0 = finetune.layer_norm_forward(some, w, b)
+    assert torch.equal(y[-200:], y0) and torch.equal(mean[-200:], mean0) and torch.equal(rstd[-200:], rstd0)
+    assert torch.equal(y[:1000], b.expand(1000, dim)) and (mean[:1000] == 0).all()
