@@ -6,8 +6,8 @@
 // A row lies in the registers of a group of lanes, or of a block, between its sums and its output, so that memory is read once;
 // the variance is summed from centered values.  All sums are in single precision.
 //
-// What bounds it is memory: forward 55 us for 16 381 rows of 4 096 numbers in bfloat16 (268 MB, 4.9 TB/s), gradient 49 us a call for
-// 50 000 rows of 256 in single precision (154 MB, 3.1 TB/s with the joining of the parts); a few rows cost a launch, 10 us a call.
+// What bounds it is memory: forward 55 us for 16 381 rows of 4 096 numbers in bfloat16 (268 MB, 4.9 TB/s), gradient 33 us a call for
+// 50 000 rows of 256 in single precision (154 MB, 4.7 TB/s with the joining of the parts); a few rows cost a launch, 10 us a call.
 #include "smx_finetune.hpp"
 
 #include <algorithm>
@@ -286,21 +286,24 @@ __global__ __launch_bounds__(256) void k_norm_bwd_columns(const NormBackward p)
     out[p.dim + col] = db;
 }
 
-// Sums of the blocks' parts, in order: a block takes 16 columns, 16 threads a column.
+// Sums of the blocks' parts, in order: a block takes 16 columns, 64 threads a column.  (16 threads with a load at a time: 21 us for 1 024
+// parts of 512 columns, as long as the kernel that makes them.)
 template <typename TW>
-__global__ __launch_bounds__(256) void k_norm_join(const float* partial, int parts, int dim, TW* dweight, TW* dbias)
+__global__ __launch_bounds__(1024) void k_norm_join(const float* partial, int parts, int dim, TW* dweight, TW* dbias)
 {
-    __shared__ float sums[16][17];
+    constexpr int Q = 64;
+    __shared__ float sums[Q][17];
     const int c = threadIdx.x % 16, q = threadIdx.x / 16, col = blockIdx.x * 16 + c;
     float sum = 0.0f;
     if (col < 2 * dim)
-        for (int i = q; i < parts; i += 16) sum += partial[(size_t)i * 2 * dim + col];
+#pragma unroll 8
+        for (int i = q; i < parts; i += Q) sum += partial[(size_t)i * 2 * dim + col];
     sums[q][c] = sum;
     __syncthreads();
     if (q == 0 && col < 2 * dim) {
         sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) sum += sums[i][c];
+        for (int i = 0; i < Q; ++i) sum += sums[i][c];
         TW* out = col < dim ? dweight : dbias;
         if (out) out[col < dim ? col : col - dim] = (TW)sum;
     }
@@ -443,7 +446,7 @@ extern "C" int smx_layer_norm_backward(int type, int weight_type, long rows, lon
                 }
                 hip_ok(hipGetLastError(), "launch");
                 if (sums)
-                    hipLaunchKernelGGL((k_norm_join<TW>), dim3((unsigned)((2 * dim + 15) / 16)), dim3(256), 0, s, static_cast<const float*>(d_workspace),
+                    hipLaunchKernelGGL((k_norm_join<TW>), dim3((unsigned)((2 * dim + 15) / 16)), dim3(1024), 0, s, static_cast<const float*>(d_workspace),
                                        (int)parts, (int)dim, static_cast<TW*>(d_dweight), static_cast<TW*>(d_dbias));
             };
             if (weight_type == type) go(T{});
