@@ -307,51 +307,83 @@ class AdamW:
     state_bits 32: moments in single precision; 8: in codes of 8 bits, 256 to a scale.  masters: parameters in single
     precision for params in 16 bits, a list like params; True makes them from params.  states: moments to go on with, a tuple a
     tensor, (exp_avg, exp_avg_sq) or (code_avg, scale_avg, code_avg_sq, scale_avg_sq); they are used in place, as params and
-    masters are, and so is what self.states holds otherwise (zeros at first).  step: steps taken before."""
+    masters are, and so is what self.states holds otherwise (zeros at first).  Both attributes can be assigned anew as a whole, under
+    the same checks; what a tensor of theirs or a parameter holds is looked at in every step.  step: steps taken before."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, masters=None, states=None, step=0):
-        self.params = list(params)
+        self.params = tuple(params)
         _need(state_bits in (32, 8), "state_bits: 32 or 8")
         _need(0 <= betas[0] < 1 and 0 <= betas[1] < 1, "betas: 0 up to, not including, 1")
         _need(lr >= 0 and eps >= 0 and weight_decay >= 0, "lr, eps and weight_decay: numbers from 0 on")
         _need(step >= 0, "step: steps taken before, none or more")
-        self.lr, self.betas, self.eps, self.weight_decay, self.state_bits, self.step_count = lr, tuple(betas), eps, weight_decay, state_bits, step
+        self.lr, self.betas, self.eps, self.weight_decay, self._bits, self.step_count = lr, tuple(betas), eps, weight_decay, state_bits, step
         for p in self.params:
             _type(p, "parameters")
             _need(p.is_contiguous(), "parameters: contiguous tensors expected")
             _need(p.is_cuda and p.device == self.params[0].device, "parameters on one GPU expected: there is no CPU path")
             if p.dtype != self.params[0].dtype:
                 raise TypeError("parameters of one type expected: an optimizer for each")
-        if masters is True:
-            masters = [p.detach().float() for p in self.params]
+        # what every parameter has to be in every step
+        self._shapes = [p.shape for p in self.params]
+        self._dtype, self._device = (self.params[0].dtype, self.params[0].get_device()) if self.params else (None, None)
+        self._masters = None
+        self.states = [self._zeros(p) for p in self.params] if states is None else states
+        self.masters = [p.detach().float() for p in self.params] if masters is True else masters
+
+    @property
+    def state_bits(self):
+        return self._bits
+
+    @property
+    def states(self):
+        """Moments, a tuple of tensors for every parameter."""
+        return self._states
+
+    @states.setter
+    def states(self, states):
+        states = tuple(tuple(s) for s in states)
+        _need(len(states) == len(self.params), "states: a tuple for every parameter expected")
+        self._held = [self._hold(i, states, self._masters) for i in range(len(states))]
+        self._states = states
+
+    @property
+    def masters(self):
+        """Parameters in single precision, a tuple like params, or None."""
+        return self._masters
+
+    @masters.setter
+    def masters(self, masters):
         if masters is not None:
-            masters = list(masters)
+            masters = tuple(masters)
             _need(len(masters) == len(self.params), "masters: one for every parameter expected")
-            for m, p in zip(masters, self.params):
-                _need(p.dtype != torch.float32, "masters are for parameters in 16 bits")
-                _need(m.dtype == torch.float32 and m.shape == p.shape and m.is_contiguous() and m.device == p.device,
-                      "masters: contiguous, float32, of the parameters' shapes and on their device expected")
-        self.masters = masters
-        if states is None:
-            states = [self._zeros(p) for p in self.params]
-        self.states = [tuple(s) for s in states]
-        _need(len(self.states) == len(self.params), "states: a tuple for every parameter expected")
-        kinds = (torch.float32, torch.float32) if state_bits == 32 else (torch.int8, torch.float32, torch.uint8, torch.float32)
-        for s, p in zip(self.states, self.params):
-            n = p.numel()
-            counts = (n, n) if state_bits == 32 else (n, -(-n // MOMENT_BLOCK)) * 2
-            _need(len(s) == len(kinds) and all(t.dtype == k and t.numel() == c and t.is_contiguous() and t.device == p.device
-                                               for t, k, c in zip(s, kinds, counts)),
-                  "states: (exp_avg, exp_avg_sq) in float32, or (code_avg int8, scale_avg float32, code_avg_sq uint8, scale_avg_sq float32), "
-                  "contiguous and on the parameters' device, expected")
-        at = (0, 1) if state_bits == 32 else (0, 2, 1, 3)          # of a state: moments, then their scales
-        self._fixed = [(0 if masters is None else self.masters[i].data_ptr(), *(s[k].data_ptr() for k in at), *((0, 0) if state_bits == 32 else ()), p.numel())
-                       for i, (s, p) in enumerate(zip(self.states, self.params))]
+        self._held = [self._hold(i, self._states, masters) for i in range(len(self.params))]
+        self._masters = masters
+
+    def _hold(self, i, states, masters):
+        """A parameter's part of smx_adamw_tensor, and aliases of the tensors that it names.  The aliases keep the memory, so that none of
+        the addresses is ever that of memory that others use; a tensor that was given other memory has another address, which is
+        compared in every step."""
+        n, bits, s = self._shapes[i].numel(), self._bits, states[i]
+        kinds = (torch.float32, torch.float32) if bits == 32 else (torch.int8, torch.float32, torch.uint8, torch.float32)
+        counts = (n, n) if bits == 32 else (n, -(-n // MOMENT_BLOCK)) * 2
+        _need(len(s) == len(kinds) and all(t.dtype == k and t.numel() == c and t.is_contiguous() and t.get_device() == self._device
+                                           for t, k, c in zip(s, kinds, counts)),
+              "states: (exp_avg, exp_avg_sq) in float32, or (code_avg int8, scale_avg float32, code_avg_sq uint8, scale_avg_sq float32), "
+              "contiguous and on the parameters' device, expected")
+        held = s
+        if masters is not None:
+            m = masters[i]
+            _need(self._dtype != torch.float32, "masters are for parameters in 16 bits")
+            _need(m.dtype == torch.float32 and m.shape == self._shapes[i] and m.is_contiguous() and m.get_device() == self._device,
+                  "masters: contiguous, float32, of the parameters' shapes and on their device expected")
+            held = (*s, m)
+        at = (0, 1) if bits == 32 else (0, 2, 1, 3)          # of a state: moments, then their scales
+        return (0 if masters is None else m.data_ptr(), *(s[k].data_ptr() for k in at), *((0, 0) if bits == 32 else ()), n), [t.detach() for t in held]
 
     def _zeros(self, p):
         n, blocks = p.numel(), -(-p.numel() // MOMENT_BLOCK)
         make = lambda k, dtype: torch.zeros(k, dtype=dtype, device=p.device)          # noqa: E731
-        if self.state_bits == 32:
+        if self._bits == 32:
             return make(n, torch.float32), make(n, torch.float32)
         return make(n, torch.int8), make(blocks, torch.float32), make(n, torch.uint8), make(blocks, torch.float32)
 
@@ -363,23 +395,30 @@ class AdamW:
         _need(len(grads) == len(self.params), "a gradient (or None) for every parameter expected")
         taken = [i for i, g in enumerate(grads) if g is not None]
         if taken:
-            params, device = self.params, self.params[0].get_device()
-            kind, own = grads[taken[0]].dtype, self.params[0].dtype
+            params, device, own = self.params, self._device, self._dtype
+            kind = grads[taken[0]].dtype
             if kind != own and kind != torch.float32:
                 raise TypeError(f"gradients: {own} or float32, not {kind}")
-            table, keep = bytearray(len(taken) * _ADAMW_TENSOR.size), []
+            table, keep, wide = bytearray(len(taken) * _ADAMW_TENSOR.size), [], self._bits == 32
+            shapes, held, states, masters = self._shapes, self._held, self._states, self._masters
             for at, i in enumerate(taken):
-                p, g = params[i], grads[i]
-                if g.dtype != kind:
-                    raise TypeError("gradients of one type expected")
-                if g.shape != p.shape or g.get_device() != device:
+                p, g, shape, s = params[i], grads[i], shapes[i], states[i]
+                if p.dtype != own or g.dtype != kind:
+                    raise TypeError(f"parameters in {own}, as they were at first, and gradients of one type expected")
+                if p.shape != shape or p.get_device() != device or not p.is_contiguous():
+                    raise ValueError("parameters contiguous, and of the shapes and on the device they had at first, expected")
+                if g.shape != shape or g.get_device() != device:
                     raise ValueError("gradients of the parameters' shapes and on their device expected")
                 if not g.is_contiguous():
                     g = g.contiguous()
                     keep.append(g)
-                master, m, v, scale_m, scale_v, n = self._fixed[i]
+                master, m, v, scale_m, scale_v, n = held[i][0]
+                if (s[0].data_ptr() != m or (s[1].data_ptr() != v if wide else s[2].data_ptr() != v or s[1].data_ptr() != scale_m or s[3].data_ptr() != scale_v)
+                        or (masters is not None and masters[i].data_ptr() != master)):
+                    held[i] = self._hold(i, states, masters)
+                    master, m, v, scale_m, scale_v, n = held[i][0]
                 _ADAMW_TENSOR.pack_into(table, at * _ADAMW_TENSOR.size, p.data_ptr(), g.data_ptr(), master, m, v, scale_m, scale_v, n)
-            _call(device, _lib_functions().smx_adamw_step, _TYPES[own], _TYPES[kind], self.state_bits, bytes(table), len(taken), self.lr, self.betas[0],
+            _call(device, _lib_functions().smx_adamw_step, _TYPES[own], _TYPES[kind], self._bits, bytes(table), len(taken), self.lr, self.betas[0],
                   self.betas[1], self.eps, self.weight_decay, self.step_count + 1)
             # (as torch's own operations in place do: a backward pass that saved the old values says so)
             torch.autograd.graph.increment_version(params if len(taken) == len(params) else [params[i] for i in taken])
