@@ -1365,13 +1365,23 @@ struct Call {
     const smx_adapted_linear& p;
     hipStream_t s;
     Arena arena;
-    const bool dry;      // nothing is launched, the workspace is counted
+    const bool dry;      // nothing is launched, the workspace is counted, and the sizes of the launches are looked at
     const int padded;
     Prepare prepare{};
     Downs downs{};
     int num_layouts = 0, num_downs = 0;
     Call(const smx_adapted_linear& p_, void* base, hipStream_t s_, bool dry_)
         : p(p_), s(s_), arena{static_cast<char*>(base)}, dry(dry_), padded((int)up(p_.rank, 16)) {}
+
+    // Every launch, also of a call that counts its workspace and launches nothing: sizes that a launch does not take are refused there,
+    // before the call has enqueued anything.
+    template <typename... P, typename... A>
+    void start(void (*kernel)(P...), long x, long y, long z, int threads, unsigned lds, const A&... args)
+    {
+        refuse_unless(x >= 1 && y >= 1 && z >= 1, "a launch of no blocks");
+        refuse_unless(x * threads < 1L << 32 && y <= 65535 && z <= 65535, "more blocks than a launch takes");
+        if (!dry) hipLaunchKernelGGL(kernel, dim3((unsigned)x, (unsigned)y, (unsigned)z), dim3(threads), lds, s, args...);
+    }
 
     template <typename T>
     void lay_out(const void* src, long src_each, long src_row, long src_k, void* dst, bool parts, long rows, int k, int matrices)
@@ -1388,8 +1398,7 @@ struct Call {
     void flush_layouts(bool count = false)
     {
         const long blocks = prepare.blocks[0] + prepare.blocks[1] + (count ? prepare.groups.blocks : 0);
-        refuse_unless(blocks < 1L << 24, "more blocks than a launch takes");      // (of 256 threads, of which there are fewer than 2^32)
-        if (!dry && blocks) hipLaunchKernelGGL((k_prepare<T>), dim3((unsigned)blocks), dim3(256), 0, s, prepare);
+        if (blocks) start(k_prepare<T>, blocks, 1, 1, 256, 0, prepare);
         prepare.blocks[0] = prepare.blocks[1] = 0;
         num_layouts = 0;
     }
@@ -1406,8 +1415,7 @@ struct Call {
             constexpr int RT = decltype(rt)::value, MT = decltype(mt)::value, WAVES = decltype(waves)::value;
             for (int i = 0; i < num_downs; ++i) downs.blocks[i] = (int)up((p.rows + 16 * MT - 1) / (16 * MT), 8);
             const long blocks = (long)downs.blocks[0] + downs.blocks[1] + (place ? downs.groups.blocks : 0);
-            refuse_unless(blocks * 64 * WAVES < 1L << 32, "more blocks than a launch takes");
-            if (!dry && blocks) hipLaunchKernelGGL((k_down<T, RT, MT, WAVES>), dim3((unsigned)blocks), dim3(64 * WAVES), 0, s, downs);
+            if (blocks) start(k_down<T, RT, MT, WAVES>, blocks, 1, 1, 64 * WAVES, 0, downs);
         };
         // Wavefronts of a block share its sums.  Few blocks leave most of the chip without work, so they get more wavefronts: 8 where the
         // sums are long (4 091 rows of 2 048 and 2 048 in f16: 12.1 us with 8 of 32 rows, 13.6 with 16 of 16 rows), and below 4 096 rows in
@@ -1463,9 +1471,8 @@ struct Call {
     template <typename T>
     void launch(Product q, bool few)
     {
-        if (dry) return;
         if (few) {
-            auto go = [&](auto mt) { hipLaunchKernelGGL((k_product_few<T, decltype(mt)::value>), dim3((q.cols + 15) / 16), dim3(512), 0, s, q); };
+            auto go = [&](auto mt) { start(k_product_few<T, decltype(mt)::value>, (q.cols + 15) / 16, 1, 1, 512, 0, q); };
             if (p.rows <= 16) go(Int<1>{});
             else if (p.rows <= 32) go(Int<2>{});
             else go(Int<4>{});
@@ -1476,17 +1483,14 @@ struct Call {
             q.col_tiles = (q.cols + tile_cols - 1) / tile_cols;
             return (long)q.row_tiles * q.col_tiles;
         };
-        auto blocks = [&] {
-            const long t = (long)q.row_tiles * q.col_tiles;
-            refuse_unless(t < 1L << 22, "more tiles than a launch takes");
-            return dim3((unsigned)((t + 7) / 8 * 8));
-        };
+        auto blocks = [&] { return up((long)q.row_tiles * q.col_tiles, 8); };
         // Tiles that run at once are done at about the same time: where those of the last such round are few, their rows get a launch of
         // smaller tiles: 8 500 rows, 4 096 x 4 096 in bfloat16, 544 tiles of 256 x 256: 256 + 32 us, and 326 in one launch.  (What is left for it
-        // is in q then; the answer is whether there is anything.)
+        // is in q then; the answer is whether there is anything.)  Where not one row of tiles fits into the full rounds all stay in one launch:
+        // 200 rows, 1 024 -> 65 792: 79 us, and 89 in smaller tiles; 100 rows to 70 000: 79 and 52.
         auto rounds = [&](int tile_rows, int tile_cols, long at_once, auto&& go) {
             const long all = tiles(tile_rows, tile_cols), over = all % at_once;
-            const long main_rows = all > at_once && over > 0 && over <= at_once / 2 ? (all - over) / q.col_tiles * tile_rows : q.rows;
+            const long full_rows = over > 0 && over <= at_once / 2 ? (all - over) / q.col_tiles * tile_rows : 0, main_rows = full_rows > 0 ? full_rows : q.rows;
             const Product whole = q;
             q.rows = main_rows;
             tiles(tile_rows, tile_cols);
@@ -1499,31 +1503,30 @@ struct Call {
             q.index += main_rows;
             return q.rows > 0;
         };
-        auto join = [&] { hipLaunchKernelGGL((k_join_splits<T>), dim3((unsigned)q.rows, (q.cols + 255) / 256), dim3(256), 0, s, q); };
+        auto join = [&] { start(k_join_splits<T>, q.rows, (q.cols + 255) / 256, 1, 256, 0, q); };
         if constexpr (std::is_same_v<T, float>) {
             if (q.splits > 1) {
                 tiles(64, 64);
-                hipLaunchKernelGGL((k_product32<1, 4>), dim3(blocks().x, q.splits), dim3(256), 0, s, q);
+                start(k_product32<1, 4>, blocks(), q.splits, 1, 256, 0, q);
                 join();
                 return;
             }
             // (large tiles from one for every CU on: 4 090 rows, 1 024 x 1 024: 56 us, and 60 in small ones; 1 500 rows: 50, and 29)
             const bool wide = tiles(128, 128) >= 256;
-            if (wide) hipLaunchKernelGGL((k_product32<2, 8>), blocks(), dim3(256), 0, s, q);
+            if (wide) start(k_product32<2, 8>, blocks(), 1, 1, 256, 0, q);
             else {
                 tiles(64, 64);
-                hipLaunchKernelGGL((k_product32<1, 4>), blocks(), dim3(256), 0, s, q);
+                start(k_product32<1, 4>, blocks(), 1, 1, 256, 0, q);
             }
             const int group = wide ? 32 : 16;
-            if (p.num_adapters)
-                hipLaunchKernelGGL(k_add_mixed, dim3((unsigned)((q.rows + group - 1) / group), (q.cols + 255) / 256, group / 8), dim3(256), 0, s, q, group);
+            if (p.num_adapters) start(k_add_mixed, (q.rows + group - 1) / group, (q.cols + 255) / 256, group / 8, 256, 0, q, group);
         } else {
             auto go = [&](auto bm, auto bn, auto wm, auto wn, auto stages) {
                 constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value, WM = decltype(wm)::value, WN = decltype(wn)::value, S = decltype(stages)::value;
                 constexpr int bytes = S * (BM + BN) * 128;
-                if constexpr (bytes > 64 * 1024)
+                if (bytes > 64 * 1024 && !dry)
                     hip_ok(hipFuncSetAttribute(reinterpret_cast<const void*>(&k_product16<T, BM, BN, WM, WN, S>), hipFuncAttributeMaxDynamicSharedMemorySize, bytes), "LDS");
-                hipLaunchKernelGGL((k_product16<T, BM, BN, WM, WN, S>), dim3(blocks().x, q.splits), dim3(64 * WM * WN), bytes, s, q);
+                start(k_product16<T, BM, BN, WM, WN, S>, blocks(), q.splits, 1, 64 * WM * WN, bytes, q);
             };
             if (q.splits > 1) {
                 tiles(64, 64);
@@ -1550,7 +1553,7 @@ struct Call {
         flush_layouts<T>();
         down(x, p.x_stride, A, (long)p.rank * p.d_in, p.d_in, p.d_in, h);
         if (!few) flush_downs<T>(false);
-        else if (!dry) hipLaunchKernelGGL((k_down_few<T>), dim3((unsigned)p.rows, padded / 4), dim3(256), 0, s, downs.down[0]);
+        else start(k_down_few<T>, p.rows, padded / 4, 1, 256, 0, downs.down[0]);
         launch<T>(q, few);
     }
 
@@ -1595,7 +1598,7 @@ struct Call {
         flush_layouts<T>(sums);
         flush_downs<T>(sums);
         if (want_x) launch<T>(q, false);
-        if (!sums || dry) return;
+        if (!sums) return;
         Outers both{};
         Outer o{};
         o.start = groups.start; o.first = groups.first; o.perm = groups.perm; o.adapters = n; o.rank = p.rank; o.padded = padded; o.piece = groups.piece;
@@ -1610,12 +1613,12 @@ struct Call {
         if (want_a) add(x, p.x_stride, g, p.d_in, partial_a, dA, each_a, p.d_in, 1);
         if (want_b) add(dy, dy_stride, h, p.d_out, partial_b, dB, each_b, 1, p.rank);
         if (rows) {
-            const dim3 grid((unsigned)most, across, (p.rank + 63) / 64);
-            if (padded == 16) hipLaunchKernelGGL((k_outer<T, 1>), grid, dim3(256), 0, s, both);
-            else if (padded == 32) hipLaunchKernelGGL((k_outer<T, 2>), grid, dim3(256), 0, s, both);
-            else hipLaunchKernelGGL((k_outer<T, 4>), grid, dim3(256), 0, s, both);
+            auto go = [&](auto kernel) { start(kernel, most, across, (p.rank + 63) / 64, 256, 0, both); };
+            if (padded == 16) go(k_outer<T, 1>);
+            else if (padded == 32) go(k_outer<T, 2>);
+            else go(k_outer<T, 4>);
         }
-        hipLaunchKernelGGL((k_join<T>), dim3((unsigned)(((long)p.rank * widest + 63) / 64), n, num), dim3(256), 0, s, both);
+        start(k_join<T>, ((long)p.rank * widest + 63) / 64, n, num, 256, 0, both);
     }
 };
 
