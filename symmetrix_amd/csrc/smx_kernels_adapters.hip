@@ -259,6 +259,7 @@ struct Prepare {
     Layout layout[2];
     long blocks[2];
     Groups groups;
+    long first;      // which of all blocks the launch's first one is
 };
 template <typename T>
 __global__ __launch_bounds__(256) void k_prepare(const Prepare p)
@@ -267,7 +268,7 @@ __global__ __launch_bounds__(256) void k_prepare(const Prepare p)
         T tile[64][65];
         int hist[kMostKeys];
     } lds;
-    long block = blockIdx.x;
+    long block = p.first + blockIdx.x;
     if (block < p.blocks[0]) {
         lay_out<T>(p.layout[0], block, lds.tile);
         return;
@@ -298,6 +299,7 @@ struct Downs {
     Down down[2];
     int blocks[2];
     Groups groups;
+    int first;      // as in Prepare
 };
 
 // A block takes 16 MT rows; its wavefronts have 128 bytes of a row by turns, and their sums are added in order.  The next 128 bytes are under
@@ -313,7 +315,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_down(const Downs both)
         int base[kMostKeys];
     } lds;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
-    int block = blockIdx.x;
+    int block = both.first + blockIdx.x;
     if (block >= both.blocks[0] + both.blocks[1]) {
         if (wave == 0) place_rows(both.groups, block - both.blocks[0] - both.blocks[1], lane, lds.base);
         return;
@@ -1383,6 +1385,14 @@ struct Call {
         if (!dry) hipLaunchKernelGGL(kernel, dim3((unsigned)x, (unsigned)y, (unsigned)z), dim3(threads), lds, s, args...);
     }
 
+    // fn(first, some): as many blocks at a time as a launch takes of 1 024 threads
+    template <typename Fn>
+    static void in_slabs(long blocks, Fn&& fn)
+    {
+        constexpr long most = 1L << 21;
+        for (long first = 0; first < blocks; first += most) fn(first, std::min(blocks - first, most));
+    }
+
     template <typename T>
     void lay_out(const void* src, long src_each, long src_row, long src_k, void* dst, bool parts, long rows, int k, int matrices)
     {
@@ -1398,7 +1408,10 @@ struct Call {
     void flush_layouts(bool count = false)
     {
         const long blocks = prepare.blocks[0] + prepare.blocks[1] + (count ? prepare.groups.blocks : 0);
-        if (blocks) start(k_prepare<T>, blocks, 1, 1, 256, 0, prepare);
+        in_slabs(blocks, [&](long first, long some) {
+            prepare.first = first;
+            start(k_prepare<T>, some, 1, 1, 256, 0, prepare);
+        });
         prepare.blocks[0] = prepare.blocks[1] = 0;
         num_layouts = 0;
     }
@@ -1415,7 +1428,10 @@ struct Call {
             constexpr int RT = decltype(rt)::value, MT = decltype(mt)::value, WAVES = decltype(waves)::value;
             for (int i = 0; i < num_downs; ++i) downs.blocks[i] = (int)up((p.rows + 16 * MT - 1) / (16 * MT), 8);
             const long blocks = (long)downs.blocks[0] + downs.blocks[1] + (place ? downs.groups.blocks : 0);
-            if (blocks) start(k_down<T, RT, MT, WAVES>, blocks, 1, 1, 64 * WAVES, 0, downs);
+            in_slabs(blocks, [&](long first, long some) {
+                downs.first = (int)first;
+                start(k_down<T, RT, MT, WAVES>, some, 1, 1, 64 * WAVES, 0, downs);
+            });
         };
         // Wavefronts of a block share its sums.  Few blocks leave most of the chip without work, so they get more wavefronts: 8 where the
         // sums are long (4 091 rows of 2 048 and 2 048 in f16: 12.1 us with 8 of 32 rows, 13.6 with 16 of 16 rows), and below 4 096 rows in
