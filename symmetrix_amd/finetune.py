@@ -148,14 +148,19 @@ def _norm_workspace(rows, dim):
     return size.value
 
 
-def layer_norm_backward(dy, x, mean, rstd, weight=None, need=(True, True, True)):
-    """Gradients of x, weight and bias (None where `need` says so); the latter two in weight's type."""
+def layer_norm_backward(dy, x, mean, rstd, weight=None, need=(True, True, True), bias_type=None):
+    """Gradients of x, weight and bias (None where `need` says so); the latter two in weight's type, or without a weight in
+    bias_type (None: the type of x)."""
     kind = _type(x, "x")
     dim = x.shape[-1]
     _need(dy.shape == x.shape and dy.dtype == x.dtype, "dy: shape and type of x expected")
     _need(mean.dtype == rstd.dtype == torch.float32 and mean.shape == rstd.shape == x.shape[:-1] and mean.is_contiguous() and rstd.is_contiguous(),
           "mean and rstd: float32, a number a row expected")
     weights = _affine(x, dim, weight, None)
+    if bias_type is not None:
+        if bias_type not in (x.dtype, torch.float32) or (weight is not None and bias_type != weights):
+            raise TypeError(f"bias_type: {x.dtype} or float32, and weight's type, not {bias_type}")
+        weights = bias_type
     device = _on(x, dy, mean, rstd, weight)
     x_rows, rows, x_stride = _rows(x, dim, "x")
     dy_rows, _, dy_stride = _rows(dy, dim, "dy")
@@ -183,8 +188,8 @@ class _LayerNorm(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         x, weight, mean, rstd = ctx.saved_tensors
-        dx, dw, db = layer_norm_backward(dy, x, mean, rstd, weight, ctx.needs_input_grad[:3])
-        return dx, dw, db if db is None else db.to(ctx.bias_type), None
+        dx, dw, db = layer_norm_backward(dy, x, mean, rstd, weight, ctx.needs_input_grad[:3], ctx.bias_type)
+        return dx, dw, db, None
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
