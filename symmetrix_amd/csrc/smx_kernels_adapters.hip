@@ -539,15 +539,24 @@ struct AdapterProduct {
     struct Factor {
         bf16x8 part[F_PARTS];
     };
-    __device__ static __forceinline__ void parts_of(const float (&x)[8], bf16x8 (&part)[2])
+    // Whether an infinity or NaN, or what rounds to one, was among a lane's numbers.
+    struct Odd {
+        float none = 0.0f;      // NaN then,
+        unsigned bits = 0;      // or the sign's place of a half set
+        __device__ __forceinline__ bool any() const { return __any(none != none || bits & 0x80008000u); }
+    };
+    __device__ static __forceinline__ void parts_of(const float (&x)[8], bf16x8 (&part)[2], float& none)
     {
+        constexpr float most = std::numeric_limits<float>::max();
 #pragma unroll
         for (int j = 0; j < 8; j += 2) {
             const f32x2 v = {x[j], x[j + 1]};
             const bf16x2 h = __builtin_convertvector(v, bf16x2);
             f32x2 rest = v - __builtin_convertvector(h, f32x2);
-            if (rest[0] != rest[0]) rest[0] = 0.0f;      // (infinities are their first part)
-            if (rest[1] != rest[1]) rest[1] = 0.0f;
+            none = fmaf(rest[0], 0.0f, none);
+            none = fmaf(rest[1], 0.0f, none);
+            if (!(fabsf(rest[0]) <= most)) rest[0] = 0.0f;      // (infinities are their first part)
+            if (!(fabsf(rest[1]) <= most)) rest[1] = 0.0f;
             const bf16x2 l = __builtin_convertvector(rest, bf16x2);
             part[0][j] = h[0]; part[0][j + 1] = h[1];
             part[1][j] = l[0]; part[1][j + 1] = l[1];
@@ -556,7 +565,7 @@ struct AdapterProduct {
     // F(col, r) = base[col * f_col + r * f_r] for the columns of a tile, r = r0 + 8 g + 0..7; eight numbers at a time where they are side by side
     // and the rank is a multiple of eight.  (No branch depends on the lane, here and below: what is behind the rank is read from its end and
     // put to zero.)
-    __device__ static __forceinline__ Factor factor(const Product& p, const T* base, int col0, int t, int r0, int lane)
+    __device__ static __forceinline__ Factor factor(const Product& p, const T* base, int col0, int t, int r0, int lane, Odd& odd)
     {
         typename Operand<T>::type v;
         if (p.f_runs) {
@@ -574,13 +583,17 @@ struct AdapterProduct {
                 v[j] = r + j < p.rank ? x : (T)0.0f;
             }
         }
+        // (an exponent of ones carries into the sign's place)
+        typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+        const u32x4 u = (__builtin_bit_cast(u32x4, v) & 0x7fff7fffu) + (std::is_same_v<T, f16> ? 0x04000400u : 0x00800080u);
+        odd.bits |= u[0] | u[1] | u[2] | u[3];
         Factor f;
         if constexpr (F_PARTS == 1) f.part[0] = v;
         else {
-            float x[8];
+            float x[8], none = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) x[j] = (float)v[j];
-            parts_of(x, f.part);
+            parts_of(x, f.part, none);
         }
         return f;
     }
@@ -588,7 +601,7 @@ struct AdapterProduct {
         bf16x8 part[2];
     };
     // h of the rows of a tile
-    __device__ static __forceinline__ Row row(const Product& p, long row0, int r0, int lane)
+    __device__ static __forceinline__ Row row(const Product& p, long row0, int r0, int lane, Odd& odd)
     {
         const int r = r0 + 8 * (lane & 3);
         const f32x4* from = reinterpret_cast<const f32x4*>(p.h + min(row0 + lane / 4, p.rows - 1) * p.padded + min(r, p.padded - 8));
@@ -598,7 +611,7 @@ struct AdapterProduct {
         v = to_operand(v, lane);
         const float x[8] = {u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]};
         Row both;
-        parts_of(x, both.part);
+        parts_of(x, both.part, odd.none);
         return both;
     }
     __device__ static __forceinline__ f32x4 run(const Factor& f, const Row& h, f32x4 c)
@@ -680,15 +693,17 @@ __device__ __forceinline__ int one_adapter(const Product& p, int lane, long row0
 }
 
 // Adds the adapters' part to sums of NM tiles of 16 rows and NT of 16 columns.  For every tile of rows one adapter after the other of
-// those that occur in it; a factor that is held as a whole stays for the next tile of rows.
+// those that occur in it; a factor that is held as a whole stays for the next tile of rows.  The answer is whether an infinity or NaN was
+// among the factors or h.
 template <typename T, int NM, int NT>
-__device__ __forceinline__ void add_adapters(const Product& p, int lane, long row0, int col0, f32x4 (&acc)[NM][NT])
+__device__ __forceinline__ bool add_adapters(const Product& p, int lane, long row0, int col0, f32x4 (&acc)[NM][NT])
 {
     typedef AdapterProduct<T> Op;
     const int n = lane & 15;
     __builtin_amdgcn_sched_barrier(0);
+    typename Op::Odd odd;
     int a = p.index[min(row0 + n, p.rows - 1)];
-    typename Op::Row first = Op::row(p, row0, 0, lane);
+    typename Op::Row first = Op::row(p, row0, 0, lane, odd);
     int held = -1;
     typename Op::Factor f[NT];
 #pragma unroll
@@ -701,11 +716,11 @@ __device__ __forceinline__ void add_adapters(const Product& p, int lane, long ro
             const unsigned whose = (unsigned)__ballot(mine) & 0xffffu;
             left &= ~whose;
             for (int r0 = 0; r0 < p.rank; r0 += Op::CHUNK) {
-                const typename Op::Row hr = r0 == 0 ? first : Op::row(p, row0 + 16 * i, r0, lane);
+                const typename Op::Row hr = r0 == 0 ? first : Op::row(p, row0 + 16 * i, r0, lane, odd);
                 if (cur != held || r0 > 0) {
 #pragma unroll
                     for (int t = 0; t < NT; ++t)
-                        f[t] = Op::factor(p, static_cast<const T*>(p.F) + cur * p.f_each, col0, t, r0, lane);
+                        f[t] = Op::factor(p, static_cast<const T*>(p.F) + cur * p.f_each, col0, t, r0, lane, odd);
                     held = p.rank <= Op::CHUNK ? cur : -1;
                 }
 #pragma unroll
@@ -718,10 +733,11 @@ __device__ __forceinline__ void add_adapters(const Product& p, int lane, long ro
         }
         if (i + 1 < NM) {
             a = p.index[min(row0 + 16 * (i + 1) + n, p.rows - 1)];
-            first = Op::row(p, row0 + 16 * (i + 1), 0, lane);
+            first = Op::row(p, row0 + 16 * (i + 1), 0, lane, odd);
         }
         __builtin_amdgcn_sched_barrier(0);
     }
+    return odd.any();
 }
 template <typename T, int NM, int NT>
 __device__ __forceinline__ void store_tiles(const Product& p, int lane, long row0, int col0, const f32x4 (&acc)[NM][NT])
@@ -750,6 +766,38 @@ __device__ __forceinline__ void store_tiles(const Product& p, int lane, long row
         }
         if (__builtin_expect(live && is_bad(p.index[row], p.adapters), 0))
             for (int c = col0 + (lane & 3); c < min(col0 + 16 * NT, p.cols); c += 4) out[c] = (T)std::numeric_limits<float>::quiet_NaN();
+    }
+}
+
+// Results that are not finite, formed again with the adapters' part in single precision: an infinity times the second part of another
+// number, which has any sign or is zero, is not what it is times the number.  (From what is stored, so that the sums need not be kept.)
+template <typename T, int NM, int NT>
+__device__ __forceinline__ void form_again(const Product& p, int lane, long row0, int col0)
+{
+    typedef typename Operand<T>::type frag;
+    const int n = lane & 15, g = lane >> 4;
+    __threadfence_block();
+#pragma unroll 1
+    for (int i = 0; i < NM * NT; ++i) {
+        const long at = row0 + i / NT * 16 + n, row = min(at, p.rows - 1);
+        const int t = i % NT, a = p.index[row], col = col0 + column_of<T>(t, 4 * g);
+        const T* x = static_cast<const T*>(p.in) + row * p.in_stride + 8 * g;
+        const T* w = static_cast<const T*>(p.W) + min(col0 + column_of<T>(t, n), p.cols - 1) * p.w_stride + 8 * g;
+        f32x4 sum{0, 0, 0, 0};
+#pragma unroll 1
+        for (int k = 0; k < p.k_padded; k += kPiece) sum = mma(*reinterpret_cast<const frag*>(w + k), *reinterpret_cast<const frag*>(x + k), sum);
+        if (at >= p.rows || !has_adapter(a, p.adapters)) continue;
+        const float* h = p.h + row * p.padded;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            T* out = static_cast<T*>(p.out) + row * p.out_stride + col + j;
+            if (col + j >= p.cols || fabsf((float)*out) <= std::numeric_limits<float>::max()) continue;
+            const T* F = static_cast<const T*>(p.F) + a * p.f_each + (col + j) * p.f_col;
+            float part = 0.0f;
+#pragma unroll 1
+            for (int r = 0; r < p.rank; ++r) part = fmaf(h[r], (float)F[r * p.f_r], part);
+            *out = (T)(sum[j] + part);
+        }
     }
 }
 
@@ -906,8 +954,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_product16(const Product p)
             store_partial<T, NM, NT>(p, lane, row_w, col_w, acc);
             return;
         }
-    add_adapters<T, NM, NT>(p, lane, row_w, col_w, acc);
+    const bool odd = add_adapters<T, NM, NT>(p, lane, row_w, col_w, acc);
     store_tiles<T, NM, NT>(p, lane, row_w, col_w, acc);
+    if (__builtin_expect(odd, 0)) form_again<T, NM, NT>(p, lane, row_w, col_w);
 }
 
 // Single precision on the bf16 matrix instructions: both operands in three parts, exactly, of whose products the six largest are formed
