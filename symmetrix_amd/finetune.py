@@ -283,8 +283,10 @@ class _AdaptedLinear(torch.autograd.Function):
 
 
 def adapted_linear(x, weight, A, B, scale, index):
-    """adapted_linear_forward, differentiable once with respect to x, A and B; weight and scale have to be fixed."""
-    _need(not weight.requires_grad and not (scale is not None and scale.requires_grad), "weight and scale are fixed: they cannot require gradients")
+    """adapted_linear_forward, differentiable once with respect to x, A and B; weight and scale have to be fixed (where gradients are
+    not recorded, as in serving, they may be parameters of a module)."""
+    _need(not torch.is_grad_enabled() or not (weight.requires_grad or (scale is not None and scale.requires_grad)),
+          "weight and scale are fixed: they cannot require gradients")
     return _AdaptedLinear.apply(x, weight, A, B, scale, index)
 
 
