@@ -330,6 +330,7 @@ class AdamW:
             _need(p.is_cuda and p.device == self.params[0].device, "parameters on one GPU expected: there is no CPU path")
             if p.dtype != self.params[0].dtype:
                 raise TypeError("parameters of one type expected: an optimizer for each")
+        self._apart(self.params, "parameters")
         # what every parameter has to be in every step
         self._shapes = [p.shape for p in self.params]
         self._dtype, self._device = (self.params[0].dtype, self.params[0].get_device()) if self.params else (None, None)
@@ -350,6 +351,7 @@ class AdamW:
     def states(self, states):
         states = tuple(tuple(s) for s in states)
         _need(len(states) == len(self.params), "states: a tuple for every parameter expected")
+        self._apart([t for s in states for t in s], "states")
         self._held = [self._hold(i, states, self._masters) for i in range(len(states))]
         self._states = states
 
@@ -363,8 +365,15 @@ class AdamW:
         if masters is not None:
             masters = tuple(masters)
             _need(len(masters) == len(self.params), "masters: one for every parameter expected")
+            self._apart(masters, "masters")
         self._held = [self._hold(i, self._states, masters) for i in range(len(self.params))]
         self._masters = masters
+
+    @staticmethod
+    def _apart(tensors, what):
+        """(A step goes over all tensors at once: memory that two of them name would be written by both.)"""
+        starts = [t.data_ptr() for t in tensors if t.numel()]
+        _need(len(set(starts)) == len(starts), f"{what}: every tensor once expected, each with memory of its own")
 
     def _hold(self, i, states, masters):
         """A parameter's part of smx_adamw_tensor, and aliases of the tensors that it names.  The aliases keep the memory, so that none of

@@ -124,3 +124,21 @@ def test_the_kind_of_moments_stays():
     with pytest.raises(AttributeError):
         opt.state_bits = 32
     assert opt.state_bits == 8
+
+
+@pytest.mark.gpu
+def test_memory_named_twice_is_refused():
+    """A step goes over all tensors at once."""
+    from symmetrix_amd import finetune
+    p = _tensors()
+    zeros = lambda: [(torch.zeros_like(t), torch.zeros_like(t)) for t in p]          # noqa: E731
+    shared, both = zeros(), zeros()
+    shared[1] = (shared[1][0], shared[1][0])
+    both[1] = (both[0][0][:7], both[1][1])
+    half = [t.half() for t in p]
+    for call in (lambda: finetune.AdamW([p[0], p[1], p[0]]), lambda: finetune.AdamW([p[0], p[0][:10]]), lambda: finetune.AdamW(p, states=shared),
+                 lambda: finetune.AdamW(p, states=both), lambda: finetune.AdamW([half[1], half[1].clone()], masters=[p[1], p[1]])):
+        with pytest.raises(ValueError, match="memory of its own"):
+            call()
+    empty = torch.zeros(0, device="cuda")
+    finetune.AdamW([p[0], empty, empty]).step([p[1].new_ones(300), empty, empty])
