@@ -315,15 +315,19 @@ class AdamW:
     precision for params in 16 bits, a list like params; True makes them from params.  states: moments to go on with, a tuple a
     tensor, (exp_avg, exp_avg_sq) or (code_avg, scale_avg, code_avg_sq, scale_avg_sq); they are used in place, as params and
     masters are, and so is what self.states holds otherwise (zeros at first).  Both attributes can be assigned anew as a whole, under
-    the same checks; what a tensor of theirs or a parameter holds is looked at in every step.  step: steps taken before."""
+    the same checks; what a tensor of theirs or a parameter holds is looked at in every step.  step: steps taken before, a number or
+    one for every parameter, as self.steps has them: a parameter takes only those steps that it has a gradient in."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, masters=None, states=None, step=0):
         self.params = tuple(params)
         _need(state_bits in (32, 8), "state_bits: 32 or 8")
         _need(0 <= betas[0] < 1 and 0 <= betas[1] < 1, "betas: 0 up to, not including, 1")
         _need(lr >= 0 and eps >= 0 and weight_decay >= 0, "lr, eps and weight_decay: numbers from 0 on")
-        _need(step >= 0, "step: steps taken before, none or more")
-        self.lr, self.betas, self.eps, self.weight_decay, self._bits, self.step_count = lr, tuple(betas), eps, weight_decay, state_bits, step
+        taken = list(step) if isinstance(step, (list, tuple)) else [step] * len(self.params)
+        _need(len(taken) == len(self.params) and all(t >= 0 for t in (taken or [step])), "step: steps taken before, none or more, a number or one for every parameter")
+        self.lr, self.betas, self.eps, self.weight_decay, self._bits = lr, tuple(betas), eps, weight_decay, state_bits
+        self.step_count = max(taken, default=0)
+        self._missed = [self.step_count - t for t in taken]          # steps without a gradient
         for p in self.params:
             _type(p, "parameters")
             _need(p.is_contiguous(), "parameters: contiguous tensors expected")
@@ -341,6 +345,11 @@ class AdamW:
     @property
     def state_bits(self):
         return self._bits
+
+    @property
+    def steps(self):
+        """The steps that every parameter has taken."""
+        return tuple(self.step_count - m for m in self._missed)
 
     @property
     def states(self):
@@ -405,7 +414,7 @@ class AdamW:
 
     def step(self, grads=None):
         """One step with the given gradients, one for every parameter (None: the parameters' own).  A parameter without a gradient
-        (None) is left as it is.  Gradients are of the parameters' type or all in float32."""
+        (None) is left as it is, and does not count the step.  Gradients are of the parameters' type or all in float32."""
         if grads is None:
             grads = [p.grad for p in self.params]
         _need(len(grads) == len(self.params), "a gradient (or None) for every parameter expected")
@@ -434,8 +443,21 @@ class AdamW:
                     held[i] = self._hold(i, states, masters)
                     master, m, v, scale_m, scale_v, n = held[i][0]
                 _ADAMW_TENSOR.pack_into(table, at * _ADAMW_TENSOR.size, p.data_ptr(), g.data_ptr(), master, m, v, scale_m, scale_v, n)
-            _call(device, _lib_functions().smx_adamw_step, _TYPES[own], _TYPES[kind], self._bits, bytes(table), len(taken), self.lr, self.betas[0],
-                  self.betas[1], self.eps, self.weight_decay, self.step_count + 1)
+            missed = self._missed
+            calls = {}          # tensors by the number of the step that it is for them
+            if any(missed):
+                _need(all(missed[i] <= self.step_count for i in taken), "step_count: less than the steps that a parameter has missed")
+                for at, i in enumerate(taken):
+                    calls.setdefault(missed[i], bytearray()).extend(table[at * _ADAMW_TENSOR.size:(at + 1) * _ADAMW_TENSOR.size])
+            else:
+                calls[0] = table
+            for late, some in calls.items():
+                _call(device, _lib_functions().smx_adamw_step, _TYPES[own], _TYPES[kind], self._bits, bytes(some), len(some) // _ADAMW_TENSOR.size, self.lr,
+                      self.betas[0], self.betas[1], self.eps, self.weight_decay, self.step_count + 1 - late)
             # (as torch's own operations in place do: a backward pass that saved the old values says so)
             torch.autograd.graph.increment_version(params if len(taken) == len(params) else [params[i] for i in taken])
+        if len(taken) < len(grads):
+            for i, g in enumerate(grads):
+                if g is None:
+                    self._missed[i] += 1
         self.step_count += 1
