@@ -152,6 +152,7 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, need=(True, True, True),
     """Gradients of x, weight and bias (None where `need` says so); the latter two in weight's type, or without a weight in
     bias_type (None: the type of x)."""
     kind = _type(x, "x")
+    _need(x.dim() >= 1 and x.shape[-1] >= 1, "x: rows of at least one number expected")
     dim = x.shape[-1]
     _need(dy.shape == x.shape and dy.dtype == x.dtype, "dy: shape and type of x expected")
     _need(mean.dtype == rstd.dtype == torch.float32 and mean.shape == rstd.shape == x.shape[:-1] and mean.is_contiguous() and rstd.is_contiguous(),
@@ -201,6 +202,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
 
 def _describe(x, weight, A, B, scale, index):
     kind = _type(x, "x")
+    _need(x.dim() >= 1, "x: rows of d_in numbers expected")
     _need(weight.dim() == 2, "weight: [d_out, d_in] expected")
     d_out, d_in = weight.shape
     _need(d_in >= 1 and d_out >= 1, "weight: at least one row and column expected")
