@@ -351,7 +351,11 @@ int smx_adapted_linear_backward(const smx_adapted_linear* p, const void* d_dy, l
  * the step goes by, of which param gets a rounded copy (parameters in 16 bits; for all tensors of a call or none).
  * state_bits 32: exp_avg and exp_avg_sq are float[numel].  state_bits 8: they are codes, signed and unsigned chars
  * [numel], and scale_avg, scale_avg_sq hold a float for every SMX_MOMENT_BLOCK of them:
- *   m = scale c |c| / 127^2,  v = scale (c / 255)^4.  Zeros are a valid start.  numel: less than 2^36. */
+ *   m = scale c |c| / 127^2,  v = scale (c / 255)^4.  Zeros are a valid start.  numel: less than 2^36.
+ * step: which one it is for the tensors of the call, counted from 1; tensors that have taken different numbers of steps
+ * go into different calls.  Tensors of a call must not overlap.  A gradient that is not finite makes its own number's
+ * moments and parameter infinite or NaN; with moments in 8 bits all SMX_MOMENT_BLOCK numbers of its scale are NaN from the next
+ * step on.  A caller that wants to leave such a step out looks at the gradients before the call. */
 typedef struct {
     void* param;
     const void* grad;

@@ -6,9 +6,12 @@
 // |m| and the fourth root of v, so that m and sqrt(v) have the same resolution, finest near zero:  m = scale c |c| / 127^2,
 // v = scale (c / 255)^4.  The moments of a step are what was read, brought to single precision; the parameters see them before they
 // are rounded.  Rounded to nearest, a moment that moves by less than half a code a step would never move, and v decays by a
-// thousandth a step; so the place where a number is rounded up moves over [0, 1) from step to step by the golden ratio, which
-// fills the interval evenly, starts elsewhere for every number of a tensor, and makes up at some steps for what is lost at others.
-// A v that is not zero keeps the code 1 at least (an m beside it that is not rounded to zero would be divided by eps).
+// thousandth a step; so the place where a number is rounded up moves over [0, 1), by 0.046 from step to step (once around in 21.6
+// steps) and by 0.618 from a number to the next.  What is lost at some is made up for at others: over the numbers of a tensor in every
+// step, and for one number over some tens of steps, which a v of beta2 = 0.99 or more remembers.  An m of beta1 = 0.9 forgets in ten, and
+// keeps a part of what it was rounded by.
+// A v that is not zero keeps the code 1 at least (an m beside it that is not rounded to zero would be divided by eps).  There is no code
+// for infinity or NaN: a scale that is one makes its 256 numbers NaN from the next step on.
 //
 // Every operation is rounded once, in the order written (no fused multiply-adds, IEEE division and root), so that the codes are those
 // of the same formulas elsewhere.

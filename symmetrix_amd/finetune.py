@@ -36,6 +36,7 @@ class _AdamwTensor(C.Structure):
 # the same as packed bytes, which are made in a fraction of the time
 _ADAPTED = struct.Struct("@5iqPqPqPPPP")
 _ADAMW_TENSOR = struct.Struct("@7Pq")
+_ADAMW_FIRST = struct.Struct("@2P")          # param and grad
 assert _ADAPTED.size == C.sizeof(_Adapted) and _ADAMW_TENSOR.size == C.sizeof(_AdamwTensor)
 
 
@@ -363,8 +364,7 @@ class AdamW:
         states = tuple(tuple(s) for s in states)
         _need(len(states) == len(self.params), "states: a tuple for every parameter expected")
         self._apart([t for s in states for t in s], "states")
-        self._held = [self._hold(i, states, self._masters) for i in range(len(states))]
-        self._states = states
+        self._hold_all(states, self._masters)
 
     @property
     def masters(self):
@@ -377,8 +377,7 @@ class AdamW:
             masters = tuple(masters)
             _need(len(masters) == len(self.params), "masters: one for every parameter expected")
             self._apart(masters, "masters")
-        self._held = [self._hold(i, self._states, masters) for i in range(len(self.params))]
-        self._masters = masters
+        self._hold_all(self._states, masters)
 
     @staticmethod
     def _apart(tensors, what):
@@ -386,10 +385,16 @@ class AdamW:
         starts = [t.data_ptr() for t in tensors if t.numel()]
         _need(len(set(starts)) == len(starts), f"{what}: every tensor once expected, each with memory of its own")
 
+    # What is held of the tensors: the descriptions that a step hands on, all but the parameters' and gradients' addresses, the addresses
+    # in them, and aliases of the tensors.  The aliases keep the memory, so that none of the addresses is ever that of memory that others
+    # use; a tensor that was given other memory has another address, which is compared in every step.
+    def _hold_all(self, states, masters):
+        held = [self._hold(i, states, masters) for i in range(len(self.params))]
+        self._table = bytearray(b"".join(_ADAMW_TENSOR.pack(0, 0, *h[0]) for h in held))
+        self._held, self._states, self._masters = held, states, masters
+
     def _hold(self, i, states, masters):
-        """A parameter's part of smx_adamw_tensor, and aliases of the tensors that it names.  The aliases keep the memory, so that none of
-        the addresses is ever that of memory that others use; a tensor that was given other memory has another address, which is
-        compared in every step."""
+        """A parameter's part of smx_adamw_tensor from its master on, and the aliases."""
         n, bits, s = self._shapes[i].numel(), self._bits, states[i]
         kinds = (torch.float32, torch.float32) if bits == 32 else (torch.int8, torch.float32, torch.uint8, torch.float32)
         counts = (n, n) if bits == 32 else (n, -(-n // MOMENT_BLOCK)) * 2
@@ -426,11 +431,11 @@ class AdamW:
             kind = grads[taken[0]].dtype
             if kind != own and kind != torch.float32:
                 raise TypeError(f"gradients: {own} or float32, not {kind}")
-            table, keep, wide = bytearray(len(taken) * _ADAMW_TENSOR.size), [], self._bits == 32
-            shapes, held, states, masters = self._shapes, self._held, self._states, self._masters
-            for at, i in enumerate(taken):
+            keep, wide, size = [], self._bits == 32, _ADAMW_TENSOR.size
+            shapes, held, states, masters, table, first = self._shapes, self._held, self._states, self._masters, self._table, _ADAMW_FIRST.pack_into
+            for i in taken:
                 p, g, shape, s = params[i], grads[i], shapes[i], states[i]
-                if p.dtype != own or g.dtype != kind:
+                if p.dtype is not own or g.dtype is not kind:
                     raise TypeError(f"parameters in {own}, as they were at first, and gradients of one type expected")
                 if p.shape != shape or p.get_device() != device or not p.is_contiguous():
                     raise ValueError("parameters contiguous, and of the shapes and on the device they had at first, expected")
@@ -439,23 +444,23 @@ class AdamW:
                 if not g.is_contiguous():
                     g = g.contiguous()
                     keep.append(g)
-                master, m, v, scale_m, scale_v, n = held[i][0]
+                master, m, v, scale_m, scale_v, _ = held[i][0]
                 if (s[0].data_ptr() != m or (s[1].data_ptr() != v if wide else s[2].data_ptr() != v or s[1].data_ptr() != scale_m or s[3].data_ptr() != scale_v)
                         or (masters is not None and masters[i].data_ptr() != master)):
                     held[i] = self._hold(i, states, masters)
-                    master, m, v, scale_m, scale_v, n = held[i][0]
-                _ADAMW_TENSOR.pack_into(table, at * _ADAMW_TENSOR.size, p.data_ptr(), g.data_ptr(), master, m, v, scale_m, scale_v, n)
+                    _ADAMW_TENSOR.pack_into(table, i * size, 0, 0, *held[i][0])
+                first(table, i * size, p.data_ptr(), g.data_ptr())
             missed = self._missed
-            calls = {}          # tensors by the number of the step that it is for them
             if any(missed):
                 _need(all(missed[i] <= self.step_count for i in taken), "step_count: less than the steps that a parameter has missed")
-                for at, i in enumerate(taken):
-                    calls.setdefault(missed[i], bytearray()).extend(table[at * _ADAMW_TENSOR.size:(at + 1) * _ADAMW_TENSOR.size])
-            else:
-                calls[0] = table
+                calls = {}          # descriptions by the number of the step that it is for their tensors
+                for i in taken:
+                    calls[missed[i]] = calls.get(missed[i], b"") + table[i * size:(i + 1) * size]
+            else:          # (no parameter has missed a step so far; some may have no gradient in this one)
+                calls = {0: bytes(table) if len(taken) == len(params) else b"".join(table[i * size:(i + 1) * size] for i in taken)}
             for late, some in calls.items():
-                _call(device, _lib_functions().smx_adamw_step, _TYPES[own], _TYPES[kind], self._bits, bytes(some), len(some) // _ADAMW_TENSOR.size, self.lr,
-                      self.betas[0], self.betas[1], self.eps, self.weight_decay, self.step_count + 1 - late)
+                _call(device, _lib_functions().smx_adamw_step, _TYPES[own], _TYPES[kind], self._bits, some, len(some) // size, self.lr, self.betas[0],
+                      self.betas[1], self.eps, self.weight_decay, self.step_count + 1 - late)
             # (as torch's own operations in place do: a backward pass that saved the old values says so)
             torch.autograd.graph.increment_version(params if len(taken) == len(params) else [params[i] for i in taken])
         if len(taken) < len(grads):
