@@ -70,3 +70,19 @@ def test_more_blocks_than_a_launch_takes(dtype):
     data, dy = _data(70, 33, 65600, 1, 4096, NAMES[dtype], "own")
     dx = finetune.adapted_linear_backward(dy, **data, need=(True, False, False))[0]
     _close(dx, *_reference(**data, dy=dy)["dx"], NAMES[dtype])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_rows_as_far_apart_as_a_tile_takes_them(dtype):
+    """2^22 numbers from row to row: offsets inside a tile of 256 rows pass 2^31 bytes, of x and of the projection."""
+    from symmetrix_amd import finetune
+    stride = 1 << 22
+    store = torch.empty(255 * stride + 64, dtype=dtype, device="cuda")
+    far = store.as_strided((256, 64), (stride, 1))
+    data, _ = _data(256, 64, 49152, 8, 3, dtype, "own")
+    far.copy_(data["x"])
+    _close(finetune.adapted_linear_forward(**dict(data, x=far)), *_reference(**data)["y"], dtype)
+    data, _ = _data(49152, 64, 256, 8, 3, dtype)
+    far.copy_(data["weight"])
+    _close(finetune.adapted_linear_forward(**dict(data, weight=far)), *_reference(**data)["y"], dtype)
