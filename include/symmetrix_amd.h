@@ -371,6 +371,75 @@ int smx_adamw_step(int param_type, int grad_type, int state_bits, const smx_adam
 int smx_moment_values(long numel, const void* d_code_avg, const float* d_scale_avg, const void* d_code_avg_sq,
                       const float* d_scale_avg_sq, float* d_exp_avg, float* d_exp_avg_sq, void* stream);
 
+/* smx_adamw_step with every gradient multiplied by *d_factor (device memory) first, as smx_grad_norm leaves it there. */
+int smx_adamw_step_scaled(int param_type, int grad_type, int state_bits, const smx_adamw_tensor* tensors, int count,
+                          double lr, double beta1, double beta2, double eps, double weight_decay, long step,
+                          const float* d_factor, void* stream);
+
+/* Rows by group: a row's index (int32, in any order) names its group, 0 to num_groups - 1; -1: none.  A row whose index is
+ * neither has NaN for results and no part in sums over rows.
+ * order[rows]: the rows, those of group 0 first, then those of 1 and so on, then those without a group, then those with an index out of
+ * range; rows of one group in their own order.  offsets[num_groups + 2]: where in it each group begins, where the rows
+ * without one do, and where those out of range do.  rows: up to 2^28, num_groups: up to SMX_MOST_ENTRIES. */
+#define SMX_MOST_GROUPS 4096
+#define SMX_MOST_ENTRIES (1 << 24)
+int smx_group_rows_workspace(long rows, int num_groups, long* bytes);
+int smx_group_rows(long rows, int num_groups, const int* d_index, int* d_order, int* d_offsets, void* d_workspace,
+                   long workspace_bytes, void* stream);
+
+/* Rows of a table: y_i = scale table[index_i]; zeros where the index is -1.  table[entries][dim], rows table_stride apart.
+ * entries: up to SMX_MOST_ENTRIES, dim: up to 2^20. */
+int smx_embedding_forward(int type, long rows, int entries, int dim, const void* d_table, long table_stride,
+                          const int* d_index, double scale, void* d_y, long y_stride, void* stream);
+/* The table's gradient, dtable[entries][dim] in the type of dy: scale times the sum of the rows of dy of every entry, in
+ * single precision and an order that the sizes and indices alone decide; zeros for entries without a row.  order and
+ * offsets: smx_group_rows of index, for callers that have them, or both NULL. */
+int smx_embedding_backward_workspace(int type, long rows, int entries, int dim, long* bytes);
+int smx_embedding_backward(int type, long rows, int entries, int dim, const void* d_dy, long dy_stride, const int* d_index,
+                           const int* d_order, const int* d_offsets, double scale, void* d_dtable, void* d_workspace, long workspace_bytes, void* stream);
+
+/* A product with a matrix of the row's own group:  y_i = weight_g x_i + bias_g,  g = index_i.
+ * weight[num_groups][d_out][d_in], rows weight_stride and matrices weight_each apart, bias[num_groups][d_out] (may be NULL)
+ * and x are of one type.  Rows without a group have zeros for results.  order and offsets: smx_group_rows of index, for
+ * callers that use them several times, or both NULL.  rows: up to 2^28, d_in and d_out: up to 2^20,
+ * num_groups: up to SMX_MOST_GROUPS. */
+typedef struct {
+    int type;
+    int d_in, d_out, num_groups;
+    long rows;
+    const void* x;
+    long x_stride;
+    const void* weight;
+    long weight_stride, weight_each;
+    const void* bias;
+    const int *index, *order, *offsets;
+} smx_grouped_linear;
+int smx_grouped_linear_workspace(const smx_grouped_linear* p, int backward, long* bytes);
+int smx_grouped_linear_forward(const smx_grouped_linear* p, void* d_y, long y_stride, void* d_workspace,
+                               long workspace_bytes, void* stream);
+/* Gradients: dx[rows][d_in], dweight[num_groups][d_out][d_in], dbias[num_groups][d_out], all of p->type; each may be NULL.
+ * Groups without a row get zeros.  (p->bias is not looked at.) */
+int smx_grouped_linear_backward(const smx_grouped_linear* p, const void* d_dy, long dy_stride, void* d_dx, long dx_stride,
+                                void* d_dweight, void* d_dbias, void* d_workspace, long workspace_bytes, void* stream);
+
+/* Gradients of many tensors (a host array of descriptions, read before the call returns), each of a type of its own:
+ *   norm = sqrt(sum over all numbers of g^2),  factor = min(1, max_norm / norm), or 1 where the norm is not finite.
+ * Squares and their sums are in double precision.  norm and factor (either may be NULL) are one float each in device
+ * memory.  max_norm: from 0 on; infinity: a factor of 1.  numel: less than 2^36. */
+typedef struct {
+    int type;
+    const void* grad;
+    void* out;
+    long numel;
+} smx_grad_tensor;
+int smx_grad_norm_workspace(const smx_grad_tensor* tensors, int count, long* bytes);
+int smx_grad_norm(const smx_grad_tensor* tensors, int count, double max_norm, float* d_norm, float* d_factor,
+                  void* d_workspace, long workspace_bytes, void* stream);
+/* out = factor grad for every tensor, rounded once; out may be grad itself, and has no memory in common with any
+ * other tensor of the call. */
+int smx_clip_grads(const smx_grad_tensor* tensors, int count, double max_norm, float* d_norm, void* d_workspace,
+                   long workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

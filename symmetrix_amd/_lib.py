@@ -33,6 +33,8 @@ EXPORTS = [
     "smx_evaluate_list", "smx_nlist_set_wait", "smx_nlist_set_chain_rounds",
     "smx_layer_norm_forward", "smx_layer_norm_backward_workspace", "smx_layer_norm_backward", "smx_adapted_linear_workspace",
     "smx_adapted_linear_forward", "smx_adapted_linear_backward", "smx_adamw_step", "smx_moment_values",
+    "smx_adamw_step_scaled", "smx_group_rows_workspace", "smx_group_rows", "smx_embedding_forward", "smx_embedding_backward_workspace", "smx_embedding_backward",
+    "smx_grouped_linear_workspace", "smx_grouped_linear_forward", "smx_grouped_linear_backward", "smx_grad_norm_workspace", "smx_grad_norm", "smx_clip_grads",
 ]
 
 

@@ -1,9 +1,11 @@
-// Shared by the operators for fine-tuned heads (layer norm, adapters beside a shared projection, AdamW): element types, loads and
+// Shared by the operators for fine-tuned heads (layer norm, adapters beside a shared projection, AdamW, tables and
+// products by group, norms of gradients): element types, loads and
 // stores of runs of numbers at any alignment, sums over lanes, and what their C entry points check.
 #pragma once
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <new>
 #include <stdexcept>
 #include <string>
@@ -14,6 +16,7 @@
 
 namespace smx {
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16;
 typedef _Float16 f16;
 
@@ -54,7 +57,6 @@ __device__ __forceinline__ void store_run(T* p, long left, const float (&v)[V])
     }
 }
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 // 1 KB of a wavefront from global memory (16 bytes per lane, at base + offset, a multiple of 16) into LDS at `to` + 16 lane.
 // In assembly: next to the compiler's own form of this load it lets every read of the LDS wait for all loads in flight; here
@@ -77,6 +79,64 @@ __device__ __forceinline__ void barrier_only()
     asm volatile("" ::: "memory");
 }
 __device__ __forceinline__ unsigned lds_address(const void* p) { return (unsigned)(unsigned long)(__attribute__((address_space(3))) const void*)p; }
+
+typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef f16 f16x8 __attribute__((ext_vector_type(8)));
+typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ f32x4 mma(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x4 mma(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+// sixteen terms of a sum in single precision: a lane holds four neighbouring ones
+__device__ __forceinline__ f32x4 mma(f32x4 a, f32x4 b, f32x4 c)
+{
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
+    return c;
+}
+// what a lane holds of an operand: 16 bytes
+template <typename T>
+struct Operand {
+    typedef T type __attribute__((ext_vector_type(kRun<T>)));
+};
+template <typename T>
+__device__ __forceinline__ typename Operand<T>::type load_operand(const T* p, long left)
+{
+    constexpr int V = kRun<T>;
+    if (left >= V) return *reinterpret_cast<const typename Run<T, V>::loose*>(p);
+    typename Operand<T>::type x;
+#pragma unroll
+    for (int j = 0; j < V; ++j) x[j] = j < left ? p[j] : (T)0.0f;
+    return x;
+}
+
+// 16 rows of 64 bytes, 16 bytes a lane: from lane 4 n + g, where neighbouring lanes have asked for neighbouring bytes of row n, to lane
+// 16 g + n, which has them in an operand.  (Asked for in the order of an operand, with every lane in another row than its neighbours, a
+// load takes about 100 cycles instead of 16, caches or not.)
+template <typename V>
+__device__ __forceinline__ V to_operand(const V& x, int lane)
+{
+    typedef int i32x4 __attribute__((ext_vector_type(4)));
+    const int from = (4 * (lane & 15) + (lane >> 4)) * 4;
+    const i32x4 u = __builtin_bit_cast(i32x4, x);
+    i32x4 v;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = __builtin_amdgcn_ds_bpermute(from, u[j]);
+    return __builtin_bit_cast(V, v);
+}
+
+// and back: what lane 16 g + n has of row n goes to lane 4 n + g
+template <typename V>
+__device__ __forceinline__ V from_operand(const V& x, int lane)
+{
+    typedef int i32x4 __attribute__((ext_vector_type(4)));
+    const int from = (16 * (lane & 3) + (lane >> 2)) * 4;
+    const i32x4 u = __builtin_bit_cast(i32x4, x);
+    i32x4 v;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = __builtin_amdgcn_ds_bpermute(from, u[j]);
+    return __builtin_bit_cast(V, v);
+}
 
 // sum over groups of G neighbouring lanes, the same in all of them
 template <int G>
@@ -154,5 +214,51 @@ void with_type(int type, Fn&& fn)
     else if (type == SMX_TYPE_BF16) fn(bf16{});
     else fn(f16{});
 }
+
+inline long up(long x, long m) { return (x + m - 1) / m * m; }
+
+// Parts of the workspace, 256 bytes aligned; counts them first and gives addresses when there is one.
+struct Arena {
+    char* base;
+    long used = 0;
+    template <typename P>
+    P* take(long count)
+    {
+        P* at = base ? reinterpret_cast<P*>(base + used) : nullptr;
+        used += up(count * (long)sizeof(P), 256);
+        return at;
+    }
+};
+
+inline void check_workspace(const void* at, long bytes, long need, const char* who)
+{
+    if (need != 0 && !(at && bytes >= need)) throw Refusal(SMX_EINVAL, std::string("the workspace is smaller than ") + who + " says");
+    refuse_unless((reinterpret_cast<size_t>(at) & 255) == 0, "the workspace: an address that is a multiple of 256");
+}
+
+template <int N>
+using Int = std::integral_constant<int, N>;
+
+// The launches of a call.
+struct Launches {
+    hipStream_t s;
+    const bool dry;      // nothing is launched, the workspace is counted, and the sizes of the launches are looked at
+    // Every launch, also of a call that counts its workspace and launches nothing: sizes that a launch does not take are refused there,
+    // before the call has enqueued anything.
+    template <typename... P, typename... A>
+    void start(void (*kernel)(P...), long x, long y, long z, int threads, unsigned lds, const A&... args)
+    {
+        refuse_unless(x >= 1 && y >= 1 && z >= 1, "a launch of no blocks");
+        refuse_unless(x * threads < 1L << 32 && y <= 65535 && z <= 65535, "more blocks than a launch takes");
+        if (!dry) hipLaunchKernelGGL(kernel, dim3((unsigned)x, (unsigned)y, (unsigned)z), dim3(threads), lds, s, args...);
+    }
+    // fn(first, some): as many blocks at a time as a launch takes of 1 024 threads
+    template <typename Fn>
+    static void in_slabs(long blocks, Fn&& fn)
+    {
+        constexpr long most = 1L << 21;
+        for (long first = 0; first < blocks; first += most) fn(first, std::min(blocks - first, most));
+    }
+};
 
 }  // namespace smx

@@ -38,6 +38,7 @@ struct AdamwTable {
     int count;
     float beta1, beta2, rest1, rest2, keep, rate, root, eps;      // rest: 1 - beta; keep: 1 - lr decay; rate: lr / (1 - beta1^t); root: 1 / sqrt(1 - beta2^t)
     unsigned turn1, turn2;           // where the rounding of the moments' codes stands
+    const float* factor;             // of the gradients; may be null
 };
 static_assert(sizeof(AdamwTable) <= 4096, "kernel arguments");
 
@@ -75,6 +76,7 @@ __global__ __launch_bounds__(256) void k_adamw(const AdamwTable a)
     const TG* grad = static_cast<const TG*>(t.grad);
     float *master = t.master, *ms = static_cast<float*>(t.exp_avg), *vs = static_cast<float*>(t.exp_avg_sq);
     const long n = t.numel;
+    const float factor = a.factor ? *a.factor : 1.0f;
 #pragma unroll
     for (int u = 0; u < kChunk / (256 * V); ++u) {
         const long at = base + (u * 256 + threadIdx.x) * V;
@@ -87,7 +89,7 @@ __global__ __launch_bounds__(256) void k_adamw(const AdamwTable a)
         load_run<V>(vs + at, n - at, v);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const Updated x = update(a, p[j], g[j], m[j], v[j]);
+            const Updated x = update(a, p[j], g[j] * factor, m[j], v[j]);
             p[j] = x.p; m[j] = x.m; v[j] = x.v;
         }
         store_run<V>(param + at, n - at, p);
@@ -136,6 +138,7 @@ __global__ __launch_bounds__(256) void k_adamw_codes(const AdamwTable a)
     int8_t* cm = static_cast<int8_t*>(t.exp_avg);
     uint8_t* cv = static_cast<uint8_t*>(t.exp_avg_sq);
     const long n = t.numel;
+    const float factor = a.factor ? *a.factor : 1.0f;
 #pragma unroll 1
     for (int u = 0; u < SCALES; ++u) {
         const long start = base + (u * 4 + wave) * kBlock, at = start + lane * V;
@@ -150,7 +153,7 @@ __global__ __launch_bounds__(256) void k_adamw_codes(const AdamwTable a)
         float most_m = 0.0f, most_v = 0.0f;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const Updated x = update(a, p[j], g[j], first_moment((int)c[j], sm), second_moment((int)d[j], sv));
+            const Updated x = update(a, p[j], g[j] * factor, first_moment((int)c[j], sm), second_moment((int)d[j], sv));
             p[j] = x.p;
             // (behind the end of the tensor there is nothing, whatever the scales are)
             m[j] = at + j < n ? x.m : 0.0f;
@@ -211,10 +214,10 @@ __global__ __launch_bounds__(256) void k_moment_values(long n, const int8_t* cm,
 
 using namespace smx;
 
-extern "C" int smx_adamw_step(int param_type, int grad_type, int state_bits, const smx_adamw_tensor* tensors, int count, double lr, double beta1,
-                              double beta2, double eps, double weight_decay, long step, void* stream)
+static int adamw_step(const char* entry, int param_type, int grad_type, int state_bits, const smx_adamw_tensor* tensors, int count, double lr, double beta1, double beta2,
+                      double eps, double weight_decay, long step, const float* d_factor, void* stream)
 {
-    return finetune_entry("smx_adamw_step", [&] {
+    return finetune_entry(entry, [&] {
         (void)type_bytes(param_type);
         refuse_unless(grad_type == param_type || grad_type == SMX_TYPE_F32, "gradients: the parameters' type or single precision");
         refuse_unless(state_bits == 32 || state_bits == 8, "state_bits: 32 or 8");
@@ -243,6 +246,7 @@ extern "C" int smx_adamw_step(int param_type, int grad_type, int state_bits, con
         a.rate = (float)(lr / (1 - std::pow(beta1, (double)step)));
         a.root = (float)(1 / std::sqrt(1 - std::pow(beta2, (double)step)));
         a.eps = (float)eps;
+        a.factor = d_factor;
         a.turn1 = (unsigned)(2 * (unsigned long)step) * 0x85EBCA6Bu;
         a.turn2 = (unsigned)(2 * (unsigned long)step + 1) * 0x85EBCA6Bu;
         const hipStream_t s = static_cast<hipStream_t>(stream);
@@ -280,6 +284,18 @@ extern "C" int smx_adamw_step(int param_type, int grad_type, int state_bits, con
         }
         launch();
     });
+}
+
+extern "C" int smx_adamw_step(int param_type, int grad_type, int state_bits, const smx_adamw_tensor* tensors, int count, double lr, double beta1,
+                              double beta2, double eps, double weight_decay, long step, void* stream)
+{
+    return adamw_step("smx_adamw_step", param_type, grad_type, state_bits, tensors, count, lr, beta1, beta2, eps, weight_decay, step, nullptr, stream);
+}
+
+extern "C" int smx_adamw_step_scaled(int param_type, int grad_type, int state_bits, const smx_adamw_tensor* tensors, int count, double lr, double beta1,
+                                     double beta2, double eps, double weight_decay, long step, const float* d_factor, void* stream)
+{
+    return adamw_step("smx_adamw_step_scaled", param_type, grad_type, state_bits, tensors, count, lr, beta1, beta2, eps, weight_decay, step, d_factor, stream);
 }
 
 extern "C" int smx_moment_values(long numel, const void* d_code_avg, const float* d_scale_avg, const void* d_code_avg_sq, const float* d_scale_avg_sq,

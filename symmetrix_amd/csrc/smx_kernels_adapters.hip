@@ -24,64 +24,6 @@ namespace smx {
 
 namespace {
 
-typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef f16 f16x8 __attribute__((ext_vector_type(8)));
-typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
-
-__device__ __forceinline__ f32x4 mma(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
-__device__ __forceinline__ f32x4 mma(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
-// sixteen terms of a sum in single precision: a lane holds four neighbouring ones
-__device__ __forceinline__ f32x4 mma(f32x4 a, f32x4 b, f32x4 c)
-{
-#pragma unroll
-    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
-    return c;
-}
-// what a lane holds of an operand: 16 bytes
-template <typename T>
-struct Operand {
-    typedef T type __attribute__((ext_vector_type(kRun<T>)));
-};
-template <typename T>
-__device__ __forceinline__ typename Operand<T>::type load_operand(const T* p, long left)
-{
-    constexpr int V = kRun<T>;
-    if (left >= V) return *reinterpret_cast<const typename Run<T, V>::loose*>(p);
-    typename Operand<T>::type x;
-#pragma unroll
-    for (int j = 0; j < V; ++j) x[j] = j < left ? p[j] : (T)0.0f;
-    return x;
-}
-
-// 16 rows of 64 bytes, 16 bytes a lane: from lane 4 n + g, where neighbouring lanes have asked for neighbouring bytes of row n, to lane
-// 16 g + n, which has them in an operand.  (Asked for in the order of an operand, with every lane in another row than its neighbours, a
-// load takes about 100 cycles instead of 16, caches or not.)
-template <typename V>
-__device__ __forceinline__ V to_operand(const V& x, int lane)
-{
-    typedef int i32x4 __attribute__((ext_vector_type(4)));
-    const int from = (4 * (lane & 15) + (lane >> 4)) * 4;
-    const i32x4 u = __builtin_bit_cast(i32x4, x);
-    i32x4 v;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = __builtin_amdgcn_ds_bpermute(from, u[j]);
-    return __builtin_bit_cast(V, v);
-}
-
-// and back: what lane 16 g + n has of row n goes to lane 4 n + g
-template <typename V>
-__device__ __forceinline__ V from_operand(const V& x, int lane)
-{
-    typedef int i32x4 __attribute__((ext_vector_type(4)));
-    const int from = (16 * (lane & 3) + (lane >> 2)) * 4;
-    const i32x4 u = __builtin_bit_cast(i32x4, x);
-    i32x4 v;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = __builtin_amdgcn_ds_bpermute(from, u[j]);
-    return __builtin_bit_cast(V, v);
-}
-
 __device__ __forceinline__ bool has_adapter(int a, int n) { return a >= 0 && a < n; }
 __device__ __forceinline__ bool is_bad(int a, int n) { return a < -1 || a >= n; }
 
@@ -1390,57 +1332,19 @@ void check(const smx_adapted_linear* p)
     refuse_unless(p->rows == 0 || (p->x && p->index), "x and index must not be null");
 }
 
-long up(long x, long m) { return (x + m - 1) / m * m; }
-
-// Parts of the workspace, 256 bytes aligned; counts them first and gives addresses when there is one.
-struct Arena {
-    char* base;
-    long used = 0;
-    template <typename P>
-    P* take(long count)
-    {
-        P* at = base ? reinterpret_cast<P*>(base + used) : nullptr;
-        used += up(count * (long)sizeof(P), 256);
-        return at;
-    }
-};
-
 // rows that direct loads into LDS can take as they are
 // (the offsets inside a tile have 32 bits)
 bool as_it_is(const void* p, long stride, long k) { return (reinterpret_cast<size_t>(p) & 15) == 0 && stride % 8 == 0 && stride <= 1 << 22 && k % kPiece == 0; }
 
-template <int N>
-using Int = std::integral_constant<int, N>;
-
-struct Call {
+struct Call : Launches {
     const smx_adapted_linear& p;
-    hipStream_t s;
     Arena arena;
-    const bool dry;      // nothing is launched, the workspace is counted, and the sizes of the launches are looked at
     const int padded;
     Prepare prepare{};
     Downs downs{};
     int num_layouts = 0, num_downs = 0;
     Call(const smx_adapted_linear& p_, void* base, hipStream_t s_, bool dry_)
-        : p(p_), s(s_), arena{static_cast<char*>(base)}, dry(dry_), padded((int)up(p_.rank, 16)) {}
-
-    // Every launch, also of a call that counts its workspace and launches nothing: sizes that a launch does not take are refused there,
-    // before the call has enqueued anything.
-    template <typename... P, typename... A>
-    void start(void (*kernel)(P...), long x, long y, long z, int threads, unsigned lds, const A&... args)
-    {
-        refuse_unless(x >= 1 && y >= 1 && z >= 1, "a launch of no blocks");
-        refuse_unless(x * threads < 1L << 32 && y <= 65535 && z <= 65535, "more blocks than a launch takes");
-        if (!dry) hipLaunchKernelGGL(kernel, dim3((unsigned)x, (unsigned)y, (unsigned)z), dim3(threads), lds, s, args...);
-    }
-
-    // fn(first, some): as many blocks at a time as a launch takes of 1 024 threads
-    template <typename Fn>
-    static void in_slabs(long blocks, Fn&& fn)
-    {
-        constexpr long most = 1L << 21;
-        for (long first = 0; first < blocks; first += most) fn(first, std::min(blocks - first, most));
-    }
+        : Launches{s_, dry_}, p(p_), arena{static_cast<char*>(base)}, padded((int)up(p_.rank, 16)) {}
 
     template <typename T>
     void lay_out(const void* src, long src_each, long src_row, long src_k, void* dst, bool parts, long rows, int k, int matrices)
@@ -1700,12 +1604,6 @@ long workspace(const smx_adapted_linear* p, bool backward)
     });
     return c.arena.used;
 }
-void check_workspace(const void* at, long bytes, long need)
-{
-    refuse_unless(need == 0 || (at && bytes >= need), "the workspace is smaller than smx_adapted_linear_workspace says");
-    refuse_unless((reinterpret_cast<size_t>(at) & 255) == 0, "the workspace: an address that is a multiple of 256");
-}
-
 }  // namespace
 
 }  // namespace smx
@@ -1727,7 +1625,7 @@ extern "C" int smx_adapted_linear_forward(const smx_adapted_linear* p, void* d_y
         check(p);
         if (p->rows == 0) return;
         refuse_unless(d_y && y_stride >= p->d_out, "y must not be null, its stride at least d_out");
-        check_workspace(d_workspace, workspace_bytes, workspace(p, false));
+        check_workspace(d_workspace, workspace_bytes, workspace(p, false), "smx_adapted_linear_workspace");
         require_gfx950();
         Call c(*p, d_workspace, static_cast<hipStream_t>(stream), false);
         with_type(p->type, [&](auto t) { c.forward<decltype(t)>(static_cast<decltype(t)*>(d_y), y_stride); });
@@ -1743,7 +1641,7 @@ extern "C" int smx_adapted_linear_backward(const smx_adapted_linear* p, const vo
         refuse_unless(p->rows == 0 || (d_dy && dy_stride >= p->d_out), "dy must not be null, its stride at least d_out");
         refuse_unless(!d_dx || dx_stride >= p->d_in, "the stride of dx: at least d_in");
         if (!d_dx && !d_dA && !d_dB) return;
-        check_workspace(d_workspace, workspace_bytes, workspace(p, true));
+        check_workspace(d_workspace, workspace_bytes, workspace(p, true), "smx_adapted_linear_workspace");
         require_gfx950();
         Call c(*p, d_workspace, static_cast<hipStream_t>(stream), false);
         with_type(p->type, [&](auto t) {

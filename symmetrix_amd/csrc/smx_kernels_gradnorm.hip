@@ -1,0 +1,249 @@
+// The norm of many tensors' numbers together, and the tensors brought to a norm at most as large as given.
+//
+//   norm = sqrt(sum g^2),   out = g min(1, max_norm / norm)
+//
+// Squares are formed and added in double precision: a product of two single-precision numbers is exact in it, and neither overflows
+// nor vanishes.  A block sums chunks by turns and leaves one number; whoever needs the norm adds these numbers, at most about 2 048, in a
+// fixed order.  That is the launch that writes the norm, or every block of the launch that clips, by itself.
+//
+// Bound by memory.
+#include "smx_finetune.hpp"
+
+#include <cmath>
+
+namespace smx {
+
+namespace {
+
+constexpr int kTensors = 96;         // of a launch: their descriptions are kernel arguments
+constexpr int kChunk = 4096;         // numbers that a block takes at a time
+constexpr int kMostParts = 2048;     // blocks, 8 for every CU
+
+struct NormTable {
+    smx_grad_tensor tensor[kTensors];
+    int first[kTensors + 1];         // chunks in front of each
+    int count;
+    double* part;                    // of the launch's blocks
+};
+static_assert(sizeof(NormTable) <= 4096, "kernel arguments");
+
+// tensor of a chunk (the same in all lanes)
+__device__ __forceinline__ int tensor_of(const NormTable& a, int chunk)
+{
+    int low = 0, high = a.count;
+    while (high - low > 1) {
+        const int mid = (low + high) / 2;
+        if (a.first[mid] <= chunk) low = mid;
+        else high = mid;
+    }
+    return low;
+}
+
+// sum over a block of 256, the same in all threads, in a fixed order
+__device__ __forceinline__ double block_total(double x, double* lds)
+{
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) x += __shfl_xor(x, d, 64);
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = x;
+    __syncthreads();
+    return (lds[0] + lds[1]) + (lds[2] + lds[3]);
+}
+
+template <typename T>
+__device__ __forceinline__ double chunk_squares(const smx_grad_tensor& t, long base)
+{
+    constexpr int V = kRun<T>, STEPS = kChunk / (256 * V);
+    const T* g = static_cast<const T*>(t.grad) + base;
+    const long left = t.numel - base;
+    double sum[2] = {0.0, 0.0};
+    float v[STEPS][V];
+#pragma unroll
+    for (int u = 0; u < STEPS; ++u) {
+        const long at = (u * 256 + threadIdx.x) * V;
+        load_run<V>(g + at, left - at, v[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < STEPS; ++u)
+#pragma unroll
+        for (int j = 0; j < V; ++j) sum[j % 2] = fma((double)v[u][j], (double)v[u][j], sum[j % 2]);
+    return sum[0] + sum[1];
+}
+
+__global__ __launch_bounds__(256) void k_squares(const NormTable a)
+{
+    __shared__ double lds[4];
+    double sum = 0.0;
+    const int chunks = a.first[a.count];
+    for (int chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
+        const int i = tensor_of(a, chunk);
+        const smx_grad_tensor& t = a.tensor[i];
+        const long base = (long)(chunk - a.first[i]) * kChunk;
+        if (t.type == SMX_TYPE_F32) sum += chunk_squares<float>(t, base);
+        else if (t.type == SMX_TYPE_BF16) sum += chunk_squares<bf16>(t, base);
+        else sum += chunk_squares<f16>(t, base);
+    }
+    sum = block_total(sum, lds);
+    if (threadIdx.x == 0) a.part[blockIdx.x] = sum;
+}
+
+struct Norm {
+    const double* part;
+    int parts;
+    double max_norm;
+    float *norm, *factor;      // written by the first block; may be null
+};
+// the factor, the same in all threads and blocks
+__device__ __forceinline__ float factor_of(const Norm& p, double* lds)
+{
+    double sum = 0.0;
+#pragma unroll 8
+    for (int i = threadIdx.x; i < p.parts; i += 256) sum += p.part[i];
+    const double norm = sqrt(block_total(sum, lds));
+    // (NaN fails the first comparison, infinity the second)
+    const float factor = norm > p.max_norm && norm < __builtin_inf() ? (float)(p.max_norm / norm) : 1.0f;
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        if (p.norm) *p.norm = (float)norm;
+        if (p.factor) *p.factor = factor;
+    }
+    return factor;
+}
+__global__ __launch_bounds__(256) void k_norm(const Norm p)
+{
+    __shared__ double lds[4];
+    factor_of(p, lds);
+}
+
+template <typename T>
+__device__ __forceinline__ void scale_chunk(const smx_grad_tensor& t, long base, float factor)
+{
+    constexpr int V = kRun<T>, STEPS = kChunk / (256 * V);
+    const T* g = static_cast<const T*>(t.grad) + base;
+    T* out = static_cast<T*>(t.out) + base;
+    const long left = t.numel - base;
+    float v[STEPS][V];
+#pragma unroll
+    for (int u = 0; u < STEPS; ++u) {
+        const long at = (u * 256 + threadIdx.x) * V;
+        load_run<V>(g + at, left - at, v[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < STEPS; ++u) {
+        const long at = (u * 256 + threadIdx.x) * V;
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[u][j] *= factor;
+        store_run<V>(out + at, left - at, v[u]);
+    }
+}
+__global__ __launch_bounds__(256) void k_clip(const NormTable a, const Norm p)
+{
+    __shared__ double lds[4];
+    const float factor = factor_of(p, lds);
+    const int chunks = a.first[a.count];
+    for (int chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
+        const int i = tensor_of(a, chunk);
+        const smx_grad_tensor& t = a.tensor[i];
+        const long base = (long)(chunk - a.first[i]) * kChunk;
+        if (factor == 1.0f && t.grad == t.out) continue;
+        if (t.type == SMX_TYPE_F32) scale_chunk<float>(t, base, factor);
+        else if (t.type == SMX_TYPE_BF16) scale_chunk<bf16>(t, base, factor);
+        else scale_chunk<f16>(t, base, factor);
+    }
+}
+
+// ---- host side
+
+long chunks_of(const smx_grad_tensor& t) { return (t.numel + kChunk - 1) / kChunk; }
+void check(const smx_grad_tensor* tensors, int count, bool sizes_only, bool outputs)
+{
+    refuse_unless(count >= 0 && (tensors || count == 0), "count must not be negative, tensors not null");
+    for (int i = 0; i < count; ++i) {
+        (void)type_bytes(tensors[i].type);
+        refuse_unless(tensors[i].numel >= 0 && tensors[i].numel < (1L << 36), "numel: 0 less than 2^36");
+        if (tensors[i].numel == 0 || sizes_only) continue;
+        refuse_unless(tensors[i].grad, "gradients must not be null");
+        refuse_unless(!outputs || tensors[i].out, "out must not be null");
+    }
+}
+
+// fn(table, its number of blocks) for as many tensors at a time as a launch takes; the answer: blocks in all, each of which has a part of
+// the sum.
+template <typename Fn>
+int in_tables(const smx_grad_tensor* tensors, int count, Fn&& fn)
+{
+    long all = 0;
+    for (int i = 0; i < count; ++i) all += chunks_of(tensors[i]);
+    int parts = 0;
+    NormTable a;
+    a.count = a.first[0] = 0;
+    auto flush = [&] {
+        const long chunks = a.first[a.count];
+        // of the parts, as many as its share of all chunks
+        const int blocks = (int)(all <= kMostParts ? chunks : std::max(1L, kMostParts * chunks / all));
+        fn(a, blocks, parts);
+        parts += blocks;
+        a.count = 0;
+    };
+    constexpr long kMostChunks = 1L << 30;
+    for (int i = 0; i < count; ++i) {
+        const long chunks = chunks_of(tensors[i]);
+        if (chunks == 0) continue;
+        if (a.count == kTensors || (a.count && a.first[a.count] + chunks > kMostChunks)) flush();
+        a.tensor[a.count] = tensors[i];
+        a.first[a.count + 1] = a.first[a.count] + (int)chunks;
+        ++a.count;
+    }
+    if (a.count) flush();
+    return parts;
+}
+long workspace(const smx_grad_tensor* tensors, int count)
+{
+    return up(8L * std::max(1, in_tables(tensors, count, [](const NormTable&, int, int) {})), 256);
+}
+
+void run(const smx_grad_tensor* tensors, int count, double max_norm, float* d_norm, float* d_factor, void* d_workspace, long workspace_bytes, void* stream, bool clip)
+{
+    check(tensors, count, false, clip);
+    refuse_unless(max_norm >= 0, "max_norm: from 0 on");
+    check_workspace(d_workspace, workspace_bytes, workspace(tensors, count), "smx_grad_norm_workspace");
+    require_gfx950();
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    double* part = static_cast<double*>(d_workspace);
+    const int parts = in_tables(tensors, count, [&](NormTable& a, int blocks, int first) {
+        a.part = part + first;
+        hipLaunchKernelGGL(k_squares, dim3(blocks), dim3(256), 0, s, a);
+    });
+    Norm n{part, parts, max_norm, d_norm, d_factor};
+    if (!clip || parts == 0) hipLaunchKernelGGL(k_norm, dim3(1), dim3(256), 0, s, n);
+    else
+        in_tables(tensors, count, [&](const NormTable& a, int blocks, int first) {
+            hipLaunchKernelGGL(k_clip, dim3(blocks), dim3(256), 0, s, a, n);
+            n.norm = nullptr;
+        });
+    hip_ok(hipGetLastError(), "launch");
+}
+
+}  // namespace
+
+}  // namespace smx
+
+using namespace smx;
+
+extern "C" int smx_grad_norm_workspace(const smx_grad_tensor* tensors, int count, long* bytes)
+{
+    return finetune_entry("smx_grad_norm_workspace", [&] {
+        check(tensors, count, true, false);
+        refuse_unless(bytes, "bytes must not be null");
+        *bytes = workspace(tensors, count);
+    });
+}
+
+extern "C" int smx_grad_norm(const smx_grad_tensor* tensors, int count, double max_norm, float* d_norm, float* d_factor, void* d_workspace, long workspace_bytes,
+                             void* stream)
+{
+    return finetune_entry("smx_grad_norm", [&] { run(tensors, count, max_norm, d_norm, d_factor, d_workspace, workspace_bytes, stream, false); });
+}
+
+extern "C" int smx_clip_grads(const smx_grad_tensor* tensors, int count, double max_norm, float* d_norm, void* d_workspace, long workspace_bytes, void* stream)
+{
+    return finetune_entry("smx_clip_grads", [&] { run(tensors, count, max_norm, d_norm, nullptr, d_workspace, workspace_bytes, stream, true); });
+}

@@ -1,0 +1,327 @@
+// Rows sorted by group, stable: a radix sort of (key, row) by digits of up to ten bits, the lowest first.
+//
+// A digit takes two launches: the digits of every block's rows are counted, and then every block places its rows behind those of
+// smaller digits and those of earlier blocks, which it sums up from the counts by itself.  Inside a wavefront the rows of a digit find
+// their places from the lanes that hold it too (a ballot for every bit), so nothing depends on the order in which blocks or
+// atomics run.  Up to 2 048 rows stay in the LDS of one block, for all digits.
+//
+// Bound by latency: a few dependent loads and barriers a launch.
+#include "smx_groups.hpp"
+
+namespace smx {
+
+namespace {
+
+constexpr int kThreads = 512, kWaves = kThreads / 64;
+constexpr int kMostDigits = 1024;
+constexpr int kSmallRows = 2048;
+
+struct Pass {
+    const int* index;      // the first pass: indices of the rows; or
+    const int* keys;       // keys and rows as the pass before left them
+    const int* rows_in;
+    int *keys_out, *rows_out;      // keys_out may be null
+    int* offsets;                  // of the only pass, or null
+    int* count;                    // [block][digit]
+    int groups, shift, bits, blocks, rows_per_block;
+    long rows;
+};
+__device__ __forceinline__ int key_at(const Pass& p, long i) { return p.index ? row_key(p.index[i], p.groups) : p.keys[i]; }
+
+// lanes of the wavefront that are alive and have this lane's digit
+__device__ __forceinline__ unsigned long same_digit(int digit, bool live, int bits)
+{
+    unsigned long same = __ballot(live);
+    for (int b = 0; b < bits; ++b) {
+        const unsigned long set = __ballot(digit >> b & 1);
+        same &= digit >> b & 1 ? set : ~set;
+    }
+    return same;
+}
+// A row's place among those of its digit that the wavefront has met so far, from next[] (the wavefront's own; its LDS operations are
+// done in order, and the fences keep the compiler to it).
+__device__ __forceinline__ int take_place(int* next, int digit, bool live, int bits, int lane)
+{
+    const unsigned long same = same_digit(digit, live, bits);
+    const int before = __popcll(same & ((1ul << lane) - 1));
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    const int first = live ? next[digit] : 0;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (live && before == 0) next[digit] = first + __popcll(same);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    return first + before;
+}
+
+__global__ __launch_bounds__(kThreads) void k_sort_count(const Pass p)
+{
+    __shared__ int hist[kMostDigits];
+    const int digits = 1 << p.bits;
+    for (int d = threadIdx.x; d < digits; d += kThreads) hist[d] = 0;
+    __syncthreads();
+    const long begin = (long)blockIdx.x * p.rows_per_block, end = min(begin + p.rows_per_block, p.rows);
+#pragma unroll 4
+    for (long i = begin + threadIdx.x; i < end; i += kThreads) atomicAdd(&hist[key_at(p, i) >> p.shift & (digits - 1)], 1);
+    __syncthreads();
+    for (int d = threadIdx.x; d < digits; d += kThreads) p.count[(long)blockIdx.x * digits + d] = hist[d];
+}
+
+// exclusive sums over the block's threads of one number each; part: a number a wavefront
+__device__ __forceinline__ int block_exclusive(int x, int* part, int& total)
+{
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int sum = x;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const int y = __shfl_up(sum, d, 64);
+        if (lane >= d) sum += y;
+    }
+    __syncthreads();
+    if (lane == 63) part[wave] = sum;
+    __syncthreads();
+    int before = 0;
+    total = 0;
+    for (int w = 0; w < (int)(blockDim.x >> 6); ++w) {
+        const int y = part[w];
+        before += w < wave ? y : 0;
+        total += y;
+    }
+    return before + sum - x;
+}
+
+__global__ __launch_bounds__(kThreads) void k_sort_place(const Pass p)
+{
+    __shared__ int next[kWaves][kMostDigits];      // at first the counts of the wavefronts' rows
+    __shared__ int all[kMostDigits], before[kMostDigits];
+    __shared__ int part[kWaves];
+    const int digits = 1 << p.bits, mask = digits - 1, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int d = threadIdx.x; d < digits; d += kThreads) {
+        all[d] = before[d] = 0;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) next[w][d] = 0;
+    }
+    __syncthreads();
+    // rows of a wavefront: neighbours
+    const long per_wave = p.rows_per_block / kWaves;
+    const long begin = (long)blockIdx.x * p.rows_per_block + wave * per_wave, end = min(begin + per_wave, p.rows);
+#pragma unroll 4
+    for (long i = begin + lane; i < end; i += 64) atomicAdd(&next[wave][key_at(p, i) >> p.shift & mask], 1);
+    // counts of all blocks, and of those before this one: a digit's by several threads where there are more threads than digits
+    const int at_once = min(digits, kThreads), parts = kThreads / at_once, mine = threadIdx.x / at_once;
+    for (int d = threadIdx.x % at_once; d < digits; d += at_once) {
+        int a = 0, b = 0;
+#pragma unroll 8
+        for (int k = mine; k < p.blocks; k += parts) {
+            const int x = p.count[(long)k * digits + d];
+            a += x;
+            b += k < (int)blockIdx.x ? x : 0;
+        }
+        atomicAdd(&all[d], a);
+        atomicAdd(&before[d], b);
+    }
+    __syncthreads();
+    int base = 0;
+    for (int d0 = 0; d0 < digits; d0 += kThreads) {
+        const int d = d0 + threadIdx.x;
+        int total;
+        const int start = base + block_exclusive(d < digits ? all[d] : 0, part, total);
+        if (d < digits) {
+            if (p.offsets && blockIdx.x == 0 && d < p.groups + 2) p.offsets[d] = start;
+            int at = start + before[d];
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                const int c = next[w][d];
+                next[w][d] = at;
+                at += c;
+            }
+        }
+        base += total;
+    }
+    __syncthreads();
+    for (long i = begin; i < end; i += 64) {
+        const bool live = i + lane < end;
+        const int key = live ? key_at(p, i + lane) : 0;
+        const int at = take_place(next[wave], key >> p.shift & mask, live, p.bits, lane);
+        if (live) {
+            p.rows_out[at] = p.index ? (int)(i + lane) : p.rows_in[i + lane];
+            if (p.keys_out) p.keys_out[at] = key;
+        }
+    }
+}
+
+// first place in sorted keys that holds `key` or more
+__device__ __forceinline__ int first_place(const int* keys, int n, int key)
+{
+    int low = 0;
+    while (n > 0) {
+        const int half = n / 2;
+        if (keys[low + half] < key) low += half + 1, n -= half + 1;
+        else n = half;
+    }
+    return low;
+}
+__global__ __launch_bounds__(256) void k_sort_offsets(const int* keys, int rows, int groups, int* offsets)
+{
+    const int g = blockIdx.x * 256 + threadIdx.x;
+    if (g < groups + 2) offsets[g] = first_place(keys, rows, g);
+}
+
+__global__ __launch_bounds__(256) void k_no_rows(int* offsets, int n)
+{
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    if (i < n) offsets[i] = 0;
+}
+
+// All digits in one block.
+struct SmallSort {
+    const int* index;
+    int rows, groups, key_bits;
+    int *order, *offsets, *keys;
+};
+__global__ __launch_bounds__(1024) void k_sort_small(const SmallSort p)
+{
+    constexpr int WAVES = 16, BITS = 8, DIGITS = 1 << BITS, PER = kSmallRows / 1024;
+    __shared__ int key_of[kSmallRows], row_of[kSmallRows];
+    __shared__ int next[WAVES][DIGITS];
+    __shared__ int part[WAVES];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int i = threadIdx.x; i < p.rows; i += 1024) {
+        key_of[i] = row_key(p.index[i], p.groups);
+        row_of[i] = i;
+    }
+    const int per_wave = ((p.rows + 16 * 64 - 1) / (16 * 64)) * 64, begin = wave * per_wave, end = min(begin + per_wave, p.rows);
+    for (int shift = 0; shift < p.key_bits; shift += BITS) {
+        __syncthreads();
+#pragma unroll
+        for (int d = threadIdx.x; d < WAVES * DIGITS; d += 1024) next[d / DIGITS][d % DIGITS] = 0;
+        __syncthreads();
+        int key[PER], row[PER], at[PER];
+#pragma unroll
+        for (int u = 0; u < PER; ++u) {      // places inside the wavefront first
+            const int i = begin + 64 * u + lane;
+            const bool live = i < end;
+            key[u] = live ? key_of[i] : 0;
+            row[u] = live ? row_of[i] : 0;
+            at[u] = begin + 64 * u < end ? take_place(next[wave], key[u] >> shift & (DIGITS - 1), live, BITS, lane) : 0;
+        }
+        __syncthreads();
+        int sum = 0, total;
+        if (threadIdx.x < DIGITS)
+            for (int w = 0; w < WAVES; ++w) sum += next[w][threadIdx.x];
+        int start = block_exclusive(sum, part, total);
+        if (threadIdx.x < DIGITS)
+            for (int w = 0; w < WAVES; ++w) {
+                const int c = next[w][threadIdx.x];
+                next[w][threadIdx.x] = start;
+                start += c;
+            }
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < PER; ++u) {
+            const int i = begin + 64 * u + lane;
+            if (i < end) {
+                const int to = next[wave][key[u] >> shift & (DIGITS - 1)] + at[u];
+                key_of[to] = key[u];
+                row_of[to] = row[u];
+            }
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < p.rows; i += 1024) {
+        p.order[i] = row_of[i];
+        if (p.keys) p.keys[i] = key_of[i];
+    }
+    if (p.offsets)
+        for (int g = threadIdx.x; g < p.groups + 2; g += 1024) p.offsets[g] = first_place(key_of, p.rows, g);
+}
+
+}  // namespace
+
+void sort_rows(Launches& launches, Arena& arena, const int* index, long rows, int groups, const RowOrder& to)
+{
+    if (rows == 0) {
+        if (to.offsets) launches.start(k_no_rows, ((long)groups + 2 + 255) / 256, 1, 1, 256, 0, to.offsets, groups + 2);
+        return;
+    }
+    int key_bits = 1;
+    while ((1L << key_bits) < (long)groups + 2) ++key_bits;
+    // (offsets of many groups by one block would take longer than the sort)
+    constexpr int kMostInside = 8192;
+    int* keys = to.keys;
+    auto offsets = [&] { launches.start(k_sort_offsets, ((long)groups + 2 + 255) / 256, 1, 1, 256, 0, (const int*)keys, (int)rows, groups, to.offsets); };
+    if (rows <= kSmallRows) {
+        const bool later = to.offsets && groups > kMostInside;
+        if (later && !keys) keys = arena.take<int>(rows);
+        launches.start(k_sort_small, 1, 1, 1, 1024, 0, SmallSort{index, (int)rows, groups, key_bits, to.order, later ? nullptr : to.offsets, keys});
+        if (later) offsets();
+        return;
+    }
+    const int passes = (key_bits + 9) / 10;
+    Pass p{};
+    p.groups = groups;
+    p.rows = rows;
+    // (every block reads the counts of all)
+    p.rows_per_block = (int)std::max(2048L, up((rows + 255) / 256, kThreads));
+    p.blocks = (int)((rows + p.rows_per_block - 1) / p.rows_per_block);
+    p.count = arena.take<int>((long)p.blocks << ((key_bits + passes - 1) / passes));
+    if (passes > 1 && !keys) keys = arena.take<int>(rows);
+    int* other_keys[2] = {passes > 1 ? arena.take<int>(rows) : nullptr, nullptr};
+    int* other_rows[2] = {passes > 1 ? arena.take<int>(rows) : nullptr, nullptr};
+    if (passes > 2) other_keys[1] = arena.take<int>(rows), other_rows[1] = arena.take<int>(rows);
+    for (int pass = 0, shift = 0; pass < passes; ++pass) {
+        const bool last = pass == passes - 1;
+        p.bits = (key_bits - shift + passes - pass - 1) / (passes - pass);
+        p.shift = shift;
+        p.index = pass == 0 ? index : nullptr;
+        p.keys = pass == 0 ? nullptr : other_keys[(pass - 1) % 2];
+        p.rows_in = pass == 0 ? nullptr : other_rows[(pass - 1) % 2];
+        p.keys_out = last ? keys : other_keys[pass % 2];
+        p.rows_out = last ? to.order : other_rows[pass % 2];
+        p.offsets = passes == 1 ? to.offsets : nullptr;
+        launches.start(k_sort_count, p.blocks, 1, 1, kThreads, 0, p);
+        launches.start(k_sort_place, p.blocks, 1, 1, kThreads, 0, p);
+        shift += p.bits;
+    }
+    if (to.offsets && passes > 1) offsets();
+}
+
+namespace {
+
+void check(long rows, int groups)
+{
+    refuse_unless(rows >= 0 && rows <= 1L << 28, "rows: 0 to 2^28");
+    refuse_unless(groups >= 0 && groups <= SMX_MOST_ENTRIES, "num_groups: 0 to 2^24");
+}
+
+}  // namespace
+
+}  // namespace smx
+
+using namespace smx;
+
+extern "C" int smx_group_rows_workspace(long rows, int num_groups, long* bytes)
+{
+    return finetune_entry("smx_group_rows_workspace", [&] {
+        check(rows, num_groups);
+        refuse_unless(bytes, "bytes must not be null");
+        Launches dry{nullptr, true};
+        Arena arena{reinterpret_cast<char*>(256)};
+        sort_rows(dry, arena, nullptr, rows, num_groups, RowOrder{nullptr, reinterpret_cast<int*>(4), nullptr});
+        *bytes = arena.used;
+    });
+}
+
+extern "C" int smx_group_rows(long rows, int num_groups, const int* d_index, int* d_order, int* d_offsets, void* d_workspace, long workspace_bytes, void* stream)
+{
+    return finetune_entry("smx_group_rows", [&] {
+        check(rows, num_groups);
+        refuse_unless(d_offsets && (rows == 0 || (d_index && d_order)), "index, order and offsets must not be null");
+        long need = 0;
+        if (smx_group_rows_workspace(rows, num_groups, &need) != SMX_OK) throw Refusal(SMX_EINVAL, "sizes");
+        check_workspace(d_workspace, workspace_bytes, need, "smx_group_rows_workspace");
+        require_gfx950();
+        Launches launches{static_cast<hipStream_t>(stream), false};
+        Arena arena{static_cast<char*>(d_workspace)};
+        sort_rows(launches, arena, d_index, rows, num_groups, RowOrder{d_order, d_offsets, nullptr});
+        hip_ok(hipGetLastError(), "launch");
+    });
+}

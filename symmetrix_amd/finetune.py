@@ -1,5 +1,6 @@
 """Operators for heads that are fine-tuned on the engine's descriptors and served beside it: layer norm, a shared projection
-with a low-rank adapter per row (systems, datasets or users, each with its own), and AdamW over many tensors.
+with a low-rank adapter per row (systems, datasets or users, each with its own), rows of a table by element, dataset or token,
+products with a matrix of the row's own group, the norm of gradients, and AdamW over many tensors.
 
 Tensors are torch's, on the GPU, in float32, bfloat16 or float16; work goes to torch's current stream of their device.  The
 forward and backward calls are plain functions; layer_norm and adapted_linear are the same for torch's automatic
@@ -8,6 +9,7 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+import math
 import struct
 
 import torch
@@ -18,6 +20,8 @@ _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 MOMENT_BLOCK = 256          # moments in 8 bits: numbers to a scale
 MAX_RANK = 128
 MAX_ADAPTERS = 4096
+MAX_GROUPS = 4096
+MAX_ENTRIES = 1 << 24
 
 
 class _Adapted(C.Structure):
@@ -33,11 +37,26 @@ class _AdamwTensor(C.Structure):
                 ("scale_avg", C.c_void_p), ("scale_avg_sq", C.c_void_p), ("numel", C.c_long)]
 
 
+class _Grouped(C.Structure):
+    """smx_grouped_linear"""
+    _fields_ = [("type", C.c_int), ("d_in", C.c_int), ("d_out", C.c_int), ("num_groups", C.c_int), ("rows", C.c_long), ("x", C.c_void_p), ("x_stride", C.c_long),
+                ("weight", C.c_void_p), ("weight_stride", C.c_long), ("weight_each", C.c_long), ("bias", C.c_void_p), ("index", C.c_void_p), ("order", C.c_void_p),
+                ("offsets", C.c_void_p)]
+
+
+class _GradTensor(C.Structure):
+    """smx_grad_tensor"""
+    _fields_ = [("type", C.c_int), ("grad", C.c_void_p), ("out", C.c_void_p), ("numel", C.c_long)]
+
+
 # the same as packed bytes, which are made in a fraction of the time
 _ADAPTED = struct.Struct("@5iqPqPqPPPP")
 _ADAMW_TENSOR = struct.Struct("@7Pq")
 _ADAMW_FIRST = struct.Struct("@2P")          # param and grad
+_GROUPED = struct.Struct("@4iqPqPqqPPPP")
+_GRAD_TENSOR = struct.Struct("@iPPq")
 assert _ADAPTED.size == C.sizeof(_Adapted) and _ADAMW_TENSOR.size == C.sizeof(_AdamwTensor)
+assert _GROUPED.size == C.sizeof(_Grouped) and _GRAD_TENSOR.size == C.sizeof(_GradTensor)
 
 
 _functions = None
@@ -56,7 +75,19 @@ def _lib_functions():
                 ("smx_adapted_linear_forward", [p, p, n, p, n, p]),
                 ("smx_adapted_linear_backward", [p, p, n, p, n, p, p, p, n, p]),
                 ("smx_adamw_step", [i, i, i, p, i, d, d, d, d, d, n, p]),
-                ("smx_moment_values", [n, p, p, p, p, p, p, p])):
+                ("smx_adamw_step_scaled", [i, i, i, p, i, d, d, d, d, d, n, p, p]),
+                ("smx_moment_values", [n, p, p, p, p, p, p, p]),
+                ("smx_group_rows_workspace", [n, i, p]),
+                ("smx_group_rows", [n, i, p, p, p, p, n, p]),
+                ("smx_embedding_forward", [i, n, i, i, p, n, p, d, p, n, p]),
+                ("smx_embedding_backward_workspace", [i, n, i, i, p]),
+                ("smx_embedding_backward", [i, n, i, i, p, n, p, p, p, d, p, p, n, p]),
+                ("smx_grouped_linear_workspace", [p, i, p]),
+                ("smx_grouped_linear_forward", [p, p, n, p, n, p]),
+                ("smx_grouped_linear_backward", [p, p, n, p, n, p, p, p, n, p]),
+                ("smx_grad_norm_workspace", [p, i, p]),
+                ("smx_grad_norm", [p, i, d, p, p, p, n, p]),
+                ("smx_clip_grads", [p, i, d, p, p, n, p])):
             getattr(L, name).argtypes = args
         _functions = L
     return _functions
@@ -293,6 +324,295 @@ def adapted_linear(x, weight, A, B, scale, index):
     return _AdaptedLinear.apply(x, weight, A, B, scale, index)
 
 
+# ---- rows by group
+
+class RowGroups:
+    """Rows sorted by group, for calls that share one index: what group_rows returns, to be given in the index's place.
+
+    order: the rows (int32), those of group 0 first, then 1 and so on, then rows without a group (-1), then those whose index is out of range.
+    offsets: where in it each group begins, where the rows without one do, and where those out of range do [num_groups + 2]."""
+
+    def __init__(self, index, num_groups, order, offsets):
+        self.index, self.num_groups, self.order, self.offsets = index, num_groups, order, offsets
+        self._version = self._now()
+
+    def _now(self):          # (tensors of inference mode count no versions)
+        return None if self.index.is_inference() else self.index._version
+
+    def of(self, num_groups):
+        _need(num_groups == self.num_groups, f"rows by {num_groups} groups expected, not by {self.num_groups}")
+        _need(self._now() == self._version, "the index has been written to since its rows were sorted")
+        return self
+
+
+@functools.lru_cache(maxsize=1024)
+def _group_rows_workspace(rows, num_groups):
+    size = C.c_long()
+    _lib.check(_lib_functions().smx_group_rows_workspace(rows, num_groups, C.byref(size)))
+    return size.value
+
+
+def _index(index, shape=None):
+    """The tensor of an index (int32, one number a row) or of RowGroups."""
+    groups = None
+    if isinstance(index, RowGroups):
+        index, groups = index.index, index
+    if index.dtype != torch.int32:
+        raise TypeError(f"index: int32 expected, not {index.dtype}")
+    _need((shape is None or index.shape == shape) and index.is_contiguous(), "index: a contiguous number a row expected")
+    return index, groups
+
+
+def group_rows(index, num_groups):
+    """The rows of an index (int32; -1: no group) sorted by group, in their own order inside each."""
+    index, _ = _index(index)
+    _need(0 <= num_groups <= MAX_ENTRIES, f"num_groups: 0 to {MAX_ENTRIES}")
+    device, rows = _on(index), index.numel()
+    order, offsets = index.new_empty((rows,)), index.new_empty((num_groups + 2,))
+    work = index.new_empty((_group_rows_workspace(rows, num_groups),), dtype=torch.uint8)
+    _call(device, _lib_functions().smx_group_rows, rows, num_groups, index.data_ptr(), order.data_ptr(), offsets.data_ptr(), work.data_ptr(), work.numel())
+    return RowGroups(index, num_groups, order, offsets)
+
+
+# ---- rows of a table
+
+def embedding_forward(table, index, scale=1.0):
+    """scale table[index] for every row of index (int32; -1: a row of zeros).  A row whose index is out of range is NaN."""
+    kind = _type(table, "table")
+    _need(table.dim() == 2 and table.shape[1] >= 1, "table: [entries, dim] expected")
+    entries, dim = table.shape
+    _need(entries <= MAX_ENTRIES and math.isfinite(scale), f"entries: up to {MAX_ENTRIES}; scale: a finite number")
+    index, groups = _index(index)
+    if groups is not None:
+        groups.of(entries)
+    device = _on(table, index)
+    table, _, stride = _rows(table, dim, "table")
+    y = table.new_empty(index.shape + (dim,))
+    _call(device, _lib_functions().smx_embedding_forward, kind, index.numel(), entries, dim, table.data_ptr(), stride, index.data_ptr(), scale, y.data_ptr(), dim)
+    return y
+
+
+@functools.lru_cache(maxsize=1024)
+def _embedding_workspace(kind, rows, entries, dim):
+    size = C.c_long()
+    _lib.check(_lib_functions().smx_embedding_backward_workspace(kind, rows, entries, dim, C.byref(size)))
+    return size.value
+
+
+def embedding_backward(dy, index, entries, scale=1.0):
+    """The gradient of a table [entries, dim]: scale times the sum of the rows of dy of every entry, in the type of dy."""
+    kind = _type(dy, "dy")
+    _need(dy.dim() >= 1 and dy.shape[-1] >= 1, "dy: rows of at least one number expected")
+    dim = dy.shape[-1]
+    _need(0 <= entries <= MAX_ENTRIES and math.isfinite(scale), f"entries: 0 to {MAX_ENTRIES}; scale: a finite number")
+    index, groups = _index(index, dy.shape[:-1])
+    device = _on(dy, index)
+    order = offsets = 0
+    if groups is not None:
+        groups.of(entries)
+        order, offsets = groups.order.data_ptr(), groups.offsets.data_ptr()
+    dy_rows, rows, stride = _rows(dy, dim, "dy")
+    dtable = dy.new_empty((entries, dim))
+    work = dy.new_empty((_embedding_workspace(kind, rows, entries, dim),), dtype=torch.uint8)
+    _call(device, _lib_functions().smx_embedding_backward, kind, rows, entries, dim, dy_rows.data_ptr(), stride, index.data_ptr(), order, offsets, scale,
+          dtable.data_ptr(), work.data_ptr(), work.numel())
+    return dtable
+
+
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, table, index, scale):
+        y = embedding_forward(table, index, scale)
+        ctx.groups = index if isinstance(index, RowGroups) else None
+        ctx.save_for_backward(index.index if ctx.groups else index)
+        ctx.entries, ctx.scale = table.shape[0], scale
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        return embedding_backward(dy, ctx.groups or ctx.saved_tensors[0], ctx.entries, ctx.scale), None, None
+
+
+def embedding(table, index, scale=1.0):
+    """embedding_forward, differentiable once with respect to table."""
+    return _Embedding.apply(table, index, scale)
+
+
+# ---- a product with a matrix of the row's own group
+
+def _grouped(x, weight, bias, index):
+    kind = _type(x, "x")
+    _need(weight.dim() == 3 and weight.shape[1] >= 1 and weight.shape[2] >= 1, "weight: [groups, d_out, d_in] expected")
+    n, d_out, d_in = weight.shape
+    _need(x.dim() >= 1 and x.shape[-1] == d_in, "x: rows of d_in numbers expected")
+    _need(n <= MAX_GROUPS, f"groups: up to {MAX_GROUPS}")
+    if weight.dtype != x.dtype or (bias is not None and bias.dtype != x.dtype):
+        raise TypeError("x, weight and bias: one type expected")
+    if bias is not None:
+        _need(bias.shape == (n, d_out) and bias.is_contiguous(), "bias: contiguous, [groups, d_out] expected")
+    index, groups = _index(index, x.shape[:-1])
+    device = _on(x, weight, bias, index)
+    order = offsets = 0
+    if groups is not None:
+        groups.of(n)
+        order, offsets = groups.order.data_ptr(), groups.offsets.data_ptr()
+    rows_of, rows, stride = _rows(x, d_in, "x")
+    if (d_in > 1 and weight.stride(2) != 1) or (d_out > 1 and weight.stride(1) < d_in) or weight.stride(0) < 0:
+        weight = weight.contiguous()
+    weight_stride, each = (weight.stride(1) if d_out > 1 else d_in), weight.stride(0)
+    p = _GROUPED.pack(kind, d_in, d_out, n, rows, rows_of.data_ptr(), stride, weight.data_ptr(), weight_stride, each, 0 if bias is None else bias.data_ptr(),
+                      index.data_ptr(), order, offsets)
+    # (the copies live until the call is made)
+    return device, p, (kind, d_in, d_out, n, rows, stride, weight_stride, each), (rows_of, weight)
+
+
+@functools.lru_cache(maxsize=1024)
+def _grouped_workspace(sizes, backward):
+    """Bytes of a call's workspace, which depends on sizes alone."""
+    kind, d_in, d_out, n, rows, stride, weight_stride, each = sizes
+    size, some = C.c_long(), 256
+    _lib.check(_lib_functions().smx_grouped_linear_workspace(
+        _GROUPED.pack(kind, d_in, d_out, n, rows, some, stride, some, weight_stride, each, 0, some, 0, 0), backward, C.byref(size)))
+    return size.value
+
+
+def grouped_linear_forward(x, weight, bias, index):
+    """y = weight[g] x + bias[g] for every row of x, g = index of the row (int32; -1: no group, zeros), or RowGroups of it.
+
+    x[..., d_in], weight[groups, d_out, d_in] and bias[groups, d_out] (or None) are of one type.  Rows may come in any order, groups may
+    have none.  A row whose index is out of range is NaN."""
+    device, p, sizes, keep = _grouped(x, weight, bias, index)
+    y = x.new_empty(x.shape[:-1] + (sizes[2],))
+    work = x.new_empty((_grouped_workspace(sizes, 0),), dtype=torch.uint8)
+    _call(device, _lib_functions().smx_grouped_linear_forward, p, y.data_ptr(), sizes[2], work.data_ptr(), work.numel())
+    return y
+
+
+def grouped_linear_backward(dy, x, weight, index, need=(True, True, True)):
+    """Gradients of x, weight and bias (None where `need` says so); zeros for groups without a row."""
+    device, p, sizes, keep = _grouped(x, weight, None, index)
+    d_in, d_out, n = sizes[1:4]
+    _need(dy.shape == x.shape[:-1] + (d_out,), "dy: a row of d_out numbers for every row of x expected")
+    if dy.dtype != x.dtype:
+        raise TypeError("dy: the type of x expected")
+    _on(x, dy)
+    dy_rows, _, dy_stride = _rows(dy, d_out, "dy")
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format) if need[0] else None
+    dw = torch.empty_like(weight, memory_format=torch.contiguous_format) if need[1] else None
+    db = x.new_empty((n, d_out)) if need[2] else None
+    work = x.new_empty((_grouped_workspace(sizes, 1),), dtype=torch.uint8)
+    _call(device, _lib_functions().smx_grouped_linear_backward, p, dy_rows.data_ptr(), dy_stride, 0 if dx is None else dx.data_ptr(), d_in,
+          0 if dw is None else dw.data_ptr(), 0 if db is None else db.data_ptr(), work.data_ptr(), work.numel())
+    return dx, dw, db
+
+
+class _GroupedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, index):
+        ctx.groups = index if isinstance(index, RowGroups) else None
+        ctx.save_for_backward(x, weight, index.index if ctx.groups else index)
+        ctx.biased = bias is not None
+        return grouped_linear_forward(x, weight, bias, index)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, index = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        return *grouped_linear_backward(dy, x, weight, ctx.groups or index, (need[0], need[1], ctx.biased and need[2])), None
+
+
+def grouped_linear(x, weight, bias, index):
+    """grouped_linear_forward, differentiable once with respect to x, weight and bias."""
+    return _GroupedLinear.apply(x, weight, bias, index)
+
+
+# ---- the norm of gradients
+
+def _describe_grads(grads, outs):
+    """The descriptions of tensors that are there (not None), their device, how many, and what has to live until the call is made."""
+    packed, keep, device = [], [], None
+    for g, o in zip(grads, outs):
+        if g is None:
+            continue
+        kind = _type(g, "gradients")
+        at = g.get_device()
+        if device is None:
+            device = _on(g)
+        elif at != device:
+            raise ValueError("gradients on one device expected")
+        if not g.is_contiguous():
+            g = g.contiguous()
+            keep.append(g)
+        packed.append(_GRAD_TENSOR.pack(kind, g.data_ptr(), 0 if o is None else o.data_ptr(), g.numel()))
+    return b"".join(packed), device, len(packed), keep
+
+
+def _norm_call(described, max_norm, clip):
+    """The norm, and the factor where nothing is clipped: float32, a number each."""
+    packed, device, count, keep = described
+    size = C.c_long()
+    L = _lib_functions()
+    _lib.check(L.smx_grad_norm_workspace(packed, count, C.byref(size)))
+    # (the numbers lie in front of the workspace: one allocation)
+    both = torch.empty((256 + size.value,), dtype=torch.uint8, device=torch.device("cuda", device))
+    norm = both[:8].view(torch.float32)
+    at = both.data_ptr()
+    if clip:
+        _call(device, L.smx_clip_grads, packed, count, max_norm, at, at + 256, size.value)
+    else:
+        _call(device, L.smx_grad_norm, packed, count, max_norm, at, at + 4, at + 256, size.value)
+    return norm
+
+
+def grad_norm(grads):
+    """The norm of all numbers of the tensors together, sqrt(sum g^2), as a float32 tensor of no dimensions.
+
+    Tensors may be of different types and shapes; None stands for a gradient that is not there."""
+    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
+    described = _describe_grads(grads, [None] * len(grads))
+    if not described[2]:
+        return torch.zeros((), device="cuda")
+    return _norm_call(described, math.inf, False)[0]
+
+
+def clip_grads(grads, max_norm, out=None):
+    """Brings the gradients to a norm of at most max_norm together, g min(1, max_norm / norm), in place or into out (tensors like
+    grads, each with memory of its own), and returns the norm that they had.  Where the norm is not finite they stay as they are."""
+    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
+    _need(max_norm >= 0, "max_norm: a number from 0 on")
+    back = []          # gradients that are clipped in a contiguous copy
+    if out is None:
+        there = [g for g in grads if g is not None]
+        for k, g in enumerate(grads):
+            if g is not None and not g.is_contiguous():
+                grads[k] = g.contiguous()
+                back.append((g, grads[k]))
+        out = grads
+    else:
+        out = [out] if isinstance(out, torch.Tensor) else list(out)
+        _need(len(out) == len(grads), "out: a tensor for every gradient expected")
+        there = [o for g, o in zip(grads, out) if g is not None]
+        for g, o in zip(grads, out):
+            if g is not None:
+                _need(o is not None, "out: a tensor for every gradient expected")
+                if o.dtype != g.dtype:
+                    raise TypeError("out: the types of the gradients expected")
+                _need(o.shape == g.shape and o.is_contiguous() and o.get_device() == g.get_device(), "out: contiguous, of the gradients' shapes and on their device, expected")
+    starts = [o.data_ptr() for g, o in zip(grads, out) if g is not None and o.numel()]
+    _need(len(set(starts)) == len(starts), "tensors that are written: every one once expected, each with memory of its own")
+    described = _describe_grads(grads, out)
+    if not described[2]:
+        return torch.zeros((), device="cuda")
+    norm = _norm_call(described, max_norm, True)
+    for g, copy in back:
+        g.copy_(copy)
+    # (as torch's own operations in place do)
+    torch.autograd.graph.increment_version(there)
+    return norm[0]
+
+
 # ---- AdamW
 
 def moment_values(code_avg, scale_avg, code_avg_sq, scale_avg_sq):
@@ -419,11 +739,16 @@ class AdamW:
             return make(n, torch.float32), make(n, torch.float32)
         return make(n, torch.int8), make(blocks, torch.float32), make(n, torch.uint8), make(blocks, torch.float32)
 
-    def step(self, grads=None):
+    def step(self, grads=None, max_norm=None):
         """One step with the given gradients, one for every parameter (None: the parameters' own).  A parameter without a gradient
-        (None) is left as it is, and does not count the step.  Gradients are of the parameters' type or all in float32."""
+        (None) is left as it is, and does not count the step.  Gradients are of the parameters' type or all in float32.
+
+        max_norm: the step goes by gradients clipped to this norm together, as clip_grads does, but without writing them; returned is
+        their norm before (a norm that is not finite clips nothing)."""
+        norm = None
         if grads is None:
             grads = [p.grad for p in self.params]
+        _need(max_norm is None or max_norm >= 0, "max_norm: a number from 0 on")
         _need(len(grads) == len(self.params), "a gradient (or None) for every parameter expected")
         taken = [i for i, g in enumerate(grads) if g is not None]
         if taken:
@@ -431,7 +756,7 @@ class AdamW:
             kind = grads[taken[0]].dtype
             if kind != own and kind != torch.float32:
                 raise TypeError(f"gradients: {own} or float32, not {kind}")
-            keep, wide, size = [], self._bits == 32, _ADAMW_TENSOR.size
+            keep, wide, size, described = [], self._bits == 32, _ADAMW_TENSOR.size, []
             shapes, held, states, masters, table, first = self._shapes, self._held, self._states, self._masters, self._table, _ADAMW_FIRST.pack_into
             for i in taken:
                 p, g, shape, s = params[i], grads[i], shapes[i], states[i]
@@ -450,6 +775,10 @@ class AdamW:
                     held[i] = self._hold(i, states, masters)
                     _ADAMW_TENSOR.pack_into(table, i * size, 0, 0, *held[i][0])
                 first(table, i * size, p.data_ptr(), g.data_ptr())
+                if max_norm is not None:
+                    described.append(_GRAD_TENSOR.pack(_TYPES[kind], g.data_ptr(), 0, g.numel()))
+            if max_norm is not None:
+                described = (b"".join(described), device, len(described), keep)
             missed = self._missed
             if any(missed):
                 _need(all(missed[i] <= self.step_count for i in taken), "step_count: less than the steps that a parameter has missed")
@@ -458,9 +787,14 @@ class AdamW:
                     calls[missed[i]] = calls.get(missed[i], b"") + table[i * size:(i + 1) * size]
             else:          # (no parameter has missed a step so far; some may have no gradient in this one)
                 calls = {0: bytes(table) if len(taken) == len(params) else b"".join(table[i * size:(i + 1) * size] for i in taken)}
+            norm = None if max_norm is None else _norm_call(described, max_norm, False)
             for late, some in calls.items():
-                _call(device, _lib_functions().smx_adamw_step, _TYPES[own], _TYPES[kind], self._bits, some, len(some) // size, self.lr, self.betas[0],
-                      self.betas[1], self.eps, self.weight_decay, self.step_count + 1 - late)
+                of = (_TYPES[own], _TYPES[kind], self._bits, some, len(some) // size, self.lr, self.betas[0], self.betas[1], self.eps, self.weight_decay,
+                      self.step_count + 1 - late)
+                if norm is None:
+                    _call(device, _lib_functions().smx_adamw_step, *of)
+                else:
+                    _call(device, _lib_functions().smx_adamw_step_scaled, *of, norm.data_ptr() + 4)
             # (as torch's own operations in place do: a backward pass that saved the old values says so)
             torch.autograd.graph.increment_version(params if len(taken) == len(params) else [params[i] for i in taken])
         if len(taken) < len(grads):
@@ -468,3 +802,5 @@ class AdamW:
                 if g is None:
                     self._missed[i] += 1
         self.step_count += 1
+        if max_norm is not None:
+            return norm[0] if norm is not None else torch.zeros((), device=torch.device("cuda", self._device) if self.params else "cuda")
