@@ -2,8 +2,9 @@
 //
 //   y_i = scale table[index_i],   dtable_t = scale sum over the rows with index t of dy_i
 //
-// Forward: neighbouring threads take neighbouring 16 bytes of a row, a thread four rows at a time.  Gradient: rows sorted by entry, then
-// a wavefront for every entry and 1 KB of its row.
+// Forward: neighbouring threads take neighbouring 16 bytes of a row, a thread four rows at a time.  Gradient: rows sorted by entry, cut
+// into pieces of equal length whatever their entries (an entry may have one row, or all), and a second launch for the entries that lie in
+// several pieces and for those without a row.
 //
 // Bound by memory.
 #include "smx_groups.hpp"
@@ -50,34 +51,177 @@ __global__ __launch_bounds__(256) void k_lookup(const Lookup p)
     }
 }
 
+// ---- sums of rows by group
+
 struct Sums {
-    const void* dy;
-    long dy_stride;
-    const int *order, *offsets;
-    void* dtable;
-    int entries, dim, slabs;
+    const void* in;
+    long in_stride;
+    const int *index, *order;
+    const int* keys;           // sorted, or null: those of index
+    int* offsets;              // written by blocks behind the pieces' where they are not there yet
+    long rows;
+    int groups, dim, slabs, piece;
+    long pieces;
+    float* partial;            // [piece][0: of a run of rows that began before the piece, 1: that goes on behind it][dim]
     float scale;
+    void* out;
+    long first;                // which of all blocks the launch's first one is
 };
+
+// Pieces of sorted rows, a wavefront for 1 KB of each row.  A group's rows that lie in one piece are summed and stored; of a
+// group that goes on in other pieces, a part.  Eight rows are under way at a time.
 template <typename T>
-__global__ __launch_bounds__(256) void k_entry_sums(const Sums p)
+__global__ __launch_bounds__(256) void k_pieces(const Sums p)
 {
-    constexpr int V = kRun<T>;
-    const long item = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int t = (int)(item / p.slabs), at = (int)(item % p.slabs) * 64 * V + (threadIdx.x & 63) * V;
-    if (t >= p.entries || at >= p.dim) return;
-    const int begin = p.offsets[t], end = p.offsets[t + 1];
+    constexpr int V = kRun<T>, U = 8;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const long items = p.pieces * p.slabs, blocks = (items + 3) / 4;
+    const long block = p.first + blockIdx.x;
+    if (block >= blocks) {      // (offsets)
+        const int g = (int)(block - blocks) * 256 + threadIdx.x;
+        if (g < p.groups + 2) p.offsets[g] = first_place(p.keys, (int)p.rows, g);
+        return;
+    }
+    const long item = block * 4 + wave;
+    if (item >= items) return;
+    const long piece = item / p.slabs;
+    const int at = (int)(item % p.slabs) * 64 * V + lane * V;
+    const long begin = piece * p.piece;
+    const int count = (int)min((long)p.piece, p.rows - begin);
+    auto key_at = [&](long i, int row) { return p.keys ? p.keys[i] : row_key(p.index[row], p.groups); };
+    const int my_row = p.order[begin + min(lane, count - 1)];
+    const int my_key = key_at(begin + min(lane, count - 1), my_row);
+    // (a key behind the groups' on either side: none)
+    const int before = begin > 0 ? key_at(begin - 1, p.keys ? 0 : p.order[begin - 1]) : -1;
+    const int behind = begin + count < p.rows ? key_at(begin + count, p.keys ? 0 : p.order[begin + count]) : -1;
+    const T* in = static_cast<const T*>(p.in) + at;
+    const bool whole = at + V <= p.dim, some = at < p.dim;
     float sum[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) sum[j] = 0.0f;
-    for (int i = begin; i < end; ++i) {
-        float v[V];
-        load_run<V>(static_cast<const T*>(p.dy) + p.order[i] * p.dy_stride + at, p.dim - at, v);
+    int key = __builtin_amdgcn_readlane(my_key, 0);
+    bool entered = key == before;
+    auto flush = [&](bool leaves) {
+        if (!some) return;
+        if (entered || leaves) {
+            store_run<V>(p.partial + (2 * piece + (entered ? 0 : 1)) * p.dim + at, p.dim - at, sum);
+        } else {
 #pragma unroll
-        for (int j = 0; j < V; ++j) sum[j] += v[j];
+            for (int j = 0; j < V; ++j) sum[j] *= p.scale;
+            store_run<V>(static_cast<T*>(p.out) + (long)key * p.dim + at, p.dim - at, sum);
+        }
+    };
+#pragma unroll 1
+    for (int i0 = 0; i0 < count; i0 += U) {
+        typename Operand<T>::type x[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const long row = __builtin_amdgcn_readlane(my_row, min(i0 + u, count - 1));
+            if (whole) x[u] = *reinterpret_cast<const typename Run<T, V>::loose*>(in + row * p.in_stride);
+            else x[u] = load_operand(in + (some ? row * p.in_stride : 0), p.dim - at);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (i0 + u >= count) break;
+            const int k = __builtin_amdgcn_readlane(my_key, i0 + u);
+            if (k >= p.groups && key >= p.groups) break;
+            if (k != key) {
+                flush(false);
+#pragma unroll
+                for (int j = 0; j < V; ++j) sum[j] = 0.0f;
+                key = k;
+                entered = false;
+            }
+#pragma unroll
+            for (int j = 0; j < V; ++j) sum[j] += (float)x[u][j];
+        }
+        if (key >= p.groups) return;      // (what lies behind belongs to no group)
+    }
+    flush(key == behind);
+}
+
+// Groups whose rows lie in several pieces: the parts, in order.  Groups without rows: zeros.  WAVES wavefronts share a group's 1 KB.
+template <typename T, int WAVES>
+__global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void k_join_pieces(const Sums p)
+{
+    constexpr int V = kRun<T>;
+    __shared__ float part[WAVES == 1 ? 1 : WAVES][64][V];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const long item = WAVES == 1 ? (p.first + blockIdx.x) * 4 + wave : p.first + blockIdx.x;
+    if (item >= (long)p.groups * p.slabs) return;
+    const int g = (int)(item / p.slabs), at = (int)(item % p.slabs) * 64 * V + lane * V;
+    const int begin = p.offsets[g], end = p.offsets[g + 1];
+    const int first = begin / p.piece, last = end > begin ? (end - 1) / p.piece : first;
+    if (end > begin && first == last) return;      // (the same in all wavefronts)
+    float sum[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) sum[j] = 0.0f;
+    const bool some = at < p.dim;
+    if (end > begin && some) {
+        // (the first part lies in its piece's second place, the others in the first)
+        auto part_of = [&](long k) { return p.partial + (2 * k + (k == first ? 1 : 0)) * p.dim + at; };
+        const int mine = WAVES == 1 ? 0 : wave;
+#pragma unroll 8
+        for (int k = first + mine; k <= last; k += WAVES) {
+            float v[V];
+            load_run<V>(part_of(k), p.dim - at, v);
+#pragma unroll
+            for (int j = 0; j < V; ++j) sum[j] += v[j];
+        }
+    }
+    if constexpr (WAVES > 1) {
+        if (end > begin) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) part[wave][lane][j] = sum[j];
+            __syncthreads();
+            if (wave > 0) return;
+#pragma unroll
+            for (int w = 1; w < WAVES; ++w)
+#pragma unroll
+                for (int j = 0; j < V; ++j) sum[j] += part[w][lane][j];
+        } else if (wave > 0) return;
+    }
+    if (!some) return;
+#pragma unroll
+    for (int j = 0; j < V; ++j) sum[j] *= p.scale;
+    store_run<V>(static_cast<T*>(p.out) + (long)g * p.dim + at, p.dim - at, sum);
+}
+
+// Few rows: a wavefront for 1 KB of a group's sum looks through the index by itself.
+template <typename T>
+__global__ __launch_bounds__(256) void k_few_rows(const Sums p)
+{
+    constexpr int V = kRun<T>, U = 8;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const long item = (p.first + blockIdx.x) * 4 + wave;
+    if (item >= (long)p.groups * p.slabs) return;
+    const int g = (int)(item / p.slabs), at = (int)(item % p.slabs) * 64 * V + lane * V;
+    float sum[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) sum[j] = 0.0f;
+    for (int i0 = 0; i0 < p.rows; i0 += 64) {
+        unsigned long left = __ballot(i0 + lane < p.rows && p.index[min((long)i0 + lane, p.rows - 1)] == g);
+        while (left) {
+            float x[U][V];
+            int n = 0;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int bit = left ? __builtin_ctzl(left) : 64;
+                left &= left - 1;
+                n += bit < 64;
+                const long row = i0 + min(bit, 63);
+                if (bit < 64) load_run<V>(static_cast<const T*>(p.in) + row * p.in_stride + at, p.dim - at, x[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (u < n)
+#pragma unroll
+                    for (int j = 0; j < V; ++j) sum[j] += x[u][j];
+        }
     }
 #pragma unroll
     for (int j = 0; j < V; ++j) sum[j] *= p.scale;
-    store_run<V>(static_cast<T*>(p.dtable) + (long)t * p.dim + at, p.dim - at, sum);
+    store_run<V>(static_cast<T*>(p.out) + (long)g * p.dim + at, p.dim - at, sum);
 }
 
 // ---- host side
@@ -89,30 +233,57 @@ void check(long rows, int entries, int dim)
     refuse_unless(dim >= 1 && dim <= 1 << 20, "dim: 1 to 2^20");
 }
 
-struct Call : Launches {
-    Arena arena;
-    template <typename T>
-    void backward(long rows, int entries, int dim, const T* dy, long dy_stride, const int* index, const int* order, const int* offsets, float scale, T* dtable)
-    {
-        constexpr int V = kRun<T>;
-        if (!order) {
-            const RowOrder sorted{arena.take<int>(rows), arena.take<int>(entries + 2L), nullptr};
-            sort_rows(*this, arena, index, rows, entries, sorted);
-            order = sorted.order;
-            offsets = sorted.offsets;
-        }
-        const int slabs = (dim + 64 * V - 1) / (64 * V);
-        start(k_entry_sums<T>, ((long)entries * slabs + 3) / 4, 1, 1, 256, 0, Sums{dy, dy_stride, order, offsets, dtable, entries, dim, slabs, scale});
-    }
-};
 long workspace(int type, long rows, int entries, int dim)
 {
-    Call c{{nullptr, true}, {reinterpret_cast<char*>(256)}};
-    with_type(type, [&](auto t) { c.backward<decltype(t)>(rows, entries, dim, nullptr, dim, nullptr, nullptr, nullptr, 1.0f, nullptr); });
-    return c.arena.used;
+    Launches dry{nullptr, true};
+    Arena arena{reinterpret_cast<char*>(256)};
+    add_rows(dry, arena, type, nullptr, dim, nullptr, rows, entries, dim, RowOrder{}, 1.0f, nullptr);
+    return arena.used;
 }
 
 }  // namespace
+
+// Rows up to which a wavefront looks through the index by itself.
+constexpr int kMostFew = 128;
+
+void add_rows(Launches& launches, Arena& arena, int type, const void* in, long in_stride, const int* index, long rows, int groups, int dim, RowOrder sorted, float scale, void* out)
+{
+    with_type(type, [&](auto t) {
+        using T = decltype(t);
+        constexpr int V = kRun<T>;
+        Sums p{};
+        p.in = in; p.in_stride = in_stride; p.index = index; p.rows = rows; p.groups = groups; p.dim = dim; p.scale = scale; p.out = out;
+        p.slabs = (dim + 64 * V - 1) / (64 * V);
+        const long entries = (long)groups * p.slabs;
+        auto start = [&](auto kernel, long blocks, int threads) {
+            Launches::in_slabs(blocks, [&](long first, long some) {
+                p.first = first;
+                launches.start(kernel, some, 1, 1, threads, 0, p);
+            });
+        };
+        if (rows <= kMostFew) {
+            start(k_few_rows<T>, (entries + 3) / 4, 256);
+            return;
+        }
+        // pieces of 8 to 64 rows, until there are 16 wavefronts for every CU
+        p.piece = 8;
+        while (p.piece < 64 && rows * p.slabs / p.piece > 4096) p.piece *= 2;
+        p.pieces = (rows + p.piece - 1) / p.piece;
+        p.partial = arena.take<float>(2 * p.pieces * dim);
+        long offset_blocks = 0;
+        if (!sorted.order) {
+            sorted = RowOrder{arena.take<int>(rows), arena.take<int>(groups + 2L), arena.take<int>(rows)};
+            // (where the sort has them anyway it writes the offsets; otherwise they are looked for beside the pieces)
+            const bool with_offsets = sort_has_offsets(rows, groups);
+            sort_rows(launches, arena, index, rows, groups, RowOrder{sorted.order, with_offsets ? sorted.offsets : nullptr, sorted.keys});
+            if (!with_offsets) offset_blocks = (groups + 2L + 255) / 256;
+        }
+        p.order = sorted.order; p.offsets = sorted.offsets; p.keys = sorted.keys;
+        start(k_pieces<T>, (p.pieces * p.slabs + 3) / 4 + offset_blocks, 256);
+        if (groups <= 4096) start(k_join_pieces<T, 16>, entries, 1024);
+        else start(k_join_pieces<T, 1>, (entries + 3) / 4, 256);
+    });
+}
 
 }  // namespace smx
 
@@ -167,11 +338,10 @@ extern "C" int smx_embedding_backward(int type, long rows, int entries, int dim,
         if (rows == 0) d_order = d_offsets = nullptr;
         check_workspace(d_workspace, workspace_bytes, workspace(type, rows, entries, dim), "smx_embedding_backward_workspace");
         require_gfx950();
-        Call c{{static_cast<hipStream_t>(stream), false}, {static_cast<char*>(d_workspace)}};
-        with_type(type, [&](auto t) {
-            using T = decltype(t);
-            c.backward<T>(rows, entries, dim, static_cast<const T*>(d_dy), dy_stride, d_index, d_order, d_offsets, (float)scale, static_cast<T*>(d_dtable));
-        });
+        Launches launches{static_cast<hipStream_t>(stream), false};
+        Arena arena{static_cast<char*>(d_workspace)};
+        add_rows(launches, arena, type, d_dy, dy_stride, d_index, rows, entries, dim, RowOrder{const_cast<int*>(d_order), const_cast<int*>(d_offsets), nullptr},
+                 (float)scale, d_dtable);
         hip_ok(hipGetLastError(), "launch");
     });
 }

@@ -148,17 +148,6 @@ __global__ __launch_bounds__(kThreads) void k_sort_place(const Pass p)
     }
 }
 
-// first place in sorted keys that holds `key` or more
-__device__ __forceinline__ int first_place(const int* keys, int n, int key)
-{
-    int low = 0;
-    while (n > 0) {
-        const int half = n / 2;
-        if (keys[low + half] < key) low += half + 1, n -= half + 1;
-        else n = half;
-    }
-    return low;
-}
 __global__ __launch_bounds__(256) void k_sort_offsets(const int* keys, int rows, int groups, int* offsets)
 {
     const int g = blockIdx.x * 256 + threadIdx.x;
@@ -170,6 +159,9 @@ __global__ __launch_bounds__(256) void k_no_rows(int* offsets, int n)
     const int i = blockIdx.x * 256 + threadIdx.x;
     if (i < n) offsets[i] = 0;
 }
+
+// (offsets of more groups by one block would take longer than the sort)
+constexpr int kMostInside = 8192;
 
 // All digits in one block.
 struct SmallSort {
@@ -236,6 +228,8 @@ __global__ __launch_bounds__(1024) void k_sort_small(const SmallSort p)
 
 }  // namespace
 
+bool sort_has_offsets(long rows, int groups) { return rows <= kSmallRows ? groups <= kMostInside : groups + 2L <= kMostDigits; }
+
 void sort_rows(Launches& launches, Arena& arena, const int* index, long rows, int groups, const RowOrder& to)
 {
     if (rows == 0) {
@@ -244,8 +238,6 @@ void sort_rows(Launches& launches, Arena& arena, const int* index, long rows, in
     }
     int key_bits = 1;
     while ((1L << key_bits) < (long)groups + 2) ++key_bits;
-    // (offsets of many groups by one block would take longer than the sort)
-    constexpr int kMostInside = 8192;
     int* keys = to.keys;
     auto offsets = [&] { launches.start(k_sort_offsets, ((long)groups + 2 + 255) / 256, 1, 1, 256, 0, (const int*)keys, (int)rows, groups, to.offsets); };
     if (rows <= kSmallRows) {
