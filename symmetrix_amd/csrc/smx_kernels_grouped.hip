@@ -2,7 +2,9 @@
 //
 //   y_i = W_g x_i + b_g,   dx_i = W_g^T dy_i,   dW_g = sum over the group's rows of dy_i x_i^T,   db_g = sum of dy_i
 //
-// Rows are taken in the order of their groups; a tile has rows of one group.
+// Rows are taken in the order of their groups, by way of the sorted order: nothing is copied into it, a tile's rows are fetched from
+// where they are and its results stored where they belong.  A tile has rows of one group.  How many tiles a group has is known on the
+// device alone, so a launch has as many blocks as there can be tiles, and every block finds its own from the groups' offsets.
 #include "smx_groups.hpp"
 
 #include <limits>
@@ -11,101 +13,787 @@ namespace smx {
 
 namespace {
 
-// C(m, c) = sum over k of A(m, k) B(k, c) for the rows of a group
+enum { FORWARD = 0, ROWS = 1, WEIGHTS = 2 };      // y, dx and dW
+
+// C(m, c) = sum over k of A(m, k) B(k, c)
+//   FORWARD, ROWS: m is a row of the tile's group, A a row of x or dy; B the group's weights, in which k or c runs along rows.
+//   WEIGHTS: k is a row of the group, A(m, k) its number m of dy and B(k, c) its number c of x.
 struct Product {
-    const void* a;             // x or dy
+    const void* a;
     long a_stride;
-    const void* b;             // the weights, or x for their gradient
-    long b_each, b_k, b_c;
+    const void* b;
+    long b_each, b_stride;
     const void* bias;          // [group][cols] or null
     const int *order, *offsets;
-    int groups, k, cols;
+    int groups, k, m, cols;    // k: of FORWARD and ROWS, m: of WEIGHTS
     long rows;
     void* out;
     long out_stride;
+    int row_tiles, col_tiles;  // row_tiles: of WEIGHTS
+    int piece;                 // of WEIGHTS: rows of a group that a block sums at most
+    float* partial;            // sums of groups of more than one piece [slot][m][cols]
 };
 
-// item -> group and its tile, where a group has ceil(rows / high) of them; false behind the last
-__device__ __forceinline__ bool tile_of(const int* offsets, int groups, long rows, int item, int high, int& group, int& tile)
+// Where a block's rows are: [begin, end) of the sorted order, group `group`; slot: of a piece of WEIGHTS, or -1.
+struct Place {
+    int group, begin, end, slot;
+};
+// Items are cut from the groups in order, `high` rows each; with `all` a group without rows has one too, and the last two groups (rows
+// without a group) have none.  The number of items; a wavefront works it out for itself, 64 groups at a time.
+__device__ __forceinline__ int items_of(int count, int high, bool all) { return max((count + high - 1) / high, all ? 1 : 0); }
+__device__ __forceinline__ int rows_of(const Product& p, int g, bool all)
 {
-    for (int g = 0; g < groups + 2; ++g) {
-        const int n = (int)((g == groups + 1 ? rows : offsets[g + 1]) - offsets[g]), tiles = (n + high - 1) / high;
-        if (item < tiles) {
-            group = g;
-            tile = item;
-            return true;
-        }
-        item -= tiles;
+    if (g >= p.groups + (all ? 0 : 2)) return -1;
+    return (int)((g == p.groups + 1 ? p.rows : (long)p.offsets[g + 1]) - p.offsets[g]);
+}
+__device__ __forceinline__ int wave_inclusive(int x, int lane)
+{
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const int y = __shfl_up(x, d, 64);
+        if (lane >= d) x += y;
     }
-    return false;
+    return x;
+}
+template <bool ALL>
+__device__ __forceinline__ int count_items(const Product& p, int high, int lane)
+{
+    int total = 0;
+    for (int g0 = 0; g0 < p.groups + 2; g0 += 64) {
+        const int count = rows_of(p, g0 + lane, ALL);
+        total += __builtin_amdgcn_readlane(wave_inclusive(count < 0 ? 0 : items_of(count, high, ALL), lane), 63);
+    }
+    return total;
+}
+template <bool ALL>
+__device__ __forceinline__ Place find_item(const Product& p, int item, int high, int lane)
+{
+    Place at{-1, 0, 0, -1};
+    int slots = 0;
+    for (int g0 = 0; g0 < p.groups + 2; g0 += 64) {
+        const int count = rows_of(p, g0 + lane, ALL), n = count < 0 ? 0 : items_of(count, high, ALL), until = wave_inclusive(n, lane);
+        const int slots_until = ALL ? wave_inclusive(n > 1 ? n : 0, lane) : 0;
+        const unsigned long behind = __ballot(until > item);
+        if (behind) {
+            const int where = __builtin_ctzl(behind), mine = item - (__builtin_amdgcn_readlane(until, where) - __builtin_amdgcn_readlane(n, where));
+            at.group = g0 + where;
+            const int first = p.offsets[at.group];
+            at.begin = first + mine * high;
+            at.end = min(first + __builtin_amdgcn_readlane(count, where), at.begin + high);
+            const int pieces = __builtin_amdgcn_readlane(n, where);
+            if (ALL && pieces > 1) at.slot = slots + __builtin_amdgcn_readlane(slots_until, where) - pieces + mine;
+            return at;
+        }
+        item -= __builtin_amdgcn_readlane(until, 63);
+        slots += ALL ? __builtin_amdgcn_readlane(slots_until, 63) : 0;
+    }
+    return at;
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void k_rows(const Product p)
+// Block -> tile: the blocks of a die (every eighth) take neighbouring tiles, four row tiles high, so that they share operands in its L2.
+__device__ __forceinline__ bool tile_of(int row_tiles, int col_tiles, long block, int& rt, int& ct)
 {
-    __shared__ float as[16][65], bs[16][65];
-    int g, tile;
-    if (!tile_of(p.offsets, p.groups, p.rows, blockIdx.x, 64, g, tile)) return;
-    const int begin = p.offsets[g] + 64 * tile, end = min((long)begin + 64, g == p.groups + 1 ? p.rows : (long)p.offsets[g + 1]), col0 = blockIdx.y * 64;
-    const int tm = threadIdx.x / 16 * 4, tc = threadIdx.x % 16 * 4;
-    float acc[4][4] = {};
-    const bool real = g < p.groups;
-    for (int k0 = 0; real && k0 < p.k; k0 += 16) {
-        for (int u = threadIdx.x; u < 1024; u += 256) {
-            const int m = u / 16, k = u % 16;
-            as[k][m] = begin + m < end && k0 + k < p.k ? (float)static_cast<const T*>(p.a)[p.order[begin + m] * p.a_stride + k0 + k] : 0.0f;
-            bs[k][m] = col0 + m < p.cols && k0 + k < p.k ? (float)static_cast<const T*>(p.b)[g * p.b_each + (k0 + k) * p.b_k + (col0 + m) * p.b_c] : 0.0f;
-        }
-        __syncthreads();
-        for (int k = 0; k < 16; ++k)
-            for (int i = 0; i < 4; ++i)
-                for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(as[k][tm + i], bs[k][tc + j], acc[i][j]);
-        __syncthreads();
+    const long tiles = (long)row_tiles * col_tiles, per = (tiles + 7) / 8, at = block % 8 * per + block / 8;
+    if (at >= tiles || block / 8 >= per) return false;
+    const int band = (int)(at / (4 * col_tiles)), high = min(4, row_tiles - 4 * band), in_band = (int)(at - (long)band * 4 * col_tiles);
+    rt = band * 4 + in_band % high;
+    ct = in_band / high;
+    return true;
+}
+// A block's place and its tile; false: there is none for it.
+template <int MODE>
+__device__ __forceinline__ bool find_tile(const Product& p, int high, int lane, Place& at, int& rt, int& ct)
+{
+    if constexpr (MODE == WEIGHTS) {
+        // (the tiles of an item by neighbouring blocks of a die)
+        const int items = count_items<true>(p, p.piece, lane);
+        const long tiles = (long)p.row_tiles * p.col_tiles, all = items * tiles, per = (all + 7) / 8, block = blockIdx.x, id = block % 8 * per + block / 8;
+        if (id >= all || block / 8 >= per) return false;
+        at = find_item<true>(p, (int)(id / tiles), p.piece, lane);
+        const int in_item = (int)(id % tiles), band = in_item / (4 * p.col_tiles), tall = min(4, p.row_tiles - 4 * band), in_band = in_item - band * 4 * p.col_tiles;
+        rt = band * 4 + in_band % tall;
+        ct = in_band / tall;
+    } else {
+        if (!tile_of(count_items<false>(p, high, lane), p.col_tiles, blockIdx.x, rt, ct)) return false;
+        at = find_item<false>(p, rt, high, lane);
     }
-    for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) {
-            if (begin + tm + i >= end || col0 + tc + j >= p.cols) continue;
-            float v = acc[i][j];
-            if (real && p.bias) v += (float)static_cast<const T*>(p.bias)[(long)g * p.cols + col0 + tc + j];
-            if (g == p.groups + 1) v = std::numeric_limits<float>::quiet_NaN();
-            static_cast<T*>(p.out)[p.order[begin + tm + i] * p.out_stride + col0 + tc + j] = (T)v;
-        }
+    return true;
 }
 
-// dW: m over columns of a (dy), k over the group's rows, c over columns of b (x)
+// What rows without a group have for results
 template <typename T>
-__global__ __launch_bounds__(256) void k_weights(const Product p)
+__device__ __forceinline__ void store_none(const Product& p, const Place& at, int col0, int wide)
 {
-    __shared__ float as[16][65], bs[16][65];
-    const int g = blockIdx.z, begin = p.offsets[g], end = p.offsets[g + 1], m0 = blockIdx.x * 64, col0 = blockIdx.y * 64;
-    const int tm = threadIdx.x / 16 * 4, tc = threadIdx.x % 16 * 4;
-    float acc[4][4] = {};
-    for (int k0 = begin; k0 < end; k0 += 16) {
-        for (int u = threadIdx.x; u < 1024; u += 256) {
-            const int m = u % 64, k = u / 64;
-            const long row = p.order[min(k0 + k, end - 1)];
-            as[k][m] = m0 + m < p.k && k0 + k < end ? (float)static_cast<const T*>(p.a)[row * p.a_stride + m0 + m] : 0.0f;
-            bs[k][m] = col0 + m < p.cols && k0 + k < end ? (float)static_cast<const T*>(p.b)[row * p.b_k + col0 + m] : 0.0f;
-        }
-        __syncthreads();
-        for (int k = 0; k < 16; ++k)
-            for (int i = 0; i < 4; ++i)
-                for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(as[k][tm + i], bs[k][tc + j], acc[i][j]);
-        __syncthreads();
+    const T v = (T)(at.group == p.groups ? 0.0f : std::numeric_limits<float>::quiet_NaN());
+    const int last = min(wide, p.cols - col0);
+    for (int i = at.begin; i < at.end; ++i) {
+        T* out = static_cast<T*>(p.out) + p.order[i] * p.out_stride + col0;
+        for (int c = threadIdx.x; c < last; c += blockDim.x) out[c] = v;
     }
-    for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j)
-            if (m0 + tm + i < p.k && col0 + tc + j < p.cols) static_cast<T*>(p.out)[((long)g * p.k + m0 + tm + i) * p.cols + col0 + tc + j] = (T)acc[i][j];
 }
-// db
-template <typename T>
-__global__ __launch_bounds__(256) void k_biases(const Product p)
+
+// Lane (n, g) holds of tile (i, t) row 16 i + n and columns 16 t + 4 g + 0..3.  What is stored goes by way of other lanes, so that four
+// neighbouring lanes have 64 neighbouring bytes.
+// row(i): where row 16 i + lane / 4 of the tile goes, or null; left: columns from the tile's first on that there are.
+template <typename T, int NM, int NT, typename Row>
+__device__ __forceinline__ void store_tiles(int lane, const f32x4 (&acc)[NM][NT], int left, Row&& row)
 {
-    const int g = blockIdx.y, m = blockIdx.x * 256 + threadIdx.x;
-    if (m >= p.k) return;
+#pragma unroll
+    for (int i = 0; i < NM; ++i) {
+        T* out = row(i);
+        if constexpr (std::is_same_v<T, float>) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const f32x4 v = from_operand(acc[i][t], lane);
+                const int col = 16 * t + 4 * (lane & 3);
+                const float u[4] = {v[0], v[1], v[2], v[3]};
+                if (out) store_run<4>(out + col, left - col, u);
+            }
+        } else {
+            typedef int i32x4 __attribute__((ext_vector_type(4)));
+            const bool odd = lane >> 4 & 1;
+            // (lane group g has, after it has exchanged four numbers with its neighbour, eight from 16 (g % 2) + 8 (g / 2) on)
+            const int from = (16 * ((lane & 1) * 2 + (lane >> 1 & 1)) + (lane >> 2)) * 4;
+#pragma unroll
+            for (int t = 0; t < NT; t += 2) {
+                typename Run<T, 8>::type v;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = (T)acc[i][t + j / 4][j % 4];
+                i32x4 d = __builtin_bit_cast(i32x4, v);
+                const int give[2] = {odd ? d[0] : d[2], odd ? d[1] : d[3]};
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int got = __shfl_xor(give[h], 16, 64);
+                    d[h] = odd ? got : d[h];
+                    d[2 + h] = odd ? d[2 + h] : got;
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) d[j] = __builtin_amdgcn_ds_bpermute(from, d[j]);
+                v = __builtin_bit_cast(typename Run<T, 8>::type, d);
+                const int col = 16 * t + 8 * (lane & 3);
+                if (!out) continue;
+                if (left - col >= 8) *reinterpret_cast<typename Run<T, 8>::loose*>(out + col) = v;
+                else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (col + j < left) out[col + j] = v[j];
+                }
+            }
+        }
+    }
+}
+
+// Bias, and where the results go: what follows the sums of all modes.  row0, col0: the wavefront's first in the tile's place.
+template <typename T, int MODE, int NM, int NT>
+__device__ __forceinline__ void finish(const Product& p, const Place& at, int lane, int row0, int col0, f32x4 (&acc)[NM][NT])
+{
+    if constexpr (MODE == WEIGHTS) {
+        if (at.slot >= 0) {
+            float* base = p.partial + (long)at.slot * p.m * p.cols + col0;
+            store_tiles<float>(lane, acc, p.cols - col0, [&](int i) {
+                const int m = row0 + 16 * i + lane / 4;
+                return m < p.m ? base + (long)m * p.cols : nullptr;
+            });
+        } else {
+            T* base = static_cast<T*>(p.out) + (long)at.group * p.m * p.cols + col0;
+            store_tiles<T>(lane, acc, p.cols - col0, [&](int i) {
+                const int m = row0 + 16 * i + lane / 4;
+                return m < p.m ? base + (long)m * p.cols : nullptr;
+            });
+        }
+    } else {
+        if (MODE == FORWARD && p.bias) {
+            const T* bias = static_cast<const T*>(p.bias) + (long)at.group * p.cols;
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const int col = col0 + 16 * t + 4 * (lane >> 4);
+                float b[4];
+                load_run<4>(bias + col, p.cols - col, b);
+#pragma unroll
+                for (int i = 0; i < NM; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[i][t][j] += b[j];
+            }
+        }
+        store_tiles<T>(lane, acc, p.cols - col0, [&](int i) {
+            const int r = at.begin + row0 + 16 * i + lane / 4;
+            return r < at.end ? static_cast<T*>(p.out) + p.order[r] * p.out_stride + col0 : nullptr;
+        });
+    }
+}
+
+// ---- operands in LDS
+//
+// Steps of K terms (64 for 16-bit types as they are, 32 for single precision in parts); an operand has `wide` rows or columns of C.  It lies
+//   along: where its terms are neighbours in memory: [wide][K], the 16-byte pieces of a row in an order that depends on the row;
+//   across: where neighbours in memory are neighbours in C: [K][wide], 32-byte pieces in an order that depends on the term; lanes get it
+//   turned by the instruction that reads it.
+// The orders are for the banks: lanes that read together meet different ones.
+template <int K>
+__device__ __forceinline__ int along_piece(int row, int piece) { return K == 64 ? piece ^ (row & 7) : piece ^ (row >> 1 & 3); }
+template <int WIDE>
+__device__ __forceinline__ int across_turn(int k) { return WIDE >= 128 ? (k & 3) | (k >> 3 & 1) << 2 : (k >> 1 & 1) | (k >> 3 & 1) << 1; }
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+// What a wavefront reads of an operand: 16 rows or columns from 16 `tile` on, 32 terms from 32 h on.
+template <typename F, int K, int WIDE, bool ACROSS>
+struct Reader {
+    unsigned at;      // of tile 0 and h 0
+    __device__ __forceinline__ Reader(unsigned base, int tile0, int lane)
+    {
+        const int n = lane & 15, g = lane >> 4;
+        if constexpr (ACROSS) at = base + (8 * g + n / 4) * (2 * WIDE) + ((tile0 ^ across_turn<WIDE>(8 * g + n / 4)) << 5) + 8 * (n & 3);
+        else at = base + (16 * tile0 + n) * (2 * K) + 16 * along_piece<K>(n, g);
+    }
+    // (tile 0 and step 0 of 16-byte pieces: a tile is 16 rows further, which along_piece does not see; h turns a bit of the piece)
+    __device__ __forceinline__ F get(int tile, int h, unsigned more) const
+    {
+        if constexpr (ACROSS) {
+            const unsigned a = (at ^ (unsigned)tile << 5) + more + h * 32 * (2 * WIDE);
+            const s16x4 u = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)a), v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(a + 4 * 2 * WIDE));
+            return __builtin_bit_cast(F, __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7));
+        } else {
+            return *(const __attribute__((address_space(3))) F*)((at ^ h << 6) + more + tile * 16 * (2 * K));
+        }
+    }
+};
+
+// 1 KB of a wavefront from global memory into LDS as load_into_lds brings it, every lane from an address of its own.
+__device__ __forceinline__ void load_into_lds_from(const void* from, unsigned to)
+{
+    unsigned m0;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
+                 : "=&s"(m0) : "v"(from), "s"(to) : "memory");
+}
+__device__ const uint4 kZeros = {0, 0, 0, 0};      // what is fetched for terms that do not exist
+
+// 16-bit types whose rows begin at multiples of 16 bytes: straight from memory into LDS, STAGES steps of 64 terms under way.
+// WM x WN wavefronts share the tile.  32 terms have their operands fetched during the 32 before.
+template <typename T, int MODE, int BM, int BN, int WM, int WN, int STAGES>
+__global__ __launch_bounds__(64 * WM * WN, 2) void k_direct(const Product p)
+{
+    constexpr int WAVES = WM * WN, NM = BM / WM / 16, NT = BN / WN / 16, PA = BM / 8 / WAVES, PB = BN / 8 / WAVES, PER = PA + PB, STAGE = (BM + BN) * 128;
+    constexpr bool A_ACROSS = MODE == WEIGHTS, B_ACROSS = MODE != FORWARD;
+    static_assert(BM / 8 % WAVES == 0 && BN / 8 % WAVES == 0, "loads of a wavefront");
+    typedef typename Operand<T>::type frag;
+    extern __shared__ __align__(1024) unsigned char lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    Place at;
+    int rt, ct;
+    if (!find_tile<MODE>(p, BM, lane, at, rt, ct)) return;
+    const int col0 = ct * BN, row0 = MODE == WEIGHTS ? rt * BM : 0, count = at.end - at.begin;
+    if (MODE != WEIGHTS && at.group >= p.groups) {
+        store_none<T>(p, at, col0, BN);
+        return;
+    }
+    const int terms = MODE == WEIGHTS ? count : p.k, stages = (terms + 63) / 64;
+    // What a lane asks for, in bytes from a base that moves from step to step: 16 bytes at a time, PA + PB times.
+    constexpr int A_PIECES = BM / 8, B_PIECES = BN / 8;      // of a term, where it lies across
+    const int* order = p.order + at.begin;
+    unsigned from_a[PA], from_b[PB];
+#pragma unroll
+    for (int u = 0; u < PA; ++u) {
+        const int slot = (wave * PA + u) * 64 + lane;      // 16 bytes of the operand in LDS
+        if constexpr (A_ACROSS) {
+            const int k = slot / A_PIECES, piece = slot % A_PIECES ^ across_turn<BM>(k) << 1;
+            from_a[u] = 2 * min(row0 + 8 * piece, p.m - 8);
+        } else {
+            const int r = slot / 8;
+            from_a[u] = (unsigned)(order[min(r, count - 1)] * p.a_stride * 2) + 16 * along_piece<64>(r, slot % 8);
+        }
+    }
+    const char* b_base = static_cast<const char*>(p.b) + (MODE == WEIGHTS ? 0 : 2 * (at.group * p.b_each + (MODE == FORWARD ? col0 * p.b_stride : 0)));
+#pragma unroll
+    for (int u = 0; u < PB; ++u) {
+        const int slot = (wave * PB + u) * 64 + lane;
+        if constexpr (B_ACROSS) {
+            const int k = slot / B_PIECES, piece = slot % B_PIECES ^ across_turn<BN>(k) << 1;
+            from_b[u] = (MODE == ROWS ? (unsigned)(2 * k * p.b_stride) : 0) + 2 * min(col0 + 8 * piece, p.cols - 8);
+        } else {
+            const int r = slot / 8;
+            from_b[u] = (unsigned)(2 * min(r, p.cols - 1 - col0) * p.b_stride) + 16 * along_piece<64>(r, slot % 8);
+        }
+    }
+    const unsigned lds0 = lds_address(lds);
+    // the rows that a wavefront's terms of a step are, for WEIGHTS (in scalar registers)
+    constexpr int TERMS = 64 / WAVES;
+    typedef const __attribute__((address_space(4))) int* scalar_ints;
+    int rows[MODE == WEIGHTS ? TERMS : 1];
+    auto look_up = [&](int s) {
+        if constexpr (MODE == WEIGHTS) {
+            const int first = 64 * s + wave * TERMS;
+            if (64 * s + 64 <= terms) {
+                const scalar_ints o = (scalar_ints)(order + first);
+#pragma unroll
+                for (int j = 0; j < TERMS; ++j) rows[j] = o[j];
+            } else {
+                const scalar_ints o = (scalar_ints)order;
+#pragma unroll
+                for (int j = 0; j < TERMS; ++j) rows[j] = o[min(first + j, terms - 1)];
+            }
+        }
+    };
+    auto row_bytes = [&](int u, int pieces, long stride) {      // of the row of a lane's term
+        const int per = 64 / pieces;      // terms of 1 KB
+        unsigned v = (unsigned)(rows[u * per] * stride * 2);
+#pragma unroll
+        for (int j = 1; j < per; ++j) v = lane >= j * pieces ? (unsigned)(rows[u * per + j] * stride * 2) : v;
+        return v;
+    };
+    auto request = [&](int s) {
+        const unsigned to = lds0 + s % STAGES * STAGE;
+        const char* a = static_cast<const char*>(p.a) + (A_ACROSS ? 0 : (long)s * 128);
+        const char* b = b_base + (MODE == FORWARD ? (long)s * 128 : MODE == ROWS ? (long)s * 128 * p.b_stride : 0);
+#pragma unroll
+        for (int u = 0; u < PA; ++u) load_into_lds(a, from_a[u] + (A_ACROSS ? row_bytes(u, A_PIECES, p.a_stride) : 0), to + (wave * PA + u) * 1024);
+#pragma unroll
+        for (int u = 0; u < PB; ++u)
+            load_into_lds(b, from_b[u] + (MODE == WEIGHTS ? row_bytes(u, B_PIECES, p.b_stride) : 0), to + BM * 128 + (wave * PB + u) * 1024);
+    };
+    auto request_last = [&](int s) {      // of a step that need not be whole
+        if (64 * s + 64 <= terms) return request(s);
+        const unsigned to = lds0 + s % STAGES * STAGE;
+        const char* a = static_cast<const char*>(p.a) + (A_ACROSS ? 0 : (long)s * 128);
+        const char* b = b_base + (MODE == FORWARD ? (long)s * 128 : MODE == ROWS ? (long)s * 128 * p.b_stride : 0);
+#pragma unroll
+        for (int u = 0; u < PA; ++u) {
+            const int slot = (wave * PA + u) * 64 + lane, k = 64 * s + (A_ACROSS ? slot / A_PIECES : 8 * along_piece<64>(slot / 8, slot % 8));
+            const char* from = a + (from_a[u] + (A_ACROSS ? row_bytes(u, A_PIECES, p.a_stride) : 0));
+            load_into_lds_from(k < terms ? from : reinterpret_cast<const char*>(&kZeros), to + (wave * PA + u) * 1024);
+        }
+#pragma unroll
+        for (int u = 0; u < PB; ++u) {
+            const int slot = (wave * PB + u) * 64 + lane, k = 64 * s + (B_ACROSS ? slot / B_PIECES : 8 * along_piece<64>(slot / 8, slot % 8));
+            const char* from = b + (from_b[u] + (MODE == WEIGHTS ? row_bytes(u, B_PIECES, p.b_stride) : 0));
+            load_into_lds_from(k < terms ? from : reinterpret_cast<const char*>(&kZeros), to + BM * 128 + (wave * PB + u) * 1024);
+        }
+    };
+    f32x4 acc[NM][NT];
+#pragma unroll
+    for (int i = 0; i < NM; ++i)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc[i][t] = f32x4{0, 0, 0, 0};
+    const int wm = wave / WN, wn = wave % WN;
+    const Reader<frag, 64, BM, A_ACROSS> read_a(lds0, wm * NM, lane);
+    const Reader<frag, 64, BN, B_ACROSS> read_b(lds0 + BM * 128, wn * NT, lane);
+    struct Frags {
+        frag x[NM], w[NT];
+    };
+    auto fetch = [&](int s, int h, Frags& f) {
+        const unsigned more = s % STAGES * STAGE;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) f.w[t] = read_b.get(t, h, more);
+#pragma unroll
+        for (int i = 0; i < NM; ++i) f.x[i] = read_a.get(i, h, more);
+    };
+    auto sums = [&](const Frags& now) {
+#pragma unroll
+        for (int i = 0; i < NM; ++i)
+#pragma unroll
+            for (int t = 0; t < NT; ++t) acc[i][t] = mma(now.w[t], now.x[i], acc[i][t]);
+    };
+    auto woven = [&] {      // sums and the fetches beside them, by turns
+        constexpr int READS = NM * (A_ACROSS ? 2 : 1) + NT * (B_ACROSS ? 2 : 1), EACH = NM * NT / READS;
+        if constexpr (EACH >= 1) {
+#pragma unroll
+            for (int i = 0; i < READS; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, EACH, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x008, NM * NT - EACH * READS, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    if (stages > 0) {
+#pragma unroll
+        for (int s = 0; s < STAGES; ++s)
+            if (s < stages) {
+                look_up(s);
+                request_last(s);
+            }
+        if (STAGES <= stages) wait_loads<(STAGES - 1) * PER>();
+        else wait_loads<0>();
+        barrier_only();
+        Frags f[2];
+        fetch(0, 0, f[0]);
+        look_up(STAGES < stages ? STAGES : 0);
+        int s = 0;
+#pragma unroll 1
+        for (; s + STAGES + 1 < stages; ++s) {
+            fetch(s, 1, f[1]);
+            sums(f[0]);
+            woven();
+            wait_loads<(STAGES - 2) * PER>();
+            barrier_only();      // the next tiles are there, and everybody has read these
+            request(s + STAGES);
+            look_up(s + STAGES + 1);
+            fetch(s + 1, 0, f[0]);
+            sums(f[1]);
+            woven();
+        }
+#pragma unroll 1
+        for (; s < stages; ++s) {      // the last request, and none
+            fetch(s, 1, f[1]);
+            sums(f[0]);
+            if (s + 1 < stages) {
+                wait_loads<0>();
+                barrier_only();
+                if (s + STAGES < stages) request_last(s + STAGES);
+                fetch(s + 1, 0, f[0]);
+            }
+            sums(f[1]);
+        }
+    }
+    finish<T, MODE, NM, NT>(p, at, lane, row0 + wm * NM * 16, col0 + wn * NT * 16, acc);
+}
+
+// ---- operands by way of registers: any alignment, and single precision, which is brought to bf16 parts on the way
+
+// Both operands of single precision in three bf16 parts, exactly, of whose products the six largest are formed (what is left out is below
+// 1.002 2^-24 of a product), small ones first.  Numbers are brought up by 2^24 first, so that the parts of small ones are normal numbers.
+constexpr float kSplitScale = 16777216.0f;
+__device__ __forceinline__ void parts_of(const float (&x)[8], bf16x8 (&part)[3])
+{
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+        f32x2 rest = {x[j] * kSplitScale, x[j + 1] * kSplitScale};
+#pragma unroll
+        for (int q = 0; q < 3; ++q) {
+            const bf16x2 h = __builtin_convertvector(rest, bf16x2);
+            part[q][j] = h[0];
+            part[q][j + 1] = h[1];
+            if (q < 2) rest -= __builtin_convertvector(h, f32x2);
+        }
+    }
+}
+// eight neighbours in memory on their way
+template <typename T>
+struct Eight {
+    typename Operand<T>::type v[8 / kRun<T>];
+};
+// those from p on, of which `left` exist; zeros for the others
+template <typename T>
+__device__ __forceinline__ Eight<T> load_eight(const T* p, int left)
+{
+    constexpr int V = kRun<T>;
+    Eight<T> x;
+#pragma unroll
+    for (int h = 0; h < 8 / V; ++h) {
+        if (left >= 8) x.v[h] = *reinterpret_cast<const typename Run<T, V>::loose*>(p + h * V);
+        else x.v[h] = load_operand(p + h * V, left - h * V);
+    }
+    return x;
+}
+
+// A sum in single precision, term by term.
+template <typename T, int MODE>
+__device__ __forceinline__ float plain_sum(const Product& p, const Place& at, int m, int c)
+{
+    const T *a = static_cast<const T*>(p.a), *b = static_cast<const T*>(p.b);
     float sum = 0.0f;
-    for (int i = p.offsets[g]; i < p.offsets[g + 1]; ++i) sum += (float)static_cast<const T*>(p.a)[p.order[i] * p.a_stride + m];
-    static_cast<T*>(p.out)[(long)g * p.k + m] = (T)sum;
+    if constexpr (MODE == WEIGHTS) {
+        for (int i = at.begin; i < at.end; ++i) sum = fmaf((float)a[p.order[i] * p.a_stride + m], (float)b[p.order[i] * p.b_stride + c], sum);
+    } else {
+        a += p.order[at.begin + m] * p.a_stride;
+        b += at.group * p.b_each + (MODE == FORWARD ? c * p.b_stride : c);
+        for (int k = 0; k < p.k; ++k) sum = fmaf((float)a[k], (float)b[MODE == FORWARD ? (long)k : k * p.b_stride], sum);
+    }
+    return sum;
+}
+
+// Steps of 32 terms; the next one's numbers are on their way to registers during the sums of this one.  Four wavefronts, 2 x 2.
+template <typename T, int MODE, int BM, int BN>
+__global__ __launch_bounds__(256, 2) void k_staged(const Product p)
+{
+    constexpr bool SINGLE = std::is_same_v<T, float>, A_ACROSS = MODE == WEIGHTS, B_ACROSS = MODE != FORWARD;
+    constexpr int PARTS = SINGLE ? 3 : 1, NM = BM / 32, NT = BN / 32, PA = BM / 64, PB = BN / 64, A_PART = BM * 64, B_PART = BN * 64;
+    typedef typename std::conditional_t<SINGLE, Operand<bf16>, Operand<T>>::type frag;
+    __shared__ __align__(1024) unsigned char lds[PARTS * (A_PART + B_PART)];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    Place at;
+    int rt, ct;
+    if (!find_tile<MODE>(p, BM, lane, at, rt, ct)) return;
+    const int col0 = ct * BN, row0 = MODE == WEIGHTS ? rt * BM : 0, count = at.end - at.begin;
+    if (MODE != WEIGHTS && at.group >= p.groups) {
+        store_none<T>(p, at, col0, BN);
+        return;
+    }
+    const int terms = MODE == WEIGHTS ? count : p.k, steps = (terms + 31) / 32;
+    const int* order = p.order + at.begin;
+    // where a thread's numbers begin and how many of the eight there are; along: k is added
+    const T* from_a[PA];
+    const T* from_b[PB];
+    int a_left[PA], b_left[PB];
+#pragma unroll
+    for (int u = 0; u < PA; ++u) {
+        const int slot = u * 256 + threadIdx.x;
+        if constexpr (A_ACROSS) {
+            const int m = row0 + slot % (BM / 8) * 8;
+            a_left[u] = p.m - m;
+            from_a[u] = static_cast<const T*>(p.a) + min(m, p.m - 1);
+        } else from_a[u] = static_cast<const T*>(p.a) + order[min(slot / 4, count - 1)] * p.a_stride + slot % 4 * 8;
+    }
+#pragma unroll
+    for (int u = 0; u < PB; ++u) {
+        const int slot = u * 256 + threadIdx.x;
+        const T* b = static_cast<const T*>(p.b) + (MODE == WEIGHTS ? 0 : at.group * p.b_each);
+        if constexpr (B_ACROSS) {
+            const int c = col0 + slot % (BN / 8) * 8;
+            b_left[u] = p.cols - c;
+            from_b[u] = b + min(c, p.cols - 1);
+        } else from_b[u] = b + min(col0 + slot / 4, p.cols - 1) * p.b_stride + slot % 4 * 8;
+    }
+    Eight<T> raw_a[PA], raw_b[PB];
+    auto request = [&](int s) {
+#pragma unroll
+        for (int u = 0; u < PA; ++u) {
+            const int slot = u * 256 + threadIdx.x;
+            if constexpr (A_ACROSS) {
+                const int k = 32 * s + slot / (BM / 8);
+                raw_a[u] = load_eight(from_a[u] + order[min(k, terms - 1)] * p.a_stride, k < terms ? a_left[u] : 0);
+            } else raw_a[u] = load_eight(from_a[u] + 32 * s, terms - 32 * s - slot % 4 * 8);
+        }
+#pragma unroll
+        for (int u = 0; u < PB; ++u) {
+            const int slot = u * 256 + threadIdx.x;
+            if constexpr (B_ACROSS) {
+                const int k = 32 * s + slot / (BN / 8);
+                raw_b[u] = load_eight(from_b[u] + (MODE == WEIGHTS ? (long)order[min(k, terms - 1)] : min(k, terms - 1)) * p.b_stride, k < terms ? b_left[u] : 0);
+            } else raw_b[u] = load_eight(from_b[u] + 32 * s, terms - 32 * s - slot % 4 * 8);
+        }
+    };
+    auto put = [&](const Eight<T>& x, unsigned char* to, int part_bytes) {
+        if constexpr (SINGLE) {
+            const float v[8] = {x.v[0][0], x.v[0][1], x.v[0][2], x.v[0][3], x.v[1][0], x.v[1][1], x.v[1][2], x.v[1][3]};
+            bf16x8 part[3];
+            parts_of(v, part);
+#pragma unroll
+            for (int q = 0; q < 3; ++q) *reinterpret_cast<bf16x8*>(to + q * part_bytes) = part[q];
+        } else *reinterpret_cast<frag*>(to) = x.v[0];
+    };
+    auto store = [&] {
+#pragma unroll
+        for (int u = 0; u < PA; ++u) {
+            const int slot = u * 256 + threadIdx.x, k = slot / (BM / 8);
+            put(raw_a[u], lds + (A_ACROSS ? k * (2 * BM) + 16 * (slot % (BM / 8) ^ across_turn<BM>(k) << 1) : slot / 4 * 64 + 16 * along_piece<32>(slot / 4, slot % 4)), A_PART);
+        }
+#pragma unroll
+        for (int u = 0; u < PB; ++u) {
+            const int slot = u * 256 + threadIdx.x, k = slot / (BN / 8);
+            put(raw_b[u], lds + PARTS * A_PART + (B_ACROSS ? k * (2 * BN) + 16 * (slot % (BN / 8) ^ across_turn<BN>(k) << 1) : slot / 4 * 64 + 16 * along_piece<32>(slot / 4, slot % 4)),
+                B_PART);
+        }
+    };
+    f32x4 acc[NM][NT];
+#pragma unroll
+    for (int i = 0; i < NM; ++i)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc[i][t] = f32x4{0, 0, 0, 0};
+    const int wm = wave / 2, wn = wave % 2;
+    const unsigned lds0 = lds_address(lds);
+    const Reader<frag, 32, BM, A_ACROSS> read_a(lds0, wm * NM, lane);
+    const Reader<frag, 32, BN, B_ACROSS> read_b(lds0 + PARTS * A_PART, wn * NT, lane);
+    if (steps > 0) request(0);
+#pragma unroll 1
+    for (int s = 0; s < steps; ++s) {
+        __syncthreads();
+        store();
+        __syncthreads();
+        if (s + 1 < steps) request(s + 1);
+        frag x[NM][PARTS];
+#pragma unroll
+        for (int i = 0; i < NM; ++i)
+#pragma unroll
+            for (int q = 0; q < PARTS; ++q) x[i][q] = read_a.get(i, 0, q * A_PART);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            frag w[PARTS];
+#pragma unroll
+            for (int q = 0; q < PARTS; ++q) w[q] = read_b.get(t, 0, q * B_PART);
+            if constexpr (SINGLE) {
+                constexpr int ix[6] = {2, 0, 1, 1, 0, 0}, iw[6] = {0, 2, 1, 0, 1, 0};
+#pragma unroll
+                for (int o = 0; o < 6; ++o)
+#pragma unroll
+                    for (int i = 0; i < NM; ++i) acc[i][t] = mma(w[iw[o]], x[i][ix[o]], acc[i][t]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < NM; ++i) acc[i][t] = mma(w[0], x[i][0], acc[i][t]);
+            }
+        }
+    }
+    const int row_w = row0 + wm * NM * 16, col_w = col0 + wn * NT * 16;
+    if constexpr (SINGLE) {
+        // (sums that are not finite for the scale, or are not at all, are formed again)
+        constexpr float kBack = 1.0f / (kSplitScale * kSplitScale);
+        float none = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NM; ++i)
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    none = fmaf(acc[i][t][j], 0.0f, none);
+                    acc[i][t][j] *= kBack;
+                }
+        if (__builtin_expect(__any(none != none), 0)) {
+#pragma unroll
+            for (int i = 0; i < NM; ++i)
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int m = row_w + 16 * i + (lane & 15), c = col_w + 16 * t + 4 * (lane >> 4) + j;
+                        if (!(fabsf(acc[i][t][j]) <= std::numeric_limits<float>::max()) && m < (MODE == WEIGHTS ? p.m : count) && c < p.cols)
+                            acc[i][t][j] = plain_sum<T, MODE>(p, at, m, c);
+                    }
+        }
+    }
+    finish<T, MODE, NM, NT>(p, at, lane, row_w, col_w, acc);
+}
+
+// Sums of the pieces of a group's dW, in order.
+template <typename T>
+__global__ __launch_bounds__(256) void k_join(const Product p)
+{
+    const int lane = threadIdx.x & 63, g = blockIdx.y;
+    const int pieces = (p.offsets[g + 1] - p.offsets[g] + p.piece - 1) / p.piece;
+    if (pieces < 2) return;
+    // (the parts of the groups in front)
+    int slots = 0;
+    for (int h = lane; h < g; h += 64) {
+        const int n = (p.offsets[h + 1] - p.offsets[h] + p.piece - 1) / p.piece;
+        slots += n > 1 ? n : 0;
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) slots += __shfl_xor(slots, d, 64);
+    const long each = (long)p.m * p.cols, e = ((long)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (e >= each) return;
+    const float* from = p.partial + slots * each + e;
+    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int i = 0; i < pieces; ++i) {
+        float v[4];
+        load_run<4>(from + i * each, each - e, v);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum[j] += v[j];
+    }
+    store_run<4>(static_cast<T*>(p.out) + g * each + e, each - e, sum);
+}
+
+// ---- few rows of a group: bound by the weights' bytes
+//
+// A block takes 16 columns of a group's product with up to 64 of its rows; eight wavefronts have 128 bytes of the weights' rows by
+// turns, four of them under way.  Up to 64 rows in all are not sorted: a block is there for every row, finds the rows of the same group
+// itself, and leaves if its own is not the first of them.
+constexpr int kMostFew = 64;
+template <typename T, int MT>
+__device__ __forceinline__ void few_rows(const Product& p, int group, const int* rows, int count, f32x4 (*part)[4][64])
+{
+    constexpr int V = kRun<T>, UNIT = 8 * V;
+    typedef typename Operand<T>::type frag;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col0 = blockIdx.x * 16, mine = (lane & 3) * V;
+    const T* W = static_cast<const T*>(p.b) + group * p.b_each + min(col0 + lane / 4, p.cols - 1) * p.b_stride + mine;
+    const T* in[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) in[i] = static_cast<const T*>(p.a) + rows[min(16 * i + lane / 4, count - 1)] * p.a_stride + mine;
+    f32x4 acc[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) acc[i] = f32x4{0, 0, 0, 0};
+    struct Unit {
+        frag w[2], x[MT][2];
+    };
+    const int full = p.k / UNIT;
+    auto fetch = [&](int u, Unit& v) {
+        const int k = min(u, full - 1) * UNIT;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            v.w[half] = *reinterpret_cast<const typename Run<T, V>::loose*>(W + k + half * (UNIT / 2));
+#pragma unroll
+            for (int i = 0; i < MT; ++i) v.x[i][half] = *reinterpret_cast<const typename Run<T, V>::loose*>(in[i] + k + half * (UNIT / 2));
+        }
+        asm volatile("" ::: "memory");      // (asked for here, not where they are used)
+    };
+    auto sums = [&](const Unit& v) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const frag w = to_operand(v.w[half], lane);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) acc[i] = mma(w, to_operand(v.x[i][half], lane), acc[i]);
+        }
+    };
+    int u = wave;
+    if (u < full) {
+        Unit unit[4];
+#pragma unroll
+        for (int q = 0; q < 3; ++q) fetch(u + 8 * q, unit[q]);
+#pragma unroll 1
+        for (;;) {
+            bool done = false;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                if (done) continue;
+                fetch(u + 24, unit[(q + 3) % 4]);
+                sums(unit[q]);
+                done = (u += 8) >= full;
+            }
+            if (done) break;
+        }
+    }
+    if (wave == full % 8 && p.k % UNIT) {      // (the end of the rows)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int k = full * UNIT + half * (UNIT / 2);
+            const frag w = to_operand(load_operand(W + k, p.k - k - mine), lane);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) acc[i] = mma(w, to_operand(load_operand(in[i] + k, p.k - k - mine), lane), acc[i]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) part[wave][i][lane] = acc[i];
+    __syncthreads();
+    for (int at = threadIdx.x; at < MT * 256; at += 512) {
+        const int row = at / 16, c = at % 16, col = col0 + c;
+        if (row >= count || col >= p.cols) continue;
+        float sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) sum += part[w][row / 16][c / 4 * 16 + row % 16][c % 4];
+        if (p.bias) sum += (float)static_cast<const T*>(p.bias)[(long)group * p.cols + col];
+        static_cast<T*>(p.out)[rows[row] * p.out_stride + col] = (T)sum;
+    }
+}
+template <typename T, bool SORTED>
+__global__ __launch_bounds__(512) void k_few(const Product p, const int* index)
+{
+    __shared__ f32x4 part[8][4][64];
+    __shared__ int rows[kMostFew];
+    const int lane = threadIdx.x & 63;
+    int group, count;
+    if constexpr (SORTED) {
+        const Place at = find_item<false>(p, blockIdx.y, kMostFew, lane);
+        if (at.group < 0) return;
+        group = at.group;
+        count = at.end - at.begin;
+        if ((int)threadIdx.x < count) rows[threadIdx.x] = p.order[at.begin + threadIdx.x];
+    } else {
+        const int all = (int)p.rows, key = row_key(index[min(lane, all - 1)], p.groups);
+        group = __builtin_amdgcn_readlane(key, blockIdx.y);
+        const unsigned long same = __ballot(lane < all && key == group);
+        if (same & ((1ul << blockIdx.y) - 1)) return;      // (an earlier row's block does it)
+        count = __popcll(same);
+        if (threadIdx.x < 64 && (same >> lane & 1)) rows[__popcll(same & ((1ul << lane) - 1))] = lane;
+    }
+    __syncthreads();
+    if (group >= p.groups) {
+        const T v = (T)(group == p.groups ? 0.0f : std::numeric_limits<float>::quiet_NaN());
+        for (int at = threadIdx.x; at < 16 * count; at += 512)
+            if ((int)blockIdx.x * 16 + at % 16 < p.cols) static_cast<T*>(p.out)[rows[at / 16] * p.out_stride + blockIdx.x * 16 + at % 16] = v;
+        return;
+    }
+    if (count <= 16) few_rows<T, 1>(p, group, rows, count, part);
+    else if (count <= 32) few_rows<T, 2>(p, group, rows, count, part);
+    else few_rows<T, 4>(p, group, rows, count, part);
 }
 
 // ---- host side
@@ -124,6 +812,11 @@ void check(const smx_grouped_linear* p)
     refuse_unless((p->order == nullptr) == (p->offsets == nullptr) || p->rows == 0, "order and offsets: both or neither");
 }
 
+// What k_direct takes: rows at multiples of 16 bytes, whole pieces of 16 bytes; the offsets inside a tile have 32 bits,
+// and so have those of rows that lie anywhere.
+bool in_pieces(const void* p, long stride, long numbers) { return (reinterpret_cast<size_t>(p) & 15) == 0 && stride % 8 == 0 && numbers % 8 == 0 && stride <= 1 << 22; }
+bool within_reach(long rows, long stride) { return rows * stride * 2 < 1L << 32; }
+
 struct Call : Launches {
     const smx_grouped_linear& p;
     Arena arena;
@@ -136,41 +829,122 @@ struct Call : Launches {
         groups.offsets = arena.take<int>(p.num_groups + 2L);
         sort_rows(*this, arena, p.index, p.rows, p.num_groups, groups);
     }
-    template <typename T>
-    void rows(const T* a, long a_stride, long b_k, long b_c, const T* bias, int k, int cols, T* out, long out_stride)
+    template <typename T, int MODE, int BM, int BN, int WM, int WN, int STAGES>
+    void direct(const Product& q, long blocks)
     {
-        Product q{a, a_stride, p.weight, p.weight_each, b_k, b_c, bias, groups.order, groups.offsets, p.num_groups, k, cols, p.rows, out, out_stride};
-        start(k_rows<T>, (p.rows + 63) / 64 + p.num_groups + 2, (cols + 63) / 64, 1, 256, 0, q);
+        constexpr int bytes = STAGES * (BM + BN) * 128;
+        auto kernel = k_direct<T, MODE, BM, BN, WM, WN, STAGES>;
+        if (bytes > 64 * 1024 && !dry) hip_ok(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes), "LDS");
+        start(kernel, up(blocks, 8), 1, 1, 64 * WM * WN, bytes, q);
+    }
+    // Tiles for all rows in the worst case: every group has one that is not full.
+    long row_tiles(int high) const { return p.rows / high + std::min(p.rows, p.num_groups + 2L); }
+
+    // y or dx
+    template <typename T, int MODE>
+    void rows(Product q, bool direct_ok)
+    {
+        auto tiles = [&](int high, int wide) {
+            q.col_tiles = (q.cols + wide - 1) / wide;
+            return row_tiles(high) * q.col_tiles;
+        };
+        if constexpr (!std::is_same_v<T, float>) {
+            if (direct_ok) {
+                if (p.rows / 256 * ((q.cols + 255) / 256) >= 192) direct<T, MODE, 256, 256, 2, 4, 2>(q, tiles(256, 256));
+                else if (p.rows / 128 * ((q.cols + 127) / 128) >= 192) direct<T, MODE, 128, 128, 2, 2, 2>(q, tiles(128, 128));
+                else direct<T, MODE, 64, 64, 2, 2, 3>(q, tiles(64, 64));
+                return;
+            }
+        }
+        if (p.rows / 128 * ((q.cols + 127) / 128) >= 192) start(k_staged<T, MODE, 128, 128>, up(tiles(128, 128), 8), 1, 1, 256, 0, q);
+        else start(k_staged<T, MODE, 64, 64>, up(tiles(64, 64), 8), 1, 1, 256, 0, q);
     }
     template <typename T>
     void forward(T* y, long y_stride)
     {
+        const T *x = static_cast<const T*>(p.x), *W = static_cast<const T*>(p.weight);
+        Product q{};
+        q.a = x; q.a_stride = p.x_stride; q.b = W; q.b_each = p.weight_each; q.b_stride = p.weight_stride; q.bias = p.bias; q.groups = p.num_groups; q.k = p.d_in; q.cols = p.d_out;
+        q.rows = p.rows; q.out = y; q.out_stride = y_stride;
+        if (p.rows <= kMostFew) {
+            start(k_few<T, false>, (p.d_out + 15) / 16, p.rows, 1, 512, 0, q, p.index);
+            return;
+        }
         sort();
-        rows<T>(static_cast<const T*>(p.x), p.x_stride, 1, p.weight_stride, static_cast<const T*>(p.bias), p.d_in, p.d_out, y, y_stride);
+        q.order = groups.order; q.offsets = groups.offsets;
+        if (p.rows <= 16L * p.num_groups) {
+            start(k_few<T, true>, (p.d_out + 15) / 16, row_tiles(kMostFew), 1, 512, 0, q, p.index);
+            return;
+        }
+        rows<T, FORWARD>(q, in_pieces(x, p.x_stride, p.d_in) && in_pieces(W, p.weight_stride, p.d_in) && p.weight_each % 8 == 0 && within_reach(p.rows, p.x_stride));
     }
     template <typename T>
     void backward(const T* dy, long dy_stride, T* dx, long dx_stride, T* dW, T* db)
     {
+        const T *x = static_cast<const T*>(p.x), *W = static_cast<const T*>(p.weight);
         sort();
-        if (dx && p.rows) rows<T>(dy, dy_stride, p.weight_stride, 1, nullptr, p.d_out, p.d_in, dx, dx_stride);
-        if (!p.num_groups) return;
-        Product q{dy, dy_stride, p.x, 0, p.x_stride, 1, nullptr, groups.order, groups.offsets, p.num_groups, p.d_out, p.d_in, p.rows, dW, 0};
-        if (dW) start(k_weights<T>, (p.d_out + 63) / 64, (p.d_in + 63) / 64, p.num_groups, 256, 0, q);
-        q.out = db;
-        if (db) start(k_biases<T>, (p.d_out + 255) / 256, p.num_groups, 1, 256, 0, q);
+        Product q{};
+        q.a = dy; q.a_stride = dy_stride; q.groups = p.num_groups; q.rows = p.rows; q.order = groups.order; q.offsets = groups.offsets;
+        const bool dy_ok = in_pieces(dy, dy_stride, p.d_out) && within_reach(p.rows, dy_stride);
+        if (dx && p.rows) {
+            q.b = W; q.b_each = p.weight_each; q.b_stride = p.weight_stride; q.k = p.d_out; q.cols = p.d_in; q.out = dx; q.out_stride = dx_stride;
+            rows<T, ROWS>(q, dy_ok && in_pieces(W, p.weight_stride, p.d_in) && p.weight_each % 8 == 0);
+        }
+        if (dW && p.num_groups) {
+            q.b = x; q.b_each = 0; q.b_stride = p.x_stride; q.m = p.d_out; q.cols = p.d_in; q.out = dW;
+            weights<T>(q, dy_ok && in_pieces(x, p.x_stride, p.d_in) && within_reach(p.rows, p.x_stride));
+        }
+        if (db && p.num_groups) add_rows(*this, arena, p.type, dy, dy_stride, p.index, p.rows, p.num_groups, p.d_out, groups, 1.0f, db);
+    }
+    template <typename T>
+    void weights(Product q, bool direct_ok)
+    {
+        auto tiles = [&](int high, int wide) {
+            q.row_tiles = (q.m + high - 1) / high;
+            q.col_tiles = (q.cols + wide - 1) / wide;
+            return (long)q.row_tiles * q.col_tiles;
+        };
+        const long used = std::max(1L, std::min(p.rows, (long)p.num_groups));
+        const bool large = tiles(256, 256) * used >= 192, medium = tiles(128, 128) * used >= 192 || p.rows >= 64 * 1024 / 8;
+        const bool direct_large = direct_ok && large && !std::is_same_v<T, float>;
+        const long each = direct_large ? tiles(256, 256) : medium ? tiles(128, 128) : tiles(64, 64);
+        // Pieces of a group's rows, until there are two blocks for every CU; long ones where there are enough without (a group may have most rows).
+        q.piece = (int)std::min(1L << 28, std::max(each * used >= 384 ? 4096L : 512L, up((p.rows * each + 511) / 512, 64)));
+        const long items = p.rows / q.piece + p.num_groups, slots = 2 * (p.rows / q.piece);
+        q.partial = arena.take<float>(slots * q.m * q.cols);
+        const long blocks = up(items * each, 8);
+        if constexpr (!std::is_same_v<T, float>) {
+            if (direct_ok) {
+                if (direct_large) direct<T, WEIGHTS, 256, 256, 2, 4, 2>(q, blocks);
+                else if (medium) direct<T, WEIGHTS, 128, 128, 2, 2, 2>(q, blocks);
+                else direct<T, WEIGHTS, 64, 64, 2, 2, 3>(q, blocks);
+            }
+        }
+        if (std::is_same_v<T, float> || !direct_ok) {
+            if (medium) start(k_staged<T, WEIGHTS, 128, 128>, blocks, 1, 1, 256, 0, q);
+            else start(k_staged<T, WEIGHTS, 64, 64>, blocks, 1, 1, 256, 0, q);
+        }
+        if (slots) start(k_join<T>, ((long)q.m * q.cols + 1023) / 1024, p.num_groups, 1, 256, 0, q);
     }
 };
 
+// (whatever the pointers' alignment is: the size does not depend on it but for dW's pieces, which are longest for the largest tiles)
 long workspace(const smx_grouped_linear* p, bool backward)
 {
-    Call c{{nullptr, true}, *p, {reinterpret_cast<char*>(256)}};
-    with_type(p->type, [&](auto t) {
-        using T = decltype(t);
-        T* some = reinterpret_cast<T*>(256);
-        if (backward) c.backward<T>(some, p->d_out, some, p->d_in, some, some);
-        else if (p->rows > 0) c.forward<T>(some, p->d_out);
-    });
-    return c.arena.used;
+    long most = 0;
+    for (int some = 256; some >= 2; some -= 254) {
+        smx_grouped_linear q = *p;
+        if (q.rows) q.x = reinterpret_cast<const void*>((size_t)some);
+        Call c{{nullptr, true}, q, {reinterpret_cast<char*>(256)}};
+        with_type(q.type, [&](auto t) {
+            using T = decltype(t);
+            T* at = reinterpret_cast<T*>((size_t)256);
+            if (backward) c.backward<T>(at, q.d_out, at, q.d_in, at, at);
+            else if (q.rows > 0) c.forward<T>(at, q.d_out);
+        });
+        most = std::max(most, c.arena.used);
+    }
+    return most;
 }
 
 }  // namespace
