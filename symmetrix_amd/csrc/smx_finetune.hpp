@@ -42,6 +42,18 @@ __device__ __forceinline__ void load_run(const T* p, long left, float (&v)[V])
         for (int j = 0; j < V; ++j) v[j] = j < left ? (float)p[j] : 0.0f;
     }
 }
+// (all V of them, in 16 bytes, which nothing is expected to read soon)
+template <int V, typename T>
+__device__ __forceinline__ void store_past(T* p, const float (&v)[V])
+{
+    static_assert(V * sizeof(T) == 16, "16 bytes");
+    typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+    typedef u32x4 loose __attribute__((aligned(2)));
+    typename Run<T, V>::type x;
+#pragma unroll
+    for (int j = 0; j < V; ++j) x[j] = (T)v[j];
+    __builtin_nontemporal_store(__builtin_bit_cast(u32x4, x), reinterpret_cast<loose*>(p));
+}
 template <int V, typename T>
 __device__ __forceinline__ void store_run(T* p, long left, const float (&v)[V])
 {

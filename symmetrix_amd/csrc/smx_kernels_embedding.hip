@@ -26,7 +26,8 @@ struct Lookup {
     float scale;
 };
 constexpr int kLookupRows = 4;      // of a thread
-template <typename T>
+constexpr long kMuch = 64L << 20;   // bytes of a result that are written past the caches
+template <typename T, bool PAST>
 __global__ __launch_bounds__(256) void k_lookup(const Lookup p)
 {
     constexpr int V = kRun<T>;
@@ -47,7 +48,11 @@ __global__ __launch_bounds__(256) void k_lookup(const Lookup p)
         }
 #pragma unroll
         for (int u = 0; u < kLookupRows; ++u)
-            if (row0 + u * at_once < p.rows) store_run<V>(static_cast<T*>(p.y) + (row0 + u * at_once) * p.y_stride + at, p.dim - at, v[u]);
+            if (row0 + u * at_once < p.rows) {
+                T* y = static_cast<T*>(p.y) + (row0 + u * at_once) * p.y_stride + at;
+                if (PAST && p.dim - at >= V) store_past<V>(y, v[u]);
+                else store_run<V>(y, p.dim - at, v[u]);
+            }
     }
 }
 
@@ -68,109 +73,168 @@ struct Sums {
     long first;                // which of all blocks the launch's first one is
 };
 
-// Pieces of sorted rows, a wavefront for 1 KB of each row.  A group's rows that lie in one piece are summed and stored; of a
-// group that goes on in other pieces, a part.  Eight rows are under way at a time.
+// Pieces of sorted rows: a block's four wavefronts have a quarter of a piece each, and 1 KB of its rows.  A group's rows that lie in one
+// piece are summed and stored; of a group that goes on in other pieces, a part.  Eight rows are under way at a time.
 template <typename T>
 __global__ __launch_bounds__(256) void k_pieces(const Sums p)
 {
     constexpr int V = kRun<T>, U = 8;
+    __shared__ float head[4][64][V], tail[4][64][V];      // of a quarter: the run that began before it, the one that goes on behind it
+    __shared__ int key_of[4][2];                          // their keys, or -1
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const long items = p.pieces * p.slabs, blocks = (items + 3) / 4;
-    const long block = p.first + blockIdx.x;
+    const long blocks = p.pieces * p.slabs, block = p.first + blockIdx.x;
     if (block >= blocks) {      // (offsets)
         const int g = (int)(block - blocks) * 256 + threadIdx.x;
         if (g < p.groups + 2) p.offsets[g] = first_place(p.keys, (int)p.rows, g);
         return;
     }
-    const long item = block * 4 + wave;
-    if (item >= items) return;
-    const long piece = item / p.slabs;
-    const int at = (int)(item % p.slabs) * 64 * V + lane * V;
-    const long begin = piece * p.piece;
-    const int count = (int)min((long)p.piece, p.rows - begin);
-    auto key_at = [&](long i, int row) { return p.keys ? p.keys[i] : row_key(p.index[row], p.groups); };
-    const int my_row = p.order[begin + min(lane, count - 1)];
-    const int my_key = key_at(begin + min(lane, count - 1), my_row);
-    // (a key behind the groups' on either side: none)
-    const int before = begin > 0 ? key_at(begin - 1, p.keys ? 0 : p.order[begin - 1]) : -1;
-    const int behind = begin + count < p.rows ? key_at(begin + count, p.keys ? 0 : p.order[begin + count]) : -1;
-    const T* in = static_cast<const T*>(p.in) + at;
+    const long piece = block / p.slabs;
+    const int at = (int)(block % p.slabs) * 64 * V + lane * V, quarter = p.piece / 4;
+    const long begin = piece * p.piece + wave * quarter;
+    const int count = (int)max(0L, min((long)quarter, p.rows - begin));
     const bool whole = at + V <= p.dim, some = at < p.dim;
-    float sum[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) sum[j] = 0.0f;
-    int key = __builtin_amdgcn_readlane(my_key, 0);
-    bool entered = key == before;
-    auto flush = [&](bool leaves) {
+    auto finish = [&](int key, float (&sum)[V]) {
         if (!some) return;
-        if (entered || leaves) {
-            store_run<V>(p.partial + (2 * piece + (entered ? 0 : 1)) * p.dim + at, p.dim - at, sum);
-        } else {
 #pragma unroll
-            for (int j = 0; j < V; ++j) sum[j] *= p.scale;
-            store_run<V>(static_cast<T*>(p.out) + (long)key * p.dim + at, p.dim - at, sum);
-        }
+        for (int j = 0; j < V; ++j) sum[j] *= p.scale;
+        store_run<V>(static_cast<T*>(p.out) + (long)key * p.dim + at, p.dim - at, sum);
     };
+    int head_key = -1, tail_key = -1;
+    if (count > 0) {
+        auto key_at = [&](long i, int row) { return p.keys ? p.keys[i] : row_key(p.index[row], p.groups); };
+        const int my_row = p.order[begin + min(lane, count - 1)];
+        const int my_key = key_at(begin + min(lane, count - 1), my_row);
+        const int before = begin > 0 ? key_at(begin - 1, p.keys ? 0 : p.order[begin - 1]) : -1;
+        const int behind = begin + count < p.rows ? key_at(begin + count, p.keys ? 0 : p.order[begin + count]) : -1;
+        const T* in = static_cast<const T*>(p.in) + at;
+        float sum[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) sum[j] = 0.0f;
+        int key = __builtin_amdgcn_readlane(my_key, 0);
+        bool entered = key == before;
+        auto flush = [&](bool leaves) {
+            if (entered) {
+                head_key = key;
+#pragma unroll
+                for (int j = 0; j < V; ++j) head[wave][lane][j] = sum[j];
+            } else if (leaves) {
+                tail_key = key;
+#pragma unroll
+                for (int j = 0; j < V; ++j) tail[wave][lane][j] = sum[j];
+            } else finish(key, sum);
+        };
 #pragma unroll 1
-    for (int i0 = 0; i0 < count; i0 += U) {
-        typename Operand<T>::type x[U];
+        for (int i0 = 0; i0 < count && key < p.groups; i0 += U) {      // (what lies behind the groups belongs to none)
+            typename Operand<T>::type x[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const long row = __builtin_amdgcn_readlane(my_row, min(i0 + u, count - 1));
-            if (whole) x[u] = *reinterpret_cast<const typename Run<T, V>::loose*>(in + row * p.in_stride);
-            else x[u] = load_operand(in + (some ? row * p.in_stride : 0), p.dim - at);
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (i0 + u >= count) break;
-            const int k = __builtin_amdgcn_readlane(my_key, i0 + u);
-            if (k >= p.groups && key >= p.groups) break;
-            if (k != key) {
-                flush(false);
-#pragma unroll
-                for (int j = 0; j < V; ++j) sum[j] = 0.0f;
-                key = k;
-                entered = false;
+            for (int u = 0; u < U; ++u) {
+                const long row = __builtin_amdgcn_readlane(my_row, min(i0 + u, count - 1));
+                if (whole) x[u] = *reinterpret_cast<const typename Run<T, V>::loose*>(in + row * p.in_stride);
+                else x[u] = load_operand(in + (some ? row * p.in_stride : 0), p.dim - at);
             }
 #pragma unroll
-            for (int j = 0; j < V; ++j) sum[j] += (float)x[u][j];
+            for (int u = 0; u < U; ++u) {
+                if (i0 + u >= count || key >= p.groups) break;
+                const int k = __builtin_amdgcn_readlane(my_key, i0 + u);
+                if (k != key) {
+                    flush(false);
+#pragma unroll
+                    for (int j = 0; j < V; ++j) sum[j] = 0.0f;
+                    key = k;
+                    entered = false;
+                }
+#pragma unroll
+                for (int j = 0; j < V; ++j) sum[j] += (float)x[u][j];
+            }
         }
-        if (key >= p.groups) return;      // (what lies behind belongs to no group)
+        if (key < p.groups) {
+            flush(key == behind);
+            if (entered && key == behind) tail_key = key;      // (a run that fills the quarter and goes on: its sum is in head)
+        }
     }
-    flush(key == behind);
+    if (lane == 0) {
+        key_of[wave][0] = head_key;
+        key_of[wave][1] = tail_key;
+    }
+    __syncthreads();
+    if (wave > 0) return;
+    // runs over several quarters, by the first wavefront
+    float sum[V];
+    int key = -1;
+    bool entered = false;
+    for (int w = 0; w < 4; ++w) {
+        const int h = __builtin_amdgcn_readfirstlane(key_of[w][0]), t = __builtin_amdgcn_readfirstlane(key_of[w][1]);
+        if (h >= 0) {
+            if (key < 0) {
+                entered = true;
+#pragma unroll
+                for (int j = 0; j < V; ++j) sum[j] = head[w][lane][j];
+            } else {
+#pragma unroll
+                for (int j = 0; j < V; ++j) sum[j] += head[w][lane][j];
+            }
+            key = h;
+            if (t == h) continue;
+            if (entered) {
+                if (some) store_run<V>(p.partial + 2 * piece * p.dim + at, p.dim - at, sum);
+            } else finish(key, sum);
+            key = -1;
+        }
+        if (t >= 0) {
+            key = t;
+            entered = false;
+#pragma unroll
+            for (int j = 0; j < V; ++j) sum[j] = tail[w][lane][j];
+        }
+    }
+    if (key >= 0 && some) store_run<V>(p.partial + (2 * piece + (entered ? 0 : 1)) * p.dim + at, p.dim - at, sum);
 }
 
-// Groups whose rows lie in several pieces: the parts, in order.  Groups without rows: zeros.  WAVES wavefronts share a group's 1 KB.
+// Groups whose rows lie in several pieces: the parts, in order.  Groups without rows: zeros.  Of few groups 16 wavefronts share 1 KB of a
+// group; of many a wavefront has up to 4 KB.
 template <typename T, int WAVES>
 __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void k_join_pieces(const Sums p)
 {
-    constexpr int V = kRun<T>;
+    constexpr int V = kRun<T>, SLABS = WAVES == 1 ? 4 : 1;
     __shared__ float part[WAVES == 1 ? 1 : WAVES][64][V];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), each = (p.slabs + SLABS - 1) / SLABS;
     const long item = WAVES == 1 ? (p.first + blockIdx.x) * 4 + wave : p.first + blockIdx.x;
-    if (item >= (long)p.groups * p.slabs) return;
-    const int g = (int)(item / p.slabs), at = (int)(item % p.slabs) * 64 * V + lane * V;
+    if (item >= (long)p.groups * each) return;
+    const int g = (int)(item / each), slab0 = (int)(item % each) * SLABS;
     const int begin = p.offsets[g], end = p.offsets[g + 1];
     const int first = begin / p.piece, last = end > begin ? (end - 1) / p.piece : first;
     if (end > begin && first == last) return;      // (the same in all wavefronts)
+    T* out = static_cast<T*>(p.out) + (long)g * p.dim;
     float sum[V];
+    if (end == begin) {
+        if (WAVES > 1 && wave > 0) return;
 #pragma unroll
-    for (int j = 0; j < V; ++j) sum[j] = 0.0f;
-    const bool some = at < p.dim;
-    if (end > begin && some) {
-        // (the first part lies in its piece's second place, the others in the first)
-        auto part_of = [&](long k) { return p.partial + (2 * k + (k == first ? 1 : 0)) * p.dim + at; };
-        const int mine = WAVES == 1 ? 0 : wave;
-#pragma unroll 8
-        for (int k = first + mine; k <= last; k += WAVES) {
-            float v[V];
-            load_run<V>(part_of(k), p.dim - at, v);
+        for (int j = 0; j < V; ++j) sum[j] = 0.0f;
 #pragma unroll
-            for (int j = 0; j < V; ++j) sum[j] += v[j];
+        for (int s = 0; s < SLABS; ++s) {
+            const int at = (slab0 + s) * 64 * V + lane * V;
+            if (at < p.dim) store_run<V>(out + at, p.dim - at, sum);
         }
+        return;
     }
-    if constexpr (WAVES > 1) {
-        if (end > begin) {
+#pragma unroll 1
+    for (int s = 0; s < SLABS; ++s) {
+        const int at = (slab0 + s) * 64 * V + lane * V;
+        const bool some = at < p.dim;
+#pragma unroll
+        for (int j = 0; j < V; ++j) sum[j] = 0.0f;
+        if (some) {
+            // (the first part lies in its piece's second place, the others in the first)
+            const int mine = WAVES == 1 ? 0 : wave;
+#pragma unroll 8
+            for (int k = first + mine; k <= last; k += WAVES) {
+                float v[V];
+                load_run<V>(p.partial + (2L * k + (k == first ? 1 : 0)) * p.dim + at, p.dim - at, v);
+#pragma unroll
+                for (int j = 0; j < V; ++j) sum[j] += v[j];
+            }
+        }
+        if constexpr (WAVES > 1) {
 #pragma unroll
             for (int j = 0; j < V; ++j) part[wave][lane][j] = sum[j];
             __syncthreads();
@@ -179,12 +243,11 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void k_join_pieces(c
             for (int w = 1; w < WAVES; ++w)
 #pragma unroll
                 for (int j = 0; j < V; ++j) sum[j] += part[w][lane][j];
-        } else if (wave > 0) return;
-    }
-    if (!some) return;
+        }
 #pragma unroll
-    for (int j = 0; j < V; ++j) sum[j] *= p.scale;
-    store_run<V>(static_cast<T*>(p.out) + (long)g * p.dim + at, p.dim - at, sum);
+        for (int j = 0; j < V; ++j) sum[j] *= p.scale;
+        if (some) store_run<V>(out + at, p.dim - at, sum);
+    }
 }
 
 // Few rows: a wavefront for 1 KB of a group's sum looks through the index by itself.
@@ -265,9 +328,9 @@ void add_rows(Launches& launches, Arena& arena, int type, const void* in, long i
             start(k_few_rows<T>, (entries + 3) / 4, 256);
             return;
         }
-        // pieces of 8 to 64 rows, until there are 16 wavefronts for every CU
-        p.piece = 8;
-        while (p.piece < 64 && rows * p.slabs / p.piece > 4096) p.piece *= 2;
+        // pieces of 32 to 256 rows, until there are 16 wavefronts for every CU
+        p.piece = 32;
+        while (p.piece < 256 && rows * p.slabs / p.piece > 1024) p.piece *= 2;
         p.pieces = (rows + p.piece - 1) / p.piece;
         p.partial = arena.take<float>(2 * p.pieces * dim);
         long offset_blocks = 0;
@@ -279,9 +342,9 @@ void add_rows(Launches& launches, Arena& arena, int type, const void* in, long i
             if (!with_offsets) offset_blocks = (groups + 2L + 255) / 256;
         }
         p.order = sorted.order; p.offsets = sorted.offsets; p.keys = sorted.keys;
-        start(k_pieces<T>, (p.pieces * p.slabs + 3) / 4 + offset_blocks, 256);
+        start(k_pieces<T>, p.pieces * p.slabs + offset_blocks, 256);
         if (groups <= 4096) start(k_join_pieces<T, 16>, entries, 1024);
-        else start(k_join_pieces<T, 1>, (entries + 3) / 4, 256);
+        else start(k_join_pieces<T, 1>, ((p.slabs + 3) / 4 * (long)groups + 3) / 4, 256);
     });
 }
 
@@ -307,7 +370,7 @@ extern "C" int smx_embedding_forward(int type, long rows, int entries, int dim, 
             const long per_block = kLookupRows * (256 / lanes);
             Launches::in_slabs((rows + per_block - 1) / per_block, [&](long first, long some) {
                 const long row = first * per_block;
-                launches.start(k_lookup<T>, some, 1, 1, 256, 0,
+                launches.start(rows * dim * (long)sizeof(T) >= kMuch ? k_lookup<T, true> : k_lookup<T, false>, some, 1, 1, 256, 0,
                                Lookup{d_table, table_stride, d_index + row, static_cast<T*>(d_y) + row * y_stride, y_stride, rows - row, entries, dim, lanes, (float)scale});
             });
         });

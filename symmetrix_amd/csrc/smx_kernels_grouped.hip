@@ -7,6 +7,7 @@
 // device alone, so a launch has as many blocks as there can be tiles, and every block finds its own from the groups' offsets.
 #include "smx_groups.hpp"
 
+#include <cmath>
 #include <limits>
 
 namespace smx {
@@ -71,17 +72,30 @@ __device__ __forceinline__ Place find_item(const Product& p, int item, int high,
     Place at{-1, 0, 0, -1};
     int slots = 0;
     for (int g0 = 0; g0 < p.groups + 2; g0 += 64) {
-        const int count = rows_of(p, g0 + lane, ALL), n = count < 0 ? 0 : items_of(count, high, ALL), until = wave_inclusive(n, lane);
+        const int count = rows_of(p, g0 + lane, ALL), n = count < 0 ? 0 : items_of(count, high, ALL);
         const int slots_until = ALL ? wave_inclusive(n > 1 ? n : 0, lane) : 0;
+        // Sums over rows: the groups with the most rows first, as far as a wavefront sees them at once, so that the last items are short.
+        int group = g0 + lane, until = n;
+        if (ALL && p.groups <= 64) {
+            int rank = 0;
+#pragma unroll 8
+            for (int h = 0; h < p.groups; ++h) {
+                const int other = __builtin_amdgcn_readlane(count, h);
+                rank += other > count || (other == count && h < lane) ? 1 : 0;
+            }
+            if (lane >= p.groups) rank = lane;
+            group = __builtin_amdgcn_ds_permute(rank * 4, lane);
+            until = __builtin_amdgcn_ds_permute(rank * 4, n);
+        }
+        until = wave_inclusive(until, lane);
         const unsigned long behind = __ballot(until > item);
         if (behind) {
-            const int where = __builtin_ctzl(behind), mine = item - (__builtin_amdgcn_readlane(until, where) - __builtin_amdgcn_readlane(n, where));
-            at.group = g0 + where;
-            const int first = p.offsets[at.group];
-            at.begin = first + mine * high;
-            at.end = min(first + __builtin_amdgcn_readlane(count, where), at.begin + high);
-            const int pieces = __builtin_amdgcn_readlane(n, where);
-            if (ALL && pieces > 1) at.slot = slots + __builtin_amdgcn_readlane(slots_until, where) - pieces + mine;
+            const int where = __builtin_ctzl(behind), from = __builtin_amdgcn_readlane(group, where) - g0, pieces = __builtin_amdgcn_readlane(n, from);
+            const int mine = item - (__builtin_amdgcn_readlane(until, where) - pieces), first = p.offsets[g0 + from];
+            at.group = g0 + from;
+            at.begin = __builtin_amdgcn_readfirstlane(first + mine * high);
+            at.end = min(at.begin - mine * high + __builtin_amdgcn_readlane(count, from), at.begin + high);
+            if (ALL && pieces > 1) at.slot = slots + __builtin_amdgcn_readlane(slots_until, from) - pieces + mine;
             return at;
         }
         item -= __builtin_amdgcn_readlane(until, 63);
@@ -90,31 +104,51 @@ __device__ __forceinline__ Place find_item(const Product& p, int item, int high,
     return at;
 }
 
-// Block -> tile: the blocks of a die (every eighth) take neighbouring tiles, four row tiles high, so that they share operands in its L2.
-__device__ __forceinline__ bool tile_of(int row_tiles, int col_tiles, long block, int& rt, int& ct)
+// Tiles of a grid, four row tiles high, one below the other: neighbours share operands.
+__device__ __forceinline__ void tile_at(int row_tiles, int col_tiles, int at, int& rt, int& ct)
 {
-    const long tiles = (long)row_tiles * col_tiles, per = (tiles + 7) / 8, at = block % 8 * per + block / 8;
-    if (at >= tiles || block / 8 >= per) return false;
-    const int band = (int)(at / (4 * col_tiles)), high = min(4, row_tiles - 4 * band), in_band = (int)(at - (long)band * 4 * col_tiles);
+    const int band = at / (4 * col_tiles), high = min(4, row_tiles - 4 * band), in_band = at - band * 4 * col_tiles;
     rt = band * 4 + in_band % high;
     ct = in_band / high;
-    return true;
 }
-// A block's place and its tile; false: there is none for it.
-template <int MODE>
-__device__ __forceinline__ bool find_tile(const Product& p, int high, int lane, Place& at, int& rt, int& ct)
+// A block's place and its tile; `parts`: into how many the tile is cut, of which the block has number `part`; false: there is no tile
+// for it.  The blocks of a die (every eighth) take neighbouring tiles, so that they share operands in its L2.
+// With CUT, of tiles that run one on a CU, those of the last round are cut where they are few: all others are done when they begin.
+constexpr int kCUs = 256;
+template <int MODE, bool CUT>
+__device__ __forceinline__ bool find_tile(const Product& p, int high, int lane, Place& at, int& rt, int& ct, int& parts, int& part)
 {
+    parts = 1;
+    part = 0;
     if constexpr (MODE == WEIGHTS) {
-        // (the tiles of an item by neighbouring blocks of a die)
-        const int items = count_items<true>(p, p.piece, lane);
-        const long tiles = (long)p.row_tiles * p.col_tiles, all = items * tiles, per = (all + 7) / 8, block = blockIdx.x, id = block % 8 * per + block / 8;
-        if (id >= all || block / 8 >= per) return false;
-        at = find_item<true>(p, (int)(id / tiles), p.piece, lane);
-        const int in_item = (int)(id % tiles), band = in_item / (4 * p.col_tiles), tall = min(4, p.row_tiles - 4 * band), in_band = in_item - band * 4 * p.col_tiles;
-        rt = band * 4 + in_band % tall;
-        ct = in_band / tall;
+        // (items take different times: every die has a share of each)
+        const int items = count_items<true>(p, p.piece, lane), tiles = p.row_tiles * p.col_tiles, share = (tiles + 7) / 8;
+        int item, tile;
+        if (tiles >= 8) {
+            item = (int)(blockIdx.x / 8) / share;
+            tile = blockIdx.x % 8 * share + (int)(blockIdx.x / 8) % share;
+            if (tile >= tiles) return false;
+        } else {
+            item = blockIdx.x / tiles;
+            tile = blockIdx.x % tiles;
+        }
+        if (item >= items) return false;
+        at = find_item<true>(p, item, p.piece, lane);
+        tile_at(p.row_tiles, p.col_tiles, tile, rt, ct);
     } else {
-        if (!tile_of(count_items<false>(p, high, lane), p.col_tiles, blockIdx.x, rt, ct)) return false;
+        const int row_tiles = count_items<false>(p, high, lane), tiles = row_tiles * p.col_tiles;
+        const int rest = CUT ? tiles % kCUs : 0, full = CUT ? tiles - rest : tiles;
+        int block = blockIdx.x, count = full, first = 0;
+        if (CUT && block >= full) {
+            parts = rest <= kCUs / 4 ? 4 : rest <= kCUs / 2 ? 2 : 1;
+            block -= full;
+            first = full;
+            count = rest * parts;
+        }
+        const int per = (count + 7) / 8, id = block % 8 * per + block / 8;
+        if (id >= count || block / 8 >= per) return false;
+        part = id % parts;
+        tile_at(row_tiles, p.col_tiles, first + id / parts, rt, ct);
         at = find_item<false>(p, rt, high, lane);
     }
     return true;
@@ -266,27 +300,25 @@ __device__ __forceinline__ void load_into_lds_from(const void* from, unsigned to
     asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
                  : "=&s"(m0) : "v"(from), "s"(to) : "memory");
 }
+// 4 bytes of every lane, from base + offset, to `to` + 4 lane
+__device__ __forceinline__ void load_words_into_lds(const void* base, unsigned offset, unsigned to)
+{
+    unsigned m0;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2\n\ts_mov_b32 m0, %0"
+                 : "=&s"(m0) : "v"(offset), "s"(base), "s"(to) : "memory");
+}
 __device__ const uint4 kZeros = {0, 0, 0, 0};      // what is fetched for terms that do not exist
 
 // 16-bit types whose rows begin at multiples of 16 bytes: straight from memory into LDS, STAGES steps of 64 terms under way.
 // WM x WN wavefronts share the tile.  32 terms have their operands fetched during the 32 before.
 template <typename T, int MODE, int BM, int BN, int WM, int WN, int STAGES>
-__global__ __launch_bounds__(64 * WM * WN, 2) void k_direct(const Product p)
+__device__ __forceinline__ void direct_tile(const Product& p, const Place& at, int row0, int col0, unsigned char* lds)
 {
     constexpr int WAVES = WM * WN, NM = BM / WM / 16, NT = BN / WN / 16, PA = BM / 8 / WAVES, PB = BN / 8 / WAVES, PER = PA + PB, STAGE = (BM + BN) * 128;
     constexpr bool A_ACROSS = MODE == WEIGHTS, B_ACROSS = MODE != FORWARD;
     static_assert(BM / 8 % WAVES == 0 && BN / 8 % WAVES == 0, "loads of a wavefront");
     typedef typename Operand<T>::type frag;
-    extern __shared__ __align__(1024) unsigned char lds[];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    Place at;
-    int rt, ct;
-    if (!find_tile<MODE>(p, BM, lane, at, rt, ct)) return;
-    const int col0 = ct * BN, row0 = MODE == WEIGHTS ? rt * BM : 0, count = at.end - at.begin;
-    if (MODE != WEIGHTS && at.group >= p.groups) {
-        store_none<T>(p, at, col0, BN);
-        return;
-    }
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), count = at.end - at.begin;
     const int terms = MODE == WEIGHTS ? count : p.k, stages = (terms + 63) / 64;
     // What a lane asks for, in bytes from a base that moves from step to step: 16 bytes at a time, PA + PB times.
     constexpr int A_PIECES = BM / 8, B_PIECES = BN / 8;      // of a term, where it lies across
@@ -316,56 +348,49 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_direct(const Product p)
         }
     }
     const unsigned lds0 = lds_address(lds);
-    // the rows that a wavefront's terms of a step are, for WEIGHTS (in scalar registers)
-    constexpr int TERMS = 64 / WAVES;
-    typedef const __attribute__((address_space(4))) int* scalar_ints;
-    int rows[MODE == WEIGHTS ? TERMS : 1];
+    // Of WEIGHTS: which rows the terms of the next steps are, four steps' in LDS behind the tiles.  A step's come a step before they are
+    // needed; asked for in front of the tiles', so that a wait for all but the youngest tiles' waits for them.
+    const unsigned rows0 = lds0 + STAGES * STAGE;
     auto look_up = [&](int s) {
+        if (MODE == WEIGHTS && wave == s % WAVES) load_words_into_lds(order, 4 * min(64 * s + lane, terms - 1), rows0 + s % 4 * 256);
+    };
+    static_assert(MODE != WEIGHTS || PA == PB, "one row for both operands");
+    auto rows_of = [&](int s, unsigned (&row)[PA]) {      // of a lane's terms
         if constexpr (MODE == WEIGHTS) {
-            const int first = 64 * s + wave * TERMS;
-            if (64 * s + 64 <= terms) {
-                const scalar_ints o = (scalar_ints)(order + first);
 #pragma unroll
-                for (int j = 0; j < TERMS; ++j) rows[j] = o[j];
-            } else {
-                const scalar_ints o = (scalar_ints)order;
-#pragma unroll
-                for (int j = 0; j < TERMS; ++j) rows[j] = o[min(first + j, terms - 1)];
-            }
+            for (int u = 0; u < PA; ++u)
+                row[u] = *(const __attribute__((address_space(3))) unsigned*)(rows0 + s % 4 * 256 + ((wave * PA + u) * 64 + lane) / A_PIECES * 4);
         }
     };
-    auto row_bytes = [&](int u, int pieces, long stride) {      // of the row of a lane's term
-        const int per = 64 / pieces;      // terms of 1 KB
-        unsigned v = (unsigned)(rows[u * per] * stride * 2);
-#pragma unroll
-        for (int j = 1; j < per; ++j) v = lane >= j * pieces ? (unsigned)(rows[u * per + j] * stride * 2) : v;
-        return v;
-    };
+    const unsigned a_row = (unsigned)p.a_stride * 2, b_row = (unsigned)p.b_stride * 2;
     auto request = [&](int s) {
         const unsigned to = lds0 + s % STAGES * STAGE;
         const char* a = static_cast<const char*>(p.a) + (A_ACROSS ? 0 : (long)s * 128);
         const char* b = b_base + (MODE == FORWARD ? (long)s * 128 : MODE == ROWS ? (long)s * 128 * p.b_stride : 0);
+        unsigned row[PA];
+        rows_of(s, row);
 #pragma unroll
-        for (int u = 0; u < PA; ++u) load_into_lds(a, from_a[u] + (A_ACROSS ? row_bytes(u, A_PIECES, p.a_stride) : 0), to + (wave * PA + u) * 1024);
+        for (int u = 0; u < PA; ++u) load_into_lds(a, from_a[u] + (A_ACROSS ? row[u] * a_row : 0), to + (wave * PA + u) * 1024);
 #pragma unroll
-        for (int u = 0; u < PB; ++u)
-            load_into_lds(b, from_b[u] + (MODE == WEIGHTS ? row_bytes(u, B_PIECES, p.b_stride) : 0), to + BM * 128 + (wave * PB + u) * 1024);
+        for (int u = 0; u < PB; ++u) load_into_lds(b, from_b[u] + (MODE == WEIGHTS ? row[u % PA] * b_row : 0), to + BM * 128 + (wave * PB + u) * 1024);
     };
     auto request_last = [&](int s) {      // of a step that need not be whole
         if (64 * s + 64 <= terms) return request(s);
         const unsigned to = lds0 + s % STAGES * STAGE;
         const char* a = static_cast<const char*>(p.a) + (A_ACROSS ? 0 : (long)s * 128);
         const char* b = b_base + (MODE == FORWARD ? (long)s * 128 : MODE == ROWS ? (long)s * 128 * p.b_stride : 0);
+        unsigned row[PA];
+        rows_of(s, row);
 #pragma unroll
         for (int u = 0; u < PA; ++u) {
             const int slot = (wave * PA + u) * 64 + lane, k = 64 * s + (A_ACROSS ? slot / A_PIECES : 8 * along_piece<64>(slot / 8, slot % 8));
-            const char* from = a + (from_a[u] + (A_ACROSS ? row_bytes(u, A_PIECES, p.a_stride) : 0));
+            const char* from = a + (from_a[u] + (A_ACROSS ? row[u] * a_row : 0));
             load_into_lds_from(k < terms ? from : reinterpret_cast<const char*>(&kZeros), to + (wave * PA + u) * 1024);
         }
 #pragma unroll
         for (int u = 0; u < PB; ++u) {
             const int slot = (wave * PB + u) * 64 + lane, k = 64 * s + (B_ACROSS ? slot / B_PIECES : 8 * along_piece<64>(slot / 8, slot % 8));
-            const char* from = b + (from_b[u] + (MODE == WEIGHTS ? row_bytes(u, B_PIECES, p.b_stride) : 0));
+            const char* from = b + (from_b[u] + (MODE == WEIGHTS ? row[u % PA] * b_row : 0));
             load_into_lds_from(k < terms ? from : reinterpret_cast<const char*>(&kZeros), to + BM * 128 + (wave * PB + u) * 1024);
         }
     };
@@ -405,20 +430,38 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_direct(const Product p)
         }
         __builtin_amdgcn_sched_barrier(0);
     };
+    // (a wavefront without rows takes part in the loads alone, and leaves the matrix cores to the others)
+    const bool idle = MODE != WEIGHTS && wm * NM * 16 >= count;
     if (stages > 0) {
+        if constexpr (MODE == WEIGHTS) {
+            static_assert(STAGES <= 3, "rows of four steps");
+            for (int i = threadIdx.x; i < (STAGES + 1) * 64; i += 64 * WAVES) *(__attribute__((address_space(3))) int*)(rows0 + 4 * i) = order[min(i, terms - 1)];
+            __syncthreads();
+        }
 #pragma unroll
         for (int s = 0; s < STAGES; ++s)
-            if (s < stages) {
-                look_up(s);
-                request_last(s);
-            }
+            if (s < stages) request_last(s);
         if (STAGES <= stages) wait_loads<(STAGES - 1) * PER>();
         else wait_loads<0>();
         barrier_only();
+        int s = 0;
+        if (idle) {
+#pragma unroll 1
+            for (; s + STAGES + 1 < stages; ++s) {
+                wait_loads<(STAGES - 2) * PER>();
+                barrier_only();
+                request(s + STAGES);
+            }
+#pragma unroll 1
+            for (; s + 1 < stages; ++s) {
+                wait_loads<0>();
+                barrier_only();
+                if (s + STAGES < stages) request_last(s + STAGES);
+            }
+            return;
+        }
         Frags f[2];
         fetch(0, 0, f[0]);
-        look_up(STAGES < stages ? STAGES : 0);
-        int s = 0;
 #pragma unroll 1
         for (; s + STAGES + 1 < stages; ++s) {
             fetch(s, 1, f[1]);
@@ -426,8 +469,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_direct(const Product p)
             woven();
             wait_loads<(STAGES - 2) * PER>();
             barrier_only();      // the next tiles are there, and everybody has read these
-            request(s + STAGES);
             look_up(s + STAGES + 1);
+            request(s + STAGES);
             fetch(s + 1, 0, f[0]);
             sums(f[1]);
             woven();
@@ -446,6 +489,39 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_direct(const Product p)
         }
     }
     finish<T, MODE, NM, NT>(p, at, lane, row0 + wm * NM * 16, col0 + wn * NT * 16, acc);
+}
+
+// LARGE: 256 x 256 by eight wavefronts, one block on a CU, those of the last round cut in two or four.
+template <typename T, int MODE, bool LARGE, int BM, int STAGES>
+__global__ __launch_bounds__(LARGE ? 512 : 256, 2) void k_direct(const Product p)
+{
+    static_assert(!LARGE || BM == 256, "tiles");
+    extern __shared__ __align__(1024) unsigned char lds[];
+    const int lane = threadIdx.x & 63;
+    Place at;
+    int rt, ct, parts, part;
+    if (!find_tile<MODE, LARGE>(p, BM, lane, at, rt, ct, parts, part)) return;
+    if (MODE != WEIGHTS && at.group >= p.groups) {
+        if (part == 0) store_none<T>(p, at, ct * BM, BM);
+        return;
+    }
+    const int row0 = MODE == WEIGHTS ? rt * BM : 0;
+    if constexpr (LARGE && MODE != WEIGHTS) {
+        if (parts > 1) {
+            const int col0 = ct * BM + part / (parts / 2) * (BM / 2);
+            if (col0 >= p.cols) return;
+            if (parts == 2) {
+                direct_tile<T, MODE, 256, 128, 4, 2, 2>(p, at, 0, col0, lds);
+            } else {
+                at.begin += part % 2 * (BM / 2);
+                at.end = min(at.end, at.begin + BM / 2);
+                if (at.begin < at.end) direct_tile<T, MODE, 128, 128, 2, 4, 4>(p, at, 0, col0, lds);
+            }
+            return;
+        }
+    }
+    if constexpr (LARGE) direct_tile<T, MODE, 256, 256, 2, 4, STAGES>(p, at, row0, ct * BM, lds);
+    else direct_tile<T, MODE, BM, BM, 2, 2, STAGES>(p, at, row0, ct * BM, lds);
 }
 
 // ---- operands by way of registers: any alignment, and single precision, which is brought to bf16 parts on the way
@@ -512,8 +588,8 @@ __global__ __launch_bounds__(256, 2) void k_staged(const Product p)
     __shared__ __align__(1024) unsigned char lds[PARTS * (A_PART + B_PART)];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Place at;
-    int rt, ct;
-    if (!find_tile<MODE>(p, BM, lane, at, rt, ct)) return;
+    int rt, ct, parts, part;
+    if (!find_tile<MODE, false>(p, BM, lane, at, rt, ct, parts, part)) return;
     const int col0 = ct * BN, row0 = MODE == WEIGHTS ? rt * BM : 0, count = at.end - at.begin;
     if (MODE != WEIGHTS && at.group >= p.groups) {
         store_none<T>(p, at, col0, BN);
@@ -668,18 +744,19 @@ __global__ __launch_bounds__(256) void k_join(const Product p)
     }
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) slots += __shfl_xor(slots, d, 64);
-    const long each = (long)p.m * p.cols, e = ((long)blockIdx.x * 256 + threadIdx.x) * 4;
-    if (e >= each) return;
-    const float* from = p.partial + slots * each + e;
-    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    const long each = (long)p.m * p.cols;
+    for (long e = ((long)blockIdx.x * 256 + threadIdx.x) * 4; e < each; e += (long)gridDim.x * 1024) {
+        const float* from = p.partial + slots * each + e;
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
-    for (int i = 0; i < pieces; ++i) {
-        float v[4];
-        load_run<4>(from + i * each, each - e, v);
+        for (int i = 0; i < pieces; ++i) {
+            float v[4];
+            load_run<4>(from + i * each, each - e, v);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) sum[j] += v[j];
+            for (int j = 0; j < 4; ++j) sum[j] += v[j];
+        }
+        store_run<4>(static_cast<T*>(p.out) + g * each + e, each - e, sum);
     }
-    store_run<4>(static_cast<T*>(p.out) + g * each + e, each - e, sum);
 }
 
 // ---- few rows of a group: bound by the weights' bytes
@@ -829,13 +906,14 @@ struct Call : Launches {
         groups.offsets = arena.take<int>(p.num_groups + 2L);
         sort_rows(*this, arena, p.index, p.rows, p.num_groups, groups);
     }
-    template <typename T, int MODE, int BM, int BN, int WM, int WN, int STAGES>
+    template <typename T, int MODE, bool LARGE, int BM, int STAGES>
     void direct(const Product& q, long blocks)
     {
-        constexpr int bytes = STAGES * (BM + BN) * 128;
-        auto kernel = k_direct<T, MODE, BM, BN, WM, WN, STAGES>;
+        constexpr int bytes = STAGES * 2 * BM * 128 + (MODE == WEIGHTS ? 1024 : 0);
+        auto kernel = k_direct<T, MODE, LARGE, BM, STAGES>;
         if (bytes > 64 * 1024 && !dry) hip_ok(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes), "LDS");
-        start(kernel, up(blocks, 8), 1, 1, 64 * WM * WN, bytes, q);
+        // (a last round of tiles cut in four has three more blocks for each)
+        start(kernel, up(blocks, 8) + (LARGE && MODE != WEIGHTS ? 3 * kCUs / 4 : 0), 1, 1, LARGE ? 512 : 256, bytes, q);
     }
     // Tiles for all rows in the worst case: every group has one that is not full.
     long row_tiles(int high) const { return p.rows / high + std::min(p.rows, p.num_groups + 2L); }
@@ -850,9 +928,9 @@ struct Call : Launches {
         };
         if constexpr (!std::is_same_v<T, float>) {
             if (direct_ok) {
-                if (p.rows / 256 * ((q.cols + 255) / 256) >= 192) direct<T, MODE, 256, 256, 2, 4, 2>(q, tiles(256, 256));
-                else if (p.rows / 128 * ((q.cols + 127) / 128) >= 192) direct<T, MODE, 128, 128, 2, 2, 2>(q, tiles(128, 128));
-                else direct<T, MODE, 64, 64, 2, 2, 3>(q, tiles(64, 64));
+                if (p.rows / 256 * ((q.cols + 255) / 256) >= 192) direct<T, MODE, true, 256, 2>(q, tiles(256, 256));
+                else if (p.rows / 128 * ((q.cols + 127) / 128) >= 192) direct<T, MODE, false, 128, 2>(q, tiles(128, 128));
+                else direct<T, MODE, false, 64, 3>(q, tiles(64, 64));
                 return;
             }
         }
@@ -896,35 +974,61 @@ struct Call : Launches {
         }
         if (db && p.num_groups) add_rows(*this, arena, p.type, dy, dy_stride, p.index, p.rows, p.num_groups, p.d_out, groups, 1.0f, db);
     }
+    // dW: which tiles, and how long the pieces of a group's rows are.  Small tiles and short pieces keep more CUs busy; large tiles
+    // take fewer bytes for a product, and pieces have to be written and read again to be joined.  What each way takes is estimated from
+    // the stages of 64 rows that a CU goes through (`stage`: us, of as many tiles as run on it at once), and the least is taken:
+    //   16 384 rows of 4 groups, 1 024 x 1 024 in bfloat16: tiles of 128 in whole groups 119 us, in two pieces 82;
+    //   50 000 rows of 12 groups, 256 x 512 in single precision: pieces of 832 rows (more blocks than run at once) 149 us, of 896 100.
+    struct Way {
+        int tile, piece;
+    };
+    Way way(int m, int cols, bool direct_ok, bool single) const
+    {
+        const double used = (double)std::max(1L, std::min(p.rows, (long)p.num_groups)), rows = (double)p.rows;
+        Way best{64, 1 << 28};
+        double least = std::numeric_limits<double>::max();
+        for (int tile = direct_ok && !single ? 256 : 128; tile >= 64; tile /= 2) {
+            const double each = (double)((m + tile - 1) / tile) * ((cols + tile - 1) / tile);
+            const double on_cu = tile == 256 ? 1 : tile == 128 ? 2 : 4;
+            const double stage = (tile == 256 ? 1.7 : tile == 128 ? 1.1 : 0.8) * (single ? 8 : direct_ok ? 1 : 2);
+            for (int parts = 1; parts <= 64; parts *= 2) {
+                // (a group's last piece is half as long as the others; groups of more than twice the usual rows are cut whatever the rest are)
+                const double piece = std::max(256.0, 64 * std::ceil((parts == 1 ? std::max(2 * rows / used, 1.5 * rows * each / (kCUs * on_cu)) : rows / used / parts) / 64));
+                const double items = rows / piece + used * (parts == 1 ? 1.0 : 0.5), blocks = items * each, rounds = blocks / (kCUs * on_cu);
+                const double usual = parts == 1 ? rows / used : piece;
+                const double time = std::max(rounds < 8 ? std::ceil(rounds) : rounds, 1.0) * (usual / 64 + 3) * stage + (parts == 1 ? 0.0 : 5 + rows / piece * m * (double)cols * 8 / 4e6);
+                if (time < least) least = time, best = Way{tile, (int)std::min(piece, (double)(1 << 28))};
+                if (piece <= 256.0) break;
+            }
+        }
+        return best;
+    }
     template <typename T>
     void weights(Product q, bool direct_ok)
     {
-        auto tiles = [&](int high, int wide) {
-            q.row_tiles = (q.m + high - 1) / high;
-            q.col_tiles = (q.cols + wide - 1) / wide;
-            return (long)q.row_tiles * q.col_tiles;
-        };
-        const long used = std::max(1L, std::min(p.rows, (long)p.num_groups));
-        const bool large = tiles(256, 256) * used >= 192, medium = tiles(128, 128) * used >= 192 || p.rows >= 64 * 1024 / 8;
-        const bool direct_large = direct_ok && large && !std::is_same_v<T, float>;
-        const long each = direct_large ? tiles(256, 256) : medium ? tiles(128, 128) : tiles(64, 64);
-        // Pieces of a group's rows, until there are two blocks for every CU; long ones where there are enough without (a group may have most rows).
-        q.piece = (int)std::min(1L << 28, std::max(each * used >= 384 ? 4096L : 512L, up((p.rows * each + 511) / 512, 64)));
-        const long items = p.rows / q.piece + p.num_groups, slots = 2 * (p.rows / q.piece);
+        constexpr bool SINGLE = std::is_same_v<T, float>;
+        const Way w = way(q.m, q.cols, direct_ok, SINGLE);
+        q.row_tiles = (q.m + w.tile - 1) / w.tile;
+        q.col_tiles = (q.cols + w.tile - 1) / w.tile;
+        q.piece = w.piece;
+        const long each = (long)q.row_tiles * q.col_tiles, items = p.rows / q.piece + p.num_groups, slots = 2 * (p.rows / q.piece);
         q.partial = arena.take<float>(slots * q.m * q.cols);
-        const long blocks = up(items * each, 8);
-        if constexpr (!std::is_same_v<T, float>) {
+        const long blocks = items * (each >= 8 ? up(each, 8) : each);
+        bool done = false;
+        if constexpr (!SINGLE) {
             if (direct_ok) {
-                if (direct_large) direct<T, WEIGHTS, 256, 256, 2, 4, 2>(q, blocks);
-                else if (medium) direct<T, WEIGHTS, 128, 128, 2, 2, 2>(q, blocks);
-                else direct<T, WEIGHTS, 64, 64, 2, 2, 3>(q, blocks);
+                if (w.tile == 256) direct<T, WEIGHTS, true, 256, 2>(q, blocks);
+                else if (w.tile == 128) direct<T, WEIGHTS, false, 128, 2>(q, blocks);
+                else direct<T, WEIGHTS, false, 64, 3>(q, blocks);
+                done = true;
             }
         }
-        if (std::is_same_v<T, float> || !direct_ok) {
-            if (medium) start(k_staged<T, WEIGHTS, 128, 128>, blocks, 1, 1, 256, 0, q);
+        if (!done) {
+            if (w.tile == 128) start(k_staged<T, WEIGHTS, 128, 128>, blocks, 1, 1, 256, 0, q);
             else start(k_staged<T, WEIGHTS, 64, 64>, blocks, 1, 1, 256, 0, q);
         }
-        if (slots) start(k_join<T>, ((long)q.m * q.cols + 1023) / 1024, p.num_groups, 1, 256, 0, q);
+        // (few blocks: most groups have nothing to join)
+        if (slots) start(k_join<T>, std::min(((long)q.m * q.cols + 1023) / 1024, std::max(1L, 2048L / p.num_groups)), p.num_groups, 1, 256, 0, q);
     }
 };
 

@@ -3,7 +3,7 @@
 // A digit takes two launches: the digits of every block's rows are counted, and then every block places its rows behind those of
 // smaller digits and those of earlier blocks, which it sums up from the counts by itself.  Inside a wavefront the rows of a digit find
 // their places from the lanes that hold it too (a ballot for every bit), so nothing depends on the order in which blocks or
-// atomics run.  Up to 2 048 rows stay in the LDS of one block, for all digits.
+// atomics run.  Up to 4 096 rows stay in the LDS of one block, for all digits.
 //
 // Bound by latency: a few dependent loads and barriers a launch.
 #include "smx_groups.hpp"
@@ -14,7 +14,7 @@ namespace {
 
 constexpr int kThreads = 512, kWaves = kThreads / 64;
 constexpr int kMostDigits = 1024;
-constexpr int kSmallRows = 2048;
+constexpr int kSmallRows = 4096;      // of one block
 
 struct Pass {
     const int* index;      // the first pass: indices of the rows; or
@@ -161,74 +161,87 @@ __global__ __launch_bounds__(256) void k_no_rows(int* offsets, int n)
 }
 
 // (offsets of more groups by one block would take longer than the sort)
-constexpr int kMostInside = 8192;
+constexpr int kMostInside = 4096;
 
-// All digits in one block.
+// All digits in one block: a wavefront has neighbouring rows, 64 at a time, at first and after every digit.
 struct SmallSort {
     const int* index;
-    int rows, groups, key_bits;
+    int rows, groups, key_bits, bits;
     int *order, *offsets, *keys;
 };
+constexpr int kSmallWaves = 16, kSmallDigits = 512;
+constexpr int small_lds(int rows) { return rows * 6 + kSmallWaves * kSmallDigits * 4; }
+template <int PER>
 __global__ __launch_bounds__(1024) void k_sort_small(const SmallSort p)
 {
-    constexpr int WAVES = 16, BITS = 8, DIGITS = 1 << BITS, PER = kSmallRows / 1024;
-    __shared__ int key_of[kSmallRows], row_of[kSmallRows];
-    __shared__ int next[WAVES][DIGITS];
-    __shared__ int part[WAVES];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int i = threadIdx.x; i < p.rows; i += 1024) {
-        key_of[i] = row_key(p.index[i], p.groups);
-        row_of[i] = i;
+    extern __shared__ int small[];
+    __shared__ int part[kSmallWaves];
+    int(*next)[kSmallDigits] = reinterpret_cast<int(*)[kSmallDigits]>(small);
+    int* key_of = small + kSmallWaves * kSmallDigits;
+    unsigned short* row_of = reinterpret_cast<unsigned short*>(key_of + 1024 * PER);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, digits = 1 << p.bits;
+    const int per_wave = ((p.rows + 1023) / 1024) * 64, begin = wave * per_wave, end = min(begin + per_wave, p.rows);
+    int key[PER], row[PER], at[PER];
+#pragma unroll
+    for (int u = 0; u < PER; ++u) {
+        row[u] = min(begin + 64 * u + lane, p.rows - 1);
+        key[u] = p.index[row[u]];
     }
-    const int per_wave = ((p.rows + 16 * 64 - 1) / (16 * 64)) * 64, begin = wave * per_wave, end = min(begin + per_wave, p.rows);
-    for (int shift = 0; shift < p.key_bits; shift += BITS) {
-        __syncthreads();
 #pragma unroll
-        for (int d = threadIdx.x; d < WAVES * DIGITS; d += 1024) next[d / DIGITS][d % DIGITS] = 0;
+    for (int u = 0; u < PER; ++u) key[u] = row_key(key[u], p.groups);
+    for (int shift = 0; shift < p.key_bits; shift += p.bits) {
+        const bool first = shift == 0, last = shift + p.bits >= p.key_bits;
+        for (int d = threadIdx.x; d < kSmallWaves * digits; d += 1024) next[d >> p.bits][d & (digits - 1)] = 0;
         __syncthreads();
-        int key[PER], row[PER], at[PER];
+        if (!first)
 #pragma unroll
-        for (int u = 0; u < PER; ++u) {      // places inside the wavefront first
-            const int i = begin + 64 * u + lane;
-            const bool live = i < end;
-            key[u] = live ? key_of[i] : 0;
-            row[u] = live ? row_of[i] : 0;
-            at[u] = begin + 64 * u < end ? take_place(next[wave], key[u] >> shift & (DIGITS - 1), live, BITS, lane) : 0;
-        }
+            for (int u = 0; u < PER; ++u)
+                if (begin + 64 * u + lane < end) {
+                    key[u] = key_of[begin + 64 * u + lane];
+                    row[u] = row_of[begin + 64 * u + lane];
+                }
+#pragma unroll
+        for (int u = 0; u < PER; ++u)      // places inside the wavefront first
+            if (begin + 64 * u < end) at[u] = take_place(next[wave], key[u] >> shift & (digits - 1), begin + 64 * u + lane < end, p.bits, lane);
         __syncthreads();
         int sum = 0, total;
-        if (threadIdx.x < DIGITS)
-            for (int w = 0; w < WAVES; ++w) sum += next[w][threadIdx.x];
+        if ((int)threadIdx.x < digits)
+#pragma unroll
+            for (int w = 0; w < kSmallWaves; ++w) sum += next[w][threadIdx.x];
         int start = block_exclusive(sum, part, total);
-        if (threadIdx.x < DIGITS)
-            for (int w = 0; w < WAVES; ++w) {
+        if ((int)threadIdx.x < digits) {
+            if (p.offsets && first && last && (int)threadIdx.x < p.groups + 2) p.offsets[threadIdx.x] = start;
+#pragma unroll
+            for (int w = 0; w < kSmallWaves; ++w) {
                 const int c = next[w][threadIdx.x];
                 next[w][threadIdx.x] = start;
                 start += c;
             }
+        }
         __syncthreads();
 #pragma unroll
-        for (int u = 0; u < PER; ++u) {
-            const int i = begin + 64 * u + lane;
-            if (i < end) {
-                const int to = next[wave][key[u] >> shift & (DIGITS - 1)] + at[u];
+        for (int u = 0; u < PER; ++u)
+            if (begin + 64 * u + lane < end) {
+                const int to = next[wave][key[u] >> shift & (digits - 1)] + at[u];
                 key_of[to] = key[u];
-                row_of[to] = row[u];
+                row_of[to] = (unsigned short)row[u];
             }
-        }
+        __syncthreads();
     }
-    __syncthreads();
     for (int i = threadIdx.x; i < p.rows; i += 1024) {
         p.order[i] = row_of[i];
         if (p.keys) p.keys[i] = key_of[i];
     }
-    if (p.offsets)
+    if (p.offsets && p.key_bits > p.bits)
         for (int g = threadIdx.x; g < p.groups + 2; g += 1024) p.offsets[g] = first_place(key_of, p.rows, g);
 }
 
 }  // namespace
 
-bool sort_has_offsets(long rows, int groups) { return rows <= kSmallRows ? groups <= kMostInside : groups + 2L <= kMostDigits; }
+bool sort_has_offsets(long rows, int groups)
+{
+    return rows <= kSmallRows ? groups <= kMostInside : groups + 2L <= kMostDigits;
+}
 
 void sort_rows(Launches& launches, Arena& arena, const int* index, long rows, int groups, const RowOrder& to)
 {
@@ -243,7 +256,16 @@ void sort_rows(Launches& launches, Arena& arena, const int* index, long rows, in
     if (rows <= kSmallRows) {
         const bool later = to.offsets && groups > kMostInside;
         if (later && !keys) keys = arena.take<int>(rows);
-        launches.start(k_sort_small, 1, 1, 1, 1024, 0, SmallSort{index, (int)rows, groups, key_bits, to.order, later ? nullptr : to.offsets, keys});
+        const int passes = (key_bits + 8) / 9;
+        const SmallSort p{index, (int)rows, groups, key_bits, (key_bits + passes - 1) / passes, to.order, later ? nullptr : to.offsets, keys};
+        auto go = [&](auto per) {
+            constexpr int PER = decltype(per)::value, bytes = small_lds(1024 * PER);
+            if (bytes > 48 * 1024 && !launches.dry)
+                hip_ok(hipFuncSetAttribute(reinterpret_cast<const void*>(k_sort_small<PER>), hipFuncAttributeMaxDynamicSharedMemorySize, bytes), "LDS");
+            launches.start(k_sort_small<PER>, 1, 1, 1, 1024, bytes, p);
+        };
+        if (rows <= 1024) go(Int<1>{});
+        else go(Int<4>{});
         if (later) offsets();
         return;
     }
@@ -252,7 +274,7 @@ void sort_rows(Launches& launches, Arena& arena, const int* index, long rows, in
     p.groups = groups;
     p.rows = rows;
     // (every block reads the counts of all)
-    p.rows_per_block = (int)std::max(2048L, up((rows + 255) / 256, kThreads));
+    p.rows_per_block = (int)std::max(1024L, up((rows + 255) / 256, kThreads));
     p.blocks = (int)((rows + p.rows_per_block - 1) / p.rows_per_block);
     p.count = arena.take<int>((long)p.blocks << ((key_bits + passes - 1) / passes));
     if (passes > 1 && !keys) keys = arena.take<int>(rows);
