@@ -17,7 +17,7 @@ namespace {
 
 constexpr int kTensors = 96;         // of a launch: their descriptions are kernel arguments
 constexpr int kChunkBytes = 16384;   // that a block takes at a time, the next ones on their way meanwhile
-constexpr int kMostParts = 1024;     // blocks, four for every CU
+constexpr int kMostParts = SMX_GRAD_NORM_PARTS;     // blocks, four for every CU
 
 struct NormTable {
     smx_grad_tensor tensor[kTensors];

@@ -39,14 +39,8 @@ struct Product {
 struct Place {
     int group, begin, end, slot;
 };
-// Items are cut from the groups in order, `high` rows each; with `all` a group without rows has one too, and the last two groups (rows
-// without a group) have none.  The number of items; a wavefront works it out for itself, 64 groups at a time.
-__device__ __forceinline__ int items_of(int count, int high, bool all) { return max((count + high - 1) / high, all ? 1 : 0); }
-__device__ __forceinline__ int rows_of(const Product& p, int g, bool all)
-{
-    if (g >= p.groups + (all ? 0 : 2)) return -1;
-    return (int)((g == p.groups + 1 ? p.rows : (long)p.offsets[g + 1]) - p.offsets[g]);
-}
+// Items are cut from the groups in order, `high` rows each; with ALL a group without rows has one too, and the last two groups (rows
+// without a group) have none.  A wavefront works out for itself where they are, 64 groups at a time, a lane each.
 __device__ __forceinline__ int wave_inclusive(int x, int lane)
 {
 #pragma unroll
@@ -57,51 +51,63 @@ __device__ __forceinline__ int wave_inclusive(int x, int lane)
     return x;
 }
 template <bool ALL>
-__device__ __forceinline__ int count_items(const Product& p, int high, int lane)
-{
-    int total = 0;
-    for (int g0 = 0; g0 < p.groups + 2; g0 += 64) {
-        const int count = rows_of(p, g0 + lane, ALL);
-        total += __builtin_amdgcn_readlane(wave_inclusive(count < 0 ? 0 : items_of(count, high, ALL), lane), 63);
+struct Items {
+    int first, count, n;      // of the lane's group: where its rows begin, how many they are, and its items
+    int until;                // items up to its last
+    __device__ __forceinline__ Items(const Product& p, int g0, int high, int lane)
+    {
+        const int g = g0 + lane, groups = p.groups + (ALL ? 0 : 2);
+        first = p.offsets[min(g, p.groups + 1)];
+        const int end = g >= p.groups + 1 ? (int)p.rows : p.offsets[min(g, p.groups) + 1];
+        count = g < groups ? end - first : -1;
+        n = count < 0 ? 0 : max((count + high - 1) / high, ALL ? 1 : 0);
+        until = wave_inclusive(n, lane);
     }
+    __device__ __forceinline__ int all() const { return __builtin_amdgcn_readlane(until, 63); }
+};
+// The number of items; here: those of the first 64 groups.
+template <bool ALL>
+__device__ __forceinline__ int count_items(const Product& p, const Items<ALL>& here, int high, int lane)
+{
+    int total = here.all();
+    for (int g0 = 64; g0 < p.groups + 2; g0 += 64) total += Items<ALL>(p, g0, high, lane).all();
     return total;
 }
 template <bool ALL>
-__device__ __forceinline__ Place find_item(const Product& p, int item, int high, int lane)
+__device__ __forceinline__ Place find_item(const Product& p, Items<ALL> here, int item, int high, int lane)
 {
     Place at{-1, 0, 0, -1};
     int slots = 0;
-    for (int g0 = 0; g0 < p.groups + 2; g0 += 64) {
-        const int count = rows_of(p, g0 + lane, ALL), n = count < 0 ? 0 : items_of(count, high, ALL);
-        const int slots_until = ALL ? wave_inclusive(n > 1 ? n : 0, lane) : 0;
+    for (int g0 = 0;;) {
+        const int slots_until = ALL ? wave_inclusive(here.n > 1 ? here.n : 0, lane) : 0;
         // Sums over rows: the groups with the most rows first, as far as a wavefront sees them at once, so that the last items are short.
-        int group = g0 + lane, until = n;
+        int group = lane, until = here.until;
         if (ALL && p.groups <= 64) {
             int rank = 0;
 #pragma unroll 8
             for (int h = 0; h < p.groups; ++h) {
-                const int other = __builtin_amdgcn_readlane(count, h);
-                rank += other > count || (other == count && h < lane) ? 1 : 0;
+                const int other = __builtin_amdgcn_readlane(here.count, h);
+                rank += other > here.count || (other == here.count && h < lane) ? 1 : 0;
             }
             if (lane >= p.groups) rank = lane;
             group = __builtin_amdgcn_ds_permute(rank * 4, lane);
-            until = __builtin_amdgcn_ds_permute(rank * 4, n);
+            until = wave_inclusive(__builtin_amdgcn_ds_permute(rank * 4, here.n), lane);
         }
-        until = wave_inclusive(until, lane);
         const unsigned long behind = __ballot(until > item);
         if (behind) {
-            const int where = __builtin_ctzl(behind), from = __builtin_amdgcn_readlane(group, where) - g0, pieces = __builtin_amdgcn_readlane(n, from);
-            const int mine = item - (__builtin_amdgcn_readlane(until, where) - pieces), first = p.offsets[g0 + from];
+            const int where = __builtin_ctzl(behind), from = __builtin_amdgcn_readlane(group, where), pieces = __builtin_amdgcn_readlane(here.n, from);
+            const int mine = item - (__builtin_amdgcn_readlane(until, where) - pieces), first = __builtin_amdgcn_readlane(here.first, from);
             at.group = g0 + from;
-            at.begin = __builtin_amdgcn_readfirstlane(first + mine * high);
-            at.end = min(at.begin - mine * high + __builtin_amdgcn_readlane(count, from), at.begin + high);
+            at.begin = first + mine * high;
+            at.end = min(first + __builtin_amdgcn_readlane(here.count, from), at.begin + high);
             if (ALL && pieces > 1) at.slot = slots + __builtin_amdgcn_readlane(slots_until, from) - pieces + mine;
             return at;
         }
-        item -= __builtin_amdgcn_readlane(until, 63);
+        item -= here.all();
         slots += ALL ? __builtin_amdgcn_readlane(slots_until, 63) : 0;
+        if ((g0 += 64) >= p.groups + 2) return at;
+        here = Items<ALL>(p, g0, high, lane);
     }
-    return at;
 }
 
 // Tiles of a grid, four row tiles high, one below the other: neighbours share operands.
@@ -122,7 +128,8 @@ __device__ __forceinline__ bool find_tile(const Product& p, int high, int lane, 
     part = 0;
     if constexpr (MODE == WEIGHTS) {
         // (items take different times: every die has a share of each)
-        const int items = count_items<true>(p, p.piece, lane), tiles = p.row_tiles * p.col_tiles, share = (tiles + 7) / 8;
+        const Items<true> here(p, 0, p.piece, lane);
+        const int items = count_items(p, here, p.piece, lane), tiles = p.row_tiles * p.col_tiles, share = (tiles + 7) / 8;
         int item, tile;
         if (tiles >= 8) {
             item = (int)(blockIdx.x / 8) / share;
@@ -133,10 +140,11 @@ __device__ __forceinline__ bool find_tile(const Product& p, int high, int lane, 
             tile = blockIdx.x % tiles;
         }
         if (item >= items) return false;
-        at = find_item<true>(p, item, p.piece, lane);
+        at = find_item(p, here, item, p.piece, lane);
         tile_at(p.row_tiles, p.col_tiles, tile, rt, ct);
     } else {
-        const int row_tiles = count_items<false>(p, high, lane), tiles = row_tiles * p.col_tiles;
+        const Items<false> here(p, 0, high, lane);
+        const int row_tiles = count_items(p, here, high, lane), tiles = row_tiles * p.col_tiles;
         const int rest = CUT ? tiles % kCUs : 0, full = CUT ? tiles - rest : tiles;
         int block = blockIdx.x, count = full, first = 0;
         if (CUT && block >= full) {
@@ -149,7 +157,7 @@ __device__ __forceinline__ bool find_tile(const Product& p, int high, int lane, 
         if (id >= count || block / 8 >= per) return false;
         part = id % parts;
         tile_at(row_tiles, p.col_tiles, first + id / parts, rt, ct);
-        at = find_item<false>(p, rt, high, lane);
+        at = find_item(p, here, rt, high, lane);
     }
     return true;
 }
@@ -217,9 +225,10 @@ __device__ __forceinline__ void store_tiles(int lane, const f32x4 (&acc)[NM][NT]
     }
 }
 
-// Bias, and where the results go: what follows the sums of all modes.  row0, col0: the wavefront's first in the tile's place.
+// Bias, and where the results go: what follows the sums of all modes.  row0, col0: the wavefront's first in the tile's place; rows: the
+// tile's, in LDS.
 template <typename T, int MODE, int NM, int NT>
-__device__ __forceinline__ void finish(const Product& p, const Place& at, int lane, int row0, int col0, f32x4 (&acc)[NM][NT])
+__device__ __forceinline__ void finish(const Product& p, const Place& at, int lane, int row0, int col0, const int* rows, f32x4 (&acc)[NM][NT])
 {
     if constexpr (MODE == WEIGHTS) {
         if (at.slot >= 0) {
@@ -250,8 +259,8 @@ __device__ __forceinline__ void finish(const Product& p, const Place& at, int la
             }
         }
         store_tiles<T>(lane, acc, p.cols - col0, [&](int i) {
-            const int r = at.begin + row0 + 16 * i + lane / 4;
-            return r < at.end ? static_cast<T*>(p.out) + p.order[r] * p.out_stride + col0 : nullptr;
+            const int r = row0 + 16 * i + lane / 4;
+            return r < at.end - at.begin ? static_cast<T*>(p.out) + rows[r] * p.out_stride + col0 : nullptr;
         });
     }
 }
@@ -348,18 +357,21 @@ __device__ __forceinline__ void direct_tile(const Product& p, const Place& at, i
         }
     }
     const unsigned lds0 = lds_address(lds);
-    // Of WEIGHTS: which rows the terms of the next steps are, four steps' in LDS behind the tiles.  A step's come a step before they are
+    int* const tile_rows = reinterpret_cast<int*>(lds + STAGES * STAGE);      // (for the results; there at the first barrier)
+    if (MODE != WEIGHTS)
+        for (int i = threadIdx.x; i < count; i += 64 * WAVES) tile_rows[i] = order[i];
+    // Of WEIGHTS: which rows the terms of the next steps are, sixteen steps' in LDS behind the tiles.  A step's come a step before they are
     // needed; asked for in front of the tiles', so that a wait for all but the youngest tiles' waits for them.
     const unsigned rows0 = lds0 + STAGES * STAGE;
     auto look_up = [&](int s) {
-        if (MODE == WEIGHTS && wave == s % WAVES) load_words_into_lds(order, 4 * min(64 * s + lane, terms - 1), rows0 + s % 4 * 256);
+        if (MODE == WEIGHTS && wave == s % WAVES) load_words_into_lds(order, 4 * min(64 * s + lane, terms - 1), rows0 + s % 16 * 256);
     };
     static_assert(MODE != WEIGHTS || PA == PB, "one row for both operands");
     auto rows_of = [&](int s, unsigned (&row)[PA]) {      // of a lane's terms
         if constexpr (MODE == WEIGHTS) {
 #pragma unroll
             for (int u = 0; u < PA; ++u)
-                row[u] = *(const __attribute__((address_space(3))) unsigned*)(rows0 + s % 4 * 256 + ((wave * PA + u) * 64 + lane) / A_PIECES * 4);
+                row[u] = *(const __attribute__((address_space(3))) unsigned*)(rows0 + s % 16 * 256 + ((wave * PA + u) * 64 + lane) / A_PIECES * 4);
         }
     };
     const unsigned a_row = (unsigned)p.a_stride * 2, b_row = (unsigned)p.b_stride * 2;
@@ -434,7 +446,7 @@ __device__ __forceinline__ void direct_tile(const Product& p, const Place& at, i
     const bool idle = MODE != WEIGHTS && wm * NM * 16 >= count;
     if (stages > 0) {
         if constexpr (MODE == WEIGHTS) {
-            static_assert(STAGES <= 3, "rows of four steps");
+            static_assert(STAGES < 15, "rows of sixteen steps");
             for (int i = threadIdx.x; i < (STAGES + 1) * 64; i += 64 * WAVES) *(__attribute__((address_space(3))) int*)(rows0 + 4 * i) = order[min(i, terms - 1)];
             __syncthreads();
         }
@@ -488,7 +500,7 @@ __device__ __forceinline__ void direct_tile(const Product& p, const Place& at, i
             sums(f[1]);
         }
     }
-    finish<T, MODE, NM, NT>(p, at, lane, row0 + wm * NM * 16, col0 + wn * NT * 16, acc);
+    finish<T, MODE, NM, NT>(p, at, lane, row0 + wm * NM * 16, col0 + wn * NT * 16, tile_rows, acc);
 }
 
 // LARGE: 256 x 256 by eight wavefronts, one block on a CU, those of the last round cut in two or four.
@@ -578,14 +590,17 @@ __device__ __forceinline__ float plain_sum(const Product& p, const Place& at, in
     return sum;
 }
 
-// Steps of 32 terms; the next one's numbers are on their way to registers during the sums of this one.  Four wavefronts, 2 x 2.
-template <typename T, int MODE, int BM, int BN>
+// Steps of 32 terms; those of the next AHEAD are on their way to registers during the sums of one.  Four wavefronts, 2 x 2.
+template <typename T, int MODE, int BM, int BN, int AHEAD>
 __global__ __launch_bounds__(256, 2) void k_staged(const Product p)
 {
     constexpr bool SINGLE = std::is_same_v<T, float>, A_ACROSS = MODE == WEIGHTS, B_ACROSS = MODE != FORWARD;
     constexpr int PARTS = SINGLE ? 3 : 1, NM = BM / 32, NT = BN / 32, PA = BM / 64, PB = BN / 64, A_PART = BM * 64, B_PART = BN * 64;
     typedef typename std::conditional_t<SINGLE, Operand<bf16>, Operand<T>>::type frag;
     __shared__ __align__(1024) unsigned char lds[PARTS * (A_PART + B_PART)];
+    // The tile's rows; or of WEIGHTS the rows of the terms of two times kLook steps, in LDS: a wait for a row's number from memory would be one for all that is on its way.
+    constexpr int kLook = 16;
+    __shared__ int look[MODE == WEIGHTS ? 2 * kLook * 32 : BM];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Place at;
     int rt, ct, parts, part;
@@ -597,6 +612,8 @@ __global__ __launch_bounds__(256, 2) void k_staged(const Product p)
     }
     const int terms = MODE == WEIGHTS ? count : p.k, steps = (terms + 31) / 32;
     const int* order = p.order + at.begin;
+    if (MODE != WEIGHTS)      // (for the results; there at the first barrier)
+        for (int i = threadIdx.x; i < count; i += 256) look[i] = order[i];
     // where a thread's numbers begin and how many of the eight there are; along: k is added
     const T* from_a[PA];
     const T* from_b[PB];
@@ -620,14 +637,20 @@ __global__ __launch_bounds__(256, 2) void k_staged(const Product p)
             from_b[u] = b + min(c, p.cols - 1);
         } else from_b[u] = b + min(col0 + slot / 4, p.cols - 1) * p.b_stride + slot % 4 * 8;
     }
-    Eight<T> raw_a[PA], raw_b[PB];
-    auto request = [&](int s) {
+    auto look_up = [&](int block) {      // of kLook steps
+        if constexpr (MODE == WEIGHTS)
+            for (int i = threadIdx.x; i < kLook * 32; i += 256) look[block % 2 * kLook * 32 + i] = order[min(block * kLook * 32 + i, terms - 1)];
+    };
+    Eight<T> raw[AHEAD][PA + PB];
+    auto request = [&](int s, Eight<T> (&to)[PA + PB]) {
+        Eight<T>* raw_a = to;
+        Eight<T>* raw_b = to + PA;
 #pragma unroll
         for (int u = 0; u < PA; ++u) {
             const int slot = u * 256 + threadIdx.x;
             if constexpr (A_ACROSS) {
                 const int k = 32 * s + slot / (BM / 8);
-                raw_a[u] = load_eight(from_a[u] + order[min(k, terms - 1)] * p.a_stride, k < terms ? a_left[u] : 0);
+                raw_a[u] = load_eight(from_a[u] + look[k % (2 * kLook * 32)] * p.a_stride, k < terms ? a_left[u] : 0);
             } else raw_a[u] = load_eight(from_a[u] + 32 * s, terms - 32 * s - slot % 4 * 8);
         }
 #pragma unroll
@@ -635,9 +658,10 @@ __global__ __launch_bounds__(256, 2) void k_staged(const Product p)
             const int slot = u * 256 + threadIdx.x;
             if constexpr (B_ACROSS) {
                 const int k = 32 * s + slot / (BN / 8);
-                raw_b[u] = load_eight(from_b[u] + (MODE == WEIGHTS ? (long)order[min(k, terms - 1)] : min(k, terms - 1)) * p.b_stride, k < terms ? b_left[u] : 0);
+                raw_b[u] = load_eight(from_b[u] + (MODE == WEIGHTS ? (long)look[k % (2 * kLook * 32)] : min(k, terms - 1)) * p.b_stride, k < terms ? b_left[u] : 0);
             } else raw_b[u] = load_eight(from_b[u] + 32 * s, terms - 32 * s - slot % 4 * 8);
         }
+        asm volatile("" ::: "memory");      // (asked for here, not where they are used)
     };
     auto put = [&](const Eight<T>& x, unsigned char* to, int part_bytes) {
         if constexpr (SINGLE) {
@@ -648,16 +672,16 @@ __global__ __launch_bounds__(256, 2) void k_staged(const Product p)
             for (int q = 0; q < 3; ++q) *reinterpret_cast<bf16x8*>(to + q * part_bytes) = part[q];
         } else *reinterpret_cast<frag*>(to) = x.v[0];
     };
-    auto store = [&] {
+    auto store = [&](const Eight<T> (&raw)[PA + PB]) {
 #pragma unroll
         for (int u = 0; u < PA; ++u) {
             const int slot = u * 256 + threadIdx.x, k = slot / (BM / 8);
-            put(raw_a[u], lds + (A_ACROSS ? k * (2 * BM) + 16 * (slot % (BM / 8) ^ across_turn<BM>(k) << 1) : slot / 4 * 64 + 16 * along_piece<32>(slot / 4, slot % 4)), A_PART);
+            put(raw[u], lds + (A_ACROSS ? k * (2 * BM) + 16 * (slot % (BM / 8) ^ across_turn<BM>(k) << 1) : slot / 4 * 64 + 16 * along_piece<32>(slot / 4, slot % 4)), A_PART);
         }
 #pragma unroll
         for (int u = 0; u < PB; ++u) {
             const int slot = u * 256 + threadIdx.x, k = slot / (BN / 8);
-            put(raw_b[u], lds + PARTS * A_PART + (B_ACROSS ? k * (2 * BN) + 16 * (slot % (BN / 8) ^ across_turn<BN>(k) << 1) : slot / 4 * 64 + 16 * along_piece<32>(slot / 4, slot % 4)),
+            put(raw[PA + u], lds + PARTS * A_PART + (B_ACROSS ? k * (2 * BN) + 16 * (slot % (BN / 8) ^ across_turn<BN>(k) << 1) : slot / 4 * 64 + 16 * along_piece<32>(slot / 4, slot % 4)),
                 B_PART);
         }
     };
@@ -670,13 +694,7 @@ __global__ __launch_bounds__(256, 2) void k_staged(const Product p)
     const unsigned lds0 = lds_address(lds);
     const Reader<frag, 32, BM, A_ACROSS> read_a(lds0, wm * NM, lane);
     const Reader<frag, 32, BN, B_ACROSS> read_b(lds0 + PARTS * A_PART, wn * NT, lane);
-    if (steps > 0) request(0);
-#pragma unroll 1
-    for (int s = 0; s < steps; ++s) {
-        __syncthreads();
-        store();
-        __syncthreads();
-        if (s + 1 < steps) request(s + 1);
+    auto sums = [&] {
         frag x[NM][PARTS];
 #pragma unroll
         for (int i = 0; i < NM; ++i)
@@ -697,6 +715,29 @@ __global__ __launch_bounds__(256, 2) void k_staged(const Product p)
 #pragma unroll
                 for (int i = 0; i < NM; ++i) acc[i][t] = mma(w[0], x[i][0], acc[i][t]);
             }
+        }
+    };
+    if (MODE == WEIGHTS && steps > 0) {
+        look_up(0);
+        look_up(1);
+        __syncthreads();
+    }
+#pragma unroll
+    for (int d = 0; d < AHEAD; ++d)
+        if (d < steps) request(d, raw[d]);
+    static_assert(kLook % AHEAD == 0, "blocks of rows begin where a round of steps does");
+#pragma unroll 1
+    for (int s0 = 0; s0 < steps; s0 += AHEAD) {
+#pragma unroll
+        for (int d = 0; d < AHEAD; ++d) {
+            const int s = s0 + d;
+            if (s >= steps) break;
+            __syncthreads();
+            store(raw[d]);
+            if (d == 0 && s > 0 && s % kLook == 0) look_up(s / kLook + 1);
+            __syncthreads();
+            if (s + AHEAD < steps) request(s + AHEAD, raw[d]);
+            sums();
         }
     }
     const int row_w = row0 + wm * NM * 16, col_w = col0 + wn * NT * 16;
@@ -726,7 +767,7 @@ __global__ __launch_bounds__(256, 2) void k_staged(const Product p)
                     }
         }
     }
-    finish<T, MODE, NM, NT>(p, at, lane, row_w, col_w, acc);
+    finish<T, MODE, NM, NT>(p, at, lane, row_w, col_w, look, acc);
 }
 
 // Sums of the pieces of a group's dW, in order.
@@ -848,7 +889,7 @@ __global__ __launch_bounds__(512) void k_few(const Product p, const int* index)
     const int lane = threadIdx.x & 63;
     int group, count;
     if constexpr (SORTED) {
-        const Place at = find_item<false>(p, blockIdx.y, kMostFew, lane);
+        const Place at = find_item(p, Items<false>(p, 0, kMostFew, lane), blockIdx.y, kMostFew, lane);
         if (at.group < 0) return;
         group = at.group;
         count = at.end - at.begin;
@@ -909,7 +950,7 @@ struct Call : Launches {
     template <typename T, int MODE, bool LARGE, int BM, int STAGES>
     void direct(const Product& q, long blocks)
     {
-        constexpr int bytes = STAGES * 2 * BM * 128 + (MODE == WEIGHTS ? 1024 : 0);
+        constexpr int bytes = STAGES * 2 * BM * 128 + (MODE == WEIGHTS ? 4096 : 1024);
         auto kernel = k_direct<T, MODE, LARGE, BM, STAGES>;
         if (bytes > 64 * 1024 && !dry) hip_ok(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes), "LDS");
         // (a last round of tiles cut in four has three more blocks for each)
@@ -930,12 +971,13 @@ struct Call : Launches {
             if (direct_ok) {
                 if (p.rows / 256 * ((q.cols + 255) / 256) >= 192) direct<T, MODE, true, 256, 2>(q, tiles(256, 256));
                 else if (p.rows / 128 * ((q.cols + 127) / 128) >= 192) direct<T, MODE, false, 128, 2>(q, tiles(128, 128));
-                else direct<T, MODE, false, 64, 3>(q, tiles(64, 64));
+                else if (tiles(64, 64) > kCUs) direct<T, MODE, false, 64, 3>(q, tiles(64, 64));
+                else direct<T, MODE, false, 64, 8>(q, tiles(64, 64));
                 return;
             }
         }
-        if (p.rows / 128 * ((q.cols + 127) / 128) >= 192) start(k_staged<T, MODE, 128, 128>, up(tiles(128, 128), 8), 1, 1, 256, 0, q);
-        else start(k_staged<T, MODE, 64, 64>, up(tiles(64, 64), 8), 1, 1, 256, 0, q);
+        if (p.rows / 128 * ((q.cols + 127) / 128) >= 192) start(k_staged<T, MODE, 128, 128, 2>, up(tiles(128, 128), 8), 1, 1, 256, 0, q);
+        else start(k_staged<T, MODE, 64, 64, 4>, up(tiles(64, 64), 8), 1, 1, 256, 0, q);
     }
     template <typename T>
     void forward(T* y, long y_stride)
@@ -1019,13 +1061,14 @@ struct Call : Launches {
             if (direct_ok) {
                 if (w.tile == 256) direct<T, WEIGHTS, true, 256, 2>(q, blocks);
                 else if (w.tile == 128) direct<T, WEIGHTS, false, 128, 2>(q, blocks);
-                else direct<T, WEIGHTS, false, 64, 3>(q, blocks);
+                else if (blocks > kCUs) direct<T, WEIGHTS, false, 64, 3>(q, blocks);
+                else direct<T, WEIGHTS, false, 64, 8>(q, blocks);
                 done = true;
             }
         }
         if (!done) {
-            if (w.tile == 128) start(k_staged<T, WEIGHTS, 128, 128>, blocks, 1, 1, 256, 0, q);
-            else start(k_staged<T, WEIGHTS, 64, 64>, blocks, 1, 1, 256, 0, q);
+            if (w.tile == 128) start(k_staged<T, WEIGHTS, 128, 128, 2>, blocks, 1, 1, 256, 0, q);
+            else start(k_staged<T, WEIGHTS, 64, 64, 4>, blocks, 1, 1, 256, 0, q);
         }
         // (few blocks: most groups have nothing to join)
         if (slots) start(k_join<T>, std::min(((long)q.m * q.cols + 1023) / 1024, std::max(1L, 2048L / p.num_groups)), p.num_groups, 1, 256, 0, q);

@@ -22,6 +22,7 @@ MAX_RANK = 128
 MAX_ADAPTERS = 4096
 MAX_GROUPS = 4096
 MAX_ENTRIES = 1 << 24
+_NORM_PARTS = 1024          # SMX_GRAD_NORM_PARTS
 
 
 class _Adapted(C.Structure):
@@ -379,9 +380,12 @@ def group_rows(index, num_groups):
 def embedding_forward(table, index, scale=1.0):
     """scale table[index] for every row of index (int32; -1: a row of zeros).  A row whose index is out of range is NaN."""
     kind = _type(table, "table")
-    _need(table.dim() == 2 and table.shape[1] >= 1, "table: [entries, dim] expected")
-    entries, dim = table.shape
-    _need(entries <= MAX_ENTRIES and math.isfinite(scale), f"entries: up to {MAX_ENTRIES}; scale: a finite number")
+    shape = table.shape
+    if len(shape) != 2 or shape[1] < 1:
+        raise ValueError("table: [entries, dim] expected")
+    entries, dim = shape
+    if entries > MAX_ENTRIES or not math.isfinite(scale):
+        raise ValueError(f"entries: up to {MAX_ENTRIES}; scale: a finite number")
     index, groups = _index(index)
     if groups is not None:
         groups.of(entries)
@@ -442,25 +446,31 @@ def embedding(table, index, scale=1.0):
 # ---- a product with a matrix of the row's own group
 
 def _grouped(x, weight, bias, index):
-    kind = _type(x, "x")
-    _need(weight.dim() == 3 and weight.shape[1] >= 1 and weight.shape[2] >= 1, "weight: [groups, d_out, d_in] expected")
-    n, d_out, d_in = weight.shape
-    _need(x.dim() >= 1 and x.shape[-1] == d_in, "x: rows of d_in numbers expected")
-    _need(n <= MAX_GROUPS, f"groups: up to {MAX_GROUPS}")
-    if weight.dtype != x.dtype or (bias is not None and bias.dtype != x.dtype):
+    kind, shape, rows_shape = _type(x, "x"), weight.shape, x.shape
+    if len(shape) != 3 or shape[1] < 1 or shape[2] < 1:
+        raise ValueError("weight: [groups, d_out, d_in] expected")
+    n, d_out, d_in = shape
+    if not rows_shape or rows_shape[-1] != d_in:
+        raise ValueError("x: rows of d_in numbers expected")
+    if n > MAX_GROUPS:
+        raise ValueError(f"groups: up to {MAX_GROUPS}")
+    if weight.dtype is not x.dtype or (bias is not None and bias.dtype is not x.dtype):
         raise TypeError("x, weight and bias: one type expected")
-    if bias is not None:
-        _need(bias.shape == (n, d_out) and bias.is_contiguous(), "bias: contiguous, [groups, d_out] expected")
-    index, groups = _index(index, x.shape[:-1])
+    if bias is not None and (bias.shape != (n, d_out) or not bias.is_contiguous()):
+        raise ValueError("bias: contiguous, [groups, d_out] expected")
+    index, groups = _index(index, rows_shape[:-1])
     device = _on(x, weight, bias, index)
     order = offsets = 0
     if groups is not None:
         groups.of(n)
         order, offsets = groups.order.data_ptr(), groups.offsets.data_ptr()
     rows_of, rows, stride = _rows(x, d_in, "x")
-    if (d_in > 1 and weight.stride(2) != 1) or (d_out > 1 and weight.stride(1) < d_in) or weight.stride(0) < 0:
+    each, weight_stride, along = weight.stride()
+    if (d_in > 1 and along != 1) or (d_out > 1 and weight_stride < d_in):
         weight = weight.contiguous()
-    weight_stride, each = (weight.stride(1) if d_out > 1 else d_in), weight.stride(0)
+        each, weight_stride, along = weight.stride()
+    if d_out == 1:
+        weight_stride = d_in
     p = _GROUPED.pack(kind, d_in, d_out, n, rows, rows_of.data_ptr(), stride, weight.data_ptr(), weight_stride, each, 0 if bias is None else bias.data_ptr(),
                       index.data_ptr(), order, offsets)
     # (the copies live until the call is made)
@@ -484,8 +494,9 @@ def grouped_linear_forward(x, weight, bias, index):
     have none.  A row whose index is out of range is NaN."""
     device, p, sizes, keep = _grouped(x, weight, bias, index)
     y = x.new_empty(x.shape[:-1] + (sizes[2],))
-    work = x.new_empty((_grouped_workspace(sizes, 0),), dtype=torch.uint8)
-    _call(device, _lib_functions().smx_grouped_linear_forward, p, y.data_ptr(), sizes[2], work.data_ptr(), work.numel())
+    size = _grouped_workspace(sizes, 0)
+    work = x.new_empty((size,), dtype=torch.uint8) if size else None
+    _call(device, _lib_functions().smx_grouped_linear_forward, p, y.data_ptr(), sizes[2], work.data_ptr() if size else 0, size)
     return y
 
 
@@ -530,40 +541,45 @@ def grouped_linear(x, weight, bias, index):
 
 # ---- the norm of gradients
 
-def _describe_grads(grads, outs):
+@functools.lru_cache(maxsize=64)
+def _grad_tensors(count):
+    return struct.Struct("@" + "iPPq" * count)
+
+
+def _describe_grads(grads, outs=None):
     """The descriptions of tensors that are there (not None), their device, how many, and what has to live until the call is made."""
-    packed, keep, device = [], [], None
-    for g, o in zip(grads, outs):
+    numbers, keep, device = [], [], None
+    for k, g in enumerate(grads):
         if g is None:
             continue
-        kind = _type(g, "gradients")
+        kind = _TYPES.get(g.dtype)
+        if kind is None:
+            _type(g, "gradients")
         at = g.get_device()
-        if device is None:
+        if at != device:
+            if device is not None:
+                raise ValueError("gradients on one device expected")
             device = _on(g)
-        elif at != device:
-            raise ValueError("gradients on one device expected")
         if not g.is_contiguous():
             g = g.contiguous()
             keep.append(g)
-        packed.append(_GRAD_TENSOR.pack(kind, g.data_ptr(), 0 if o is None else o.data_ptr(), g.numel()))
-    return b"".join(packed), device, len(packed), keep
+        numbers += (kind, g.data_ptr(), 0 if outs is None else outs[k].data_ptr(), g.numel())
+    count = len(numbers) // 4
+    return _grad_tensors(count).pack(*numbers), device, count, keep
 
 
-def _norm_call(described, max_norm, clip):
-    """The norm, and the factor where nothing is clipped: float32, a number each."""
+def _norm_call(described, max_norm, clip, factor=False):
+    """The norm, a float32 number, and with `factor` what keeps the factor, where its memory begins."""
     packed, device, count, keep = described
-    size = C.c_long()
-    L = _lib_functions()
-    _lib.check(L.smx_grad_norm_workspace(packed, count, C.byref(size)))
-    # (the numbers lie in front of the workspace: one allocation)
-    both = torch.empty((256 + size.value,), dtype=torch.uint8, device=torch.device("cuda", device))
-    norm = both[:8].view(torch.float32)
-    at = both.data_ptr()
+    place, size = torch.device("cuda", device), (8 * (_NORM_PARTS + count) + 255) // 256 * 256
+    norm = torch.empty((), dtype=torch.float32, device=place)
+    work = torch.empty((size + 256 if factor else size,), dtype=torch.uint8, device=place)
+    at = work.data_ptr()
     if clip:
-        _call(device, L.smx_clip_grads, packed, count, max_norm, at, at + 256, size.value)
+        _call(device, _lib_functions().smx_clip_grads, packed, count, max_norm, norm.data_ptr(), at, size)
     else:
-        _call(device, L.smx_grad_norm, packed, count, max_norm, at, at + 4, at + 256, size.value)
-    return norm
+        _call(device, _lib_functions().smx_grad_norm, packed, count, max_norm, norm.data_ptr(), at if factor else 0, at + 256 if factor else at, size)
+    return (norm, work) if factor else norm
 
 
 def grad_norm(grads):
@@ -571,10 +587,10 @@ def grad_norm(grads):
 
     Tensors may be of different types and shapes; None stands for a gradient that is not there."""
     grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
-    described = _describe_grads(grads, [None] * len(grads))
+    described = _describe_grads(grads)
     if not described[2]:
         return torch.zeros((), device="cuda")
-    return _norm_call(described, math.inf, False)[0]
+    return _norm_call(described, math.inf, False)
 
 
 def clip_grads(grads, max_norm, out=None):
@@ -610,7 +626,7 @@ def clip_grads(grads, max_norm, out=None):
         g.copy_(copy)
     # (as torch's own operations in place do)
     torch.autograd.graph.increment_version(there)
-    return norm[0]
+    return norm
 
 
 # ---- AdamW
@@ -777,8 +793,6 @@ class AdamW:
                 first(table, i * size, p.data_ptr(), g.data_ptr())
                 if max_norm is not None:
                     described.append(_GRAD_TENSOR.pack(_TYPES[kind], g.data_ptr(), 0, g.numel()))
-            if max_norm is not None:
-                described = (b"".join(described), device, len(described), keep)
             missed = self._missed
             if any(missed):
                 _need(all(missed[i] <= self.step_count for i in taken), "step_count: less than the steps that a parameter has missed")
@@ -787,14 +801,15 @@ class AdamW:
                     calls[missed[i]] = calls.get(missed[i], b"") + table[i * size:(i + 1) * size]
             else:          # (no parameter has missed a step so far; some may have no gradient in this one)
                 calls = {0: bytes(table) if len(taken) == len(params) else b"".join(table[i * size:(i + 1) * size] for i in taken)}
-            norm = None if max_norm is None else _norm_call(described, max_norm, False)
+            if max_norm is not None:
+                norm, factor = _norm_call((b"".join(described), device, len(described), keep), max_norm, False, factor=True)
             for late, some in calls.items():
                 of = (_TYPES[own], _TYPES[kind], self._bits, some, len(some) // size, self.lr, self.betas[0], self.betas[1], self.eps, self.weight_decay,
                       self.step_count + 1 - late)
                 if norm is None:
                     _call(device, _lib_functions().smx_adamw_step, *of)
                 else:
-                    _call(device, _lib_functions().smx_adamw_step_scaled, *of, norm.data_ptr() + 4)
+                    _call(device, _lib_functions().smx_adamw_step_scaled, *of, factor.data_ptr())
             # (as torch's own operations in place do: a backward pass that saved the old values says so)
             torch.autograd.graph.increment_version(params if len(taken) == len(params) else [params[i] for i in taken])
         if len(taken) < len(grads):
@@ -803,4 +818,4 @@ class AdamW:
                     self._missed[i] += 1
         self.step_count += 1
         if max_norm is not None:
-            return norm[0] if norm is not None else torch.zeros((), device=torch.device("cuda", self._device) if self.params else "cuda")
+            return norm if norm is not None else torch.zeros((), device=torch.device("cuda", self._device) if self.params else "cuda")
