@@ -560,17 +560,23 @@ template <typename T>
 struct Eight {
     typename Operand<T>::type v[8 / kRun<T>];
 };
-// those from p on, of which `left` exist; zeros for the others
+// those from p on, all of which exist, or `left` of them; zeros for the others
+template <typename T>
+__device__ __forceinline__ Eight<T> load_eight(const T* p)
+{
+    constexpr int V = kRun<T>;
+    Eight<T> x;
+#pragma unroll
+    for (int h = 0; h < 8 / V; ++h) x.v[h] = *reinterpret_cast<const typename Run<T, V>::loose*>(p + h * V);
+    return x;
+}
 template <typename T>
 __device__ __forceinline__ Eight<T> load_eight(const T* p, int left)
 {
     constexpr int V = kRun<T>;
     Eight<T> x;
 #pragma unroll
-    for (int h = 0; h < 8 / V; ++h) {
-        if (left >= 8) x.v[h] = *reinterpret_cast<const typename Run<T, V>::loose*>(p + h * V);
-        else x.v[h] = load_operand(p + h * V, left - h * V);
-    }
+    for (int h = 0; h < 8 / V; ++h) x.v[h] = load_operand(p + h * V, left - h * V);
     return x;
 }
 
@@ -590,6 +596,11 @@ __device__ __forceinline__ float plain_sum(const Product& p, const Place& at, in
     return sum;
 }
 
+// (16-bit types have more blocks on a CU instead)
+template <typename T>
+constexpr int kAhead128 = std::is_same_v<T, float> ? 2 : 1;
+template <typename T>
+constexpr int kAhead64 = std::is_same_v<T, float> ? 4 : 2;
 // Steps of 32 terms; those of the next AHEAD are on their way to registers during the sums of one.  Four wavefronts, 2 x 2.
 template <typename T, int MODE, int BM, int BN, int AHEAD>
 __global__ __launch_bounds__(256, 2) void k_staged(const Product p)
@@ -642,24 +653,36 @@ __global__ __launch_bounds__(256, 2) void k_staged(const Product p)
             for (int i = threadIdx.x; i < kLook * 32; i += 256) look[block % 2 * kLook * 32 + i] = order[min(block * kLook * 32 + i, terms - 1)];
     };
     Eight<T> raw[AHEAD][PA + PB];
+    // (Where every number exists nothing depends on the lane: behind a branch of some lanes all loads would be waited for.)
+    const bool a_whole = !A_ACROSS || row0 + BM <= p.m, b_whole = !B_ACROSS || col0 + BN <= p.cols;
     auto request = [&](int s, Eight<T> (&to)[PA + PB]) {
-        Eight<T>* raw_a = to;
-        Eight<T>* raw_b = to + PA;
+        const bool whole = 32 * s + 32 <= terms;
+        auto term = [&](int u, int wide) { return 32 * s + (u * 256 + (int)threadIdx.x) / (wide / 8); };
+        auto row_of = [&](int k) { return look[k % (2 * kLook * 32)]; };
+        if (whole && a_whole) {
 #pragma unroll
-        for (int u = 0; u < PA; ++u) {
-            const int slot = u * 256 + threadIdx.x;
-            if constexpr (A_ACROSS) {
-                const int k = 32 * s + slot / (BM / 8);
-                raw_a[u] = load_eight(from_a[u] + look[k % (2 * kLook * 32)] * p.a_stride, k < terms ? a_left[u] : 0);
-            } else raw_a[u] = load_eight(from_a[u] + 32 * s, terms - 32 * s - slot % 4 * 8);
+            for (int u = 0; u < PA; ++u) to[u] = load_eight(from_a[u] + (A_ACROSS ? row_of(term(u, BM)) * p.a_stride : 32 * s));
+        } else {
+#pragma unroll
+            for (int u = 0; u < PA; ++u) {
+                const int k = term(u, BM);
+                if constexpr (A_ACROSS) to[u] = load_eight(from_a[u] + row_of(k) * p.a_stride, k < terms ? a_left[u] : 0);
+                else to[u] = load_eight(from_a[u] + 32 * s, terms - 32 * s - (int)threadIdx.x % 4 * 8);
+            }
         }
+        if (whole && b_whole) {
 #pragma unroll
-        for (int u = 0; u < PB; ++u) {
-            const int slot = u * 256 + threadIdx.x;
-            if constexpr (B_ACROSS) {
-                const int k = 32 * s + slot / (BN / 8);
-                raw_b[u] = load_eight(from_b[u] + (MODE == WEIGHTS ? (long)look[k % (2 * kLook * 32)] : min(k, terms - 1)) * p.b_stride, k < terms ? b_left[u] : 0);
-            } else raw_b[u] = load_eight(from_b[u] + 32 * s, terms - 32 * s - slot % 4 * 8);
+            for (int u = 0; u < PB; ++u) {
+                const int k = term(u, BN);
+                to[PA + u] = load_eight(from_b[u] + (MODE == WEIGHTS ? row_of(k) * p.b_stride : B_ACROSS ? k * p.b_stride : 32 * s));
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < PB; ++u) {
+                const int k = term(u, BN);
+                if constexpr (B_ACROSS) to[PA + u] = load_eight(from_b[u] + (MODE == WEIGHTS ? (long)row_of(k) : min(k, terms - 1)) * p.b_stride, k < terms ? b_left[u] : 0);
+                else to[PA + u] = load_eight(from_b[u] + 32 * s, terms - 32 * s - (int)threadIdx.x % 4 * 8);
+            }
         }
         asm volatile("" ::: "memory");      // (asked for here, not where they are used)
     };
@@ -717,6 +740,11 @@ __global__ __launch_bounds__(256, 2) void k_staged(const Product p)
             }
         }
     };
+    // (what was put into the LDS, and what is read from it; a barrier of the language would wait for what is on its way to registers too)
+    auto all_there = [&] {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        barrier_only();
+    };
     if (MODE == WEIGHTS && steps > 0) {
         look_up(0);
         look_up(1);
@@ -732,12 +760,14 @@ __global__ __launch_bounds__(256, 2) void k_staged(const Product p)
         for (int d = 0; d < AHEAD; ++d) {
             const int s = s0 + d;
             if (s >= steps) break;
-            __syncthreads();
+            all_there();
             store(raw[d]);
             if (d == 0 && s > 0 && s % kLook == 0) look_up(s / kLook + 1);
-            __syncthreads();
+            all_there();
             if (s + AHEAD < steps) request(s + AHEAD, raw[d]);
+            __builtin_amdgcn_s_setprio(1);
             sums();
+            __builtin_amdgcn_s_setprio(0);
         }
     }
     const int row_w = row0 + wm * NM * 16, col_w = col0 + wn * NT * 16;
@@ -800,14 +830,17 @@ __global__ __launch_bounds__(256) void k_join(const Product p)
     }
 }
 
-// ---- few rows of a group: bound by the weights' bytes
+// ---- few rows: bound by the weights' bytes
 //
-// A block takes 16 columns of a group's product with up to 64 of its rows; eight wavefronts have 128 bytes of the weights' rows by
-// turns, four of them under way.  Up to 64 rows in all are not sorted: a block is there for every row, finds the rows of the same group
-// itself, and leaves if its own is not the first of them.
+// Up to 64 rows are not sorted: a block has 16 columns of the product of a row's group, finds the rows of the same group itself, and leaves if
+// its own is not the first of them.  Eight wavefronts have 128 bytes of the weights' rows by turns, three or four of them under way; 16 or
+// 32 rows at a time, so that two blocks have room on a CU (with 64 at a time there was one: 64 us for the first call below).
+// 48 rows of 32 groups, 2 048 x 2 048 in bfloat16: 48 us, 5.6 TB/s of the weights' bytes; 16 of 16, 4 096 x 4 096: 89 us, 6.0.
+// In tiles of 64: 24 rows of 3 groups, 192 -> 128 in single precision 15 us, here 11; 32 rows of one, 4 096 x 4 096 in bfloat16 20 us, here 12; but 64 of
+// 4 groups 27, here 31.
 constexpr int kMostFew = 64;
 template <typename T, int MT>
-__device__ __forceinline__ void few_rows(const Product& p, int group, const int* rows, int count, f32x4 (*part)[4][64])
+__device__ __forceinline__ void few_rows(const Product& p, int group, const int* rows, int count, f32x4 (*part)[2][64])
 {
     constexpr int V = kRun<T>, UNIT = 8 * V;
     typedef typename Operand<T>::type frag;
@@ -843,16 +876,17 @@ __device__ __forceinline__ void few_rows(const Product& p, int group, const int*
     };
     int u = wave;
     if (u < full) {
-        Unit unit[4];
+        constexpr int UNITS = MT == 1 ? 4 : 3;
+        Unit unit[UNITS];
 #pragma unroll
-        for (int q = 0; q < 3; ++q) fetch(u + 8 * q, unit[q]);
+        for (int q = 0; q < UNITS - 1; ++q) fetch(u + 8 * q, unit[q]);
 #pragma unroll 1
         for (;;) {
             bool done = false;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
+            for (int q = 0; q < UNITS; ++q) {
                 if (done) continue;
-                fetch(u + 24, unit[(q + 3) % 4]);
+                fetch(u + 8 * (UNITS - 1), unit[(q + UNITS - 1) % UNITS]);
                 sums(unit[q]);
                 done = (u += 8) >= full;
             }
@@ -868,6 +902,7 @@ __device__ __forceinline__ void few_rows(const Product& p, int group, const int*
             for (int i = 0; i < MT; ++i) acc[i] = mma(w, to_operand(load_operand(in[i] + k, p.k - k - mine), lane), acc[i]);
         }
     }
+    __syncthreads();
 #pragma unroll
     for (int i = 0; i < MT; ++i) part[wave][i][lane] = acc[i];
     __syncthreads();
@@ -881,27 +916,17 @@ __device__ __forceinline__ void few_rows(const Product& p, int group, const int*
         static_cast<T*>(p.out)[rows[row] * p.out_stride + col] = (T)sum;
     }
 }
-template <typename T, bool SORTED>
-__global__ __launch_bounds__(512) void k_few(const Product p, const int* index)
+template <typename T>
+__global__ __launch_bounds__(512, 4) void k_few(const Product p, const int* index)
 {
-    __shared__ f32x4 part[8][4][64];
+    __shared__ f32x4 part[8][2][64];
     __shared__ int rows[kMostFew];
-    const int lane = threadIdx.x & 63;
-    int group, count;
-    if constexpr (SORTED) {
-        const Place at = find_item(p, Items<false>(p, 0, kMostFew, lane), blockIdx.y, kMostFew, lane);
-        if (at.group < 0) return;
-        group = at.group;
-        count = at.end - at.begin;
-        if ((int)threadIdx.x < count) rows[threadIdx.x] = p.order[at.begin + threadIdx.x];
-    } else {
-        const int all = (int)p.rows, key = row_key(index[min(lane, all - 1)], p.groups);
-        group = __builtin_amdgcn_readlane(key, blockIdx.y);
-        const unsigned long same = __ballot(lane < all && key == group);
-        if (same & ((1ul << blockIdx.y) - 1)) return;      // (an earlier row's block does it)
-        count = __popcll(same);
-        if (threadIdx.x < 64 && (same >> lane & 1)) rows[__popcll(same & ((1ul << lane) - 1))] = lane;
-    }
+    const int lane = threadIdx.x & 63, all = (int)p.rows, key = row_key(index[min(lane, all - 1)], p.groups);
+    const int group = __builtin_amdgcn_readlane(key, blockIdx.y);
+    const unsigned long same = __ballot(lane < all && key == group);
+    if (same & ((1ul << blockIdx.y) - 1)) return;      // (an earlier row's block does it)
+    const int count = __popcll(same);
+    if (threadIdx.x < 64 && (same >> lane & 1)) rows[__popcll(same & ((1ul << lane) - 1))] = lane;
     __syncthreads();
     if (group >= p.groups) {
         const T v = (T)(group == p.groups ? 0.0f : std::numeric_limits<float>::quiet_NaN());
@@ -910,8 +935,8 @@ __global__ __launch_bounds__(512) void k_few(const Product p, const int* index)
         return;
     }
     if (count <= 16) few_rows<T, 1>(p, group, rows, count, part);
-    else if (count <= 32) few_rows<T, 2>(p, group, rows, count, part);
-    else few_rows<T, 4>(p, group, rows, count, part);
+    else
+        for (int first = 0; first < count; first += 32) few_rows<T, 2>(p, group, rows + first, min(32, count - first), part);
 }
 
 // ---- host side
@@ -976,8 +1001,8 @@ struct Call : Launches {
                 return;
             }
         }
-        if (p.rows / 128 * ((q.cols + 127) / 128) >= 192) start(k_staged<T, MODE, 128, 128, 2>, up(tiles(128, 128), 8), 1, 1, 256, 0, q);
-        else start(k_staged<T, MODE, 64, 64, 4>, up(tiles(64, 64), 8), 1, 1, 256, 0, q);
+        if (p.rows / 128 * ((q.cols + 127) / 128) >= 192) start(k_staged<T, MODE, 128, 128, kAhead128<T>>, up(tiles(128, 128), 8), 1, 1, 256, 0, q);
+        else start(k_staged<T, MODE, 64, 64, kAhead64<T>>, up(tiles(64, 64), 8), 1, 1, 256, 0, q);
     }
     template <typename T>
     void forward(T* y, long y_stride)
@@ -987,15 +1012,11 @@ struct Call : Launches {
         q.a = x; q.a_stride = p.x_stride; q.b = W; q.b_each = p.weight_each; q.b_stride = p.weight_stride; q.bias = p.bias; q.groups = p.num_groups; q.k = p.d_in; q.cols = p.d_out;
         q.rows = p.rows; q.out = y; q.out_stride = y_stride;
         if (p.rows <= kMostFew) {
-            start(k_few<T, false>, (p.d_out + 15) / 16, p.rows, 1, 512, 0, q, p.index);
+            start(k_few<T>, (p.d_out + 15) / 16, p.rows, 1, 512, 0, q, p.index);
             return;
         }
         sort();
         q.order = groups.order; q.offsets = groups.offsets;
-        if (p.rows <= 16L * p.num_groups) {
-            start(k_few<T, true>, (p.d_out + 15) / 16, row_tiles(kMostFew), 1, 512, 0, q, p.index);
-            return;
-        }
         rows<T, FORWARD>(q, in_pieces(x, p.x_stride, p.d_in) && in_pieces(W, p.weight_stride, p.d_in) && p.weight_each % 8 == 0 && within_reach(p.rows, p.x_stride));
     }
     template <typename T>
@@ -1031,14 +1052,16 @@ struct Call : Launches {
         double least = std::numeric_limits<double>::max();
         for (int tile = direct_ok && !single ? 256 : 128; tile >= 64; tile /= 2) {
             const double each = (double)((m + tile - 1) / tile) * ((cols + tile - 1) / tile);
-            const double on_cu = tile == 256 ? 1 : tile == 128 ? 2 : 4;
+            const double on_cu = tile == 256 ? 1 : tile == 128 ? 2 : 4, at_once = kCUs * on_cu;
             const double stage = (tile == 256 ? 1.7 : tile == 128 ? 1.1 : 0.8) * (single ? 8 : direct_ok ? 1 : 2);
-            for (int parts = 1; parts <= 64; parts *= 2) {
+            for (int parts : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 48, 64}) {
                 // (a group's last piece is half as long as the others; groups of more than twice the usual rows are cut whatever the rest are)
-                const double piece = std::max(256.0, 64 * std::ceil((parts == 1 ? std::max(2 * rows / used, 1.5 * rows * each / (kCUs * on_cu)) : rows / used / parts) / 64));
-                const double items = rows / piece + used * (parts == 1 ? 1.0 : 0.5), blocks = items * each, rounds = blocks / (kCUs * on_cu);
+                const double piece = std::max(256.0, 64 * std::ceil((parts == 1 ? std::max(2 * rows / used, 1.5 * rows * each / at_once) : rows / used / parts) / 64));
+                const double items = rows / piece + used * (parts == 1 ? 1.0 : 0.5), blocks = items * each, rounds = blocks / at_once;
                 const double usual = parts == 1 ? rows / used : piece;
-                const double time = std::max(rounds < 8 ? std::ceil(rounds) : rounds, 1.0) * (usual / 64 + 3) * stage + (parts == 1 ? 0.0 : 5 + rows / piece * m * (double)cols * 8 / 4e6);
+                // (fewer blocks on a CU than could be there are faster, though not in proportion)
+                const double shared = std::min(1.0, std::max(0.6, std::ceil(blocks / kCUs) / on_cu));
+                const double time = std::max(rounds < 8 ? std::ceil(rounds) : rounds, 1.0) * (usual / 64 + 3) * stage * shared + (parts == 1 ? 0.0 : 5 + rows / piece * m * (double)cols * 8 / 4e6);
                 if (time < least) least = time, best = Way{tile, (int)std::min(piece, (double)(1 << 28))};
                 if (piece <= 256.0) break;
             }
@@ -1067,8 +1090,8 @@ struct Call : Launches {
             }
         }
         if (!done) {
-            if (w.tile == 128) start(k_staged<T, WEIGHTS, 128, 128, 2>, blocks, 1, 1, 256, 0, q);
-            else start(k_staged<T, WEIGHTS, 64, 64, 4>, blocks, 1, 1, 256, 0, q);
+            if (w.tile == 128) start(k_staged<T, WEIGHTS, 128, 128, kAhead128<T>>, blocks, 1, 1, 256, 0, q);
+            else start(k_staged<T, WEIGHTS, 64, 64, kAhead64<T>>, blocks, 1, 1, 256, 0, q);
         }
         // (few blocks: most groups have nothing to join)
         if (slots) start(k_join<T>, std::min(((long)q.m * q.cols + 1023) / 1024, std::max(1L, 2048L / p.num_groups)), p.num_groups, 1, 256, 0, q);
