@@ -559,26 +559,19 @@ __device__ __forceinline__ void parts_of(const float (&x)[8], bf16x8 (&part)[3])
 template <typename T>
 struct Eight {
     typename Operand<T>::type v[8 / kRun<T>];
+    // from p on, all of which exist
+    __device__ __forceinline__ void load(const T* p)
+    {
+#pragma unroll
+        for (int h = 0; h < 8 / kRun<T>; ++h) v[h] = *reinterpret_cast<const typename Run<T, kRun<T>>::loose*>(p + h * kRun<T>);
+    }
+    // of which `left` exist; zeros for the others
+    __device__ __forceinline__ void load(const T* p, int left)
+    {
+#pragma unroll
+        for (int h = 0; h < 8 / kRun<T>; ++h) v[h] = load_operand(p + h * kRun<T>, left - h * kRun<T>);
+    }
 };
-// those from p on, all of which exist, or `left` of them; zeros for the others
-template <typename T>
-__device__ __forceinline__ Eight<T> load_eight(const T* p)
-{
-    constexpr int V = kRun<T>;
-    Eight<T> x;
-#pragma unroll
-    for (int h = 0; h < 8 / V; ++h) x.v[h] = *reinterpret_cast<const typename Run<T, V>::loose*>(p + h * V);
-    return x;
-}
-template <typename T>
-__device__ __forceinline__ Eight<T> load_eight(const T* p, int left)
-{
-    constexpr int V = kRun<T>;
-    Eight<T> x;
-#pragma unroll
-    for (int h = 0; h < 8 / V; ++h) x.v[h] = load_operand(p + h * V, left - h * V);
-    return x;
-}
 
 // A sum in single precision, term by term.
 template <typename T, int MODE>
@@ -596,22 +589,18 @@ __device__ __forceinline__ float plain_sum(const Product& p, const Place& at, in
     return sum;
 }
 
-// (16-bit types have more blocks on a CU instead)
-template <typename T>
-constexpr int kAhead128 = std::is_same_v<T, float> ? 2 : 1;
-template <typename T>
-constexpr int kAhead64 = std::is_same_v<T, float> ? 4 : 2;
-// Steps of 32 terms; those of the next AHEAD are on their way to registers during the sums of one.  Four wavefronts, 2 x 2.
+// Steps of 32 terms in single precision, of 64 in 16 bits (whose sums are short); those of the next AHEAD are on their way to registers during the sums of one.  Four wavefronts, 2 x 2.
 template <typename T, int MODE, int BM, int BN, int AHEAD>
 __global__ __launch_bounds__(256, 2) void k_staged(const Product p)
 {
     constexpr bool SINGLE = std::is_same_v<T, float>, A_ACROSS = MODE == WEIGHTS, B_ACROSS = MODE != FORWARD;
-    constexpr int PARTS = SINGLE ? 3 : 1, NM = BM / 32, NT = BN / 32, PA = BM / 64, PB = BN / 64, A_PART = BM * 64, B_PART = BN * 64;
+    constexpr int PARTS = SINGLE ? 3 : 1, STEP = SINGLE ? 32 : 64, PIECES = STEP / 8, NM = BM / 32, NT = BN / 32, PA = BM * PIECES / 256, PB = BN * PIECES / 256;
+    constexpr int A_PART = BM * STEP * 2, B_PART = BN * STEP * 2;
     typedef typename std::conditional_t<SINGLE, Operand<bf16>, Operand<T>>::type frag;
     __shared__ __align__(1024) unsigned char lds[PARTS * (A_PART + B_PART)];
     // The tile's rows; or of WEIGHTS the rows of the terms of two times kLook steps, in LDS: a wait for a row's number from memory would be one for all that is on its way.
     constexpr int kLook = 16;
-    __shared__ int look[MODE == WEIGHTS ? 2 * kLook * 32 : BM];
+    __shared__ int look[MODE == WEIGHTS ? 2 * kLook * STEP : BM];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Place at;
     int rt, ct, parts, part;
@@ -621,7 +610,7 @@ __global__ __launch_bounds__(256, 2) void k_staged(const Product p)
         store_none<T>(p, at, col0, BN);
         return;
     }
-    const int terms = MODE == WEIGHTS ? count : p.k, steps = (terms + 31) / 32;
+    const int terms = MODE == WEIGHTS ? count : p.k, steps = (terms + STEP - 1) / STEP;
     const int* order = p.order + at.begin;
     if (MODE != WEIGHTS)      // (for the results; there at the first barrier)
         for (int i = threadIdx.x; i < count; i += 256) look[i] = order[i];
@@ -636,7 +625,7 @@ __global__ __launch_bounds__(256, 2) void k_staged(const Product p)
             const int m = row0 + slot % (BM / 8) * 8;
             a_left[u] = p.m - m;
             from_a[u] = static_cast<const T*>(p.a) + min(m, p.m - 1);
-        } else from_a[u] = static_cast<const T*>(p.a) + order[min(slot / 4, count - 1)] * p.a_stride + slot % 4 * 8;
+        } else from_a[u] = static_cast<const T*>(p.a) + order[min(slot / PIECES, count - 1)] * p.a_stride + slot % PIECES * 8;
     }
 #pragma unroll
     for (int u = 0; u < PB; ++u) {
@@ -646,45 +635,39 @@ __global__ __launch_bounds__(256, 2) void k_staged(const Product p)
             const int c = col0 + slot % (BN / 8) * 8;
             b_left[u] = p.cols - c;
             from_b[u] = b + min(c, p.cols - 1);
-        } else from_b[u] = b + min(col0 + slot / 4, p.cols - 1) * p.b_stride + slot % 4 * 8;
+        } else from_b[u] = b + min(col0 + slot / PIECES, p.cols - 1) * p.b_stride + slot % PIECES * 8;
     }
     auto look_up = [&](int block) {      // of kLook steps
         if constexpr (MODE == WEIGHTS)
-            for (int i = threadIdx.x; i < kLook * 32; i += 256) look[block % 2 * kLook * 32 + i] = order[min(block * kLook * 32 + i, terms - 1)];
+            for (int i = threadIdx.x; i < kLook * STEP; i += 256) look[block % 2 * kLook * STEP + i] = order[min(block * kLook * STEP + i, terms - 1)];
     };
     Eight<T> raw[AHEAD][PA + PB];
-    // (Where every number exists nothing depends on the lane: behind a branch of some lanes all loads would be waited for.)
-    const bool a_whole = !A_ACROSS || row0 + BM <= p.m, b_whole = !B_ACROSS || col0 + BN <= p.cols;
-    auto request = [&](int s, Eight<T> (&to)[PA + PB]) {
-        const bool whole = 32 * s + 32 <= terms;
-        auto term = [&](int u, int wide) { return 32 * s + (u * 256 + (int)threadIdx.x) / (wide / 8); };
-        auto row_of = [&](int k) { return look[k % (2 * kLook * 32)]; };
-        if (whole && a_whole) {
+    auto term = [&](int s, int u, int wide) { return STEP * s + (u * 256 + (int)threadIdx.x) / (wide / 8); };
+    auto row_of = [&](int k) { return look[k % (2 * kLook * STEP)]; };
+    // Of a step all numbers of which exist, without a branch; and of any.
+    auto request_whole = [&](int s, Eight<T> (&to)[PA + PB]) {
 #pragma unroll
-            for (int u = 0; u < PA; ++u) to[u] = load_eight(from_a[u] + (A_ACROSS ? row_of(term(u, BM)) * p.a_stride : 32 * s));
-        } else {
+        for (int u = 0; u < PA; ++u) to[u].load(from_a[u] + (A_ACROSS ? row_of(term(s, u, BM)) * p.a_stride : STEP * s));
 #pragma unroll
-            for (int u = 0; u < PA; ++u) {
-                const int k = term(u, BM);
-                if constexpr (A_ACROSS) to[u] = load_eight(from_a[u] + row_of(k) * p.a_stride, k < terms ? a_left[u] : 0);
-                else to[u] = load_eight(from_a[u] + 32 * s, terms - 32 * s - (int)threadIdx.x % 4 * 8);
-            }
-        }
-        if (whole && b_whole) {
-#pragma unroll
-            for (int u = 0; u < PB; ++u) {
-                const int k = term(u, BN);
-                to[PA + u] = load_eight(from_b[u] + (MODE == WEIGHTS ? row_of(k) * p.b_stride : B_ACROSS ? k * p.b_stride : 32 * s));
-            }
-        } else {
-#pragma unroll
-            for (int u = 0; u < PB; ++u) {
-                const int k = term(u, BN);
-                if constexpr (B_ACROSS) to[PA + u] = load_eight(from_b[u] + (MODE == WEIGHTS ? (long)row_of(k) : min(k, terms - 1)) * p.b_stride, k < terms ? b_left[u] : 0);
-                else to[PA + u] = load_eight(from_b[u] + 32 * s, terms - 32 * s - (int)threadIdx.x % 4 * 8);
-            }
+        for (int u = 0; u < PB; ++u) {
+            const int k = term(s, u, BN);
+            to[PA + u].load(from_b[u] + (MODE == WEIGHTS ? row_of(k) * p.b_stride : B_ACROSS ? k * p.b_stride : STEP * s));
         }
         asm volatile("" ::: "memory");      // (asked for here, not where they are used)
+    };
+    auto request = [&](int s, Eight<T> (&to)[PA + PB]) {
+#pragma unroll
+        for (int u = 0; u < PA; ++u) {
+            const int k = term(s, u, BM);
+            if constexpr (A_ACROSS) to[u].load(from_a[u] + row_of(k) * p.a_stride, k < terms ? a_left[u] : 0);
+            else to[u].load(from_a[u] + STEP * s, terms - STEP * s - (int)threadIdx.x % PIECES * 8);
+        }
+#pragma unroll
+        for (int u = 0; u < PB; ++u) {
+            const int k = term(s, u, BN);
+            if constexpr (B_ACROSS) to[PA + u].load(from_b[u] + (MODE == WEIGHTS ? (long)row_of(k) : min(k, terms - 1)) * p.b_stride, k < terms ? b_left[u] : 0);
+            else to[PA + u].load(from_b[u] + STEP * s, terms - STEP * s - (int)threadIdx.x % PIECES * 8);
+        }
     };
     auto put = [&](const Eight<T>& x, unsigned char* to, int part_bytes) {
         if constexpr (SINGLE) {
@@ -699,12 +682,12 @@ __global__ __launch_bounds__(256, 2) void k_staged(const Product p)
 #pragma unroll
         for (int u = 0; u < PA; ++u) {
             const int slot = u * 256 + threadIdx.x, k = slot / (BM / 8);
-            put(raw[u], lds + (A_ACROSS ? k * (2 * BM) + 16 * (slot % (BM / 8) ^ across_turn<BM>(k) << 1) : slot / 4 * 64 + 16 * along_piece<32>(slot / 4, slot % 4)), A_PART);
+            put(raw[u], lds + (A_ACROSS ? k * (2 * BM) + 16 * (slot % (BM / 8) ^ across_turn<BM>(k) << 1) : slot / PIECES * (2 * STEP) + 16 * along_piece<STEP>(slot / PIECES, slot % PIECES)), A_PART);
         }
 #pragma unroll
         for (int u = 0; u < PB; ++u) {
             const int slot = u * 256 + threadIdx.x, k = slot / (BN / 8);
-            put(raw[PA + u], lds + PARTS * A_PART + (B_ACROSS ? k * (2 * BN) + 16 * (slot % (BN / 8) ^ across_turn<BN>(k) << 1) : slot / 4 * 64 + 16 * along_piece<32>(slot / 4, slot % 4)),
+            put(raw[PA + u], lds + PARTS * A_PART + (B_ACROSS ? k * (2 * BN) + 16 * (slot % (BN / 8) ^ across_turn<BN>(k) << 1) : slot / PIECES * (2 * STEP) + 16 * along_piece<STEP>(slot / PIECES, slot % PIECES)),
                 B_PART);
         }
     };
@@ -715,28 +698,31 @@ __global__ __launch_bounds__(256, 2) void k_staged(const Product p)
         for (int t = 0; t < NT; ++t) acc[i][t] = f32x4{0, 0, 0, 0};
     const int wm = wave / 2, wn = wave % 2;
     const unsigned lds0 = lds_address(lds);
-    const Reader<frag, 32, BM, A_ACROSS> read_a(lds0, wm * NM, lane);
-    const Reader<frag, 32, BN, B_ACROSS> read_b(lds0 + PARTS * A_PART, wn * NT, lane);
+    const Reader<frag, STEP, BM, A_ACROSS> read_a(lds0, wm * NM, lane);
+    const Reader<frag, STEP, BN, B_ACROSS> read_b(lds0 + PARTS * A_PART, wn * NT, lane);
     auto sums = [&] {
-        frag x[NM][PARTS];
 #pragma unroll
-        for (int i = 0; i < NM; ++i)
+        for (int h = 0; h < STEP / 32; ++h) {
+            frag x[NM][PARTS];
 #pragma unroll
-            for (int q = 0; q < PARTS; ++q) x[i][q] = read_a.get(i, 0, q * A_PART);
+            for (int i = 0; i < NM; ++i)
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            frag w[PARTS];
+                for (int q = 0; q < PARTS; ++q) x[i][q] = read_a.get(i, h, q * A_PART);
 #pragma unroll
-            for (int q = 0; q < PARTS; ++q) w[q] = read_b.get(t, 0, q * B_PART);
-            if constexpr (SINGLE) {
-                constexpr int ix[6] = {2, 0, 1, 1, 0, 0}, iw[6] = {0, 2, 1, 0, 1, 0};
+            for (int t = 0; t < NT; ++t) {
+                frag w[PARTS];
 #pragma unroll
-                for (int o = 0; o < 6; ++o)
+                for (int q = 0; q < PARTS; ++q) w[q] = read_b.get(t, h, q * B_PART);
+                if constexpr (SINGLE) {
+                    constexpr int ix[6] = {2, 0, 1, 1, 0, 0}, iw[6] = {0, 2, 1, 0, 1, 0};
 #pragma unroll
-                    for (int i = 0; i < NM; ++i) acc[i][t] = mma(w[iw[o]], x[i][ix[o]], acc[i][t]);
-            } else {
+                    for (int o = 0; o < 6; ++o)
 #pragma unroll
-                for (int i = 0; i < NM; ++i) acc[i][t] = mma(w[0], x[i][0], acc[i][t]);
+                        for (int i = 0; i < NM; ++i) acc[i][t] = mma(w[iw[o]], x[i][ix[o]], acc[i][t]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < NM; ++i) acc[i][t] = mma(w[0], x[i][0], acc[i][t]);
+                }
             }
         }
     };
@@ -750,24 +736,41 @@ __global__ __launch_bounds__(256, 2) void k_staged(const Product p)
         look_up(1);
         __syncthreads();
     }
-#pragma unroll
-    for (int d = 0; d < AHEAD; ++d)
-        if (d < steps) request(d, raw[d]);
     static_assert(kLook % AHEAD == 0, "blocks of rows begin where a round of steps does");
+    // Steps that are whole, in a loop of their own: what is on its way is waited for by count there, behind a branch altogether.
+    const int whole = (!A_ACROSS || row0 + BM <= p.m) && (!B_ACROSS || col0 + BN <= p.cols) ? terms / STEP : 0;
+    auto step = [&](int s, int d, auto&& next) {
+        all_there();
+        store(raw[d]);
+        if (d == 0 && s > 0 && s % kLook == 0) look_up(s / kLook + 1);
+        all_there();
+        next(s + AHEAD, raw[d]);
+        __builtin_amdgcn_s_setprio(1);      // (the matrix cores before another block's splits)
+        sums();
+        __builtin_amdgcn_s_setprio(0);
+    };
+    int s0 = 0;
+    if (whole >= 2 * AHEAD) {
+#pragma unroll
+        for (int d = 0; d < AHEAD; ++d) request_whole(d, raw[d]);
 #pragma unroll 1
-    for (int s0 = 0; s0 < steps; s0 += AHEAD) {
+        for (; s0 + 2 * AHEAD <= whole; s0 += AHEAD) {
+#pragma unroll
+            for (int d = 0; d < AHEAD; ++d) step(s0 + d, d, request_whole);
+        }
+    } else {
+#pragma unroll
+        for (int d = 0; d < AHEAD; ++d)
+            if (d < steps) request(d, raw[d]);
+    }
+#pragma unroll 1
+    for (; s0 < steps; s0 += AHEAD) {
 #pragma unroll
         for (int d = 0; d < AHEAD; ++d) {
-            const int s = s0 + d;
-            if (s >= steps) break;
-            all_there();
-            store(raw[d]);
-            if (d == 0 && s > 0 && s % kLook == 0) look_up(s / kLook + 1);
-            all_there();
-            if (s + AHEAD < steps) request(s + AHEAD, raw[d]);
-            __builtin_amdgcn_s_setprio(1);
-            sums();
-            __builtin_amdgcn_s_setprio(0);
+            if (s0 + d >= steps) break;
+            step(s0 + d, d, [&](int s, Eight<T> (&to)[PA + PB]) {
+                if (s < steps) request(s, to);
+            });
         }
     }
     const int row_w = row0 + wm * NM * 16, col_w = col0 + wn * NT * 16;
@@ -1001,8 +1004,8 @@ struct Call : Launches {
                 return;
             }
         }
-        if (p.rows / 128 * ((q.cols + 127) / 128) >= 192) start(k_staged<T, MODE, 128, 128, kAhead128<T>>, up(tiles(128, 128), 8), 1, 1, 256, 0, q);
-        else start(k_staged<T, MODE, 64, 64, kAhead64<T>>, up(tiles(64, 64), 8), 1, 1, 256, 0, q);
+        if (p.rows / 128 * ((q.cols + 127) / 128) >= 192) start(k_staged<T, MODE, 128, 128, (std::is_same_v<T, float> ? 2 : 1)>, up(tiles(128, 128), 8), 1, 1, 256, 0, q);
+        else start(k_staged<T, MODE, 64, 64, (std::is_same_v<T, float> ? 4 : 2)>, up(tiles(64, 64), 8), 1, 1, 256, 0, q);
     }
     template <typename T>
     void forward(T* y, long y_stride)
@@ -1090,8 +1093,8 @@ struct Call : Launches {
             }
         }
         if (!done) {
-            if (w.tile == 128) start(k_staged<T, WEIGHTS, 128, 128, kAhead128<T>>, blocks, 1, 1, 256, 0, q);
-            else start(k_staged<T, WEIGHTS, 64, 64, kAhead64<T>>, blocks, 1, 1, 256, 0, q);
+            if (w.tile == 128) start(k_staged<T, WEIGHTS, 128, 128, (std::is_same_v<T, float> ? 2 : 1)>, blocks, 1, 1, 256, 0, q);
+            else start(k_staged<T, WEIGHTS, 64, 64, (std::is_same_v<T, float> ? 4 : 2)>, blocks, 1, 1, 256, 0, q);
         }
         // (few blocks: most groups have nothing to join)
         if (slots) start(k_join<T>, std::min(((long)q.m * q.cols + 1023) / 1024, std::max(1L, 2048L / p.num_groups)), p.num_groups, 1, 256, 0, q);
