@@ -33,6 +33,8 @@ struct Product {
     int row_tiles, col_tiles;  // row_tiles: of WEIGHTS
     int piece;                 // of WEIGHTS: rows of a group that a block sums at most
     float* partial;            // sums of groups of more than one piece [slot][m][cols]
+    void* sums;                // of WEIGHTS by way of registers: db [group][m], or null
+    float* partial_sums;       // its parts [slot][m]
 };
 
 // Where a block's rows are: [begin, end) of the sorted order, group `group`; slot: of a piece of WEIGHTS, or -1.
@@ -162,15 +164,17 @@ __device__ __forceinline__ bool find_tile(const Product& p, int high, int lane, 
     return true;
 }
 
-// What rows without a group have for results
+// What rows without a group have for results: eight numbers a thread, rows and columns at once.
 template <typename T>
 __device__ __forceinline__ void store_none(const Product& p, const Place& at, int col0, int wide)
 {
-    const T v = (T)(at.group == p.groups ? 0.0f : std::numeric_limits<float>::quiet_NaN());
-    const int last = min(wide, p.cols - col0);
-    for (int i = at.begin; i < at.end; ++i) {
-        T* out = static_cast<T*>(p.out) + p.order[i] * p.out_stride + col0;
-        for (int c = threadIdx.x; c < last; c += blockDim.x) out[c] = v;
+    const float v = at.group == p.groups ? 0.0f : std::numeric_limits<float>::quiet_NaN();
+    const float eight[8] = {v, v, v, v, v, v, v, v};
+    const int pieces = wide / 8, all = (at.end - at.begin) * pieces;
+#pragma unroll 4
+    for (int e = threadIdx.x; e < all; e += blockDim.x) {
+        const int row = p.order[at.begin + e / pieces], col = col0 + e % pieces * 8;
+        if (col < p.cols) store_run<8>(static_cast<T*>(p.out) + row * p.out_stride + col, p.cols - col, eight);
     }
 }
 
@@ -697,6 +701,14 @@ __global__ __launch_bounds__(256, 2) void k_staged(const Product p)
 #pragma unroll
         for (int t = 0; t < NT; ++t) acc[i][t] = f32x4{0, 0, 0, 0};
     const int wm = wave / 2, wn = wave % 2;
+    // db: the sums of dy alone, as one column more whose numbers are ones, of the first column of tiles
+    const bool with_sums = MODE == WEIGHTS && p.sums && ct == 0 && wn == 0;
+    f32x4 ones_acc[MODE == WEIGHTS ? NM : 1];
+    frag ones;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) ones[j] = 1.0f;
+#pragma unroll
+    for (int i = 0; i < (MODE == WEIGHTS ? NM : 1); ++i) ones_acc[i] = f32x4{0, 0, 0, 0};
     const unsigned lds0 = lds_address(lds);
     const Reader<frag, STEP, BM, A_ACROSS> read_a(lds0, wm * NM, lane);
     const Reader<frag, STEP, BN, B_ACROSS> read_b(lds0 + PARTS * A_PART, wn * NT, lane);
@@ -708,6 +720,12 @@ __global__ __launch_bounds__(256, 2) void k_staged(const Product p)
             for (int i = 0; i < NM; ++i)
 #pragma unroll
                 for (int q = 0; q < PARTS; ++q) x[i][q] = read_a.get(i, h, q * A_PART);
+            if (MODE == WEIGHTS && with_sums) {
+#pragma unroll
+                for (int q = PARTS - 1; q >= 0; --q)
+#pragma unroll
+                    for (int i = 0; i < NM; ++i) ones_acc[i] = mma(ones, x[i][q], ones_acc[i]);
+            }
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 frag w[PARTS];
@@ -800,10 +818,27 @@ __global__ __launch_bounds__(256, 2) void k_staged(const Product p)
                     }
         }
     }
+    if (MODE == WEIGHTS && with_sums && lane < 16) {
+#pragma unroll
+        for (int i = 0; i < NM; ++i) {
+            const int m = row_w + 16 * i + lane;
+            if (m >= p.m) continue;
+            float sum = ones_acc[MODE == WEIGHTS ? i : 0][0];
+            if (SINGLE) {
+                if (fabsf(sum) <= std::numeric_limits<float>::max()) sum *= 1.0f / kSplitScale;
+                else {
+                    sum = 0.0f;
+                    for (int k = at.begin; k < at.end; ++k) sum += (float)static_cast<const T*>(p.a)[p.order[k] * p.a_stride + m];
+                }
+            }
+            if (at.slot >= 0) p.partial_sums[(long)at.slot * p.m + m] = sum;
+            else static_cast<T*>(p.sums)[(long)at.group * p.m + m] = (T)sum;
+        }
+    }
     finish<T, MODE, NM, NT>(p, at, lane, row_w, col_w, look, acc);
 }
 
-// Sums of the pieces of a group's dW, in order.
+// Sums of the pieces of a group's dW and db, in order.
 template <typename T>
 __global__ __launch_bounds__(256) void k_join(const Product p)
 {
@@ -831,6 +866,12 @@ __global__ __launch_bounds__(256) void k_join(const Product p)
         }
         store_run<4>(static_cast<T*>(p.out) + g * each + e, each - e, sum);
     }
+    if (p.sums)
+        for (int m = blockIdx.x * 256 + threadIdx.x; m < p.m; m += gridDim.x * 256) {
+            float sum = 0.0f;
+            for (int i = 0; i < pieces; ++i) sum += p.partial_sums[(long)(slots + i) * p.m + m];
+            static_cast<T*>(p.sums)[(long)g * p.m + m] = (T)sum;
+        }
 }
 
 // ---- few rows: bound by the weights' bytes
@@ -995,16 +1036,24 @@ struct Call : Launches {
             q.col_tiles = (q.cols + wide - 1) / wide;
             return row_tiles(high) * q.col_tiles;
         };
+        // The largest tiles that are enough for three quarters of the CUs, that columns fill by three quarters, and groups of the usual size too.
+        // (In bfloat16, 16 384 rows of 4 groups, 1 024 columns: 128 terms 14.9 us and 15.6 in tiles of 128, 1 024 terms 34 and 44.  63 855 rows of
+        // 15 groups, 96 -> 32: tiles of 256 20 us.)
+        const long used = std::min(p.rows, std::max(1L, (long)p.num_groups));
+        auto fits = [&](int tile) {
+            const long across = (q.cols + tile - 1) / tile;
+            return p.rows / tile * across >= 192 && 4L * q.cols >= 3 * across * tile && p.rows >= used * tile;
+        };
         if constexpr (!std::is_same_v<T, float>) {
             if (direct_ok) {
-                if (p.rows / 256 * ((q.cols + 255) / 256) >= 192) direct<T, MODE, true, 256, 2>(q, tiles(256, 256));
-                else if (p.rows / 128 * ((q.cols + 127) / 128) >= 192) direct<T, MODE, false, 128, 2>(q, tiles(128, 128));
+                if (fits(256)) direct<T, MODE, true, 256, 2>(q, tiles(256, 256));
+                else if (fits(128)) direct<T, MODE, false, 128, 2>(q, tiles(128, 128));
                 else if (tiles(64, 64) > kCUs) direct<T, MODE, false, 64, 3>(q, tiles(64, 64));
                 else direct<T, MODE, false, 64, 8>(q, tiles(64, 64));
                 return;
             }
         }
-        if (p.rows / 128 * ((q.cols + 127) / 128) >= 192) start(k_staged<T, MODE, 128, 128, (std::is_same_v<T, float> ? 2 : 1)>, up(tiles(128, 128), 8), 1, 1, 256, 0, q);
+        if (fits(128)) start(k_staged<T, MODE, 128, 128, (std::is_same_v<T, float> ? 2 : 1)>, up(tiles(128, 128), 8), 1, 1, 256, 0, q);
         else start(k_staged<T, MODE, 64, 64, (std::is_same_v<T, float> ? 4 : 2)>, up(tiles(64, 64), 8), 1, 1, 256, 0, q);
     }
     template <typename T>
@@ -1034,11 +1083,12 @@ struct Call : Launches {
             q.b = W; q.b_each = p.weight_each; q.b_stride = p.weight_stride; q.k = p.d_out; q.cols = p.d_in; q.out = dx; q.out_stride = dx_stride;
             rows<T, ROWS>(q, dy_ok && in_pieces(W, p.weight_stride, p.d_in) && p.weight_each % 8 == 0);
         }
+        bool summed = false;      // (db)
         if (dW && p.num_groups) {
             q.b = x; q.b_each = 0; q.b_stride = p.x_stride; q.m = p.d_out; q.cols = p.d_in; q.out = dW;
-            weights<T>(q, dy_ok && in_pieces(x, p.x_stride, p.d_in) && within_reach(p.rows, p.x_stride));
+            summed = weights<T>(q, db, dy_ok && in_pieces(x, p.x_stride, p.d_in) && within_reach(p.rows, p.x_stride));
         }
-        if (db && p.num_groups) add_rows(*this, arena, p.type, dy, dy_stride, p.index, p.rows, p.num_groups, p.d_out, groups, 1.0f, db);
+        if (db && p.num_groups && (dry || !summed)) add_rows(*this, arena, p.type, dy, dy_stride, p.index, p.rows, p.num_groups, p.d_out, groups, 1.0f, db);
     }
     // dW: which tiles, and how long the pieces of a group's rows are.  Small tiles and short pieces keep more CUs busy; large tiles
     // take fewer bytes for a product, and pieces have to be written and read again to be joined.  What each way takes is estimated from
@@ -1071,8 +1121,9 @@ struct Call : Launches {
         }
         return best;
     }
+    // The answer is whether db is there too.
     template <typename T>
-    void weights(Product q, bool direct_ok)
+    bool weights(Product q, T* db, bool direct_ok)
     {
         constexpr bool SINGLE = std::is_same_v<T, float>;
         const Way w = way(q.m, q.cols, direct_ok, SINGLE);
@@ -1081,23 +1132,27 @@ struct Call : Launches {
         q.piece = w.piece;
         const long each = (long)q.row_tiles * q.col_tiles, items = p.rows / q.piece + p.num_groups, slots = 2 * (p.rows / q.piece);
         q.partial = arena.take<float>(slots * q.m * q.cols);
+        const bool summed = SINGLE || !direct_ok;
+        if (summed) {
+            q.sums = db;
+            q.partial_sums = arena.take<float>(slots * q.m);
+        }
         const long blocks = items * (each >= 8 ? up(each, 8) : each);
-        bool done = false;
         if constexpr (!SINGLE) {
             if (direct_ok) {
                 if (w.tile == 256) direct<T, WEIGHTS, true, 256, 2>(q, blocks);
                 else if (w.tile == 128) direct<T, WEIGHTS, false, 128, 2>(q, blocks);
                 else if (blocks > kCUs) direct<T, WEIGHTS, false, 64, 3>(q, blocks);
                 else direct<T, WEIGHTS, false, 64, 8>(q, blocks);
-                done = true;
             }
         }
-        if (!done) {
+        if (summed) {
             if (w.tile == 128) start(k_staged<T, WEIGHTS, 128, 128, (std::is_same_v<T, float> ? 2 : 1)>, blocks, 1, 1, 256, 0, q);
             else start(k_staged<T, WEIGHTS, 64, 64, (std::is_same_v<T, float> ? 4 : 2)>, blocks, 1, 1, 256, 0, q);
         }
         // (few blocks: most groups have nothing to join)
         if (slots) start(k_join<T>, std::min(((long)q.m * q.cols + 1023) / 1024, std::max(1L, 2048L / p.num_groups)), p.num_groups, 1, 256, 0, q);
+        return summed;
     }
 };
 

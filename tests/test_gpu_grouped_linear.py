@@ -243,8 +243,13 @@ def test_parts_that_are_asked_for(dtype):
     data, dy = _data(700, 96, 64, 5, NAMES[dtype])
     every = finetune.grouped_linear_backward(dy, data["x"], data["weight"], data["index"])
     for need in ((True, False, False), (False, True, False), (False, False, True), (True, False, True), (False, False, False)):
-        for got, want, asked in zip(finetune.grouped_linear_backward(dy, data["x"], data["weight"], data["index"], need), every, need):
-            assert (got is None) if not asked else torch.equal(got, want)
+        for k, got, want, asked in zip(range(3), finetune.grouped_linear_backward(dy, data["x"], data["weight"], data["index"], need), every, need):
+            if not asked:
+                assert got is None
+            elif k == 2 and not need[1]:          # (alone, and beside the weights' gradient: sums in another order)
+                _close(got, *_reference(**data, dy=dy)["dbias"], NAMES[dtype])
+            else:
+                assert torch.equal(got, want)
 
 
 @pytest.mark.gpu
