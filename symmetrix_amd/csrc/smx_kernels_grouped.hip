@@ -33,7 +33,7 @@ struct Product {
     int row_tiles, col_tiles;  // row_tiles: of WEIGHTS
     int piece;                 // of WEIGHTS: rows of a group that a block sums at most
     float* partial;            // sums of groups of more than one piece [slot][m][cols]
-    void* sums;                // of WEIGHTS by way of registers: db [group][m], or null
+    void* sums;                // of WEIGHTS in single precision: db [group][m], or null
     float* partial_sums;       // its parts [slot][m]
 };
 
@@ -593,12 +593,13 @@ __device__ __forceinline__ float plain_sum(const Product& p, const Place& at, in
     return sum;
 }
 
-// Steps of 32 terms in single precision, of 64 in 16 bits (whose sums are short); those of the next AHEAD are on their way to registers during the sums of one.  Four wavefronts, 2 x 2.
+// Steps of 32 terms, or of 64 where a step's sums are short (in 16 bits; not of WEIGHTS, whose registers they would take); those of the next AHEAD
+// are on their way to registers during the sums of one.  Four wavefronts, 2 x 2.
 template <typename T, int MODE, int BM, int BN, int AHEAD>
 __global__ __launch_bounds__(256, 2) void k_staged(const Product p)
 {
     constexpr bool SINGLE = std::is_same_v<T, float>, A_ACROSS = MODE == WEIGHTS, B_ACROSS = MODE != FORWARD;
-    constexpr int PARTS = SINGLE ? 3 : 1, STEP = SINGLE ? 32 : 64, PIECES = STEP / 8, NM = BM / 32, NT = BN / 32, PA = BM * PIECES / 256, PB = BN * PIECES / 256;
+    constexpr int PARTS = SINGLE ? 3 : 1, STEP = SINGLE || MODE == WEIGHTS ? 32 : 64, PIECES = STEP / 8, NM = BM / 32, NT = BN / 32, PA = BM * PIECES / 256, PB = BN * PIECES / 256;
     constexpr int A_PART = BM * STEP * 2, B_PART = BN * STEP * 2;
     typedef typename std::conditional_t<SINGLE, Operand<bf16>, Operand<T>>::type frag;
     __shared__ __align__(1024) unsigned char lds[PARTS * (A_PART + B_PART)];
@@ -701,14 +702,16 @@ __global__ __launch_bounds__(256, 2) void k_staged(const Product p)
 #pragma unroll
         for (int t = 0; t < NT; ++t) acc[i][t] = f32x4{0, 0, 0, 0};
     const int wm = wave / 2, wn = wave % 2;
-    // db: the sums of dy alone, as one column more whose numbers are ones, of the first column of tiles
-    const bool with_sums = MODE == WEIGHTS && p.sums && ct == 0 && wn == 0;
-    f32x4 ones_acc[MODE == WEIGHTS ? NM : 1];
+    // db: the sums of dy alone, as one column more whose numbers are ones, of the first column of tiles.  (Not in 16 bits: 8 000 rows, 1 025 -> 2 049
+    // in bfloat16: 105 us, and 135 with their registers.)
+    constexpr bool SUMS = SINGLE && MODE == WEIGHTS;
+    const bool with_sums = SUMS && p.sums && ct == 0 && wn == 0;
+    f32x4 ones_acc[SUMS ? NM : 1];
     frag ones;
 #pragma unroll
     for (int j = 0; j < 8; ++j) ones[j] = 1.0f;
 #pragma unroll
-    for (int i = 0; i < (MODE == WEIGHTS ? NM : 1); ++i) ones_acc[i] = f32x4{0, 0, 0, 0};
+    for (int i = 0; i < (SUMS ? NM : 1); ++i) ones_acc[i] = f32x4{0, 0, 0, 0};
     const unsigned lds0 = lds_address(lds);
     const Reader<frag, STEP, BM, A_ACROSS> read_a(lds0, wm * NM, lane);
     const Reader<frag, STEP, BN, B_ACROSS> read_b(lds0 + PARTS * A_PART, wn * NT, lane);
@@ -720,11 +723,11 @@ __global__ __launch_bounds__(256, 2) void k_staged(const Product p)
             for (int i = 0; i < NM; ++i)
 #pragma unroll
                 for (int q = 0; q < PARTS; ++q) x[i][q] = read_a.get(i, h, q * A_PART);
-            if (MODE == WEIGHTS && with_sums) {
+            if (SUMS && with_sums) {
 #pragma unroll
                 for (int q = PARTS - 1; q >= 0; --q)
 #pragma unroll
-                    for (int i = 0; i < NM; ++i) ones_acc[i] = mma(ones, x[i][q], ones_acc[i]);
+                    for (int i = 0; i < NM; ++i) ones_acc[SUMS ? i : 0] = mma(ones, x[i][q], ones_acc[SUMS ? i : 0]);
             }
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
@@ -818,18 +821,16 @@ __global__ __launch_bounds__(256, 2) void k_staged(const Product p)
                     }
         }
     }
-    if (MODE == WEIGHTS && with_sums && lane < 16) {
+    if (SUMS && with_sums && lane < 16) {
 #pragma unroll
         for (int i = 0; i < NM; ++i) {
             const int m = row_w + 16 * i + lane;
             if (m >= p.m) continue;
-            float sum = ones_acc[MODE == WEIGHTS ? i : 0][0];
-            if (SINGLE) {
-                if (fabsf(sum) <= std::numeric_limits<float>::max()) sum *= 1.0f / kSplitScale;
-                else {
-                    sum = 0.0f;
-                    for (int k = at.begin; k < at.end; ++k) sum += (float)static_cast<const T*>(p.a)[p.order[k] * p.a_stride + m];
-                }
+            float sum = ones_acc[SUMS ? i : 0][0];
+            if (fabsf(sum) <= std::numeric_limits<float>::max()) sum *= 1.0f / kSplitScale;
+            else {
+                sum = 0.0f;
+                for (int k = at.begin; k < at.end; ++k) sum += (float)static_cast<const T*>(p.a)[p.order[k] * p.a_stride + m];
             }
             if (at.slot >= 0) p.partial_sums[(long)at.slot * p.m + m] = sum;
             else static_cast<T*>(p.sums)[(long)at.group * p.m + m] = (T)sum;
@@ -869,6 +870,7 @@ __global__ __launch_bounds__(256) void k_join(const Product p)
     if (p.sums)
         for (int m = blockIdx.x * 256 + threadIdx.x; m < p.m; m += gridDim.x * 256) {
             float sum = 0.0f;
+#pragma unroll 8
             for (int i = 0; i < pieces; ++i) sum += p.partial_sums[(long)(slots + i) * p.m + m];
             static_cast<T*>(p.sums)[(long)g * p.m + m] = (T)sum;
         }
@@ -1132,8 +1134,7 @@ struct Call : Launches {
         q.piece = w.piece;
         const long each = (long)q.row_tiles * q.col_tiles, items = p.rows / q.piece + p.num_groups, slots = 2 * (p.rows / q.piece);
         q.partial = arena.take<float>(slots * q.m * q.cols);
-        const bool summed = SINGLE || !direct_ok;
-        if (summed) {
+        if (SINGLE) {
             q.sums = db;
             q.partial_sums = arena.take<float>(slots * q.m);
         }
@@ -1146,13 +1147,13 @@ struct Call : Launches {
                 else direct<T, WEIGHTS, false, 64, 8>(q, blocks);
             }
         }
-        if (summed) {
+        if (SINGLE || !direct_ok) {
             if (w.tile == 128) start(k_staged<T, WEIGHTS, 128, 128, (std::is_same_v<T, float> ? 2 : 1)>, blocks, 1, 1, 256, 0, q);
             else start(k_staged<T, WEIGHTS, 64, 64, (std::is_same_v<T, float> ? 4 : 2)>, blocks, 1, 1, 256, 0, q);
         }
         // (few blocks: most groups have nothing to join)
         if (slots) start(k_join<T>, std::min(((long)q.m * q.cols + 1023) / 1024, std::max(1L, 2048L / p.num_groups)), p.num_groups, 1, 256, 0, q);
-        return summed;
+        return SINGLE;
     }
 };
 
