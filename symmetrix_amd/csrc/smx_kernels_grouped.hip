@@ -33,7 +33,7 @@ struct Product {
     int row_tiles, col_tiles;  // row_tiles: of WEIGHTS
     int piece;                 // of WEIGHTS: rows of a group that a block sums at most
     float* partial;            // sums of groups of more than one piece [slot][m][cols]
-    void* sums;                // of WEIGHTS in single precision: db [group][m], or null
+    void* sums;                // of WEIGHTS: db [group][m], or null
     float* partial_sums;       // its parts [slot][m]
 };
 
@@ -269,6 +269,13 @@ __device__ __forceinline__ void finish(const Product& p, const Place& at, int la
     }
 }
 
+template <typename T>
+__device__ __forceinline__ void store_sum(const Product& p, const Place& at, int m, float sum)      // of db
+{
+    if (at.slot >= 0) p.partial_sums[(long)at.slot * p.m + m] = sum;
+    else static_cast<T*>(p.sums)[(long)at.group * p.m + m] = (T)sum;
+}
+
 // ---- operands in LDS
 //
 // Steps of K terms (64 for 16-bit types as they are, 32 for single precision in parts); an operand has `wide` rows or columns of C.  It lies
@@ -434,6 +441,28 @@ __device__ __forceinline__ void direct_tile(const Product& p, const Place& at, i
 #pragma unroll
             for (int t = 0; t < NT; ++t) acc[i][t] = mma(now.w[t], now.x[i], acc[i][t]);
     };
+    // db: the sums of dy alone, as one column more whose numbers are ones, of the first column of tiles; the wavefronts that have the same rows
+    // of A share them.  (Of small tiles: 12 731 rows, 192 -> 224, 47 groups in bfloat16: 28 us with a launch for db, 16.  Larger ones have no registers
+    // for it: 16 384 rows, 4 096 -> 2 048: 305 us without, 532.)
+    constexpr bool SUMS = MODE == WEIGHTS && BM == 64;
+    constexpr int OWN = NM / WN;
+    const bool with_sums = SUMS && p.sums && col0 == 0;
+    f32x4 ones_acc[SUMS ? OWN : 1];
+#pragma unroll
+    for (int o = 0; o < (SUMS ? OWN : 1); ++o) ones_acc[o] = f32x4{0, 0, 0, 0};
+    auto add_sums = [&](const Frags& now) {
+        if constexpr (SUMS) {
+            if (!with_sums) return;
+            frag ones;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) ones[j] = (T)1.0f;
+#pragma unroll
+            for (int w = 0; w < WN; ++w)
+                if (wn == w)
+#pragma unroll
+                    for (int o = 0; o < OWN; ++o) ones_acc[o] = mma(ones, now.x[w * OWN + o], ones_acc[o]);
+        }
+    };
     auto woven = [&] {      // sums and the fetches beside them, by turns
         constexpr int READS = NM * (A_ACROSS ? 2 : 1) + NT * (B_ACROSS ? 2 : 1), EACH = NM * NT / READS;
         if constexpr (EACH >= 1) {
@@ -483,6 +512,7 @@ __device__ __forceinline__ void direct_tile(const Product& p, const Place& at, i
             fetch(s, 1, f[1]);
             sums(f[0]);
             woven();
+            add_sums(f[0]);
             wait_loads<(STAGES - 2) * PER>();
             barrier_only();      // the next tiles are there, and everybody has read these
             look_up(s + STAGES + 1);
@@ -490,11 +520,13 @@ __device__ __forceinline__ void direct_tile(const Product& p, const Place& at, i
             fetch(s + 1, 0, f[0]);
             sums(f[1]);
             woven();
+            add_sums(f[1]);
         }
 #pragma unroll 1
         for (; s < stages; ++s) {      // the last request, and none
             fetch(s, 1, f[1]);
             sums(f[0]);
+            add_sums(f[0]);
             if (s + 1 < stages) {
                 wait_loads<0>();
                 barrier_only();
@@ -502,8 +534,15 @@ __device__ __forceinline__ void direct_tile(const Product& p, const Place& at, i
                 fetch(s + 1, 0, f[0]);
             }
             sums(f[1]);
+            add_sums(f[1]);
         }
     }
+    if (SUMS && with_sums && lane < 16)
+#pragma unroll
+        for (int o = 0; o < OWN; ++o) {
+            const int m = row0 + (wm * NM + wn * OWN + o) * 16 + lane;
+            if (m < p.m) store_sum<T>(p, at, m, ones_acc[SUMS ? o : 0][0]);
+        }
     finish<T, MODE, NM, NT>(p, at, lane, row0 + wm * NM * 16, col0 + wn * NT * 16, tile_rows, acc);
 }
 
@@ -702,9 +741,8 @@ __global__ __launch_bounds__(256, 2) void k_staged(const Product p)
 #pragma unroll
         for (int t = 0; t < NT; ++t) acc[i][t] = f32x4{0, 0, 0, 0};
     const int wm = wave / 2, wn = wave % 2;
-    // db: the sums of dy alone, as one column more whose numbers are ones, of the first column of tiles.  (Not in 16 bits: 8 000 rows, 1 025 -> 2 049
-    // in bfloat16: 105 us, and 135 with their registers.)
-    constexpr bool SUMS = SINGLE && MODE == WEIGHTS;
+    // db: the sums of dy alone, as one column more whose numbers are ones, of the first column of tiles
+    constexpr bool SUMS = MODE == WEIGHTS;
     const bool with_sums = SUMS && p.sums && ct == 0 && wn == 0;
     f32x4 ones_acc[SUMS ? NM : 1];
     frag ones;
@@ -827,13 +865,14 @@ __global__ __launch_bounds__(256, 2) void k_staged(const Product p)
             const int m = row_w + 16 * i + lane;
             if (m >= p.m) continue;
             float sum = ones_acc[SUMS ? i : 0][0];
-            if (fabsf(sum) <= std::numeric_limits<float>::max()) sum *= 1.0f / kSplitScale;
-            else {
-                sum = 0.0f;
-                for (int k = at.begin; k < at.end; ++k) sum += (float)static_cast<const T*>(p.a)[p.order[k] * p.a_stride + m];
+            if (SINGLE) {
+                if (fabsf(sum) <= std::numeric_limits<float>::max()) sum *= 1.0f / kSplitScale;
+                else {
+                    sum = 0.0f;
+                    for (int k = at.begin; k < at.end; ++k) sum += (float)static_cast<const T*>(p.a)[p.order[k] * p.a_stride + m];
+                }
             }
-            if (at.slot >= 0) p.partial_sums[(long)at.slot * p.m + m] = sum;
-            else static_cast<T*>(p.sums)[(long)at.group * p.m + m] = (T)sum;
+            store_sum<T>(p, at, m, sum);
         }
     }
     finish<T, MODE, NM, NT>(p, at, lane, row_w, col_w, look, acc);
@@ -1123,7 +1162,7 @@ struct Call : Launches {
         }
         return best;
     }
-    // The answer is whether db is there too.
+    // The answer is whether db is there too, if it is asked for.
     template <typename T>
     bool weights(Product q, T* db, bool direct_ok)
     {
@@ -1134,7 +1173,8 @@ struct Call : Launches {
         q.piece = w.piece;
         const long each = (long)q.row_tiles * q.col_tiles, items = p.rows / q.piece + p.num_groups, slots = 2 * (p.rows / q.piece);
         q.partial = arena.take<float>(slots * q.m * q.cols);
-        if (SINGLE) {
+        const bool summed = SINGLE || !direct_ok || w.tile == 64;
+        if (summed) {
             q.sums = db;
             q.partial_sums = arena.take<float>(slots * q.m);
         }
@@ -1153,7 +1193,7 @@ struct Call : Launches {
         }
         // (few blocks: most groups have nothing to join)
         if (slots) start(k_join<T>, std::min(((long)q.m * q.cols + 1023) / 1024, std::max(1L, 2048L / p.num_groups)), p.num_groups, 1, 256, 0, q);
-        return SINGLE;
+        return summed;
     }
 };
 
