@@ -548,22 +548,36 @@ def _grad_tensors(count):
 
 def _describe_grads(grads, outs=None):
     """The descriptions of tensors that are there (not None), their device, how many, and what has to live until the call is made."""
-    numbers, keep, device = [], [], None
-    for k, g in enumerate(grads):
+    numbers, keep, device, types = [], [], None, _TYPES
+    for g, o in zip(grads, outs or grads):
         if g is None:
             continue
-        kind = _TYPES.get(g.dtype)
+        dtype = g.dtype
+        kind = types.get(dtype)
         if kind is None:
             _type(g, "gradients")
-        at = g.get_device()
+        at, n = g.get_device(), g.numel()
         if at != device:
             if device is not None:
                 raise ValueError("gradients on one device expected")
             device = _on(g)
+        to = 0
+        if outs is not None and o is not g:
+            if o is None:
+                raise ValueError("out: a tensor for every gradient expected")
+            if o.dtype is not dtype:
+                raise TypeError("out: the types of the gradients expected")
+            if o.get_device() != at or o.shape != g.shape or not o.is_contiguous():
+                raise ValueError("out: contiguous, of the gradients' shapes and on their device, expected")
+            to = o.data_ptr()
         if not g.is_contiguous():
             g = g.contiguous()
             keep.append(g)
-        numbers += (kind, g.data_ptr(), 0 if outs is None else outs[k].data_ptr(), g.numel())
+        from_ = g.data_ptr()
+        numbers += (kind, from_, to or from_, n)
+    if outs is not None:
+        starts = [to for to, n in zip(numbers[2::4], numbers[3::4]) if n]
+        _need(len(set(starts)) == len(starts), "tensors that are written: every one once expected, each with memory of its own")
     count = len(numbers) // 4
     return _grad_tensors(count).pack(*numbers), device, count, keep
 
@@ -598,26 +612,18 @@ def clip_grads(grads, max_norm, out=None):
     grads, each with memory of its own), and returns the norm that they had.  Where the norm is not finite they stay as they are."""
     grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
     _need(max_norm >= 0, "max_norm: a number from 0 on")
-    back = []          # gradients that are clipped in a contiguous copy
+    back, there = [], grads          # gradients that are clipped in a contiguous copy, and tensors that are written
     if out is None:
-        there = [g for g in grads if g is not None]
+        out = list(grads)
         for k, g in enumerate(grads):
             if g is not None and not g.is_contiguous():
-                grads[k] = g.contiguous()
-                back.append((g, grads[k]))
-        out = grads
+                out[k] = g.contiguous()
+                back.append((g, out[k]))
+        if back:
+            grads = out
     else:
-        out = [out] if isinstance(out, torch.Tensor) else list(out)
+        there = out = [out] if isinstance(out, torch.Tensor) else list(out)
         _need(len(out) == len(grads), "out: a tensor for every gradient expected")
-        there = [o for g, o in zip(grads, out) if g is not None]
-        for g, o in zip(grads, out):
-            if g is not None:
-                _need(o is not None, "out: a tensor for every gradient expected")
-                if o.dtype != g.dtype:
-                    raise TypeError("out: the types of the gradients expected")
-                _need(o.shape == g.shape and o.is_contiguous() and o.get_device() == g.get_device(), "out: contiguous, of the gradients' shapes and on their device, expected")
-    starts = [o.data_ptr() for g, o in zip(grads, out) if g is not None and o.numel()]
-    _need(len(set(starts)) == len(starts), "tensors that are written: every one once expected, each with memory of its own")
     described = _describe_grads(grads, out)
     if not described[2]:
         return torch.zeros((), device="cuda")
@@ -625,7 +631,7 @@ def clip_grads(grads, max_norm, out=None):
     for g, copy in back:
         g.copy_(copy)
     # (as torch's own operations in place do)
-    torch.autograd.graph.increment_version(there)
+    torch.autograd.graph.increment_version([o for o, g in zip(there, grads) if g is not None])
     return norm
 
 
