@@ -42,7 +42,8 @@ struct Place {
     int group, begin, end, slot;
 };
 // Items are cut from the groups in order, `high` rows each; with ALL a group without rows has one too, and the last two groups (rows
-// without a group) have none.  A wavefront works out for itself where they are, 64 groups at a time, a lane each.
+// without a group) have none.  Every block works out for itself where they are: of up to 62 groups every wavefront, a lane a group; of more
+// the block, a thread some neighbouring groups (20 000 rows of 1 024 groups, 256 x 256 in bfloat16: 43 us; every wavefront 64 groups at a time: 98).
 __device__ __forceinline__ int wave_inclusive(int x, int lane)
 {
 #pragma unroll
@@ -54,63 +55,109 @@ __device__ __forceinline__ int wave_inclusive(int x, int lane)
 }
 template <bool ALL>
 struct Items {
-    int first, count, n;      // of the lane's group: where its rows begin, how many they are, and its items
-    int until;                // items up to its last
-    __device__ __forceinline__ Items(const Product& p, int g0, int high, int lane)
+    const Product& p;
+    const int high, lane;
+    int first = 0, count = -1, n = 0;      // of the lane's group: where its rows begin, how many they are, and its items
+    int until;                             // items up to the lane's, or thread's, last
+    int slots_until;                       // and of groups of several
+    int total;                             // all items
+    __device__ __forceinline__ bool few() const { return p.groups + 2 <= 64; }
+    __device__ __forceinline__ int rows_of(int g, int& begin) const
     {
-        const int g = g0 + lane, groups = p.groups + (ALL ? 0 : 2);
-        first = p.offsets[min(g, p.groups + 1)];
+        begin = p.offsets[min(g, p.groups + 1)];
         const int end = g >= p.groups + 1 ? (int)p.rows : p.offsets[min(g, p.groups) + 1];
-        count = g < groups ? end - first : -1;
-        n = count < 0 ? 0 : max((count + high - 1) / high, ALL ? 1 : 0);
-        until = wave_inclusive(n, lane);
+        return g < p.groups + (ALL ? 0 : 2) ? end - begin : -1;
     }
-    __device__ __forceinline__ int all() const { return __builtin_amdgcn_readlane(until, 63); }
-};
-// The number of items; here: those of the first 64 groups.
-template <bool ALL>
-__device__ __forceinline__ int count_items(const Product& p, const Items<ALL>& here, int high, int lane)
-{
-    int total = here.all();
-    for (int g0 = 64; g0 < p.groups + 2; g0 += 64) total += Items<ALL>(p, g0, high, lane).all();
-    return total;
-}
-template <bool ALL>
-__device__ __forceinline__ Place find_item(const Product& p, Items<ALL> here, int item, int high, int lane)
-{
-    Place at{-1, 0, 0, -1};
-    int slots = 0;
-    for (int g0 = 0;;) {
-        const int slots_until = ALL ? wave_inclusive(here.n > 1 ? here.n : 0, lane) : 0;
-        // Sums over rows: the groups with the most rows first, as far as a wavefront sees them at once, so that the last items are short.
-        int group = lane, until = here.until;
-        if (ALL && p.groups <= 64) {
-            int rank = 0;
-#pragma unroll 8
-            for (int h = 0; h < p.groups; ++h) {
-                const int other = __builtin_amdgcn_readlane(here.count, h);
-                rank += other > here.count || (other == here.count && h < lane) ? 1 : 0;
-            }
-            if (lane >= p.groups) rank = lane;
-            group = __builtin_amdgcn_ds_permute(rank * 4, lane);
-            until = wave_inclusive(__builtin_amdgcn_ds_permute(rank * 4, here.n), lane);
+    __device__ __forceinline__ int items_of(int rows) const { return rows < 0 ? 0 : max((rows + high - 1) / high, ALL ? 1 : 0); }
+    __device__ __forceinline__ int per_thread() const { return (p.groups + 2 + (int)blockDim.x - 1) / (int)blockDim.x; }
+    // (part: two numbers a wavefront)
+    __device__ __forceinline__ Items(const Product& p_, int high_, int lane_, int (*part)[2]) : p(p_), high(high_), lane(lane_)
+    {
+        if (few()) {
+            count = rows_of(lane, first);
+            n = items_of(count);
+            until = wave_inclusive(n, lane);
+            slots_until = ALL ? wave_inclusive(n > 1 ? n : 0, lane) : 0;
+            total = __builtin_amdgcn_readlane(until, 63);
+            return;
         }
-        const unsigned long behind = __ballot(until > item);
-        if (behind) {
-            const int where = __builtin_ctzl(behind), from = __builtin_amdgcn_readlane(group, where), pieces = __builtin_amdgcn_readlane(here.n, from);
-            const int mine = item - (__builtin_amdgcn_readlane(until, where) - pieces), first = __builtin_amdgcn_readlane(here.first, from);
-            at.group = g0 + from;
-            at.begin = first + mine * high;
-            at.end = min(first + __builtin_amdgcn_readlane(here.count, from), at.begin + high);
-            if (ALL && pieces > 1) at.slot = slots + __builtin_amdgcn_readlane(slots_until, from) - pieces + mine;
+        int slots = 0;
+        const int g0 = threadIdx.x * per_thread(), wave = threadIdx.x >> 6;
+#pragma unroll 4
+        for (int g = g0; g < g0 + per_thread(); ++g) {
+            int begin;
+            const int k = items_of(rows_of(g, begin));
+            n += k;
+            slots += ALL && k > 1 ? k : 0;
+        }
+        until = wave_inclusive(n, lane);
+        slots_until = wave_inclusive(slots, lane);
+        if (lane == 63) {
+            part[wave][0] = until;
+            part[wave][1] = slots_until;
+        }
+        __syncthreads();
+        total = 0;
+        int before = 0, slots_before = 0;
+        for (int w = 0; w < (int)(blockDim.x >> 6); ++w) {
+            before += w < wave ? part[w][0] : 0;
+            slots_before += w < wave ? part[w][1] : 0;
+            total += part[w][0];
+        }
+        until += before;
+        slots_until += slots_before;
+        total = __builtin_amdgcn_readfirstlane(total);
+        count = slots;
+    }
+    __device__ __forceinline__ Place find(int item, Place* found) const
+    {
+        Place at{-1, 0, 0, -1};
+        if (few()) {
+            // Sums over rows: the groups with the most rows first, so that the last items are short.
+            int group = lane, last = until;
+            if (ALL) {
+                int rank = 0;
+#pragma unroll 8
+                for (int h = 0; h < p.groups; ++h) {
+                    const int other = __builtin_amdgcn_readlane(count, h);
+                    rank += other > count || (other == count && h < lane) ? 1 : 0;
+                }
+                if (lane >= p.groups) rank = lane;
+                group = __builtin_amdgcn_ds_permute(rank * 4, lane);
+                last = wave_inclusive(__builtin_amdgcn_ds_permute(rank * 4, n), lane);
+            }
+            const unsigned long behind = __ballot(last > item);
+            const int where = __builtin_ctzl(behind), from = __builtin_amdgcn_readlane(group, where), pieces = __builtin_amdgcn_readlane(n, from);
+            const int mine = item - (__builtin_amdgcn_readlane(last, where) - pieces), begin = __builtin_amdgcn_readlane(first, from);
+            at.group = from;
+            at.begin = begin + mine * high;
+            at.end = min(begin + __builtin_amdgcn_readlane(count, from), at.begin + high);
+            if (ALL && pieces > 1) at.slot = __builtin_amdgcn_readlane(slots_until, from) - pieces + mine;
             return at;
         }
-        item -= here.all();
-        slots += ALL ? __builtin_amdgcn_readlane(slots_until, 63) : 0;
-        if ((g0 += 64) >= p.groups + 2) return at;
-        here = Items<ALL>(p, g0, high, lane);
+        if (item < until && item >= until - n) {      // (one thread's)
+            int left = item - (until - n), slots = slots_until - count;
+            for (int g = threadIdx.x * per_thread();; ++g) {
+                int begin;
+                const int rows = rows_of(g, begin), k = items_of(rows);
+                if (left < k) {
+                    at.group = g;
+                    at.begin = begin + left * high;
+                    at.end = min(begin + rows, at.begin + high);
+                    if (ALL && k > 1) at.slot = slots + left;
+                    break;
+                }
+                left -= k;
+                slots += ALL && k > 1 ? k : 0;
+            }
+            *found = at;
+        }
+        __syncthreads();
+        at = *found;
+        return Place{__builtin_amdgcn_readfirstlane(at.group), __builtin_amdgcn_readfirstlane(at.begin), __builtin_amdgcn_readfirstlane(at.end),
+                     __builtin_amdgcn_readfirstlane(at.slot)};
     }
-}
+};
 
 // Tiles of a grid, four row tiles high, one below the other: neighbours share operands.
 __device__ __forceinline__ void tile_at(int row_tiles, int col_tiles, int at, int& rt, int& ct)
@@ -126,12 +173,14 @@ constexpr int kCUs = 256;
 template <int MODE, bool CUT>
 __device__ __forceinline__ bool find_tile(const Product& p, int high, int lane, Place& at, int& rt, int& ct, int& parts, int& part)
 {
+    __shared__ int sums[8][2];
+    __shared__ Place found;
     parts = 1;
     part = 0;
+    const Items<MODE == WEIGHTS> items(p, MODE == WEIGHTS ? p.piece : high, lane, sums);
     if constexpr (MODE == WEIGHTS) {
         // (items take different times: every die has a share of each)
-        const Items<true> here(p, 0, p.piece, lane);
-        const int items = count_items(p, here, p.piece, lane), tiles = p.row_tiles * p.col_tiles, share = (tiles + 7) / 8;
+        const int tiles = p.row_tiles * p.col_tiles, share = (tiles + 7) / 8;
         int item, tile;
         if (tiles >= 8) {
             item = (int)(blockIdx.x / 8) / share;
@@ -141,12 +190,11 @@ __device__ __forceinline__ bool find_tile(const Product& p, int high, int lane, 
             item = blockIdx.x / tiles;
             tile = blockIdx.x % tiles;
         }
-        if (item >= items) return false;
-        at = find_item(p, here, item, p.piece, lane);
+        if (item >= items.total) return false;
+        at = items.find(item, &found);
         tile_at(p.row_tiles, p.col_tiles, tile, rt, ct);
     } else {
-        const Items<false> here(p, 0, high, lane);
-        const int row_tiles = count_items(p, here, high, lane), tiles = row_tiles * p.col_tiles;
+        const int row_tiles = items.total, tiles = row_tiles * p.col_tiles;
         const int rest = CUT ? tiles % kCUs : 0, full = CUT ? tiles - rest : tiles;
         int block = blockIdx.x, count = full, first = 0;
         if (CUT && block >= full) {
@@ -159,7 +207,7 @@ __device__ __forceinline__ bool find_tile(const Product& p, int high, int lane, 
         if (id >= count || block / 8 >= per) return false;
         part = id % parts;
         tile_at(row_tiles, p.col_tiles, first + id / parts, rt, ct);
-        at = find_item(p, here, rt, high, lane);
+        at = items.find(rt, &found);
     }
     return true;
 }
@@ -616,18 +664,28 @@ struct Eight {
     }
 };
 
-// A sum in single precision, term by term.
+// Sums of a tile of 16 x 16 in single precision, on its own instructions: row m0 + n and columns c0 + 4 g + 0..3 of lane (n, g).
 template <typename T, int MODE>
-__device__ __forceinline__ float plain_sum(const Product& p, const Place& at, int m, int c)
+__device__ __forceinline__ f32x4 plain_sums(const Product& p, const Place& at, int lane, int m0, int c0)
 {
     const T *a = static_cast<const T*>(p.a), *b = static_cast<const T*>(p.b);
-    float sum = 0.0f;
-    if constexpr (MODE == WEIGHTS) {
-        for (int i = at.begin; i < at.end; ++i) sum = fmaf((float)a[p.order[i] * p.a_stride + m], (float)b[p.order[i] * p.b_stride + c], sum);
-    } else {
+    const int n = lane & 15, g = lane >> 4, count = at.end - at.begin, terms = MODE == WEIGHTS ? count : p.k;
+    const int m = min(m0 + n, (MODE == WEIGHTS ? p.m : count) - 1), c = min(c0 + n, p.cols - 1);
+    if (MODE != WEIGHTS) {
         a += p.order[at.begin + m] * p.a_stride;
         b += at.group * p.b_each + (MODE == FORWARD ? c * p.b_stride : c);
-        for (int k = 0; k < p.k; ++k) sum = fmaf((float)a[k], (float)b[MODE == FORWARD ? (long)k : k * p.b_stride], sum);
+    }
+    f32x4 sum{0, 0, 0, 0};
+#pragma unroll 4
+    for (int k0 = 0; k0 < terms; k0 += 4) {
+        const int k = k0 + g;
+        float u = 0.0f, v = 0.0f;
+        if (k < terms) {
+            const long row = MODE == WEIGHTS ? p.order[at.begin + k] : k;
+            u = (float)(MODE == WEIGHTS ? a[row * p.a_stride + m] : a[k]);
+            v = (float)(MODE == FORWARD ? b[k] : MODE == ROWS ? b[row * p.b_stride] : b[row * p.b_stride + c]);
+        }
+        sum = __builtin_amdgcn_mfma_f32_16x16x4f32(v, u, sum, 0, 0, 0);
     }
     return sum;
 }
@@ -850,13 +908,16 @@ __global__ __launch_bounds__(256, 2) void k_staged(const Product p)
 #pragma unroll
             for (int i = 0; i < NM; ++i)
 #pragma unroll
-                for (int t = 0; t < NT; ++t)
+                for (int t = 0; t < NT; ++t) {
+                    bool all = true;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int m = row_w + 16 * i + (lane & 15), c = col_w + 16 * t + 4 * (lane >> 4) + j;
-                        if (!(fabsf(acc[i][t][j]) <= std::numeric_limits<float>::max()) && m < (MODE == WEIGHTS ? p.m : count) && c < p.cols)
-                            acc[i][t][j] = plain_sum<T, MODE>(p, at, m, c);
-                    }
+                    for (int j = 0; j < 4; ++j) all = all && fabsf(acc[i][t][j]) <= std::numeric_limits<float>::max();
+                    if (__all(all)) continue;
+                    const f32x4 again = plain_sums<T, MODE>(p, at, lane, row_w + 16 * i, col_w + 16 * t);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (!(fabsf(acc[i][t][j]) <= std::numeric_limits<float>::max())) acc[i][t][j] = again[j];
+                }
         }
     }
     if (SUMS && with_sums && lane < 16) {
