@@ -165,3 +165,16 @@ def test_refusals():
         with pytest.raises(ValueError):
             call()
     assert g.eq(1).all()
+
+
+@pytest.mark.gpu
+def test_a_tensor_of_more_than_four_gigabytes():
+    from symmetrix_amd import finetune
+    n = 2_200_000_011
+    big, small = torch.full((n,), 0.5, device="cuda", dtype=torch.bfloat16), torch.full((3,), 2.0, device="cuda")
+    big[-1] = 64.0
+    want = math.sqrt(0.25 * (n - 1) + 64.0 ** 2 + 12.0)
+    _is_norm(finetune.grad_norm([big, small]), want)
+    _is_norm(finetune.clip_grads([big, small], want / 4), want)
+    # a quarter, but for the factor's rounding, which 8 bits do not show
+    assert float(big[-1]) == 16.0 and bool((big[:-1] == 0.125).all()) and ((small - 0.5).abs() <= 0.5 * 2.0 ** -23).all()

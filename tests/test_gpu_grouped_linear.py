@@ -314,3 +314,57 @@ def test_refusals():
         finetune.grouped_linear_backward(dy[:, :5], data["x"], data["weight"], data["index"])
     with pytest.raises(TypeError):
         finetune.grouped_linear_backward(dy.half(), data["x"], data["weight"], data["index"])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_rows_apart_by_more_than_four_gigabytes(dtype):
+    """Offsets of rows and matrices that 32 bits do not hold, in tiles of every size."""
+    from symmetrix_amd import finetune
+    dtype = NAMES[dtype]
+    rows, d_in, d_out, n = 80_011, 64, 72, 3
+    store = torch.empty(rows * 40_000, device="cuda", dtype=dtype)          # 6.4 or 12.8 GB, of which little is touched
+    x, dy = store.view(rows, 40_000)[:, :d_in], store.view(rows, 40_000)[:, 8_000:8_000 + d_out]
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x.normal_(generator=g)
+    dy.normal_(generator=g)
+    each = store.numel() // (n + 1) // 8 * 8
+    weight = store[16_000:].as_strided((n, d_out, d_in), (each, 40_000, 1))          # (among the rows)
+    weight.normal_(generator=g).mul_(d_in ** -0.5)
+    assert rows * 40_000 * store.element_size() > 1 << 32 and each * n * store.element_size() > 1 << 32
+    data = dict(x=x, weight=weight, bias=None, index=_index(rows, n, "mixed"))
+    _check(data, dy)
+    some = slice(rows - 50, rows)
+    _check(dict(data, x=x[some], index=data["index"][some]), dy[some])
+    far = dict(data, x=x[some].contiguous(), index=data["index"][some])
+    assert torch.equal(finetune.grouped_linear_forward(**far), finetune.grouped_linear_forward(**dict(data, x=x[some], index=far["index"])))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(NAMES))
+def test_many_groups_of_several_tiles(dtype):
+    """More groups than a wavefront has lanes, of no rows, of one, and of several tiles and pieces."""
+    for rows, d_in, d_out, n, order in ((9000, 64, 40, 63, "few"), (9000, 64, 40, 62, "few"), (20_000, 72, 64, 700, "few"), (4000, 33, 20, 2049, "one"), (30_000, 64, 64, 65, "mixed")):
+        _check(*_data(rows, d_in, d_out, n, NAMES[dtype], order))
+
+
+@pytest.mark.gpu
+def test_every_sum_not_finite():
+    """A row of infinities and NaN makes its own results what the formula says, whatever else shares its tile."""
+    from symmetrix_amd import finetune
+    for rows in (50, 300, 3000):
+        data, _ = _data(rows, 40, 24, 3, torch.float32, seed=rows)
+        data["index"].clamp_(min=0)
+        data["x"][::7] = float("inf")
+        data["x"][3::7] = float("nan")
+        data["weight"].abs_()
+        data["weight"][2].neg_()
+        y = finetune.grouped_linear_forward(**data)
+        high, low = torch.full((24,), float("inf"), device="cuda"), torch.full((24,), float("-inf"), device="cuda")
+        for i in range(0, rows, 7):
+            assert torch.equal(y[i], low if int(data["index"][i]) == 2 else high)
+        assert y[3::7].isnan().all()
+        others = torch.ones(rows, dtype=torch.bool, device="cuda")
+        others[::7] = others[3::7] = False
+        want, off = _reference(**{**data, "x": torch.where(others[:, None], data["x"], 0.0)})["y"]
+        _close(y[others], want[others], off[others], torch.float32)

@@ -224,3 +224,27 @@ def test_refusals():
     index.add_(1)          # the rows are sorted by what the index held before
     with pytest.raises(ValueError):
         finetune.embedding_forward(table, groups)
+
+
+@pytest.mark.gpu
+def test_tables_and_results_of_more_than_four_gigabytes():
+    """Numbers that are powers of two tell a row, and sums of a few of them are exact."""
+    from symmetrix_amd import finetune
+    entries, dim, rows = 70_001, 40_008, 70_003
+    table = torch.empty(entries, dim, device="cuda", dtype=torch.bfloat16)
+    marks = 2.0 ** (torch.arange(entries, device="cuda") % 15).to(torch.bfloat16)
+    table.copy_(marks[:, None].expand(-1, dim))
+    index = torch.tensor([entries - 1, 0, -1, entries - 2, 53_688, 53_689], dtype=torch.int32, device="cuda")
+    y = finetune.embedding_forward(table, index)
+    want = torch.where(index >= 0, marks[index.long().clamp(min=0)], 0.0)
+    assert torch.equal(y, want[:, None].expand(-1, dim).to(torch.bfloat16))
+    del y
+    index = (torch.arange(rows, device="cuda") * 7 % 5).to(torch.int32)
+    y = finetune.embedding_forward(table, index)
+    assert y.numel() * 2 > 1 << 32 and torch.equal(y, marks[index.long()][:, None].expand(-1, dim))
+    del table
+    # the gradient: 70 003 rows of which each adds its mark to one of 30 000 entries, two or three an entry
+    index = (torch.arange(rows, device="cuda") % 30_000).to(torch.int32)
+    got = finetune.embedding_backward(y, index, 30_000)
+    each = torch.zeros(30_000, device="cuda", dtype=torch.float64).index_add_(0, index.long(), y[:, 0].double())
+    assert torch.equal(got, each.to(torch.bfloat16)[:, None].expand(-1, dim))
