@@ -419,8 +419,10 @@ __device__ __forceinline__ void direct_tile(const Product& p, const Place& at, i
     int* const tile_rows = reinterpret_cast<int*>(lds + STAGES * STAGE);      // (for the results; there at the first barrier)
     if (MODE != WEIGHTS)
         for (int i = threadIdx.x; i < count; i += 64 * WAVES) tile_rows[i] = order[i];
-    // Of WEIGHTS: which rows the terms of the next steps are, sixteen steps' in LDS behind the tiles.  A step's come a step before they are
-    // needed; asked for in front of the tiles', so that a wait for all but the youngest tiles' waits for them.
+    // Of WEIGHTS: which rows the terms of the next steps are, sixteen steps' in LDS behind the tiles.  They are asked for AHEAD steps before
+    // they are needed, in front of that step's tiles: AHEAD (and no fewer) steps' tiles later, a wait for all but the youngest STAGES - 2 steps'
+    // has waited for them too, and a barrier shows them to the other wavefronts.
+    constexpr int AHEAD = STAGES > 3 ? STAGES - 2 : 1;
     const unsigned rows0 = lds0 + STAGES * STAGE;
     auto look_up = [&](int s) {
         if (MODE == WEIGHTS && wave == s % WAVES) load_words_into_lds(order, 4 * min(64 * s + lane, terms - 1), rows0 + s % 16 * 256);
@@ -527,8 +529,8 @@ __device__ __forceinline__ void direct_tile(const Product& p, const Place& at, i
     const bool idle = MODE != WEIGHTS && wm * NM * 16 >= count;
     if (stages > 0) {
         if constexpr (MODE == WEIGHTS) {
-            static_assert(STAGES < 15, "rows of sixteen steps");
-            for (int i = threadIdx.x; i < (STAGES + 1) * 64; i += 64 * WAVES) *(__attribute__((address_space(3))) int*)(rows0 + 4 * i) = order[min(i, terms - 1)];
+            static_assert(STAGES + AHEAD < 16, "rows of sixteen steps");
+            for (int i = threadIdx.x; i < (STAGES + AHEAD) * 64; i += 64 * WAVES) *(__attribute__((address_space(3))) int*)(rows0 + 4 * i) = order[min(i, terms - 1)];
             __syncthreads();
         }
 #pragma unroll
@@ -563,7 +565,7 @@ __device__ __forceinline__ void direct_tile(const Product& p, const Place& at, i
             add_sums(f[0]);
             wait_loads<(STAGES - 2) * PER>();
             barrier_only();      // the next tiles are there, and everybody has read these
-            look_up(s + STAGES + 1);
+            look_up(s + STAGES + AHEAD);
             request(s + STAGES);
             fetch(s + 1, 0, f[0]);
             sums(f[1]);

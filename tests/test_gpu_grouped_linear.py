@@ -368,3 +368,18 @@ def test_every_sum_not_finite():
         others[::7] = others[3::7] = False
         want, off = _reference(**{**data, "x": torch.where(others[:, None], data["x"], 0.0)})["y"]
         _close(y[others], want[others], off[others], torch.float32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+def test_long_groups_in_few_tiles(dtype):
+    """Sums over many rows with eight steps under way, whose rows' numbers come from memory while others' tiles do."""
+    from symmetrix_amd import finetune
+    for rows, d_in, d_out, n in ((2000, 96, 96, 3), (1500, 64, 64, 2), (900, 64, 136, 1), (5000, 128, 64, 4), (3000, 32, 200, 3), (8000, 64, 64, 9)):
+        data, dy = _data(rows, d_in, d_out, n, NAMES[dtype], "own", seed=rows)
+        _check(data, dy)
+        args = dy, data["x"], data["weight"], data["index"], (False, True, True)
+        first = finetune.grouped_linear_backward(*args)
+        for _ in range(20):
+            again = finetune.grouped_linear_backward(*args)
+            assert torch.equal(again[1], first[1]) and torch.equal(again[2], first[2])
