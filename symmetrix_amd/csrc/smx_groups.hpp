@@ -27,8 +27,13 @@ struct RowOrder {
 };
 // Whether the sort writes offsets without a launch for them.
 bool sort_has_offsets(long rows, int groups);
+// Memory that is filled with zeros beside the sort, which leaves most of the card idle.
+struct Zeros {
+    char* at = nullptr;      // a multiple of 2, as bytes is
+    long bytes = 0;
+};
 // Enqueues the sort; what it needs beside its results comes from the arena.
-void sort_rows(Launches& launches, Arena& arena, const int* index, long rows, int groups, const RowOrder& to);
+void sort_rows(Launches& launches, Arena& arena, const int* index, long rows, int groups, const RowOrder& to, const Zeros& zeros = {});
 
 // out[group][dim] = scale times the sum of the group's rows of in, and zeros where it has none; in `type`.  The rows' order in the
 // sums is theirs.  sorted.order null: the rows are sorted here.

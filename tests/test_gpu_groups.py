@@ -248,3 +248,32 @@ def test_tables_and_results_of_more_than_four_gigabytes():
     got = finetune.embedding_backward(y, index, 30_000)
     each = torch.zeros(30_000, device="cuda", dtype=torch.float64).index_add_(0, index.long(), y[:, 0].double())
     assert torch.equal(got, each.to(torch.bfloat16)[:, None].expand(-1, dim))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(NAMES))
+def test_few_of_many_entries(dtype):
+    """More entries than rows: zeros beside the sort, at every alignment of the table's gradient, and one entry with half of the rows."""
+    from symmetrix_amd import _lib, finetune
+    import ctypes as C
+    dtype = NAMES[dtype]
+    for rows, n, dim in ((129, 5000, 7), (1500, 1500, 33), (4096, 9001, 64), (4097, 4100, 129), (9000, 40_000, 24), (5000, 70_000, 520)):
+        g = torch.Generator(device="cuda").manual_seed(rows)
+        dy = torch.randn(rows, dim, generator=g, device="cuda").to(dtype)
+        index = _index(rows, n, "bad", seed=n)
+        index[::2] = n - 3
+        want, off = _sums(dy, index, n)
+        got = finetune.embedding_backward(dy, index, n)
+        _close(got, want, off, dtype)
+        assert torch.equal(got, finetune.embedding_backward(dy, finetune.group_rows(index, n), n))
+        # the C call into the middle of an array: what is beside it stays
+        size, kind = C.c_long(), list(NAMES.values()).index(dtype)          # (as SMX_TYPE_* are numbered)
+        lib = finetune._lib_functions()
+        _lib.check(lib.smx_embedding_backward_workspace(kind, rows, n, dim, C.byref(size)))
+        work = torch.empty(size.value, dtype=torch.uint8, device="cuda")
+        for shift in (1, 3, 8):
+            room = torch.full((n * dim + 16,), 7.0, device="cuda", dtype=dtype)
+            out = room[shift:shift + n * dim]
+            _lib.check(lib.smx_embedding_backward(kind, rows, n, dim, dy.data_ptr(), dim, index.data_ptr(), 0, 0, 1.0, out.data_ptr(), work.data_ptr(), size.value,
+                                                  torch.cuda.current_stream().cuda_stream))
+            assert torch.equal(out.view(n, dim), got) and (room[:shift] == 7).all() and (room[shift + n * dim:] == 7).all()
