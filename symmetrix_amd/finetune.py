@@ -617,6 +617,7 @@ def clip_grads(grads, max_norm, out=None):
         out = list(grads)
         for k, g in enumerate(grads):
             if g is not None and not g.is_contiguous():
+                _need(all(n <= 1 or step for n, step in zip(g.shape, g.stride())), "gradients that are clipped in place: numbers with memory of their own expected")
                 out[k] = g.contiguous()
                 back.append((g, out[k]))
         if back:

@@ -178,3 +178,29 @@ def test_a_tensor_of_more_than_four_gigabytes():
     _is_norm(finetune.clip_grads([big, small], want / 4), want)
     # a quarter, but for the factor's rounding, which 8 bits do not show
     assert float(big[-1]) == 16.0 and bool((big[:-1] == 0.125).all()) and ((small - 0.5).abs() <= 0.5 * 2.0 ** -23).all()
+
+
+def test_a_broadcast_gradient_is_not_clipped_in_place():
+    from symmetrix_amd import finetune
+    with pytest.raises(ValueError, match="memory of their own"):
+        finetune.clip_grads([torch.ones(3), torch.ones(()).expand(4, 5)], 1.0)
+
+
+@pytest.mark.gpu
+def test_broadcast_gradients():
+    """As sums have them: one number in memory for all."""
+    from symmetrix_amd import finetune
+    p, q = torch.zeros(40, 3, device="cuda", requires_grad=True), torch.ones(7, device="cuda", requires_grad=True)
+    grads = list(torch.autograd.grad(p.sum() + (q * q).sum(), [p, q]))
+    assert grads[0].stride() == (0, 0)
+    want = math.sqrt(120 + 28)
+    _is_norm(finetune.grad_norm(grads), want)
+    with pytest.raises(ValueError):
+        finetune.clip_grads(grads, 1.0)
+    assert grads[1].eq(2).all()
+    out = [torch.empty(40, 3, device="cuda"), torch.empty(7, device="cuda")]
+    _is_norm(finetune.clip_grads(grads, 1.0, out=out), want)
+    assert ((out[0].double() - 1 / want).abs() <= 2.0 ** -23).all() and ((out[1].double() - 2 / want).abs() <= 2.0 ** -22).all()
+    a = finetune.AdamW([p], lr=0.1, weight_decay=0.0)
+    _is_norm(a.step([grads[0]], max_norm=1.0), math.sqrt(120))
+    assert ((p + 0.1).abs() <= 1e-6).all()
