@@ -1148,13 +1148,15 @@ struct Call : Launches {
             q.col_tiles = (q.cols + wide - 1) / wide;
             return row_tiles(high) * q.col_tiles;
         };
-        // The largest tiles that are enough for three quarters of the CUs, that columns fill by three quarters, and groups of the usual size too.
-        // (In bfloat16, 16 384 rows of 4 groups, 1 024 columns: 128 terms 14.9 us and 15.6 in tiles of 128, 1 024 terms 34 and 44.  63 855 rows of
-        // 15 groups, 96 -> 32: tiles of 256 20 us.)
+        // The largest tiles that are enough for three quarters of the CUs (of the usual group the last tile is half full), that columns fill by three
+        // quarters, and that groups of the usual size fill; those of 128 also by half, since they read the weights once for two of 64.
+        // In bfloat16, 16 384 rows of 4 groups, 1 024 columns: 128 terms 14.9 us and 15.6 in tiles of 128, 1 024 terms 34 and 44.  63 855 rows of
+        // 15 groups, 96 -> 32: tiles of 256 20 us.  1 000 rows of 8 groups, 4 096 x 4 096, y and dx: 66 and 61 us in tiles of 128, 92 and 86 of 64;
+        // 4 000 rows of 48 groups, 2 048 x 2 048: 115 and 96, and 109 and 114; 5 000 rows of 60, 512 -> 1 024 in single precision: 51 and 68, and 66 and 75.
         const long used = std::min(p.rows, std::max(1L, (long)p.num_groups));
         auto fits = [&](int tile) {
             const long across = (q.cols + tile - 1) / tile;
-            return p.rows / tile * across >= 192 && 4L * q.cols >= 3 * across * tile && p.rows >= used * tile;
+            return (p.rows / tile + used / 2) * across >= 192 && 4L * q.cols >= 3 * across * tile && (tile == 128 ? 2 : 1) * p.rows >= used * tile;
         };
         if constexpr (!std::is_same_v<T, float>) {
             if (direct_ok) {
