@@ -612,19 +612,16 @@ def clip_grads(grads, max_norm, out=None):
     grads, each with memory of its own), and returns the norm that they had.  Where the norm is not finite they stay as they are."""
     grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
     _need(max_norm >= 0, "max_norm: a number from 0 on")
-    back, there = [], grads          # gradients that are clipped in a contiguous copy, and tensors that are written
-    if out is None:
-        out = list(grads)
-        for k, g in enumerate(grads):
-            if g is not None and not g.is_contiguous():
-                _need(all(n <= 1 or step for n, step in zip(g.shape, g.stride())), "gradients that are clipped in place: numbers with memory of their own expected")
-                out[k] = g.contiguous()
-                back.append((g, out[k]))
-        if back:
-            grads = out
-    else:
-        there = out = [out] if isinstance(out, torch.Tensor) else list(out)
-        _need(len(out) == len(grads), "out: a tensor for every gradient expected")
+    there = list(grads)
+    if out is not None:
+        there = [out] if isinstance(out, torch.Tensor) else list(out)
+        _need(len(there) == len(grads), "out: a tensor for every gradient expected")
+    back, out = [], list(there)          # gradients that are clipped in place by way of a contiguous copy, and the copies
+    for k, g in enumerate(there):
+        if g is not None and g is grads[k] and not g.is_contiguous():
+            _need(all(n <= 1 or step for n, step in zip(g.shape, g.stride())), "gradients that are clipped in place: numbers with memory of their own expected")
+            grads[k] = out[k] = g.contiguous()
+            back.append((g, out[k]))
     described = _describe_grads(grads, out)
     if not described[2]:
         return torch.zeros((), device="cuda")
