@@ -438,7 +438,7 @@ int smx_grad_norm_workspace(const smx_grad_tensor* tensors, int count, long* byt
 int smx_grad_norm(const smx_grad_tensor* tensors, int count, double max_norm, float* d_norm, float* d_factor,
                   void* d_workspace, long workspace_bytes, void* stream);
 /* out = factor grad for every tensor, rounded once; out may be grad itself, and has no memory in common with any
- * other tensor of the call. */
+ * other tensor of the call nor with a part of grad (such calls are refused). */
 int smx_clip_grads(const smx_grad_tensor* tensors, int count, double max_norm, float* d_norm, void* d_workspace,
                    long workspace_bytes, void* stream);
 

@@ -9,7 +9,9 @@
 // Bound by memory: 150 million numbers in bfloat16 are read for the norm in 47 us, 6.4 TB/s, and read and written clipped in 100, 6.0 TB/s.
 #include "smx_finetune.hpp"
 
+#include <algorithm>
 #include <cmath>
+#include <vector>
 
 namespace smx {
 
@@ -238,6 +240,31 @@ void check(const smx_grad_tensor* tensors, int count, bool sizes_only, bool outp
     }
 }
 
+// What is written has memory of its own: none of another result's, none of another tensor's gradient, and of its own gradient all or none.
+// (Blocks read gradients that others have written already, or will.)
+void check_apart(const smx_grad_tensor* tensors, int count)
+{
+    struct Range {
+        size_t from, to;
+    };
+    auto range = [](const void* at, const smx_grad_tensor& t) {
+        const size_t from = reinterpret_cast<size_t>(at);
+        return Range{from, from + t.numel * type_bytes(t.type)};
+    };
+    std::vector<Range> out;
+    out.reserve(count);
+    for (int i = 0; i < count; ++i)
+        if (tensors[i].numel) out.push_back(range(tensors[i].out, tensors[i]));
+    std::sort(out.begin(), out.end(), [](const Range& a, const Range& b) { return a.from < b.from; });
+    for (size_t k = 1; k < out.size(); ++k) refuse_unless(out[k - 1].to <= out[k].from, "results of tensors share memory");
+    for (int i = 0; i < count; ++i) {
+        if (tensors[i].numel == 0 || tensors[i].grad == tensors[i].out) continue;
+        const Range r = range(tensors[i].grad, tensors[i]);
+        const auto behind = std::partition_point(out.begin(), out.end(), [&](const Range& o) { return o.to <= r.from; });
+        refuse_unless(behind == out.end() || behind->from >= r.to, "a result shares memory with a gradient that is not its own, or with a part of it");
+    }
+}
+
 // fn(table, its number of blocks) for as many tensors at a time as a launch takes; the answer: blocks in all, each of which has a part of
 // the sum.
 template <typename Fn>
@@ -276,6 +303,7 @@ long workspace(const smx_grad_tensor* tensors, int count)
 void run(const smx_grad_tensor* tensors, int count, double max_norm, float* d_norm, float* d_factor, void* d_workspace, long workspace_bytes, void* stream, bool clip)
 {
     check(tensors, count, false, clip);
+    if (clip) check_apart(tensors, count);
     refuse_unless(max_norm >= 0, "max_norm: from 0 on");
     check_workspace(d_workspace, workspace_bytes, workspace(tensors, count), "smx_grad_norm_workspace");
     require_gfx950();

@@ -575,11 +575,14 @@ def _describe_grads(grads, outs=None):
             keep.append(g)
         from_ = g.data_ptr()
         numbers += (kind, from_, to or from_, n)
-    if outs is not None:
-        starts = [to for to, n in zip(numbers[2::4], numbers[3::4]) if n]
-        _need(len(set(starts)) == len(starts), "tensors that are written: every one once expected, each with memory of its own")
     count = len(numbers) // 4
     return _grad_tensors(count).pack(*numbers), device, count, keep
+
+
+def _span(t):
+    """Where the tensor's numbers begin and end in memory."""
+    at = t.data_ptr()
+    return at, at + (1 + sum((n - 1) * step for n, step in zip(t.shape, t.stride()))) * t.element_size() if t.numel() else at
 
 
 def _norm_call(described, max_norm, clip, factor=False):
@@ -622,6 +625,13 @@ def clip_grads(grads, max_norm, out=None):
             _need(all(n <= 1 or step for n, step in zip(g.shape, g.stride())), "gradients that are clipped in place: numbers with memory of their own expected")
             grads[k] = out[k] = g.contiguous()
             back.append((g, out[k]))
+    if back:          # (of what is written as it is, the call itself finds out)
+        spans = {(g.data_ptr(), g.shape, g.stride()): _span(g) for g, _ in back}
+        _need(len(spans) == len(back), "tensors that are written: every one once expected, each with memory of its own")
+        for g, o in zip(grads, out):
+            if g is not None and o is not None and o is not g:
+                from_, to = _span(o)
+                _need(all(to <= a or b <= from_ for a, b in spans.values()), "tensors that are written: every one once expected, each with memory of its own")
     described = _describe_grads(grads, out)
     if not described[2]:
         return torch.zeros((), device="cuda")
