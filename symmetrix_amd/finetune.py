@@ -623,8 +623,8 @@ def clip_grads(grads, max_norm, out=None):
     for k, g in enumerate(there):
         if g is not None and g is grads[k] and not g.is_contiguous():
             _need(all(n <= 1 or step for n, step in zip(g.shape, g.stride())), "gradients that are clipped in place: numbers with memory of their own expected")
-            grads[k] = out[k] = g.contiguous()
-            back.append((g, out[k]))
+            grads[k] = out[k] = g.detach().contiguous()
+            back.append((g.detach(), out[k]))
     if back:          # (of what is written as it is, the call itself finds out)
         spans = {(g.data_ptr(), g.shape, g.stride()): _span(g) for g, _ in back}
         _need(len(spans) == len(back), "tensors that are written: every one once expected, each with memory of its own")

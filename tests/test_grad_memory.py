@@ -106,3 +106,22 @@ def test_refused_before_anything_is_written():
     out = [torch.empty(600, device="cuda"), torch.empty(600, device="cuda")]
     norm = finetune.clip_grads([buf[:600], buf[400:]], 1.0, out=out)
     assert abs(float(norm) - math.sqrt(300)) <= 2.0 ** -23 * math.sqrt(300) and torch.equal(out[0], out[1]) and buf.eq(0.5).all()
+
+
+@pytest.mark.gpu
+def test_gradients_that_hang_on_a_graph():
+    """Recorded gradients (create_graph) and tensors that require gradients are clipped too, in any order of dimensions; nothing is recorded."""
+    from symmetrix_amd import finetune
+    for turn in (False, True):
+        make = lambda: _turned(40, 30) if turn else _turned(40, 30).contiguous()          # noqa: E731
+        want = make()
+        norm = finetune.clip_grads(want, 3.0)
+        leaf = make().requires_grad_()
+        x = torch.ones_like(leaf, requires_grad=True)
+        recorded, = torch.autograd.grad((x * x * leaf).sum() * 0.5, x, create_graph=True)
+        recorded = recorded if recorded.is_contiguous() != turn else recorded.t().contiguous().t()
+        assert recorded.requires_grad
+        for g in (leaf, recorded):
+            version, node = g._version, g.grad_fn
+            assert torch.equal(finetune.clip_grads([g], 3.0), norm)
+            assert torch.equal(g.detach(), want) and g._version > version and g.requires_grad and g.grad_fn is node
