@@ -328,21 +328,25 @@ def adapted_linear(x, weight, A, B, scale, index):
 # ---- rows by group
 
 class RowGroups:
-    """Rows sorted by group, for calls that share one index: what group_rows returns, to be given in the index's place.
+    """Rows sorted by group, for calls that share one index: what group_rows returns, to be given in the index's place, and refused once the
+    index, order or offsets have been written to.  (A captured graph cannot refuse: one that uses RowGroups from outside of it needs the index
+    as it was; one that is to follow the index has group_rows in it.)
 
     order: the rows (int32), those of group 0 first, then 1 and so on, then rows without a group (-1), then those whose index is out of range.
     offsets: where in it each group begins, where the rows without one do, and where those out of range do [num_groups + 2]."""
 
     def __init__(self, index, num_groups, order, offsets):
+        _need(order.dtype == offsets.dtype == torch.int32 and order.numel() == index.numel() and offsets.numel() == num_groups + 2
+              and order.is_contiguous() and offsets.is_contiguous(), "order and offsets as group_rows returns them expected")
         self.index, self.num_groups, self.order, self.offsets = index, num_groups, order, offsets
-        self._version = self._now()
+        self._versions = self._now()
 
-    def _now(self):          # (tensors of inference mode count no versions)
-        return None if self.index.is_inference() else self.index._version
+    def _now(self):          # (group_rows makes none of inference mode, which count no versions)
+        return [None if t.is_inference() else t._version for t in (self.index, self.order, self.offsets)]
 
     def of(self, num_groups):
         _need(num_groups == self.num_groups, f"rows by {num_groups} groups expected, not by {self.num_groups}")
-        _need(self._now() == self._version, "the index has been written to since its rows were sorted")
+        _need(self._now() == self._versions, "the index, order or offsets have been written to since the rows were sorted")
         return self
 
 
@@ -365,10 +369,17 @@ def _index(index, shape=None):
 
 
 def group_rows(index, num_groups):
-    """The rows of an index (int32; -1: no group) sorted by group, in their own order inside each."""
+    """The rows of an index (int32; -1: no group) sorted by group, in their own order inside each.
+
+    An index of torch's inference mode, which counts no writes, is copied: calls by its RowGroups go by what it held."""
+    if torch.is_inference_mode_enabled():
+        with torch.inference_mode(False):          # (so that order and offsets count theirs)
+            return group_rows(index, num_groups)
     index, _ = _index(index)
     _need(0 <= num_groups <= MAX_ENTRIES, f"num_groups: 0 to {MAX_ENTRIES}")
     device, rows = _on(index), index.numel()
+    if index.is_inference():
+        index = index.clone()
     order, offsets = index.new_empty((rows,)), index.new_empty((num_groups + 2,))
     work = index.new_empty((_group_rows_workspace(rows, num_groups),), dtype=torch.uint8)
     _call(device, _lib_functions().smx_group_rows, rows, num_groups, index.data_ptr(), order.data_ptr(), offsets.data_ptr(), work.data_ptr(), work.numel())
