@@ -388,7 +388,7 @@ int smx_group_rows(long rows, int num_groups, const int* d_index, int* d_order, 
                    long workspace_bytes, void* stream);
 
 /* Rows of a table: y_i = scale table[index_i]; zeros where the index is -1.  table[entries][dim], rows table_stride apart.
- * entries: up to SMX_MOST_ENTRIES, dim: up to 2^20. */
+ * entries: up to SMX_MOST_ENTRIES, dim: up to 2^20, scale: 0 or a normal number of single precision, which it is rounded to. */
 int smx_embedding_forward(int type, long rows, int entries, int dim, const void* d_table, long table_stride,
                           const int* d_index, double scale, void* d_y, long y_stride, void* stream);
 /* The table's gradient, dtable[entries][dim] in the type of dy: scale times the sum of the rows of dy of every entry, in

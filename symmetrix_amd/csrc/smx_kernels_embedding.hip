@@ -9,6 +9,7 @@
 // Bound by memory.  32 749 rows of 4 096 in bfloat16 looked up: 74 us, 5.9 TB/s of what has to move (81 a call; 91 with results by way of the caches).
 #include "smx_groups.hpp"
 
+#include <cmath>
 #include <limits>
 
 namespace smx {
@@ -300,6 +301,13 @@ void check(long rows, int entries, int dim)
     refuse_unless(dim >= 1 && dim <= 1 << 20, "dim: 1 to 2^20");
 }
 
+// (kernels multiply in single precision)
+void check_scale(double scale)
+{
+    const float f = (float)scale;
+    refuse_unless(scale == 0 || (std::isfinite(f) && std::fabs(f) >= std::numeric_limits<float>::min()), "scale: 0 or a normal number of single precision");
+}
+
 long workspace(int type, long rows, int entries, int dim)
 {
     Launches dry{nullptr, true};
@@ -367,6 +375,7 @@ extern "C" int smx_embedding_forward(int type, long rows, int entries, int dim, 
     return finetune_entry("smx_embedding_forward", [&] {
         (void)type_bytes(type);
         check(rows, entries, dim);
+        check_scale(scale);
         if (rows == 0) return;
         refuse_unless(d_index && d_y && (d_table || entries == 0), "table, index and y must not be null");
         refuse_unless(table_stride >= dim && y_stride >= dim, "strides of table and y: at least dim");
@@ -403,6 +412,7 @@ extern "C" int smx_embedding_backward(int type, long rows, int entries, int dim,
     return finetune_entry("smx_embedding_backward", [&] {
         (void)type_bytes(type);
         check(rows, entries, dim);
+        check_scale(scale);
         if (entries == 0) return;
         refuse_unless(d_dtable && (rows == 0 || (d_dy && d_index)), "dy, index and dtable must not be null");
         refuse_unless(dy_stride >= dim, "the stride of dy: at least dim");

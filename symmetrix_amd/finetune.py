@@ -389,7 +389,9 @@ def group_rows(index, num_groups):
 # ---- rows of a table
 
 def embedding_forward(table, index, scale=1.0):
-    """scale table[index] for every row of index (int32; -1: a row of zeros).  A row whose index is out of range is NaN."""
+    """scale table[index] for every row of index (int32; -1: a row of zeros).  A row whose index is out of range is NaN.
+
+    scale: 0 or a normal number of single precision, which it is rounded to."""
     kind = _type(table, "table")
     shape = table.shape
     if len(shape) != 2 or shape[1] < 1:
