@@ -336,17 +336,17 @@ class RowGroups:
     offsets: where in it each group begins, where the rows without one do, and where those out of range do [num_groups + 2]."""
 
     def __init__(self, index, num_groups, order, offsets):
-        _need(order.dtype == offsets.dtype == torch.int32 and order.numel() == index.numel() and offsets.numel() == num_groups + 2
-              and order.is_contiguous() and offsets.is_contiguous(), "order and offsets as group_rows returns them expected")
+        if order.dtype != torch.int32 or offsets.dtype != torch.int32 or order.numel() != index.numel() or offsets.numel() != num_groups + 2 \
+                or not (order.is_contiguous() and offsets.is_contiguous() and order.get_device() == offsets.get_device() == index.get_device()):
+            raise ValueError("order and offsets as group_rows returns them expected")
+        if index.is_inference() or order.is_inference() or offsets.is_inference():
+            raise ValueError("tensors that count their versions expected, not of inference mode")
         self.index, self.num_groups, self.order, self.offsets = index, num_groups, order, offsets
-        self._versions = self._now()
-
-    def _now(self):          # (group_rows makes none of inference mode, which count no versions)
-        return [None if t.is_inference() else t._version for t in (self.index, self.order, self.offsets)]
+        self._versions = index._version, order._version, offsets._version
 
     def of(self, num_groups):
         _need(num_groups == self.num_groups, f"rows by {num_groups} groups expected, not by {self.num_groups}")
-        _need(self._now() == self._versions, "the index, order or offsets have been written to since the rows were sorted")
+        _need((self.index._version, self.order._version, self.offsets._version) == self._versions, "the index, order or offsets have been written to since the rows were sorted")
         return self
 
 

@@ -28,6 +28,11 @@ def test_made_by_hand():
                            (torch.zeros(8, dtype=torch.int32)[::2], g.offsets)):
         with pytest.raises(ValueError):
             finetune.RowGroups(g.index, 3, order, offsets)
+    with torch.inference_mode():
+        uncounted = g.index.clone()
+    for tensors in ((uncounted, g.order, g.offsets), (g.index, uncounted, g.offsets)):
+        with pytest.raises(ValueError, match="inference"):
+            finetune.RowGroups(tensors[0], 3, *tensors[1:])
 
 
 @pytest.mark.gpu
