@@ -424,7 +424,7 @@ int smx_grouped_linear_backward(const smx_grouped_linear* p, const void* d_dy, l
 
 /* Gradients of many tensors (a host array of descriptions, read before the call returns), each of a type of its own:
  *   norm = sqrt(sum over all numbers of g^2),  factor = min(1, max_norm / norm), or 1 where the norm is not finite.
- * Squares and their sums are in double precision.  norm and factor (either may be NULL) are one float each in device
+ * Squares, their sums and the comparison are in double precision.  norm and factor (either may be NULL) are one float each in device
  * memory.  max_norm: from 0 on; infinity: a factor of 1.  numel: less than 2^36.  The workspace is at most
  * 8 (SMX_GRAD_NORM_PARTS + count) bytes, rounded up to a multiple of 256. */
 #define SMX_GRAD_NORM_PARTS 1024

@@ -7,9 +7,9 @@
 // device alone, so a launch has as many blocks as there can be tiles, and every block finds its own from the groups' offsets.
 //
 // Bound by the matrix instructions but for few rows, which are bound by the weights' bytes.  16-bit types, whole pieces of 16 bytes (k_direct):
-// straight from memory into LDS; 16 381 rows of 16 groups, 4 096 -> 2 048 in bfloat16, 310 to 325 us, 0.85 to 0.89 PFLOP/s (groups of the
-// same even size 1.0, a library's product of that size 1.3 to 1.5).  Single precision and any alignment (k_staged): by way of registers;
-// gradient of 50 000 rows of 12 groups, 256 -> 512: dx and dW 91 us each, 144 TFLOP/s (8 192 rows, 2 048 x 2 048: 190 to 200; a library's
+// straight from memory into LDS; 16 381 rows of 16 groups, 4 096 -> 2 048 in bfloat16, 286 us a call with the sort, 0.96 PFLOP/s (the kernel alone, slowed by
+// a profiler, 320 to 340; groups of the same even size 1.0 PFLOP/s, a library's product of that size 1.3 to 1.5).  Single precision and any alignment (k_staged): by way of registers;
+// gradient of 50 000 rows of 12 groups, 256 -> 512: dx and dW 91 us each, 144 TFLOP/s (8 192 rows, 2 048 x 2 048: 190 to 210; a library's
 // product 146).
 #include "smx_groups.hpp"
 
@@ -603,7 +603,8 @@ __device__ __forceinline__ void direct_tile(const Product& p, const Place& at, i
 }
 
 // LARGE: 256 x 256 by eight wavefronts, one block on a CU, those of the last round cut in two or four (16 381 rows as above: 345 us uncut).
-// Gradient of 8 179 rows of 8 groups, 2 048 x 2 048 in float16: dx 78 us, dW 74.
+// Gradient of 8 179 rows of 8 groups, 2 048 x 2 048 in float16: dx 78 us, dW 74.  (dx's takes all 256 registers and keeps one more in memory, which the last
+// steps of a tile alone read; dW's tiles are not cut.)
 template <typename T, int MODE, bool LARGE, int BM, int STAGES>
 __global__ __launch_bounds__(LARGE ? 512 : 256, 2) void k_direct(const Product p)
 {
@@ -639,7 +640,9 @@ __global__ __launch_bounds__(LARGE ? 512 : 256, 2) void k_direct(const Product p
 // ---- operands by way of registers: any alignment, and single precision, which is brought to bf16 parts on the way
 
 // Both operands of single precision in three bf16 parts, exactly, of whose products the six largest are formed (what is left out is below
-// 1.002 2^-24 of a product), small ones first.  Numbers are brought up by 2^24 first, so that the parts of small ones are normal numbers.
+// 1.002 2^-24 of a product), small ones first.  Numbers are brought up by 2^24 first, so that the parts of small ones are normal numbers.  Numbers from
+// 2^104 on and sums from 2^80 on do not fit then (db: from 2^104 on); what they make infinite or NaN is formed again, as sums that are not finite are, in twenty
+// times the time (8 192 rows, 2 048 x 2 048: 0.33 ms, 7.4).
 constexpr float kSplitScale = 16777216.0f;
 __device__ __forceinline__ void parts_of(const float (&x)[8], bf16x8 (&part)[3])
 {
@@ -1152,7 +1155,8 @@ struct Call : Launches {
         // quarters, and that groups of the usual size fill; those of 128 also by half, since they read the weights once for two of 64.
         // In bfloat16, 16 384 rows of 4 groups, 1 024 columns: 128 terms 14.9 us and 15.6 in tiles of 128, 1 024 terms 34 and 44.  63 855 rows of
         // 15 groups, 96 -> 32: tiles of 256 20 us.  1 000 rows of 8 groups, 4 096 x 4 096, y and dx: 66 and 61 us in tiles of 128, 92 and 86 of 64;
-        // 4 000 rows of 48 groups, 2 048 x 2 048: 115 and 96, and 109 and 114; 5 000 rows of 60, 512 -> 1 024 in single precision: 51 and 68, and 66 and 75.
+        // 4 000 rows of 48 groups, 2 048 x 2 048: 116 and 96, and 110 and 114 (one rule for both: dx gains more than y loses, where y loses at all);
+        // 5 000 rows of 60, 512 -> 1 024 in single precision: 51 and 68, and 66 and 75.  (Groups of even size.)
         const long used = std::min(p.rows, std::max(1L, (long)p.num_groups));
         auto fits = [&](int tile) {
             const long across = (q.cols + tile - 1) / tile;
