@@ -180,3 +180,36 @@ def test_rows_of_infinities_and_nan(d_in, d_out, dtype):
         others = torch.ones(rows, dtype=torch.bool, device="cuda")
         others[::7] = others[3::7] = False
         assert torch.equal(y[others], clean[others])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(NAMES))
+@pytest.mark.parametrize("rows,d_in,d_out", [(20, 96, 80), (20, 101, 63), (400, 96, 80), (400, 101, 63), (8200, 64, 1536), (8200, 1536, 64)])
+def test_subnormal_numbers(rows, d_in, d_out, dtype):
+    """Numbers below the normal ones of their type times large ones: whole multiples of one small number, fewer than 2^24 of it in any sum, so that
+    sums in single precision are exact and results are rounded once."""
+    from symmetrix_amd import finetune
+    dtype = NAMES[dtype]
+    least, large = {torch.float32: (2.0 ** -149, 2.0 ** 100), torch.bfloat16: (2.0 ** -133, 2.0 ** 100), torch.float16: (2.0 ** -24, 2.0 ** 8)}[dtype]
+    g = torch.Generator(device="cuda").manual_seed(rows + d_in)
+    whole = lambda high, *s: torch.randint(-high, high + 1, s, generator=g, device="cuda").double()          # noqa: E731
+    index = torch.randint(0, 3, (rows,), generator=g, device="cuda", dtype=torch.int32)
+    x, dy, w = whole(3, rows, d_in), whole(2, rows, d_out), whole(1, 3, d_out, d_in)
+    assert (3 * 2 * rows) < 1 << 24
+    small, big = (lambda t: (t * least).to(dtype)), (lambda t: (t * large).to(dtype))
+    assert torch.equal(small(x).double(), x * least) and torch.equal(big(dy).double(), dy * large)
+    unit = least * large
+    y = finetune.grouped_linear_forward(small(x), big(w), None, index)
+    dx, _, _ = finetune.grouped_linear_backward(small(dy), small(x), big(w), index)
+    _, dw, db = finetune.grouped_linear_backward(big(dy), small(x), big(w), index)
+    for k in range(3):
+        at = (index == k).nonzero()[:, 0]
+        assert torch.equal(y[at], (x[at] @ w[k].t() * unit).to(dtype))
+        assert torch.equal(dx[at], (dy[at] @ w[k] * unit).to(dtype))
+        assert torch.equal(dw[k], (dy[at].t() @ x[at] * unit).to(dtype))
+        assert torch.equal(db[k], (dy[at].sum(0) * large).to(dtype))
+    _, _, db = finetune.grouped_linear_backward(small(dy), small(x), big(w), index)
+    table = finetune.embedding_backward(small(dy), index, 3)
+    for k in range(3):
+        want = (dy[index == k].sum(0) * least).to(dtype)
+        assert torch.equal(db[k], want) and torch.equal(table[k], want)
